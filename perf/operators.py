@@ -132,12 +132,12 @@ def values(codes, scales):
 
 def pack(codes, scales):
     """Codes [Np, Kp] and scale bytes [Np, Kp / 32] of a weight -> fragments
-    [Np / 16, Kp / 128][2 halves][4 blocks][16 rows][16 bytes] and their scales
-    [Np / 16, Kp / 128][16 rows][4 blocks]."""
+    [Np / 16, Kp / 128][8 chunks of 16 columns][16 rows][16 bytes] and their
+    scales [Np / 16, Kp / 128][16 rows][4 blocks]."""
     np_, kp = codes.shape
-    c = codes.view(torch.uint8).view(np_ // 16, 16, kp // 128, 4, 2, 16)
+    c = codes.view(torch.uint8).view(np_ // 16, 16, kp // 128, 8, 16)
     s = scales.view(np_ // 16, 16, kp // 128, 4)
-    return c.permute(0, 2, 4, 3, 1, 5).contiguous(), s.permute(0, 2, 1, 3).contiguous()
+    return c.permute(0, 2, 3, 1, 4).contiguous(), s.permute(0, 2, 1, 3).contiguous()
 
 
 def mx_out(y):

@@ -315,8 +315,9 @@ def _table():
     return torch.tensor(v, dtype=torch.float64, device=DEV)
 
 
-def _exact_mx(y):
-    """Rounded values (over the scale) and scales of f64 rows, the rows padded to 128 columns."""
+def _exact_mx(y, rounded=True):
+    """Values over their scale (rounded to codes, or as they are) and scales of
+    f64 rows, the rows padded to 128 columns."""
     rows, cols = y.shape
     wide = torch.zeros(rows, _up(cols, 128), dtype=torch.float64, device=y.device)
     wide[:, :cols] = y
@@ -326,6 +327,8 @@ def _exact_mx(y):
     scale = torch.where(top > 448 * scale, 2 * scale, scale)
     scale = torch.where((top <= 224 * scale) & (scale > 2.0 ** -127), scale / 2, scale)
     t = t / scale[..., None]
+    if not rounded:
+        return t.reshape(rows, -1), scale
     step = torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6))) - 3)
     step = torch.where(t.abs() >= 16 * step, 2 * step, step)
     step = torch.where((t.abs() < 8 * step) & (step > 2.0 ** -9), step / 2, step)
@@ -333,8 +336,8 @@ def _exact_mx(y):
     return codes.reshape(rows, -1), scale
 
 
-def _exact_out(y):
-    codes, scale = _exact_mx(y)
+def _exact_out(y, rounded=True):
+    codes, scale = _exact_mx(y, rounded)
     return codes, scale.reshape(len(y), -1, 4).transpose(0, 1)
 
 
@@ -373,7 +376,8 @@ def exact(case, seed):
         return g / (1 + torch.exp(-g)) * u
 
     if kind == "swiglu":
-        return _exact_out(swiglu(_exact_rows(s), s["w"], case["n"]))
+        # as a bf16 result: before the rounding to the output's bits
+        return _exact_out(swiglu(_exact_rows(s), s["w"], case["n"]), rounded=False)
     if kind == "linear":
         y = product(_exact_rows(s), s["w"], case["n"])
         for more in (s["bias"], s["residual"]):

@@ -2,7 +2,8 @@
  * pa_dense.h -- the dense side around the paged-attention path, for an
  * end-to-end decoder step: RMSNorm or LayerNorm (with the residual add fused
  * in), the SwiGLU activation, and the linear projections (skinny-M for
- * decode steps, a tiled GEMM for prompt chunks).  Conventions as pa.h (device
+ * decode steps, a tiled GEMM for prompt chunks), and the same projections over
+ * MXFP8 rows and weights.  Conventions as pa.h (device
  * pointers, stream-ordered, PA_OK or a negative pa_status); dtype
  * PA_DTYPE_F32 or PA_DTYPE_BF16, math in f32.
  */
@@ -148,6 +149,86 @@ int32_t pa_linear_rope_cache(void* out, const void* x, const void* weight, const
 int32_t pa_linear_pack_qkv(void* packed, const void* weight, const void* col_scale,
                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                            int32_t cols, int32_t dtype, pa_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* The projections in MXFP8                                               */
+/* ---------------------------------------------------------------------- */
+
+/* MXFP8 (the OCP microscaling format with E4M3 elements): a row's columns go
+ * in blocks of 32 with one power-of-two scale each, the format that the matrix
+ * cores multiply directly.  No counterpart in the reference, whose FP8 is a KV
+ * cache type with codes of its own (PA_DTYPE_FP8_E4M3); here the codes are OCP
+ * E4M3 (bias 7, +-448 the largest, 0x7F / 0xFF NaN, no infinities).
+ *   a = the largest |y| among the block's finite values
+ *   e = the smallest integer >= -127 with a <= 448 * 2^e; scale byte e + 127
+ *   code = y * 2^-e rounded to the nearest E4M3 value, ties to even; NaN and
+ *          +-inf become NaN codes
+ * so no finite value saturates, and a value is its code times 2^(byte - 127).
+ * Columns are padded to Kp, the next multiple of 128, with zero codes.
+ *   rows     codes [rows, Kp] uint8; scales [Kp / 128][R][4] uint8, R = rows
+ *            rounded up to 16: byte b of (s, r) scales columns 128 s + 32 b ..
+ *            + 31 of row r.  The scales of rows behind `rows` are neither
+ *            written nor used.
+ *   weights  [N, K], N padded to Np, the next multiple of 16, with zero rows:
+ *            codes [Np / 16][Kp / 128][8][16][16], 16-row x 128-column
+ *            fragments of 2 KB in the order of the matrix instructions'
+ *            operands: chunk c of row r holds columns 16 c .. 16 c + 15;
+ *            scales [Np / 16][Kp / 128][16][4].
+ * Code arrays are 16-byte aligned, scale arrays 4-byte. */
+
+/* Kp: the bytes of one row of codes. */
+size_t pa_mx_row_bytes(int32_t cols);
+/* Bytes of the scales of `rows` MXFP8 rows, and of a weight of `rows` rows. */
+size_t pa_mx_scale_bytes(int32_t rows, int32_t cols);
+/* Bytes of the codes of a weight of `rows` rows. */
+size_t pa_mx_weight_bytes(int32_t rows, int32_t cols);
+
+/* Quantises rows to MXFP8 (the attention's output in front of an MXFP8 O
+ * projection): x [rows, cols] of dtype with x_stride elements between rows
+ * (0 = cols, else at least cols), any alignment; codes and scales as above.
+ * x does not overlap them. */
+int32_t pa_quantize_mx(uint8_t* codes, uint8_t* scales, const void* x, int32_t rows,
+                       int32_t cols, int64_t x_stride, int32_t dtype, pa_stream_t stream);
+
+/* pa_rms_norm with an MXFP8 output:
+ *   if add != NULL:  sum[r] = residual[r] + add[r]  (rounded to dtype)
+ *   y[r] = s / sqrt(mean(s^2) + eps) * weight,  s = sum[r], or residual[r]
+ *   codes, scales = MXFP8 of y (f32, not rounded in between)
+ * residual / add / sum [rows, hidden] and weight [hidden] contiguous, of dtype;
+ * sum is needed with add only and may be residual itself (in place), but
+ * overlaps nothing otherwise. */
+int32_t pa_rms_norm_mx(uint8_t* codes, uint8_t* scales, void* sum, const void* residual,
+                       const void* add, const void* weight, int32_t rows, int32_t hidden,
+                       float eps, int32_t dtype, pa_stream_t stream);
+
+/* Quantises a weight [rows, cols] of dtype (contiguous) into the weight layout
+ * above: a load-time step. */
+int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void* weight, int32_t rows,
+                          int32_t cols, int32_t dtype, pa_stream_t stream);
+
+/* pa_linear on MXFP8 rows and weights:
+ *   act PA_ACT_NONE:      out[r][n] = sum_k x[r][k] * weight[n][k]
+ *                                     (+ bias[n]) (+ residual[r][n])
+ *   act PA_ACT_SILU_MUL:  weight is the gate|up matrix [2 N, K], N a multiple
+ *                         of 32, out[r][n] = silu(g) * u of the two products of
+ *                         column n; bias and residual must be NULL.
+ * out_scales NULL: out [rows, N] bf16, contiguous, 16-byte aligned, rounded
+ * once, from the f32 result.  out_scales given (PA_ACT_SILU_MUL only): the
+ * result goes out as MXFP8 rows, codes to out, for the projection after it.
+ *   bias [N] or NULL, residual [rows, N] or NULL, bf16, contiguous; residual
+ *   may be out itself (the residual stream updated in place), but out overlaps
+ *   no other argument.
+ * The sums are f32, over groups of 16 columns whose exact products the matrix
+ * instructions align to the group's largest, keeping 13 binary places below
+ * its leading one: a result is off by about 2^-14 of its largest products,
+ * well below the bf16 rounding unless terms cancel.
+ * Any rows, N (with PA_ACT_NONE) and K up to 2^22.  The order of a row's f32
+ * sums, and with it the last bit of an output, may depend on rows, N and K
+ * (equal calls give equal bits). */
+int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x, const uint8_t* x_scales,
+                     const uint8_t* weight, const uint8_t* weight_scales, const void* bias,
+                     const void* residual, int32_t rows, int32_t out_features,
+                     int32_t in_features, int32_t act, pa_stream_t stream);
 
 /* Greedy sampling's argmax_logits (crates/traits/src/sampling.rs:439-453) on
  * every row of a logit matrix: out[r] = the first column holding the row's

@@ -1,0 +1,333 @@
+"""The MXFP8 operators against their definitions in 64 bits (mx_plain.py), at
+the sizes, layouts and values where they can go wrong."""
+import zlib
+
+import pytest
+import torch
+
+import mx_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.bfloat16, torch.float32]
+EPS = 1e-6
+
+
+def gen(*key):
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def hidden_states(g, rows, cols, dtype=torch.float32):
+    x = torch.randn(rows, cols, generator=g, device=DEV)
+    x *= 1 + 20 * (torch.rand(cols, generator=g, device=DEV) < 0.02)
+    return x.to(dtype)
+
+
+def same_as_definition(mx, y):
+    """Codes and scales of values that need no rounding before them: equal."""
+    v, s = plain.quantize(y)
+    got, _ = plain.row_values(mx)
+    assert torch.equal(plain.row_scales(mx), s)
+    assert torch.equal(torch.nan_to_num(got, 1e9), torch.nan_to_num(v, 1e9))
+
+
+SIZES = [(1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129), (5, 896), (64, 1000),
+         (33, 2048), (7, 2049), (4, 4096), (3, 8200), (2, 12289), (1000, 40), (4099, 96)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantize(pa, rows, cols, dtype):
+    x = hidden_states(gen(rows, cols), rows, cols, dtype)
+    same_as_definition(pa.quantize_mx(x), x.double())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_strided_and_misaligned(pa, dtype):
+    wide = hidden_states(gen(1), 37, 513, dtype)
+    for lo, hi in ((0, 512), (1, 301), (3, 500), (509, 513)):
+        x = wide[:, lo:hi]
+        same_as_definition(pa.quantize_mx(x), x.double())
+    one = wide[5:6, 7:200]
+    same_as_definition(pa.quantize_mx(one), one.double())
+
+
+def test_quantize_values(pa):
+    """Every magnitude: powers of two around the scale's borders, ties between
+    codes, subnormal floats and codes, zeros, the largest floats."""
+    v = []
+    for e in (-149, -148, -140, -136, -127, -126, -120, -10, -1, 0, 1, 8, 100, 127):
+        for m in (1.0, 1.0 + 2.0 ** -23, 1.0625, 1.125, 1.1875, 1.5, 1.75, 1.75 + 2.0 ** -23,
+                  2.0 - 2.0 ** -23):
+            v.append(m * 2.0 ** e)
+    v = torch.tensor(v, dtype=torch.float64).to(torch.float32)
+    v = torch.cat([v, -v, torch.zeros(2)]).to(DEV)
+    # each as the largest of its block, over blocks of its own fractions
+    frac = torch.cat([torch.tensor([1.0]), 2.0 ** -torch.arange(0, 21).float(),
+                      torch.tensor([0.9375, 0.53125, 0.28125, 0.0009765625, 3e-4, 1e-5, 0., -0.,
+                                    -0.71875, -0.3])])[:32].to(DEV)
+    x = v[:, None] * frac
+    same_as_definition(pa.quantize_mx(x.contiguous()), x.double())
+    # every half step between codes is a tie
+    t = torch.arange(0, 1025, device=DEV).float() * 2.0 ** -10
+    t = torch.cat([t, torch.arange(1, 449, device=DEV).float(), t * 448])
+    x = torch.cat([t, -t, t.new_zeros(-2 * len(t) % 31)]).view(-1, 31)
+    x = torch.cat([torch.full((len(x), 1), 448.0, device=DEV), x], 1)
+    same_as_definition(pa.quantize_mx(x), x.double())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_non_finite(pa, dtype):
+    """NaN and infinities become NaN codes and leave the rest of their block."""
+    x = hidden_states(gen(2), 6, 96, dtype)
+    x[0, 3] = float("nan")
+    x[1, 40] = float("inf")
+    x[2, 95] = -float("inf")
+    x[3, :32] = float("nan")
+    x[4] = float("inf")
+    same_as_definition(pa.quantize_mx(x), x.double())
+
+
+def test_outputs_stay_in_their_rows(pa):
+    """The scales of the rows behind the last and what follows the arrays stay."""
+    rows, cols = 21, 300
+    x = hidden_states(gen(3), rows, cols)
+    codes = torch.full((rows + 3, 384), 0xAB, dtype=torch.uint8, device=DEV)
+    scales = torch.full((3 * 32 * 4 + 64,), 0xCD, dtype=torch.uint8, device=DEV)
+    out = pa.MxRows(codes[:rows], scales[:3 * 32 * 4].view(3, 32, 4), rows, cols)
+    assert pa.quantize_mx(x, out=out) is out
+    same_as_definition(out, x.double())
+    assert (codes[rows:] == 0xAB).all() and (scales[3 * 32 * 4:] == 0xCD).all()
+    assert (out.scales[:, rows:] == 0xCD).all()
+    w = torch.ones(cols, device=DEV)
+    out.scales[:, :rows] = 0
+    pa.rms_norm_mx(x, w, EPS, out=out)
+    assert (codes[rows:] == 0xAB).all() and (out.scales[:, rows:] == 0xCD).all()
+
+
+# ---- RMSNorm ---------------------------------------------------------------
+
+
+def norm_reference(x, add, w):
+    s = x.double() if add is None else (x.float() + add.float()).to(x.dtype).double()
+    y = s / (s.pow(2).mean(1, keepdim=True) + EPS).sqrt() * w.double()
+    # f32: the squares' sum rounds in a lane's chain of at most max(32, K / 32)
+    # additions and eight more, half of it left by the root; the mean, eps, the
+    # root, the division and three products round once each
+    k = x.shape[1]
+    return s, y, y.abs() * (max(32, k / 32) / 2 + 4 + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_add", [False, True])
+@pytest.mark.parametrize("rows,cols", SIZES + [(2, 20000)])
+def test_rms_norm(pa, rows, cols, dtype, with_add):
+    g = gen(rows, cols, with_add)
+    x = hidden_states(g, rows, cols, dtype)
+    w = (1 + 0.2 * torch.randn(cols, generator=g, device=DEV)).to(dtype)
+    add = hidden_states(g, rows, cols, dtype) if with_add else None
+    s, y, err = norm_reference(x, add, w)
+    before = x.clone()
+    total = torch.empty_like(x) if with_add else None
+    mx = pa.rms_norm_mx(x, w, EPS, add=add, residual_out=total)
+    assert torch.equal(x, before)
+    if with_add:
+        assert torch.equal(total.double(), s)
+    plain.assert_rounds(mx, y, err)
+    # in place: the same sum and the same codes
+    mx2 = pa.rms_norm_mx(x, w, EPS, add=add)
+    assert torch.equal(mx.codes, mx2.codes)
+    assert torch.equal(plain.row_scales(mx), plain.row_scales(mx2))
+    assert torch.equal(x.double(), s)
+
+
+def test_rms_norm_special_rows(pa):
+    """A row of zeros, one of the smallest values, one with an infinity, one
+    with a NaN, one whose squares overflow: as the formula in f32 has them."""
+    x = torch.ones(5, 256, device=DEV)
+    x[0] = 0
+    x[1] = 1e-30
+    x[2, 7] = float("inf")
+    x[3, 200] = float("nan")
+    x[4] = 1e30
+    w = torch.ones(256, device=DEV)
+    v = plain.dequantize(pa.rms_norm_mx(x, w, EPS))
+    assert (v[0] == 0).all()
+    # 1e-30 / sqrt(eps), as its block's only value: within half a step of 2^-4
+    assert ((v[1] / 1e-27 - 1).abs() <= 2.0 ** -4).all()
+    assert torch.isnan(v[2, 7]) and (torch.cat([v[2, :7], v[2, 8:]]) == 0).all()
+    assert torch.isnan(v[3]).all()
+    assert (v[4] == 0).all()  # 1 / sqrt(inf)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rms_norm_misaligned(pa, dtype):
+    """Contiguous tensors that start one element behind a 16-byte border."""
+    rows, cols = 9, 333
+    g = gen(4)
+
+    def odd(n):
+        return torch.randn(n + 1, generator=g, device=DEV).to(dtype)[1:]
+
+    x, add, w = odd(rows * cols).view(rows, cols), odd(rows * cols).view(rows, cols), odd(cols)
+    s, y, err = norm_reference(x, add, w)
+    plain.assert_rounds(pa.rms_norm_mx(x, w, EPS, add=add), y, err)
+    assert torch.equal(x.double(), s)
+
+
+# ---- products --------------------------------------------------------------
+
+
+def weight(pa, g, n, k, dtype=torch.bfloat16):
+    return pa.MxWeight((torch.randn(n, k, generator=g, device=DEV) * k ** -0.5).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 40), (100, 896), (3, 2050), (33, 5000)])
+def test_pack(pa, n, k, dtype):
+    w = hidden_states(gen(n, k), n, k, dtype)
+    mx = pa.MxWeight(w)
+    v, s = plain.quantize(w.double())
+    ref = (v.view(n, -1, 32) * torch.exp2(s.double() - 127)[..., None]).view(n, -1)
+    assert not ref[:, k:].any()
+    assert torch.equal(plain.weight_values(mx), ref[:, :k])
+    # the rows and columns behind the last are zero codes
+    np_ = plain.up(n, 16)
+    codes = mx.codes.view(np_ // 16, -1, 8, 16, 16).permute(0, 3, 1, 2, 4).reshape(np_, -1)
+    assert not codes[n:].any() and not codes[:, k:].any()
+
+
+def product(x, w):
+    """The product in 64 bits, and what it may be off.  The matrix instructions
+    align the (exact) products of 16 consecutive columns to the largest of them
+    and keep 13 binary places below its leading one: 16 products each lose less
+    than 2^-13 of the largest, which is at most the product of the largest
+    magnitudes of both operands.  (Measured on the instructions with one small
+    product between two large ones of opposite sign: within 16 columns it is
+    kept down to 2^-13 of them, beside other columns to 2^-23.)  The groups'
+    sums are added in f32: fewer than K roundings of at most the sum of all
+    magnitudes."""
+    def tops(v):
+        pad = -v.shape[1] % 16
+        return torch.nn.functional.pad(v.abs(), (0, pad)).view(len(v), -1, 16).amax(-1)
+
+    err = tops(x) @ tops(w).t() * (16 * 2.0 ** -13)
+    return x @ w.t(), err + x.abs() @ w.abs().t() * (x.shape[1] * 2.0 ** -24)
+
+
+def near_bf16(out, ref, err):
+    bad = ~((out.double() - ref).abs() <= err + (ref.abs() + err) * 2.0 ** -8 + 1e-38)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3].tolist())
+
+
+# rows around the tiles' heights, widths off the tiles and off the 16-byte
+# stores, K off the blocks and steps
+PRODUCTS = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (3, 64, 128), (7, 100, 129), (16, 896, 896),
+            (17, 1152, 896), (31, 900, 300), (32, 4864, 896), (33, 40, 4864), (48, 2050, 640),
+            (64, 896, 4864), (65, 72, 257), (100, 1001, 1000), (127, 128, 128), (128, 130, 2048),
+            (129, 257, 384), (200, 520, 4096), (255, 255, 255), (256, 256, 256), (257, 300, 512),
+            (333, 896, 4864), (513, 1025, 130), (618, 2056, 1152), (1025, 640, 896),
+            (2100, 1100, 300), (5000, 900, 160)]
+
+
+@pytest.mark.parametrize("epi", ["none", "bias", "residual", "both"])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_linear(pa, m, n, k, epi):
+    g = gen(m, n, k, epi)
+    x = pa.quantize_mx(hidden_states(g, m, k))
+    w = weight(pa, g, n, k)
+    bias = res = None
+    if epi in ("bias", "both"):  # at an odd offset: the bias has no alignment of its own
+        bias = torch.randn(n + 1, generator=g, device=DEV).to(torch.bfloat16)[1:]
+    if epi in ("residual", "both"):
+        res = hidden_states(g, m, n, torch.bfloat16)
+    ref, err = product(plain.dequantize(x)[:, :k], plain.weight_values(w))
+    for more in (bias, res):
+        if more is not None:
+            err = err + (ref.abs() + err + more.double().abs()) * 2.0 ** -24
+            ref = ref + more.double()
+    out = pa.linear_mx(x, w, bias=bias, residual=res)
+    near_bf16(out, ref, err)
+    assert torch.equal(out, pa.linear_mx(x, w, bias=bias, residual=res))
+    if res is not None:  # the residual stream updated in place
+        assert pa.linear_mx(x, w, bias=bias, residual=res, out=res) is res
+        assert torch.equal(out, res)
+
+
+GATED = [(1, 32, 1), (2, 32, 40), (3, 64, 128), (16, 96, 300), (17, 4864, 896), (32, 160, 896),
+         (33, 128, 129), (64, 416, 1000), (65, 32, 64), (100, 224, 256), (130, 288, 896),
+         (257, 1056, 384), (333, 4864, 896), (700, 352, 1100), (1100, 2080, 160),
+         (4000, 192, 256)]
+
+
+def gated_reference(x, w, n):
+    gu, err = product(x, w)
+    gate, up, eg, eu = gu[:, :n], gu[:, n:], err[:, :n], err[:, n:]
+    silu = gate / (1 + torch.exp(-gate))
+    y = silu * up
+    # |silu'| < 1.1; the exponential, the sum, the division and two products
+    return y, 1.1 * eg * (up.abs() + eu) + silu.abs() * eu + y.abs() * 16 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("m,n,k", GATED)
+def test_linear_swiglu(pa, m, n, k):
+    g = gen(m, n, k)
+    x = pa.quantize_mx(hidden_states(g, m, k))
+    w = weight(pa, g, 2 * n, k)
+    y, err = gated_reference(plain.dequantize(x)[:, :k], plain.weight_values(w), n)
+    out = pa.linear_mx(x, w, act=pa.ops.ACT_SILU_MUL)
+    near_bf16(out, y, err)
+    mx = pa.linear_mx(x, w, act=pa.ops.ACT_SILU_MUL, mx_out=True)
+    plain.assert_rounds(mx, y, err)
+    again = pa.linear_mx(x, w, act=pa.ops.ACT_SILU_MUL, mx_out=True)
+    assert torch.equal(mx.codes, again.codes)
+    assert torch.equal(plain.row_scales(mx), plain.row_scales(again))
+
+
+@pytest.mark.parametrize("m", [5, 70, 300])
+def test_linear_outputs_stay_in_their_rows(pa, m):
+    """What follows an output, and the scales of the rows behind the last, stay."""
+    g = gen(m)
+    n, k = 96, 200
+    x = pa.quantize_mx(hidden_states(g, m, k))
+    w = weight(pa, g, 2 * n, k)
+    r = plain.up(m, 16)
+    codes = torch.full((m + 2, 128), 0xAB, dtype=torch.uint8, device=DEV)
+    scales = torch.full((r * 4 + 64,), 0xCD, dtype=torch.uint8, device=DEV)
+    out = pa.MxRows(codes[:m], scales[:r * 4].view(1, r, 4), m, n)
+    pa.linear_mx(x, w, act=pa.ops.ACT_SILU_MUL, out=out, mx_out=True)
+    assert (codes[m:] == 0xAB).all() and (scales[r * 4:] == 0xCD).all()
+    assert (out.scales[:, m:] == 0xCD).all()
+    assert not out.codes[:, n:].any() and not out.scales[0, :m, 3].any()
+    for n in (96, 90):
+        buf = torch.full((m + 2, n), 7.0, dtype=torch.bfloat16, device=DEV)
+        pa.linear_mx(x, weight(pa, g, n, k), out=buf[:m])
+        assert (buf[m:] == 7).all()
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_linear_non_finite(pa, m):
+    """A NaN in a row of x reaches that row of the output alone, one in a row
+    of the weight that column; products beyond f32 are infinite."""
+    g = gen(m)
+    n, k = 80, 300
+    xf = hidden_states(g, m, k)
+    xf[1, 299] = float("nan")
+    wf = torch.randn(n, k, generator=g, device=DEV)
+    wf[70, 0] = float("inf")
+    out = pa.linear_mx(pa.quantize_mx(xf), pa.MxWeight(wf))
+    nan = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    nan[1] = True
+    nan[:, 70] = True
+    assert torch.equal(torch.isnan(out), nan) and torch.isfinite(out[~nan]).all()
+    big = torch.full((m, 128), 2.0 ** 70, device=DEV)
+    assert (pa.linear_mx(pa.quantize_mx(big), pa.MxWeight(big)) == float("inf")).all()
+    small = torch.full((m, 128), 2.0 ** -90, device=DEV)
+    assert (pa.linear_mx(pa.quantize_mx(small), pa.MxWeight(small)) == 0).all()
+
+
+def test_linear_scale_range(pa):
+    """Scales from both ends of their range cancel in a product."""
+    x = pa.quantize_mx(torch.full((3, 160), 2.0 ** 100, device=DEV))
+    w = pa.MxWeight(torch.full((20, 160), 2.0 ** -101, device=DEV))
+    assert (pa.linear_mx(x, w) == 80).all()

@@ -1,0 +1,114 @@
+"""The MXFP8 entry points' sizes and refusals: checked on the host before any
+launch, so without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib(pa):
+    return pa._lib.load()
+
+
+P = C.c_void_p(64)
+ODD = C.c_void_p(65)
+
+
+def test_sizes(lib):
+    assert [lib.pa_mx_row_bytes(c) for c in (1, 128, 129, 896, 4864, 0, -1)] == \
+        [128, 128, 256, 896, 4864, 0, 0]
+    assert lib.pa_mx_scale_bytes(1, 1) == 16 * 4
+    assert lib.pa_mx_scale_bytes(17, 896) == 32 * 7 * 4
+    assert lib.pa_mx_scale_bytes(0, 896) == 0
+    assert lib.pa_mx_weight_bytes(33, 130) == 48 * 256
+    # beyond 32 bits
+    assert lib.pa_mx_weight_bytes(1 << 20, 1 << 14) == 1 << 34
+
+
+def quantize(lib, codes=P, scales=P, x=P, rows=4, cols=100, stride=0, dtype=1):
+    return lib.pa_quantize_mx(codes, scales, x, rows, cols, stride, dtype, None)
+
+
+def test_quantize_refusals(lib):
+    assert quantize(lib, rows=0, codes=None, scales=None, x=None) == 0
+    assert quantize(lib, rows=-1) == -1
+    assert quantize(lib, cols=0) == -1
+    assert quantize(lib, dtype=2) == -1 and b"dtype" in lib.pa_last_error()
+    assert quantize(lib, stride=99) == -1 and b"overlap" in lib.pa_last_error()
+    assert quantize(lib, stride=-100) == -1
+    assert quantize(lib, cols=(1 << 22) + 1) == -3
+    for name in ("codes", "scales", "x"):
+        assert quantize(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
+        assert quantize(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
+
+
+def norm(lib, codes=P, scales=P, sum=P, residual=P, add=P, weight=P, rows=4, hidden=100, dtype=1):
+    return lib.pa_rms_norm_mx(codes, scales, sum, residual, add, weight, rows, hidden, 1e-6, dtype,
+                              None)
+
+
+def test_norm_refusals(lib):
+    assert norm(lib, rows=0, codes=None) == 0
+    assert norm(lib, rows=-1) == -1
+    assert norm(lib, hidden=0) == -1
+    assert norm(lib, dtype=7) == -1
+    assert norm(lib, hidden=(1 << 22) + 1) == -3
+    assert norm(lib, sum=None) == -1 and b"needs sum" in lib.pa_last_error()
+    for name in ("codes", "scales", "residual", "weight"):
+        assert norm(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
+    for name in ("codes", "scales", "sum", "residual", "add", "weight"):
+        assert norm(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
+
+
+def pack(lib, codes=P, scales=P, weight=P, rows=4, cols=100, dtype=1):
+    return lib.pa_linear_mx_pack(codes, scales, weight, rows, cols, dtype, None)
+
+
+def test_pack_refusals(lib):
+    assert pack(lib, rows=0) == -1
+    assert pack(lib, cols=0) == -1
+    assert pack(lib, dtype=2) == -1
+    assert pack(lib, cols=(1 << 22) + 1) == -3
+    for name in ("codes", "scales", "weight"):
+        assert pack(lib, **{name: None}) == -1
+        assert pack(lib, **{name: ODD}) == -1
+
+
+def linear(lib, out=P, out_scales=None, x=P, xs=P, w=P, ws=P, bias=None, residual=None, rows=4,
+           n=96, k=100, act=0):
+    return lib.pa_linear_mx(out, out_scales, x, xs, w, ws, bias, residual, rows, n, k, act, None)
+
+
+def test_linear_refusals(lib):
+    assert linear(lib, rows=0, out=None, x=None) == 0
+    assert linear(lib, rows=-1) == -1
+    assert linear(lib, n=0) == -1
+    assert linear(lib, k=0) == -1
+    assert linear(lib, act=2) == -1 and b"activation" in lib.pa_last_error()
+    assert linear(lib, act=1, bias=P) == -1
+    assert linear(lib, act=1, residual=P) == -1
+    assert linear(lib, out_scales=P) == -1 and b"SwiGLU" in lib.pa_last_error()
+    assert linear(lib, act=1, n=48) == -3 and b"multiple of 32" in lib.pa_last_error()
+    assert linear(lib, k=(1 << 22) + 1) == -3
+    assert linear(lib, n=1 << 24, k=1 << 22) == -3
+    for name in ("out", "x", "xs", "w", "ws"):
+        assert linear(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
+    for name in ("out", "x", "xs", "w", "ws", "bias", "residual"):
+        assert linear(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
+    assert linear(lib, act=1, out_scales=ODD) == -1
+
+
+def test_wrappers_refuse_host_tensors(pa):
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError):
+        pa.quantize_mx(x)
+    with pytest.raises(ValueError):
+        pa.rms_norm_mx(x, torch.ones(64), 1e-6)
+    with pytest.raises(ValueError):
+        pa.MxWeight(x)
+    with pytest.raises(ValueError):
+        pa.linear_mx(x, x)
+    with pytest.raises(ValueError):
+        pa.MxRows(torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 16, 4, dtype=torch.uint8),
+                  4, 64)

@@ -10,6 +10,8 @@ raises.
 from . import _lib
 from .ops import (
     BLOCK_SIZE,
+    MxRows,
+    MxWeight,
     PaError,
     argmax,
     block_hash,
@@ -22,7 +24,10 @@ from .ops import (
     rope_inv_freq,
     layer_norm,
     linear,
+    linear_mx,
+    quantize_mx,
     rms_norm,
+    rms_norm_mx,
     rope_reshape_and_cache,
     silu_mul,
     slot_mapping,
@@ -31,6 +36,8 @@ from .kv_cache import PagedKvCache, StepBatch
 
 __all__ = [
     "BLOCK_SIZE",
+    "MxRows",
+    "MxWeight",
     "PaError",
     "PagedKvCache",
     "StepBatch",
@@ -45,7 +52,10 @@ __all__ = [
     "rope_inv_freq",
     "layer_norm",
     "linear",
+    "linear_mx",
+    "quantize_mx",
     "rms_norm",
+    "rms_norm_mx",
     "rope_reshape_and_cache",
     "silu_mul",
     "slot_mapping",

@@ -37,6 +37,13 @@ SIGNATURES = {
                          _i32, _p]),
     "pa_linear_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
     "pa_linear_pack": (_i32, [_p, _p, _p, _i32, _i32, _i32, _p]),
+    "pa_mx_row_bytes": (_sz, [_i32]),
+    "pa_mx_scale_bytes": (_sz, [_i32, _i32]),
+    "pa_mx_weight_bytes": (_sz, [_i32, _i32]),
+    "pa_quantize_mx": (_i32, [_p, _p, _p, _i32, _i32, _i64, _i32, _p]),
+    "pa_rms_norm_mx": (_i32, [_p, _p, _p, _p, _p, _p, _i32, _i32, _f32, _i32, _p]),
+    "pa_linear_mx_pack": (_i32, [_p, _p, _p, _i32, _i32, _i32, _p]),
+    "pa_linear_mx": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p]),
     "pa_argmax": (_i32, [_p, _p, _i32, _i32, _i64, _i32, _p]),
     "pa_linear_rope_cache": (_i32, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
                                     _p, _p, _p, _p, _p, _i32, _i32, _p]),

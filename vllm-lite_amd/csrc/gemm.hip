@@ -4,42 +4,15 @@
 #include <algorithm>
 
 #include "gemm_tiling.hpp"
+#include "lds_copy.hpp"
 #include "pa_common.hpp"
 #include "pa_internal.hpp"
 
 namespace pa {
 namespace {
 
-// A wavefront's copy HBM -> LDS of 16 bytes per lane: lane l's bytes come
-// from base + off (off per lane) and land at LDS address lds + 16 l.  Written
-// out in assembly: with the builtin the compiler cannot tell that the operand
-// reads which follow use another LDS buffer, and makes them wait for the copy
-// (vmcnt(0) right after every copy).  The kernel orders copies and reads
-// itself (wait_copies and a barrier at the top of every step).  A load to LDS
-// needs one wait state after the write of m0, which the compiler does not add
-// inside assembly: the s_nop.
-#pragma clang diagnostic ignored "-Winline-asm"  // m0 as a clobber
-__device__ inline void lds_copy16(const uint8_t* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(off), "s"(base), "s"(lds)
-               : "memory", "m0");
-}
-__device__ inline void lds_copy16(const uint8_t* base, uint64_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :
-               : "v"(base + off), "s"(lds)
-               : "memory", "m0");
-}
 // Round to nearest even with the conversion instruction.
 __device__ inline uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
-// Waits until at most N of this wavefront's copies are in flight and its LDS
-// reads and writes are done.
-template <int N>
-__device__ inline void wait_copies() {
-  static_assert(N <= 63, "vmcnt range");
-  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 0xF) | ((N >> 4) << 14));
-}
 
 // Workgroup = KG groups of WM x WN wavefronts.  Wavefront (wm, wn) of a group
 // computes TM x TN tiles of 32 x 32 (v_mfma_f32_32x32x16_bf16), so the

@@ -1,0 +1,68 @@
+// MXFP8 blocks on the device: 32 columns, one power-of-two scale, E4M3 codes
+// (the format's definition and layouts: include/pa_dense.h).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace pa {
+
+// MXFP8 column steps of 128 (one dword of scale bytes per row).
+inline int64_t mx_steps(int64_t cols) { return (cols + 127) / 128; }
+inline int64_t mx_pad_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
+constexpr int kMxMaxCols = 1 << 22;
+
+// Lane permutations within 16 lanes.  Once a value is equal over each aligned
+// group of 4 (8) lanes, the half mirror (mirror) brings the other group's.
+template <int CTRL>
+__device__ inline uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
+
+// |y| as bits, 0 for NaN and infinities: finite magnitudes order as integers.
+__device__ inline uint32_t mx_magnitude(float y) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, y) & 0x7FFFFFFFu;
+  return u < 0x7F800000u ? u : 0u;
+}
+// The scale byte of a block whose largest finite magnitude has bits a: with
+// a = 1.m 2^x, a <= 448 2^e = 1.75 2^(8 + e) asks for e >= x - 8, and one more
+// where m is above .75 (the carry); at least 0 (subnormal and zero blocks).
+__device__ inline uint32_t mx_scale_byte(uint32_t a) {
+  const uint32_t x = (a + 0x1FFFFFu) >> 23;
+  return x > 8 ? x - 8 : 0;
+}
+// 2^(127 - byte), by which a block's values are multiplied (bytes 0 .. 247).
+__device__ inline float mx_inverse(uint32_t byte) {
+  return __builtin_bit_cast(float, (254u - byte) << 23);
+}
+// Two codes: round to nearest even in the conversion (|y| <= 448 here; an
+// infinity is made a NaN first, as E4M3 has none).
+__device__ inline float mx_finite(float y) {
+  return __builtin_fabsf(y) < __builtin_inff() ? y : __builtin_nanf("");
+}
+__device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float inv) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(mx_finite(a) * inv, mx_finite(b) * inv, 0, false);
+  v = __builtin_amdgcn_cvt_pk_fp8_f32(mx_finite(c) * inv, mx_finite(d) * inv, v, true);
+  return (uint32_t)v;
+}
+
+// Eight consecutive columns per lane, a block over 4 lanes, 128 columns over
+// 16 lanes, which all run this.  Returns the lane's codes; dword gets the four
+// scale bytes of the 128 columns (in every lane).
+__device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a = max(a, mx_magnitude(y[e]));
+  a = max(a, dpp<kDppXor1>(a));
+  a = max(a, dpp<kDppXor2>(a));
+  const uint32_t byte = mx_scale_byte(a);
+  const float inv = mx_inverse(byte);
+  uint32_t d = byte << (8 * ((threadIdx.x >> 2) & 3));
+  d |= dpp<kDppHalfMirror>(d);
+  d |= dpp<kDppMirror>(d);
+  dword = d;
+  return uint2{mx_codes4(y[0], y[1], y[2], y[3], inv), mx_codes4(y[4], y[5], y[6], y[7], inv)};
+}
+
+}  // namespace pa

@@ -1,0 +1,436 @@
+// pa_linear_mx: Y[M, N] = X[M, K] · W[N, K]ᵀ on MXFP8 rows and weights
+// (layouts: include/pa_dense.h), a tiled GEMM on the scaled matrix
+// instructions.
+#include <algorithm>
+#include <type_traits>
+
+#include "lds_copy.hpp"
+#include "mx_common.hpp"
+#include "pa_common.hpp"
+#include "pa_internal.hpp"
+#include "../../include/pa_dense.h"
+
+namespace pa {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct MxLinear {
+  void* out;
+  uint8_t* out_scales;
+  const uint8_t *x, *xs, *w, *ws;
+  const uint16_t *bias, *residual;
+  int M, N;
+  int steps;      // of 128 columns
+  int64_t pad_m;  // rows of a scale column of x (and of the output)
+};
+
+// Workgroup = KG groups of WM x WN wavefronts.  Wavefront (wm, wn) of a group
+// computes TM x TN tiles of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4), so the
+// workgroup tile is BM = 32 WM TM rows of X by BN = 32 WN TN rows of W.  Group
+// kg takes the K steps (128 columns) kg, KG + kg, ..., and the groups' sums
+// meet in LDS at the end.  A stage is one step of every group, copied HBM ->
+// LDS into one of S buffers, S - 1 stages ahead of use, one barrier per stage.
+//
+// LDS, per step: X rows of 128 bytes with their 16-byte chunks XOR-swizzled by
+// the row (the 16 rows that an operand read serves at once hit distinct bank
+// slots), W fragments as they lie in memory, one scale dword per row of each.
+// Operands of a product over 64 columns: lane (n, g) = (lane % 32, lane / 32)
+// holds columns 16 g .. + 15 and 32 + 16 g .. + 15 of row n, and the scale
+// byte of columns 32 g .. + 31.  The products compute the transposed tile (A =
+// W, B = X): lane (n, g) holds X row n and, in register r, output column
+// 8 (r / 4) + 4 g + r % 4.
+//
+// SILU: the tile's BN weight rows are BN/2 gate rows, then the matching up
+// rows; a wavefront takes TN/2 gate tiles and their up tiles.
+template <bool SILU, int WM, int WN, int TM, int TN, int KG, int S>
+__global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLinear p, int ntm,
+                                                                    int ntn) {
+  constexpr int GW = WM * WN, NT = 64 * GW * KG;
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, BNO = SILU ? BN / 2 : BN;
+  constexpr int CA = BM / 8 / GW, CB = BN / 8 / GW;         // 1 KB copies per wavefront
+  constexpr int SC = (BM + BN) / 64, CS = (SC + GW - 1) / GW;  // 256 B copies of scales
+  constexpr int PER = CA + CB + CS;
+  static_assert(CA * GW * 8 == BM && CB * GW * 8 == BN && BM % 64 == 0 && BN % 64 == 0 &&
+                    (!SILU || (TN % 2 == 0 && (BN / 2) % 16 == 0)),
+                "tiles");
+  constexpr int STEP = (BM + BN) * 132, STAGE = KG * STEP;  // codes, then scale dwords
+  constexpr int SX = (BM + BN) * 128, SW = SX + BM * 4;
+  constexpr int ORB = BNO * 2 + 16;  // bytes per row of the staged output tile
+  constexpr int RED = BM * BN * 4 * (KG - 1);
+  constexpr int SM0 = S * STAGE > BM * ORB ? S * STAGE : BM * ORB;
+  constexpr int SM = SM0 > RED ? SM0 : RED;
+  static_assert(SM + 4 * BN <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[SM];
+  __shared__ float sbias[SILU ? 1 : BN];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / GW, wt = wave % GW;
+  const int wm = wt / WN, wn = wt % WN;
+  const int n = lane & 31, g = lane >> 5;
+  const int M = p.M, N = p.N, nk = p.steps;
+  // Tile order: workgroups are dealt round-robin to the 8 XCDs; XCD i takes
+  // the i-th contiguous range of an order that goes through groups of row
+  // tiles (all of them up to 8, so that W is streamed once; else 4), column
+  // tiles outer within a group, so the tiles in flight on an XCD share X and
+  // W rows in its L2.
+  const int group_m = ntm <= 8 ? ntm : 4;
+  const int total = ntm * ntn, per_xcd = (total + 7) / 8;
+  const int tile = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= per_xcd || tile >= total) return;
+  const int first_m = tile / (group_m * ntn) * group_m;
+  const int gsz = min(group_m, ntm - first_m), in_grp = tile % (group_m * ntn);
+  const int m0 = (first_m + in_grp % gsz) * BM;
+  const int c0 = in_grp / gsz * BNO;  // first output column
+  const int tiles_n = (N + 15) / 16;  // 16-row fragments of W (of its gate half)
+  auto swz = [](int r) -> int { return (r / 2) % 8; };
+
+  // This wavefront's copies of a step: scalar bases, 32-bit lane offsets.
+  const uint8_t* xb = p.x + (int64_t)m0 * nk * 128;
+  uint32_t xo[CA];
+#pragma unroll
+  for (int u = 0; u < CA; ++u) {
+    const int r = (CA * wt + u) * 8 + lane / 8;
+    xo[u] = (uint32_t)min(r, M - 1 - m0) * (uint32_t)(nk * 128) + ((lane % 8) ^ swz(r)) * 16;
+  }
+  // the fragment of W that holds row r of the tile
+  auto frag = [&](int r) __attribute__((always_inline)) -> int {
+    const bool up = SILU && r >= BN / 2;
+    return min((c0 + (up ? r - BN / 2 : r)) / 16, tiles_n - 1) + (up ? tiles_n : 0);
+  };
+  const uint8_t* wb[CB];  // half a fragment each
+#pragma unroll
+  for (int u = 0; u < CB; ++u) {
+    const int piece = CB * wt + u;
+    wb[u] = p.w + (int64_t)frag(piece * 8) * nk * 2048 + piece % 2 * 1024;
+  }
+  // Scales, 64 rows a copy: first X's, then W's; the last ones twice where
+  // the copies do not divide among the wavefronts.
+  const uint8_t* sb[CS];
+  uint32_t so[CS], sl[CS];
+  int64_t sstep[CS];  // bytes from one step's scales to the next's
+  const int f0 = frag(0);
+#pragma unroll
+  for (int u = 0; u < CS; ++u) {
+    const int c = (wt + GW * u) % SC, r = (c * 64 < BM ? 0 : -BM) + c * 64 + lane;
+    if (c * 64 < BM) {
+      sb[u] = p.xs + (int64_t)m0 * 4;
+      so[u] = (uint32_t)min(r, M - 1 - m0) * 4;
+      sstep[u] = p.pad_m * 4;
+    } else {
+      sb[u] = p.ws + (int64_t)f0 * nk * 64;
+      so[u] = (uint32_t)(frag(r) - f0) * (uint32_t)(nk * 64) + r % 16 * 4;
+      sstep[u] = 64;
+    }
+    sl[u] = SX + c * 256;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  auto issue = [&](int stage, int buf) __attribute__((always_inline)) {
+    // a group without a step in the last stage copies the last step again
+    const int kt = min(stage * KG + kg, nk - 1);
+    const uint32_t l0 = lds0 + buf * STAGE + kg * STEP;
+    const uint32_t la = __builtin_amdgcn_readfirstlane(l0 + CA * wt * 1024);
+    const uint32_t lb = __builtin_amdgcn_readfirstlane(l0 + BM * 128 + CB * wt * 1024);
+#pragma unroll
+    for (int u = 0; u < CA; ++u) lds_copy16(xb + (int64_t)kt * 128, xo[u], la + u * 1024);
+#pragma unroll
+    for (int u = 0; u < CB; ++u)
+      lds_copy16(wb[u] + (int64_t)kt * 2048, (uint32_t)lane * 16, lb + u * 1024);
+#pragma unroll
+    for (int u = 0; u < CS; ++u)
+      lds_copy4(sb[u] + kt * sstep[u], so[u], __builtin_amdgcn_readfirstlane(l0 + sl[u]));
+  };
+  // tile rows of this lane's operands (SILU: gate tiles, then their up tiles)
+  int arow[TM], brow[TN];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) arow[t] = (wm * TM + t) * 32 + n;
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+    brow[t] = SILU ? (t < TN / 2 ? (wn * TN / 2 + t) * 32 + n
+                                 : BN / 2 + (wn * TN / 2 + t - TN / 2) * 32 + n)
+                   : (wn * TN + t) * 32 + n;
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+  auto two16 = [](const uint8_t* lo, const uint8_t* hi) __attribute__((always_inline)) {
+    return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(lo),
+                                   *reinterpret_cast<const i32x4*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  const int ns = (nk + KG - 1) / KG;
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t)
+    if (t < ns) issue(t, t);
+  for (int st = 0, buf = 0, ibuf = S - 1; st < ns; ++st) {
+    // this wavefront's copies of the stage have landed (near the end fewer
+    // stages are in flight and all are waited for) ...
+    if (ns - st > S - 2)
+      wait_copies<(S - 2) * PER>();
+    else
+      wait_copies<0>();
+    // ... and after the barrier everyone's, and everyone is done with the
+    // stage before, whose buffer the next copies fill
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (st + S - 1 < ns) issue(st + S - 1, ibuf);
+    if (KG == 1 || st * KG + kg < nk) {
+      const uint8_t* at = lds + buf * STAGE + kg * STEP;
+      const uint8_t* bt = at + BM * 128;
+      // this lane's byte of the first 64 columns in bits 0-7, of the second in 16-23
+      int sa[TM], sw[TN];
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+        sa[t] = *reinterpret_cast<const uint32_t*>(at + SX + arow[t] * 4) >> (8 * g);
+#pragma unroll
+      for (int t = 0; t < TN; ++t)
+        sw[t] = *reinterpret_cast<const uint32_t*>(at + SW + brow[t] * 4) >> (8 * g);
+      auto half = [&](auto hc) __attribute__((always_inline)) {
+        constexpr int h = decltype(hc)::value;
+        i32x8 af[TM], bf[TN];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+          const uint8_t* row = at + arow[t] * 128;
+          af[t] = two16(row + ((4 * h + g) ^ swz(arow[t])) * 16,
+                        row + ((4 * h + 2 + g) ^ swz(arow[t])) * 16);
+        }
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const uint8_t* f = bt + brow[t] / 16 * 2048 + brow[t] % 16 * 16;
+          bf[t] = two16(f + (4 * h + g) * 256, f + (4 * h + 2 + g) * 256);
+        }
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TN; ++b)
+            acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                bf[b], af[a], acc[a][b], 0, 0, 2 * h, sw[b], 2 * h, sa[a]);
+      };
+      half(std::integral_constant<int, 0>{});
+      half(std::integral_constant<int, 1>{});
+    }
+    buf = buf == S - 1 ? 0 : buf + 1;
+    ibuf = ibuf == S - 1 ? 0 : ibuf + 1;
+  }
+  __syncthreads();
+  // the K groups' sums, in group order
+  if constexpr (KG > 1) {
+    float* red = reinterpret_cast<float*>(lds);
+    auto slot = [&](int z, int a, int b, int q) __attribute__((always_inline)) {
+      return red + (((z * GW + wt) * TM * TN + a * TN + b) * 4 + q) * 256 + lane * 4;
+    };
+    if (kg > 0) {
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(slot(kg - 1, a, b, q)) =
+                float4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2],
+                       acc[a][b][4 * q + 3]};
+    }
+    __syncthreads();
+    if (kg == 0) {
+#pragma unroll
+      for (int z = 0; z < KG - 1; ++z)
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TN; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float4 v = *reinterpret_cast<const float4*>(slot(z, a, b, q));
+              acc[a][b][4 * q] += v.x;
+              acc[a][b][4 * q + 1] += v.y;
+              acc[a][b][4 * q + 2] += v.z;
+              acc[a][b][4 * q + 3] += v.w;
+            }
+    }
+    __syncthreads();
+  }
+  if constexpr (SILU) {
+    constexpr int TB = TN / 2;
+    // silu(g) u, 0 in the columns behind the last (an MXFP8 output's padding)
+    if (KG == 1 || kg == 0) {
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) {
+          const bool real = c0 + (wn * TB + b) * 32 < N;  // N is a multiple of 32
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float gate = acc[a][b][i];
+            const float y = gate / (1.0f + expf(-gate)) * acc[a][b + TB][i];
+            acc[a][b][i] = real ? y : 0.f;
+          }
+        }
+    }
+    if (p.out_scales) {
+      constexpr int CRB = BNO + 16, NBLK = BNO / 32;  // bytes per staged row, blocks per row
+      static_assert(BM * (CRB + NBLK) <= SM, "staged codes");
+      if (KG == 1 || kg == 0) {
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TB; ++b) {
+            // a block's 32 columns are this lane's 16 and those of lane ^ 32
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, mx_magnitude(acc[a][b][i]));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+            const uint32_t byte = mx_scale_byte(top);
+            const float inv = mx_inverse(byte);
+            const int blk = wn * TB + b;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint32_t*>(lds + arow[a] * CRB + blk * 32 + 8 * q + 4 * g) =
+                  mx_codes4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2],
+                            acc[a][b][4 * q + 3], inv);
+            if (g == 0) lds[BM * CRB + arow[a] * NBLK + blk] = (uint8_t)byte;
+          }
+      }
+      __syncthreads();
+      const int pitch = (N + 127) / 128 * 128;
+      uint8_t* out = static_cast<uint8_t*>(p.out);
+      for (int i = threadIdx.x; i < BM * (BNO / 16); i += NT) {
+        const int r = i / (BNO / 16), cc = i % (BNO / 16) * 16;
+        if (m0 + r < M && c0 + cc < pitch)
+          *reinterpret_cast<uint4*>(out + (int64_t)(m0 + r) * pitch + c0 + cc) =
+              *reinterpret_cast<const uint4*>(lds + r * CRB + cc);
+      }
+      for (int i = threadIdx.x; i < BM * NBLK; i += NT) {
+        const int r = i % BM, blk = i / BM, at = c0 / 32 + blk;
+        if (m0 + r < M && at * 32 < pitch)
+          p.out_scales[((at / 4) * p.pad_m + m0 + r) * 4 + at % 4] =
+              lds[BM * CRB + r * NBLK + blk];
+      }
+      return;
+    }
+  }
+  // bf16 output.  The residual rows and the bias into LDS ...
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+  constexpr int CPRO = BNO / 8;
+  if constexpr (!SILU) {
+    if (p.residual)
+      for (int i = threadIdx.x; i < BM * CPRO; i += NT) {
+        const int r = i / CPRO, cc = i % CPRO * 8;
+        if (m0 + r >= M || c0 + cc >= N) continue;
+        const uint16_t* src = p.residual + (int64_t)(m0 + r) * N + c0 + cc;
+        uint8_t* dst = lds + r * ORB + cc * 2;
+        if (N % 8 == 0)
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+        else
+          for (int e = 0; e < 8 && c0 + cc + e < N; ++e)
+            reinterpret_cast<uint16_t*>(dst)[e] = src[e];
+      }
+    for (int i = threadIdx.x; i < BN; i += NT)
+      sbias[i] = p.bias && c0 + i < N ? bf16_bits_to_f32(p.bias[c0 + i]) : 0.f;
+    __syncthreads();
+  }
+  // ... the results beside them, rounded once ...
+  if (KG == 1 || kg == 0) {
+    constexpr int TB = SILU ? TN / 2 : TN;
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = (wn * TB + b) * 32 + 8 * q + 4 * g;
+          uint64_t* at = reinterpret_cast<uint64_t*>(lds + arow[a] * ORB + col * 2);
+          const uint64_t prev = !SILU && p.residual ? *at : 0;
+          uint16_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = acc[a][b][4 * q + e];
+            if constexpr (!SILU) {
+              y += sbias[col + e];
+              y += bf16_bits_to_f32((uint16_t)(prev >> (16 * e)));
+            }
+            v[e] = f32_to_bf16_bits(y);
+          }
+          *at = *reinterpret_cast<const uint64_t*>(v);
+        }
+  }
+  __syncthreads();
+  // ... and the rows out, 8 columns per thread at a time
+  for (int i = threadIdx.x; i < BM * CPRO; i += NT) {
+    const int r = i / CPRO, cc = i % CPRO * 8;
+    const int row = m0 + r, col = c0 + cc;
+    if (row >= M || col >= N) continue;
+    const uint8_t* src = lds + r * ORB + cc * 2;
+    uint16_t* dst = out + (int64_t)row * N + col;
+    if (N % 8 == 0)
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+    else
+      for (int e = 0; e < 8 && col + e < N; ++e)
+        dst[e] = reinterpret_cast<const uint16_t*>(src)[e];
+  }
+}
+
+template <int WM, int WN, int TM, int TN, int KG, int S>
+int32_t launch(const MxLinear& p, bool silu, hipStream_t stream) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NT = 64 * WM * WN * KG;
+  const int bno = silu ? BN / 2 : BN;
+  // an MXFP8 output's padding is written too
+  const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
+  const int64_t ntm = ((int64_t)p.M + BM - 1) / BM, ntn = (cols + bno - 1) / bno;
+  PA_REQUIRE(ntm * ntn < (1ll << 30), PA_ERR_UNSUPPORTED, "pa_linear_mx: %d x %d outputs", p.M,
+             p.N);
+  const dim3 grid(8 * (uint32_t)((ntm * ntn + 7) / 8));
+  if (silu)
+    mx_gemm_kernel<true, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
+  else
+    mx_gemm_kernel<false, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
+  return check_launch("pa_linear_mx");
+}
+
+}  // namespace
+}  // namespace pa
+
+using namespace pa;
+
+extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x,
+                                const uint8_t* x_scales, const uint8_t* weight,
+                                const uint8_t* weight_scales, const void* bias,
+                                const void* residual, int32_t rows, int32_t out_features,
+                                int32_t in_features, int32_t act, pa_stream_t stream) {
+  clear_error();
+  const bool silu = act == PA_ACT_SILU_MUL;
+  PA_REQUIRE(act == PA_ACT_NONE || silu, PA_ERR_INVALID_ARG, "pa_linear_mx: unknown activation %d",
+             act);
+  PA_REQUIRE(rows >= 0 && out_features > 0 && in_features > 0, PA_ERR_INVALID_ARG,
+             "pa_linear_mx: bad sizes");
+  PA_REQUIRE(!silu || (!bias && !residual), PA_ERR_INVALID_ARG,
+             "pa_linear_mx: bias or residual with the SwiGLU epilogue");
+  PA_REQUIRE(silu || !out_scales, PA_ERR_INVALID_ARG,
+             "pa_linear_mx: an MXFP8 output needs the SwiGLU epilogue");
+  PA_REQUIRE(!silu || out_features % 32 == 0, PA_ERR_UNSUPPORTED,
+             "pa_linear_mx: SwiGLU over %d columns (a multiple of 32)", out_features);
+  // 32-bit lane offsets: 255 rows of codes, and the scales from a gate row to
+  // its up row
+  PA_REQUIRE(in_features <= kMxMaxCols && mx_pad_rows(out_features) / 16 * mx_steps(in_features) *
+                                                  64 < (1ll << 31),
+             PA_ERR_UNSUPPORTED, "pa_linear_mx: a weight of %d x %d", out_features, in_features);
+  if (rows == 0) return PA_OK;
+  PA_REQUIRE(out && x && x_scales && weight && weight_scales, PA_ERR_INVALID_ARG,
+             "pa_linear_mx: null pointer");
+  PA_REQUIRE(((uintptr_t)out | (uintptr_t)x | (uintptr_t)weight) % 16 == 0, PA_ERR_INVALID_ARG,
+             "pa_linear_mx: out, x and weight must be 16-byte aligned");
+  PA_REQUIRE(((uintptr_t)x_scales | (uintptr_t)weight_scales | (uintptr_t)out_scales) % 4 == 0,
+             PA_ERR_INVALID_ARG, "pa_linear_mx: scales must be 4-byte aligned");
+  PA_REQUIRE((uintptr_t)bias % 2 == 0 && (uintptr_t)residual % 16 == 0, PA_ERR_INVALID_ARG,
+             "pa_linear_mx: the residual must be 16-byte aligned, the bias to its elements");
+  const MxLinear p{out,      out_scales,
+                   x,        x_scales,
+                   weight,   weight_scales,
+                   (const uint16_t*)bias, (const uint16_t*)residual,
+                   rows,     out_features,
+                   (int)mx_steps(in_features), mx_pad_rows(rows)};
+  return launch<2, 2, 2, 2, 1, 2>(p, silu, (hipStream_t)stream);
+}

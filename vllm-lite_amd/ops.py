@@ -523,3 +523,165 @@ def linear(x, weight, bias=None, act=ACT_NONE, out=None, rms_eps=None, add_to_ou
                                       workspace.numel() if workspace is not None else 0,
                                       _dtype_code(x), _stream(x)))
     return out
+
+
+# ---- the projections in MXFP8 (pa_dense.h) ---------------------------------
+
+
+def _mx_call(fn, device, *args):
+    """Calls a libpa entry point on the current stream of `device`, with that
+    device current."""
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        _check(fn, getattr(lib, fn)(*args, C.c_void_p(
+            torch.cuda.current_stream(device).cuda_stream)))
+
+
+def _mx_dev(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected a contiguous tensor on {device}")
+
+
+class MxRows:
+    """MXFP8 rows [rows, cols]: codes uint8 [rows, Kp] (Kp = cols rounded up to
+    128), scales uint8 [Kp / 128, R, 4] (R = rows rounded up to 16), see
+    pa_dense.h."""
+
+    def __init__(self, codes, scales, rows, cols):
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        kp = -(-cols // 128) * 128
+        if codes.shape != (rows, kp) or scales.shape != (kp // 128, -(-rows // 16) * 16, 4):
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are "
+                             f"not MXFP8 rows of {rows} x {cols}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda:
+            raise ValueError("MXFP8 rows are uint8 device tensors")
+        _mx_dev(codes.device, codes=codes, scales=scales)
+
+    @classmethod
+    def empty(cls, rows, cols, device="cuda"):
+        if rows < 0 or cols <= 0:
+            raise ValueError(f"MXFP8 rows of {rows} x {cols}")
+        kp = -(-cols // 128) * 128
+        return cls(torch.empty(rows, kp, dtype=torch.uint8, device=device),
+                   torch.empty(kp // 128, -(-rows // 16) * 16, 4, dtype=torch.uint8,
+                               device=device), rows, cols)
+
+
+def _mx_out(out, rows, cols, device):
+    if out is None:
+        return MxRows.empty(rows, cols, device)
+    if (out.rows, out.cols) != (rows, cols) or out.codes.device != device:
+        raise ValueError(f"out holds {out.rows} x {out.cols} on {out.codes.device}, not "
+                         f"{rows} x {cols} on {device}")
+    return out
+
+
+def quantize_mx(x, out=None):
+    """pa_quantize_mx: x [rows, cols] (bf16 or f32, unit stride along a row,
+    rows that do not overlap) -> MxRows."""
+    if not x.is_cuda or x.dim() != 2:
+        raise ValueError("quantize_mx: expected a device tensor [rows, cols]")
+    rows, cols = x.shape
+    if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
+        raise ValueError("quantize_mx: rows must have unit stride and not overlap")
+    code = _dtype_code(x)
+    out = _mx_out(out, rows, cols, x.device)
+    _mx_call("pa_quantize_mx", x.device, _ptr(out.codes), _ptr(out.scales), _ptr(x), rows, cols,
+             x.stride(0) if rows > 1 else cols, code)
+    return out
+
+
+def rms_norm_mx(residual, weight, eps, add=None, residual_out=None, out=None):
+    """pa_rms_norm_mx: residual + add (when given; into residual_out, by
+    default residual itself), then its RMSNorm as MxRows; [rows, hidden]."""
+    if not residual.is_cuda or residual.dim() != 2:
+        raise ValueError("rms_norm_mx: expected a device tensor [rows, hidden]")
+    rows, hidden = residual.shape
+    if weight.shape != (hidden,) or weight.dtype != residual.dtype:
+        raise ValueError("weight must be [hidden] in the residual dtype")
+    for name, t in (("add", add), ("residual_out", residual_out)):
+        if t is not None and (t.shape != residual.shape or t.dtype != residual.dtype):
+            raise ValueError(f"{name} must match residual")
+    if add is None and residual_out is not None:
+        raise ValueError("residual_out holds the sum with add")
+    if add is not None and residual_out is None:
+        residual_out = residual
+    _mx_dev(residual.device, residual=residual, weight=weight, add=add,
+            residual_out=residual_out)
+    code = _dtype_code(residual)
+    out = _mx_out(out, rows, hidden, residual.device)
+    _mx_call("pa_rms_norm_mx", residual.device, _ptr(out.codes), _ptr(out.scales),
+             _ptr(residual_out), _ptr(residual), _ptr(add), _ptr(weight), rows, hidden,
+             float(eps), code)
+    return out
+
+
+class MxWeight:
+    """A weight [N, K] (bf16 or f32, contiguous) quantised to MXFP8 in the
+    layout that linear_mx reads (pa_linear_mx_pack)."""
+
+    def __init__(self, weight):
+        if not weight.is_cuda or weight.dim() != 2 or not weight.is_contiguous():
+            raise ValueError("MxWeight: expected a contiguous device tensor [N, K]")
+        lib = _lib.load()
+        n, k = self.shape = tuple(weight.shape)
+        code = _dtype_code(weight)
+        self.codes = torch.empty(lib.pa_mx_weight_bytes(n, k), dtype=torch.uint8,
+                                 device=weight.device)
+        self.scales = torch.empty(lib.pa_mx_scale_bytes(n, k), dtype=torch.uint8,
+                                  device=weight.device)
+        _mx_call("pa_linear_mx_pack", weight.device, _ptr(self.codes), _ptr(self.scales),
+                 _ptr(weight), n, k, code)
+
+    @classmethod
+    def from_packed(cls, codes, scales, rows, cols):
+        """A weight [rows, cols] whose packed codes and scales (flat uint8)
+        are at hand, e.g. from a checkpoint."""
+        lib = _lib.load()
+        self = cls.__new__(cls)
+        self.shape, self.codes, self.scales = (rows, cols), codes, scales
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda or \
+                codes.shape != (lib.pa_mx_weight_bytes(rows, cols),) or \
+                scales.shape != (lib.pa_mx_scale_bytes(rows, cols),):
+            raise ValueError(f"not the packed MXFP8 codes and scales of {rows} x {cols}")
+        _mx_dev(codes.device, codes=codes, scales=scales)
+        return self
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_out=False):
+    """pa_linear_mx: x MxRows [rows, K], weight MxWeight [N, K] (or the fused
+    gate|up [2 N, K] with act=ACT_SILU_MUL) -> [rows, N] bf16, with bias [N]
+    and residual [rows, N] (bf16; out may be the residual itself) added before
+    the one rounding; mx_out (with ACT_SILU_MUL): -> MxRows."""
+    if not isinstance(x, MxRows) or not isinstance(weight, MxWeight):
+        raise ValueError("linear_mx takes MxRows and an MxWeight")
+    silu = act == ACT_SILU_MUL
+    device, rows = x.codes.device, x.rows
+    n = weight.shape[0] // 2 if silu else weight.shape[0]
+    if weight.shape[1] != x.cols or (silu and weight.shape[0] % 2):
+        raise ValueError(f"weight {weight.shape} does not match x {x.rows} x {x.cols}")
+    if mx_out and not silu:
+        raise ValueError("an MXFP8 output needs the SwiGLU epilogue")
+    if weight.codes.device != device:
+        raise ValueError(f"weight on {weight.codes.device}, x on {device}")
+    for name, t, shape in (("bias", bias, (n,)), ("residual", residual, (rows, n))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.bfloat16):
+            raise ValueError(f"{name} must be bf16 {shape}")
+    if mx_out:
+        out = _mx_out(out, rows, n, device)
+        data, scales = out.codes, out.scales
+    else:
+        if out is None:
+            out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+        elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16:
+            raise ValueError(f"out must be bf16 {(rows, n)}")
+        data, scales = out, None
+    _mx_dev(device, bias=bias, residual=residual, out=data)
+    _mx_call("pa_linear_mx", device, _ptr(data), _ptr(scales), _ptr(x.codes), _ptr(x.scales),
+             _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(residual), rows, n,
+             x.cols, act)
+    return out

@@ -6,6 +6,7 @@
 
 #include "lds_copy.hpp"
 #include "mx_common.hpp"
+#include "mx_tiling.hpp"
 #include "pa_common.hpp"
 #include "pa_internal.hpp"
 #include "../../include/pa_dense.h"
@@ -126,20 +127,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     sl[u] = SX + c * 256;
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
-  auto issue = [&](int stage, int buf) __attribute__((always_inline)) {
-    // a group without a step in the last stage copies the last step again
+  // copy u of a stage's PER; a group without a step in the last stage copies
+  // the last step again
+  auto copy = [&](int stage, int buf, int u) __attribute__((always_inline)) {
     const int kt = min(stage * KG + kg, nk - 1);
     const uint32_t l0 = lds0 + buf * STAGE + kg * STEP;
-    const uint32_t la = __builtin_amdgcn_readfirstlane(l0 + CA * wt * 1024);
-    const uint32_t lb = __builtin_amdgcn_readfirstlane(l0 + BM * 128 + CB * wt * 1024);
-#pragma unroll
-    for (int u = 0; u < CA; ++u) lds_copy16(xb + (int64_t)kt * 128, xo[u], la + u * 1024);
-#pragma unroll
-    for (int u = 0; u < CB; ++u)
-      lds_copy16(wb[u] + (int64_t)kt * 2048, (uint32_t)lane * 16, lb + u * 1024);
-#pragma unroll
-    for (int u = 0; u < CS; ++u)
-      lds_copy4(sb[u] + kt * sstep[u], so[u], __builtin_amdgcn_readfirstlane(l0 + sl[u]));
+    if (u < CA)
+      lds_copy16(xb + (int64_t)kt * 128, xo[u],
+                 __builtin_amdgcn_readfirstlane(l0 + (CA * wt + u) * 1024));
+    else if (u < CA + CB)
+      lds_copy16(wb[u - CA] + (int64_t)kt * 2048, (uint32_t)lane * 16,
+                 __builtin_amdgcn_readfirstlane(l0 + BM * 128 + (CB * wt + u - CA) * 1024));
+    else
+      lds_copy4(sb[u - CA - CB] + kt * sstep[u - CA - CB], so[u - CA - CB],
+                __builtin_amdgcn_readfirstlane(l0 + sl[u - CA - CB]));
   };
   // tile rows of this lane's operands (SILU: gate tiles, then their up tiles)
   int arow[TM], brow[TN];
@@ -157,65 +158,113 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     for (int b = 0; b < TN; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
-  auto two16 = [](const uint8_t* lo, const uint8_t* hi) __attribute__((always_inline)) {
-    return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(lo),
-                                   *reinterpret_cast<const i32x4*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
+  // The operands of half a step (64 columns), read while the half before is
+  // multiplied, in 2 (TM + TN) reads.
+  struct Half {
+    i32x4 a[TM][2], b[TN][2];
+  };
+  constexpr int READS = 2 * (TM + TN), PRODUCTS = TM * TN;
+  auto read = [&](int buf, int h, int u, Half& o) __attribute__((always_inline)) {
+    const uint8_t* at = lds + buf * STAGE + kg * STEP;
+    const int c = 4 * h + 2 * (u % 2) + g, t = u / 2;
+    if (t < TN)
+      o.b[t][u % 2] = *reinterpret_cast<const i32x4*>(at + BM * 128 + brow[t] / 16 * 2048 +
+                                                      brow[t] % 16 * 16 + c * 256);
+    else
+      o.a[t - TN][u % 2] = *reinterpret_cast<const i32x4*>(
+          at + arow[t - TN] * 128 + (c ^ swz(arow[t - TN])) * 16);
+  };
+  // This lane's scale bytes: of the first 64 columns in bits 0-7, of the
+  // second in 16-23.
+  struct Scales {
+    int a[TM], b[TN];
+  };
+  auto read_scales = [&](int st, int buf, Scales& o) __attribute__((always_inline)) {
+    const uint8_t* at = lds + buf * STAGE + kg * STEP;
+    // a group without a step in the last stage multiplies by 2^-127 twice,
+    // which leaves nothing in f32
+    const int keep = KG == 1 || st * KG + kg < nk ? -1 : 0;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+      o.b[t] = (*reinterpret_cast<const int*>(at + SW + brow[t] * 4) >> (8 * g)) & keep;
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+      o.a[t] = (*reinterpret_cast<const int*>(at + SX + arow[t] * 4) >> (8 * g)) & keep;
+  };
+  // Half h's products, with the next half's reads and a stage's copies
+  // between them: nothing else of this wavefront would run meanwhile, and
+  // a block of reads in front would leave the matrix core waiting.
+  auto half = [&](auto hc, const Half& o, const Scales& s, auto&& beside)
+                  __attribute__((always_inline)) {
+    constexpr int h = decltype(hc)::value;
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+      const int a = i / TN, b = i % TN;
+      acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          __builtin_shufflevector(o.b[b][0], o.b[b][1], 0, 1, 2, 3, 4, 5, 6, 7),
+          __builtin_shufflevector(o.a[a][0], o.a[a][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[a][b], 0, 0,
+          2 * h, s.b[b], 2 * h, s.a[a]);
+      beside(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   const int ns = (nk + KG - 1) / KG;
 #pragma unroll
-  for (int t = 0; t < S - 1; ++t)
-    if (t < ns) issue(t, t);
-  for (int st = 0, buf = 0, ibuf = S - 1; st < ns; ++st) {
-    // this wavefront's copies of the stage have landed (near the end fewer
-    // stages are in flight and all are waited for) ...
-    if (ns - st > S - 2)
-      wait_copies<(S - 2) * PER>();
-    else
-      wait_copies<0>();
-    // ... and after the barrier everyone's, and everyone is done with the
-    // stage before, whose buffer the next copies fill
+  for (int t = 0; t < S; ++t)
+    if (t < ns)
+#pragma unroll
+      for (int u = 0; u < PER; ++u) copy(t, t, u);
+  Half h0, h1;
+  Scales sc, sn;
+  int buf = 0;
+  // piece i of PRODUCTS of n things, the first `early` products taking them
+  auto share = [](int i, int n, int early, auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = min(i, early) * n / early; u < min(i + 1, early) * n / early; ++u) f(u);
+  };
+  constexpr int EARLY = PRODUCTS > 4 ? PRODUCTS / 2 : PRODUCTS;
+  // Stage st and the step to the one after it.  Between the halves this
+  // wavefront's copies of the next stage have landed (in_flight: those of the
+  // stages behind it), and after the barrier everyone's, and everyone has read
+  // all of this stage, whose buffer takes the stage S further on.  No
+  // branches: the compiler would move the products behind them.
+  auto step = [&](int st, auto in_flight, auto copies) __attribute__((always_inline)) {
+    half(std::integral_constant<int, 0>{}, h0, sc, [&](int i) __attribute__((always_inline)) {
+      share(i, READS, EARLY, [&](int u) __attribute__((always_inline)) { read(buf, 1, u, h1); });
+    });
+    wait_copies<decltype(in_flight)::value>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (st + S - 1 < ns) issue(st + S - 1, ibuf);
-    if (KG == 1 || st * KG + kg < nk) {
-      const uint8_t* at = lds + buf * STAGE + kg * STEP;
-      const uint8_t* bt = at + BM * 128;
-      // this lane's byte of the first 64 columns in bits 0-7, of the second in 16-23
-      int sa[TM], sw[TN];
+    const int nb = buf == S - 1 ? 0 : buf + 1;
+    read_scales(st + 1, nb, sn);
+    half(std::integral_constant<int, 1>{}, h1, sc, [&](int i) __attribute__((always_inline)) {
+      share(i, READS, EARLY, [&](int u) __attribute__((always_inline)) { read(nb, 0, u, h0); });
+      if constexpr (decltype(copies)::value)
+        share(i, PER, PRODUCTS,
+              [&](int u) __attribute__((always_inline)) { copy(st + S, buf, u); });
+    });
+    buf = nb;
+    sc = sn;
+  };
+  if (ns >= S)
+    wait_copies<(S - 1) * PER>();
+  else
+    wait_copies<0>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read_scales(0, 0, sc);
 #pragma unroll
-      for (int t = 0; t < TM; ++t)
-        sa[t] = *reinterpret_cast<const uint32_t*>(at + SX + arow[t] * 4) >> (8 * g);
-#pragma unroll
-      for (int t = 0; t < TN; ++t)
-        sw[t] = *reinterpret_cast<const uint32_t*>(at + SW + brow[t] * 4) >> (8 * g);
-      auto half = [&](auto hc) __attribute__((always_inline)) {
-        constexpr int h = decltype(hc)::value;
-        i32x8 af[TM], bf[TN];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-          const uint8_t* row = at + arow[t] * 128;
-          af[t] = two16(row + ((4 * h + g) ^ swz(arow[t])) * 16,
-                        row + ((4 * h + 2 + g) ^ swz(arow[t])) * 16);
-        }
-#pragma unroll
-        for (int t = 0; t < TN; ++t) {
-          const uint8_t* f = bt + brow[t] / 16 * 2048 + brow[t] % 16 * 16;
-          bf[t] = two16(f + (4 * h + g) * 256, f + (4 * h + 2 + g) * 256);
-        }
-#pragma unroll
-        for (int a = 0; a < TM; ++a)
-#pragma unroll
-          for (int b = 0; b < TN; ++b)
-            acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                bf[b], af[a], acc[a][b], 0, 0, 2 * h, sw[b], 2 * h, sa[a]);
-      };
-      half(std::integral_constant<int, 0>{});
-      half(std::integral_constant<int, 1>{});
-    }
-    buf = buf == S - 1 ? 0 : buf + 1;
-    ibuf = ibuf == S - 1 ? 0 : ibuf + 1;
-  }
+  for (int u = 0; u < READS; ++u) read(0, 0, u, h0);
+  int st = 0;
+  for (; st < ns - S; ++st)
+    step(st, std::integral_constant<int, (S - 2) * PER>{}, std::true_type{});
+  for (; st < ns - 1; ++st) step(st, std::integral_constant<int, 0>{}, std::false_type{});
+  half(std::integral_constant<int, 0>{}, h0, sc, [&](int i) __attribute__((always_inline)) {
+    share(i, READS, EARLY, [&](int u) __attribute__((always_inline)) { read(buf, 1, u, h1); });
+  });
+  half(std::integral_constant<int, 1>{}, h1, sc, [](int) {});
   __syncthreads();
   // the K groups' sums, in group order
   if constexpr (KG > 1) {
@@ -432,5 +481,12 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
                    (const uint16_t*)bias, (const uint16_t*)residual,
                    rows,     out_features,
                    (int)mx_steps(in_features), mx_pad_rows(rows)};
-  return launch<2, 2, 2, 2, 1, 2>(p, silu, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  switch (choose_mx_tiling(rows, silu ? 2 * out_features : out_features, in_features)) {
+    case kMx256x256: return launch<2, 2, 4, 4, 1, 2>(p, silu, s);
+    case kMx256x128: return launch<4, 2, 2, 2, 1, 3>(p, silu, s);
+    case kMx128x128Pair: return launch<2, 2, 2, 2, 1, 2>(p, silu, s);
+    case kMx128x128: return launch<2, 2, 2, 2, 1, 4>(p, silu, s);
+    default: return launch<2, 1, 1, 2, 2, 4>(p, silu, s);
+  }
 }

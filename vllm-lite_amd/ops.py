@@ -530,23 +530,35 @@ def linear(x, weight, bias=None, act=ACT_NONE, out=None, rms_eps=None, add_to_ou
 
 def _mx_call(fn, device, *args):
     """Calls a libpa entry point on the current stream of `device`, with that
-    device current."""
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        _check(fn, getattr(lib, fn)(*args, C.c_void_p(
-            torch.cuda.current_stream(device).cuda_stream)))
+    device current.  Pointers as plain integers, and the raw stream: a decode
+    step's calls are a few microseconds each, of which the objects in between
+    would be most (quantize_mx of 32 rows: 12.7 us with them)."""
+    index = device.index
+    call = getattr(_lib.load(), fn)
+    if torch.cuda.current_device() == index:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _check(fn, rc)
 
 
-def _mx_dev(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{name}: expected a contiguous tensor on {device}")
+def _mx_dev(device, name, t):
+    if t is not None and (t.device != device or not t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous tensor on {device}")
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 class MxRows:
     """MXFP8 rows [rows, cols]: codes uint8 [rows, Kp] (Kp = cols rounded up to
     128), scales uint8 [Kp / 128, R, 4] (R = rows rounded up to 16), see
     pa_dense.h."""
+
+    __slots__ = ("codes", "scales", "rows", "cols")
 
     def __init__(self, codes, scales, rows, cols):
         self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
@@ -556,16 +568,21 @@ class MxRows:
                              f"not MXFP8 rows of {rows} x {cols}")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda:
             raise ValueError("MXFP8 rows are uint8 device tensors")
-        _mx_dev(codes.device, codes=codes, scales=scales)
+        _mx_dev(codes.device, "codes", codes)
+        _mx_dev(codes.device, "scales", scales)
 
     @classmethod
     def empty(cls, rows, cols, device="cuda"):
+        """Rows whose arrays are allocated and not filled."""
         if rows < 0 or cols <= 0:
             raise ValueError(f"MXFP8 rows of {rows} x {cols}")
+        self = cls.__new__(cls)
         kp = -(-cols // 128) * 128
-        return cls(torch.empty(rows, kp, dtype=torch.uint8, device=device),
-                   torch.empty(kp // 128, -(-rows // 16) * 16, 4, dtype=torch.uint8,
-                               device=device), rows, cols)
+        self.codes = torch.empty((rows, kp), dtype=torch.uint8, device=device)
+        self.scales = torch.empty((kp // 128, -(-rows // 16) * 16, 4), dtype=torch.uint8,
+                                  device=device)
+        self.rows, self.cols = rows, cols
+        return self
 
 
 def _mx_out(out, rows, cols, device):
@@ -587,8 +604,8 @@ def quantize_mx(x, out=None):
         raise ValueError("quantize_mx: rows must have unit stride and not overlap")
     code = _dtype_code(x)
     out = _mx_out(out, rows, cols, x.device)
-    _mx_call("pa_quantize_mx", x.device, _ptr(out.codes), _ptr(out.scales), _ptr(x), rows, cols,
-             x.stride(0) if rows > 1 else cols, code)
+    _mx_call("pa_quantize_mx", x.device, out.codes.data_ptr(), out.scales.data_ptr(),
+             x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, code)
     return out
 
 
@@ -607,12 +624,15 @@ def rms_norm_mx(residual, weight, eps, add=None, residual_out=None, out=None):
         raise ValueError("residual_out holds the sum with add")
     if add is not None and residual_out is None:
         residual_out = residual
-    _mx_dev(residual.device, residual=residual, weight=weight, add=add,
-            residual_out=residual_out)
+    device = residual.device
+    _mx_dev(device, "residual", residual)
+    _mx_dev(device, "weight", weight)
+    _mx_dev(device, "add", add)
+    _mx_dev(device, "residual_out", residual_out)
     code = _dtype_code(residual)
-    out = _mx_out(out, rows, hidden, residual.device)
-    _mx_call("pa_rms_norm_mx", residual.device, _ptr(out.codes), _ptr(out.scales),
-             _ptr(residual_out), _ptr(residual), _ptr(add), _ptr(weight), rows, hidden,
+    out = _mx_out(out, rows, hidden, device)
+    _mx_call("pa_rms_norm_mx", device, out.codes.data_ptr(), out.scales.data_ptr(),
+             _at(residual_out), residual.data_ptr(), _at(add), weight.data_ptr(), rows, hidden,
              float(eps), code)
     return out
 
@@ -631,8 +651,8 @@ class MxWeight:
                                  device=weight.device)
         self.scales = torch.empty(lib.pa_mx_scale_bytes(n, k), dtype=torch.uint8,
                                   device=weight.device)
-        _mx_call("pa_linear_mx_pack", weight.device, _ptr(self.codes), _ptr(self.scales),
-                 _ptr(weight), n, k, code)
+        _mx_call("pa_linear_mx_pack", weight.device, self.codes.data_ptr(),
+                 self.scales.data_ptr(), weight.data_ptr(), n, k, code)
 
     @classmethod
     def from_packed(cls, codes, scales, rows, cols):
@@ -645,7 +665,8 @@ class MxWeight:
                 codes.shape != (lib.pa_mx_weight_bytes(rows, cols),) or \
                 scales.shape != (lib.pa_mx_scale_bytes(rows, cols),):
             raise ValueError(f"not the packed MXFP8 codes and scales of {rows} x {cols}")
-        _mx_dev(codes.device, codes=codes, scales=scales)
+        _mx_dev(codes.device, "codes", codes)
+        _mx_dev(codes.device, "scales", scales)
         return self
 
     def nbytes(self):
@@ -668,20 +689,24 @@ def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_ou
         raise ValueError("an MXFP8 output needs the SwiGLU epilogue")
     if weight.codes.device != device:
         raise ValueError(f"weight on {weight.codes.device}, x on {device}")
-    for name, t, shape in (("bias", bias, (n,)), ("residual", residual, (rows, n))):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.bfloat16):
-            raise ValueError(f"{name} must be bf16 {shape}")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != torch.bfloat16):
+        raise ValueError(f"bias must be bf16 {(n,)}")
+    if residual is not None and (residual.shape != (rows, n) or
+                                 residual.dtype != torch.bfloat16):
+        raise ValueError(f"residual must be bf16 {(rows, n)}")
     if mx_out:
         out = _mx_out(out, rows, n, device)
         data, scales = out.codes, out.scales
     else:
         if out is None:
-            out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
-        elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16:
+            out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
+        elif out.shape != (rows, n) or out.dtype != torch.bfloat16:
             raise ValueError(f"out must be bf16 {(rows, n)}")
         data, scales = out, None
-    _mx_dev(device, bias=bias, residual=residual, out=data)
-    _mx_call("pa_linear_mx", device, _ptr(data), _ptr(scales), _ptr(x.codes), _ptr(x.scales),
-             _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(residual), rows, n,
-             x.cols, act)
+    _mx_dev(device, "bias", bias)
+    _mx_dev(device, "residual", residual)
+    _mx_dev(device, "out", data)
+    _mx_call("pa_linear_mx", device, data.data_ptr(), _at(scales), x.codes.data_ptr(),
+             x.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), _at(bias),
+             _at(residual), rows, n, x.cols, act)
     return out

@@ -31,7 +31,7 @@ def same_as_definition(mx, y):
     assert torch.equal(torch.nan_to_num(got, 1e9), torch.nan_to_num(v, 1e9))
 
 
-SIZES = [(1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129), (5, 896), (64, 1000),
+SIZES = [(2500, 130), (2048, 2300), (1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129), (5, 896), (64, 1000),
          (33, 2048), (7, 2049), (4, 4096), (3, 8200), (2, 12289), (1000, 40), (4099, 96)]
 
 
@@ -120,7 +120,7 @@ def norm_reference(x, add, w):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("with_add", [False, True])
-@pytest.mark.parametrize("rows,cols", SIZES + [(2, 20000)])
+@pytest.mark.parametrize("rows,cols", SIZES + [(2, 16000), (2, 20000), (2100, 200), (2065, 4097)])
 def test_rms_norm(pa, rows, cols, dtype, with_add):
     g = gen(rows, cols, with_add)
     x = hidden_states(g, rows, cols, dtype)

@@ -1,6 +1,7 @@
 // MXFP8 rows and weights (pa_dense.h): quantising rows, RMSNorm with an MXFP8
 // output, and the weights' layout.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx_common.hpp"
 #include "pa_common.hpp"
@@ -23,32 +24,22 @@ struct Vec8<float> {
 
 // Columns 8 ch .. 8 ch + 7 of a row, 0 behind the last.
 template <typename T>
-__device__ inline void load8(const T* row, int64_t ch, int cols, float (&y)[8]) {
-  if (8 * ch + 8 <= cols) {
-    const auto v = *reinterpret_cast<const typename Vec8<T>::V*>(row + 8 * ch);
+__device__ inline typename Vec8<T>::V load8(const T* row, int64_t ch, int cols) {
+  if (8 * ch + 8 <= cols) return *reinterpret_cast<const typename Vec8<T>::V*>(row + 8 * ch);
+  typename Vec8<T>::V v = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (float)v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = 8 * ch + e < cols ? Elem<T>::load(row + 8 * ch + e) : 0.f;
-  }
+  for (int e = 0; e < 8; ++e)
+    if (8 * ch + e < cols) v[e] = Elem<T>::load(row + 8 * ch + e);
+  return v;
 }
 template <typename T>
-__device__ inline void store8(T* row, int64_t ch, int cols, const float (&y)[8]) {
+__device__ inline void store8(T* row, int64_t ch, int cols, const typename Vec8<T>::V& v) {
   if (8 * ch + 8 <= cols) {
-    typename Vec8<T>::V v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (sizeof(T) == 2)
-        v[e] = (__bf16)y[e];
-      else
-        v[e] = y[e];
-    }
     *reinterpret_cast<typename Vec8<T>::V*>(row + 8 * ch) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (8 * ch + e < cols) Elem<T>::store(row + 8 * ch + e, y[e]);
+      if (8 * ch + e < cols) Elem<T>::store(row + 8 * ch + e, v[e]);
   }
 }
 
@@ -75,21 +66,55 @@ struct WeightLayout {
   }
 };
 
-// Eight columns per thread, 16 threads per (row, step of 128 columns).  Rows
-// `rows` .. `out_rows` are written as zeros (the padding of a weight).
+// The first of a workgroup's R rows (R a power of two up to 32).  near:
+// workgroups are dealt round-robin to the 8 XCDs; the rows of a group of 32,
+// whose scales share cache lines, then go to one XCD, so that its L2 puts the
+// lines together.
+__device__ inline int64_t first_row(int64_t block, int R, int near) {
+  if (!near) return block * R;
+  const int64_t i = block / 8;
+  const int per = 32 / R;
+  return (i / per * 8 + block % 8) * 32 + i % per * R;
+}
+constexpr int64_t kNearRows = 2048;
+inline int64_t row_groups(int64_t rows, int R) {
+  return rows >= kNearRows ? (rows + 255) / 256 * (256 / R) : (rows + R - 1) / R;
+}
+
+// Eight columns per thread, 16 threads per (row, step of 128 columns), a
+// workgroup 2^lg steps of 16 / 2^lg rows at a time, and `times` of these one
+// after another.  Rows `rows` .. `out_rows` are written as zeros (the padding
+// of a weight).
 template <typename T, typename Layout>
 __global__ __launch_bounds__(256) void quantize_mx_kernel(Layout out, const T* __restrict__ x,
                                                           int64_t rows, int64_t out_rows, int cols,
-                                                          int64_t stride) {
-  const int64_t unit = blockIdx.x * (int64_t)16 + threadIdx.x / 16;
-  const int64_t row = unit / out.steps, s = unit % out.steps;
-  if (row >= out_rows) return;  // 16 lanes together
-  const int64_t ch = 16 * s + threadIdx.x % 16;
-  float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (row < rows) load8(x + row * stride, ch, cols, y);
-  uint32_t dword;
-  *out.code(row, ch) = mx_quantize8(y, dword);
-  if (threadIdx.x % 16 == 0) *out.scale(row, s) = dword;
+                                                          int64_t stride, int lg, int times,
+                                                          int near) {
+  typedef typename Vec8<T>::V V;
+  const int unit = threadIdx.x / 16;
+  const int64_t row = first_row(blockIdx.x, 16 >> lg, near) + (unit >> lg);
+  int s = ((int)blockIdx.y * times << lg) + (unit & ((1 << lg) - 1));
+  const int end = min((int)out.steps, ((int)blockIdx.y + 1) * times << lg);
+  if (row >= out_rows || s >= end) return;  // 16 lanes together
+  auto load = [&](int st) __attribute__((always_inline)) {
+    V v = 0;
+    if (row < rows) v = load8(x + row * stride, 16 * st + threadIdx.x % 16, cols);
+    return v;
+  };
+  V v = load(s);
+  for (;;) {
+    const int next = s + (1 << lg);
+    const V v1 = next < end ? load(next) : v;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (float)v[e];
+    uint32_t dword;
+    *out.code(row, 16 * s + threadIdx.x % 16) = mx_quantize8(y, dword);
+    if (threadIdx.x % 16 == 0) *out.scale(row, s) = dword;
+    if (next >= end) break;
+    s = next;
+    v = v1;
+  }
 }
 
 template <int G>
@@ -105,100 +130,106 @@ __device__ inline float row_sum(float v, float* red) {
 }
 
 // G lanes per row (64: a wavefront, 256: the workgroup), chunk i of lane l is
-// columns 8 (l + G i) ..; kHeld: the row fits kNormHeld chunks a lane and stays
-// in registers, else it is read again for the second pass.
-constexpr int kNormHeld = 4;
-template <typename T, int G, bool kHeld>
+// columns 8 (l + G i) ..  C > 0: the row fits C chunks a lane and stays in
+// registers; C = 0: it is read again for the second pass.
+template <typename T, int G, int C>
 __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum, const T* residual,
                                                           const T* __restrict__ add,
                                                           const T* __restrict__ w, int64_t rows,
-                                                          int hidden, float eps) {
+                                                          int hidden, float eps, int near) {
+  typedef typename Vec8<T>::V V;
+  using E = std::conditional_t<sizeof(T) == 2, __bf16, float>;
   __shared__ float red[4];
   const int lane = threadIdx.x % G;
-  const int64_t row = blockIdx.x * (int64_t)(256 / G) + threadIdx.x / G;
-  if (row >= rows) return;  // a whole wavefront, or at G = 256 never
+  const int64_t row = first_row(blockIdx.x, 256 / G, near) + threadIdx.x / G;
+  if (row >= rows) return;  // a whole wavefront, or at G = 256 the workgroup
   const int nch = (int)out.steps * 16;
   const T* x = residual + row * hidden;
   const T* a = add ? add + row * hidden : nullptr;
   T* o = add ? sum + row * hidden : nullptr;
   float ss = 0.f;
   // the row's value: with add the sum, kept in the storage dtype and stored
-  auto take = [&](int ch, float (&v)[8], const float (&av)[8]) __attribute__((always_inline)) {
+  auto take = [&](int ch, V& v, const V& av) __attribute__((always_inline)) {
     if (a) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] += av[e];
-        if constexpr (sizeof(T) == 2) v[e] = (float)(__bf16)v[e];
-      }
+      for (int e = 0; e < 8; ++e) v[e] = (E)((float)v[e] + (float)av[e]);
       store8(o, ch, hidden, v);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+    for (int e = 0; e < 8; ++e) ss += (float)v[e] * (float)v[e];
   };
-  auto write = [&](int ch, float (&v)[8], float inv) __attribute__((always_inline)) {
-    float wv[8];
-    load8(w, ch, hidden, wv);
+  auto write = [&](int ch, const V& v, const V& wv, float inv) __attribute__((always_inline)) {
     // the product with the weight first: exact for bf16
+    float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * wv[e] * inv;
+    for (int e = 0; e < 8; ++e) y[e] = (float)v[e] * (float)wv[e] * inv;
     uint32_t dword;
-    *out.code(row, ch) = mx_quantize8(v, dword);
+    *out.code(row, ch) = mx_quantize8(y, dword);
     if (threadIdx.x % 16 == 0) *out.scale(row, ch / 16) = dword;
   };
-  if constexpr (kHeld) {
+  if constexpr (C > 0) {
     // all loads first: sum may be residual itself, so none moves over a store
-    float v[kNormHeld][8], av[kNormHeld][8];
+    V v[C], av[C], wv[C];
 #pragma unroll
-    for (int i = 0; i < kNormHeld; ++i)
+    for (int i = 0; i < C; ++i)
       if (lane + G * i < nch) {
-        load8(x, lane + G * i, hidden, v[i]);
-        if (a) load8(a, lane + G * i, hidden, av[i]);
+        v[i] = load8(x, lane + G * i, hidden);
+        if (a) av[i] = load8(a, lane + G * i, hidden);
+        wv[i] = load8(w, lane + G * i, hidden);
       }
 #pragma unroll
-    for (int i = 0; i < kNormHeld; ++i)
+    for (int i = 0; i < C; ++i)
       if (lane + G * i < nch) take(lane + G * i, v[i], av[i]);
     const float inv = 1.0f / sqrtf(row_sum<G>(ss, red) / (float)hidden + eps);
 #pragma unroll
-    for (int i = 0; i < kNormHeld; ++i)
-      if (lane + G * i < nch) write(lane + G * i, v[i], inv);
+    for (int i = 0; i < C; ++i)
+      if (lane + G * i < nch) write(lane + G * i, v[i], wv[i], inv);
   } else {
-    float v[8], av[8];
     for (int ch = lane; ch < nch; ch += G) {
-      load8(x, ch, hidden, v);
-      if (a) load8(a, ch, hidden, av);
+      V v = load8(x, ch, hidden), av;
+      if (a) av = load8(a, ch, hidden);
       take(ch, v, av);
     }
     const float inv = 1.0f / sqrtf(row_sum<G>(ss, red) / (float)hidden + eps);
-    for (int ch = lane; ch < nch; ch += G) {
-      load8<T>(a ? o : x, ch, hidden, v);
-      write(ch, v, inv);
-    }
+    for (int ch = lane; ch < nch; ch += G)
+      write(ch, load8<T>(a ? o : x, ch, hidden), load8(w, ch, hidden), inv);
   }
 }
 
 template <typename T, typename Layout>
 int32_t launch_quantize(const char* what, const Layout& out, const void* x, int64_t rows,
                         int64_t out_rows, int cols, int64_t stride, hipStream_t s) {
-  const int64_t groups = (out_rows * out.steps + 15) / 16;
-  PA_REQUIRE(groups < (1ll << 31), PA_ERR_UNSUPPORTED, "%s: %lld x %d is too large", what,
-             (long long)rows, cols);
-  quantize_mx_kernel<T, Layout><<<(uint32_t)groups, 256, 0, s>>>(out, (const T*)x, rows, out_rows,
-                                                                 cols, stride);
+  int lg = 0;  // as many steps side by side as there are, up to 16
+  while (lg < 4 && 1 << lg < out.steps) ++lg;
+  const int64_t groups = row_groups(out_rows, 16 >> lg);
+  // many rows: whole rows to a workgroup (7569 x 4096: 20 us, 22 with the steps
+  // over workgroups); few: the steps too
+  const int across = (int)((out.steps + (1 << lg) - 1) >> lg);
+  const int times = out_rows >= kNearRows ? across : 1;
+  quantize_mx_kernel<T, Layout>
+      <<<dim3((uint32_t)groups, (uint32_t)((across + times - 1) / times)), 256, 0, s>>>(
+          out, (const T*)x, rows, out_rows, cols, stride, lg, times, out_rows >= kNearRows);
   return check_launch(what);
 }
 
-template <typename T>
+template <typename T, int G, int C>
 int32_t launch_norm(const RowLayout& out, void* sum, const void* residual, const void* add,
-                    const void* w, int rows, int hidden, float eps, hipStream_t s) {
-  auto run = [&](auto kernel, int per) {
-    kernel<<<(rows + per - 1) / per, 256, 0, s>>>(out, (T*)sum, (const T*)residual, (const T*)add,
-                                                  (const T*)w, rows, hidden, eps);
-    return check_launch("pa_rms_norm_mx");
-  };
-  const int64_t nch = out.steps * 16;
-  if (nch <= 64 * kNormHeld) return run(rms_norm_mx_kernel<T, 64, true>, 4);
-  if (nch <= 256 * kNormHeld) return run(rms_norm_mx_kernel<T, 256, true>, 1);
-  return run(rms_norm_mx_kernel<T, 256, false>, 1);
+                    const void* w, int64_t rows, int hidden, float eps, hipStream_t s) {
+  rms_norm_mx_kernel<T, G, C><<<(uint32_t)row_groups(rows, 256 / G), 256, 0, s>>>(
+      out, (T*)sum, (const T*)residual, (const T*)add, (const T*)w, rows, hidden, eps,
+      rows >= kNearRows);
+  return check_launch("pa_rms_norm_mx");
+}
+template <typename T, typename... Args>
+int32_t launch_norm(const RowLayout& out, const Args&... args) {
+  const int64_t nch = out.steps * 16;  // chunks of 8 columns
+  if (nch <= 64) return launch_norm<T, 64, 1>(out, args...);
+  if (nch <= 128) return launch_norm<T, 64, 2>(out, args...);
+  if (nch <= 256) return launch_norm<T, 256, 1>(out, args...);
+  if (nch <= 512) return launch_norm<T, 256, 2>(out, args...);
+  if (nch <= 1024) return launch_norm<T, 256, 4>(out, args...);
+  if (nch <= 2048) return launch_norm<T, 256, 8>(out, args...);
+  return launch_norm<T, 256, 0>(out, args...);
 }
 
 }  // namespace
@@ -276,6 +307,8 @@ extern "C" int32_t pa_rms_norm_mx(uint8_t* codes, uint8_t* scales, void* sum,
                      dtype_size(dtype) == 0,
              PA_ERR_INVALID_ARG, "pa_rms_norm_mx: rows are not aligned to their elements");
   const RowLayout out{codes, scales, mx_steps(hidden), mx_pad_rows(rows)};
-  return (dtype == PA_DTYPE_BF16 ? launch_norm<uint16_t> : launch_norm<float>)(
-      out, sum, residual, add, weight, rows, hidden, eps, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PA_DTYPE_BF16)
+    return launch_norm<uint16_t>(out, sum, residual, add, weight, (int64_t)rows, hidden, eps, s);
+  return launch_norm<float>(out, sum, residual, add, weight, (int64_t)rows, hidden, eps, s);
 }

@@ -20,10 +20,24 @@ __device__ inline uint32_t dpp(uint32_t v) {
 }
 constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
 
-// |y| as bits, 0 for NaN and infinities: finite magnitudes order as integers.
-__device__ inline uint32_t mx_magnitude(float y) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, y) & 0x7FFFFFFFu;
-  return u < 0x7F800000u ? u : 0u;
+// The largest finite magnitude of N values, as the bits of a float (0 if none
+// is finite).  A maximum of floats finds it wherever all are finite; a NaN or
+// an infinity among them shows in the maximum, or (a quiet NaN) is passed over.
+template <int N>
+__device__ inline uint32_t mx_top(const float (&y)[N]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, __builtin_fabsf(y[e]));
+  if (__any(!(m < __builtin_inff()))) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const uint32_t u = __builtin_bit_cast(uint32_t, y[e]) & 0x7FFFFFFFu;
+      a = max(a, u < 0x7F800000u ? u : 0u);
+    }
+    return a;
+  }
+  return __builtin_bit_cast(uint32_t, m);
 }
 // The scale byte of a block whose largest finite magnitude has bits a: with
 // a = 1.m 2^x, a <= 448 2^e = 1.75 2^(8 + e) asks for e >= x - 8, and one more
@@ -36,14 +50,11 @@ __device__ inline uint32_t mx_scale_byte(uint32_t a) {
 __device__ inline float mx_inverse(uint32_t byte) {
   return __builtin_bit_cast(float, (254u - byte) << 23);
 }
-// Two codes: round to nearest even in the conversion (|y| <= 448 here; an
-// infinity is made a NaN first, as E4M3 has none).
-__device__ inline float mx_finite(float y) {
-  return __builtin_fabsf(y) < __builtin_inff() ? y : __builtin_nanf("");
-}
+// Four codes, rounded to nearest even in the conversion: at most 448, or a NaN
+// code for a NaN and (E4M3 has no infinities) an infinity.
 __device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float inv) {
-  int v = __builtin_amdgcn_cvt_pk_fp8_f32(mx_finite(a) * inv, mx_finite(b) * inv, 0, false);
-  v = __builtin_amdgcn_cvt_pk_fp8_f32(mx_finite(c) * inv, mx_finite(d) * inv, v, true);
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  v = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, v, true);
   return (uint32_t)v;
 }
 
@@ -51,9 +62,7 @@ __device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float i
 // 16 lanes, which all run this.  Returns the lane's codes; dword gets the four
 // scale bytes of the 128 columns (in every lane).
 __device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) a = max(a, mx_magnitude(y[e]));
+  uint32_t a = mx_top(y);
   a = max(a, dpp<kDppXor1>(a));
   a = max(a, dpp<kDppXor2>(a));
   const uint32_t byte = mx_scale_byte(a);

@@ -328,9 +328,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
 #pragma unroll
           for (int b = 0; b < TB; ++b) {
             // a block's 32 columns are this lane's 16 and those of lane ^ 32
-            uint32_t top = 0;
+            float y[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = max(top, mx_magnitude(acc[a][b][i]));
+            for (int i = 0; i < 16; ++i) y[i] = acc[a][b][i];
+            uint32_t top = mx_top(y);
             top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
             const uint32_t byte = mx_scale_byte(top);
             const float inv = mx_inverse(byte);
@@ -338,8 +339,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               *reinterpret_cast<uint32_t*>(lds + arow[a] * CRB + blk * 32 + 8 * q + 4 * g) =
-                  mx_codes4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2],
-                            acc[a][b][4 * q + 3], inv);
+                  mx_codes4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3], inv);
             if (g == 0) lds[BM * CRB + arow[a] * NBLK + blk] = (uint8_t)byte;
           }
       }
@@ -439,6 +439,166 @@ int32_t launch(const MxLinear& p, bool silu, hipStream_t stream) {
   return check_launch("pa_linear_mx");
 }
 
+// Few rows (decode steps): the weights' bytes bound the call, so they stream
+// from memory straight to registers.  Yᵀ tiles on
+// v_mfma_scale_f32_16x16x128_f8f6f4: A = a fragment of W (16 rows), B = 16 rows
+// of X (from L2); lane (c, j) = (lane % 16, lane / 16) holds columns 16 j .. + 15
+// and 64 + 16 j .. + 15 of row c of both and the scale byte of columns 32 j ..
+// + 31, and of a product Yᵀ[W row 4 j + r][X row c].  A workgroup computes TG NT
+// W tiles x MT X tiles: TG groups of kw wavefronts, which take NT tiles and an
+// equal share of the K steps each, load a step while they multiply the one
+// before, and sum in LDS, from where every thread finishes four columns of one
+// row.  SILU: one group takes two gate tiles, the other their up tiles, so that
+// a workgroup holds whole blocks of 32 output columns.
+template <bool SILU, int MT, int NT, int MAXW>
+__global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, int kw) {
+  static_assert(!SILU || NT == 2, "two gate and two up tiles");
+  constexpr int TG = SILU ? 2 : 1, TILES = TG * NT, NO = NT;  // NO: output tiles
+  extern __shared__ f32x4 part[];  // [kw][TILES][MT][64]
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, j = lane >> 4;
+  const int M = p.M, N = p.N, nk = p.steps;
+  const int tiles_n = (N + 15) / 16;  // of W (of its gate half)
+  const int kp = TG == 1 ? wave : wave % kw, tg = TG == 1 ? 0 : wave / kw;
+  const int s0 = (int)((int64_t)kp * nk / kw), s1 = (int)((int64_t)(kp + 1) * nk / kw);
+  const uint8_t *wp[NT], *sp[NT], *xp[MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    // tiles behind the last read it again
+    const int f = min((int)blockIdx.x * NO + (SILU ? 0 : tg * NT) + t, tiles_n - 1) +
+                  (SILU ? tg * tiles_n : 0);
+    wp[t] = p.w + (int64_t)f * nk * 2048 + lane * 16;
+    sp[t] = p.ws + (int64_t)f * nk * 64 + c * 4;
+  }
+  int xrow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    xrow[t] = min(16 * t + c, M - 1);  // rows behind the last read it again
+    xp[t] = p.x + (int64_t)xrow[t] * nk * 128 + j * 16;
+  }
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int q = 0; q < MT; ++q) acc[t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Stage {
+    i32x4 w[NT][2], x[MT][2];
+    int ws[NT], xs[MT];
+  };
+  auto load = [&](int s, Stage& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint8_t* at = wp[t] + (int64_t)s * 2048;
+      o.w[t][0] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(at));
+      o.w[t][1] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(at + 1024));
+      o.ws[t] = *reinterpret_cast<const int*>(sp[t] + (int64_t)s * 64);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uint8_t* at = xp[t] + (int64_t)s * 128;
+      o.x[t][0] = *reinterpret_cast<const i32x4*>(at);
+      o.x[t][1] = *reinterpret_cast<const i32x4*>(at + 64);
+      o.xs[t] = *reinterpret_cast<const int*>(p.xs + ((int64_t)s * p.pad_m + xrow[t]) * 4);
+    }
+  };
+  auto multiply = [&](const Stage& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < MT; ++q)
+        acc[t][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            __builtin_shufflevector(o.w[t][0], o.w[t][1], 0, 1, 2, 3, 4, 5, 6, 7),
+            __builtin_shufflevector(o.x[q][0], o.x[q][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[t][q], 0,
+            0, 0, o.ws[t] >> (8 * j), 0, o.xs[q] >> (8 * j));
+  };
+  Stage a, b;
+  if (s0 < s1) load(s0, a);
+  for (int s = s0; s < s1; s += 2) {
+    if (s + 1 < s1) load(s + 1, b);
+    multiply(a);
+    if (s + 1 >= s1) break;
+    if (s + 2 < s1) load(s + 2, a);
+    multiply(b);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int q = 0; q < MT; ++q)
+      part[((kp * TILES + tg * NT + t) * MT + q) * 64 + lane] = acc[t][q];
+  __syncthreads();
+  // columns 4 i % (4 NO) .. + 3 of row i / (4 NO), partial sums in K order
+  const int rows = min(M, 16 * MT);
+  auto total = [&](int tile, int row, int quad) __attribute__((always_inline)) {
+    f32x4 v = part[(tile * MT + row / 16) * 64 + row % 16 + 16 * quad];
+    for (int w = 1; w < kw; ++w)
+      v += part[((w * TILES + tile) * MT + row / 16) * 64 + row % 16 + 16 * quad];
+    return v;
+  };
+  for (int i = threadIdx.x; i < 16 * MT * 4 * NO; i += 64 * TG * kw) {
+    const int row = i / (4 * NO), quad = i % (4 * NO);
+    if (row >= rows) break;  // whole rows: the shuffles below stay within one
+    const int col = ((int)blockIdx.x * 4 * NO + quad) * 4;
+    f32x4 y = total(quad / 4, row, quad % 4);
+    if constexpr (SILU) {
+      const f32x4 up = total(NO + quad / 4, row, quad % 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = col < N ? y[e] / (1.0f + expf(-y[e])) * up[e] : 0.f;  // N: a multiple of 32
+      if (p.out_scales) {
+        // a block is eight consecutive threads' columns
+        const float four[4] = {y[0], y[1], y[2], y[3]};
+        uint32_t top = mx_top(four);
+        top = max(top, dpp<kDppXor1>(top));
+        top = max(top, dpp<kDppXor2>(top));
+        top = max(top, dpp<kDppHalfMirror>(top));
+        const uint32_t byte = mx_scale_byte(top);
+        const int pitch = (N + 127) / 128 * 128;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (int64_t)row * pitch + col) =
+            mx_codes4(y[0], y[1], y[2], y[3], mx_inverse(byte));
+        if (quad % 8 == 0)
+          p.out_scales[((int64_t)(col / 128) * p.pad_m + row) * 4 + col / 32 % 4] = (uint8_t)byte;
+        continue;
+      }
+    }
+    const int64_t at = (int64_t)row * N + col;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+    uint16_t prev[4] = {0, 0, 0, 0}, v[4];
+    const bool wide = N % 4 == 0;
+    if (wide && col >= N) continue;
+    if (!SILU && p.residual) {
+      if (wide)
+        *reinterpret_cast<uint64_t*>(prev) =
+            *reinterpret_cast<const uint64_t*>(p.residual + at);
+      else
+        for (int e = 0; e < 4 && col + e < N; ++e) prev[e] = p.residual[at + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float f = y[e];
+      if (!SILU && p.bias && col + e < N) f += bf16_bits_to_f32(p.bias[col + e]);
+      if (!SILU) f += bf16_bits_to_f32(prev[e]);
+      v[e] = f32_to_bf16_bits(f);
+    }
+    if (wide)
+      *reinterpret_cast<uint64_t*>(out) = *reinterpret_cast<const uint64_t*>(v);
+    else
+      for (int e = 0; e < 4 && col + e < N; ++e) out[e] = v[e];
+  }
+}
+
+template <bool SILU, int MT, int NT, int MAXW>
+int32_t launch_skinny(const MxLinear& p, int kw, hipStream_t stream) {
+  constexpr int TG = SILU ? 2 : 1;
+  kw = std::min(kw, p.steps);
+  // an MXFP8 output's padding is written too
+  const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
+  const dim3 grid((uint32_t)((cols + 16 * NT - 1) / (16 * NT)));
+  const size_t lds = (size_t)kw * TG * NT * MT * 64 * sizeof(f32x4);
+  mx_skinny_kernel<SILU, MT, NT, MAXW><<<grid, 64 * TG * kw, lds, stream>>>(p, kw);
+  return check_launch("pa_linear_mx");
+}
+
 }  // namespace
 }  // namespace pa
 
@@ -482,6 +642,16 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
                    rows,     out_features,
                    (int)mx_steps(in_features), mx_pad_rows(rows)};
   hipStream_t s = (hipStream_t)stream;
+  if (const MxSkinny k = choose_mx_skinny(rows, out_features, silu); k.kw) {
+    const bool one = rows <= 16;  // one tile of X rows
+    if (silu)
+      return one ? launch_skinny<true, 1, 2, 8>(p, k.kw, s) : launch_skinny<true, 2, 2, 8>(p, k.kw, s);
+    if (k.nt == 2)
+      return one ? launch_skinny<false, 1, 2, 8>(p, k.kw, s)
+                 : launch_skinny<false, 2, 2, 8>(p, k.kw, s);
+    return one ? launch_skinny<false, 1, 1, 16>(p, k.kw, s)
+               : launch_skinny<false, 2, 1, 16>(p, k.kw, s);
+  }
   switch (choose_mx_tiling(rows, silu ? 2 * out_features : out_features, in_features)) {
     case kMx256x256: return launch<2, 2, 4, 4, 1, 2>(p, silu, s);
     case kMx256x128: return launch<4, 2, 2, 2, 1, 3>(p, silu, s);

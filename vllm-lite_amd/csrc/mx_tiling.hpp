@@ -41,4 +41,30 @@ inline MxTiling choose_mx_tiling(int M, int wrows, int K) {
   return best;
 }
 
+// The kernel for few rows: W tiles per wavefront and wavefronts that share K
+// (kw 0: the tiled kernel instead).  Measured at 32 rows, us:
+//   N x K                4096 x 12288  4096 x 4096  896 x 4864  1152 x 896
+//   1 tile, 16 wavefronts    16.4          7.9          8.5        3.8
+//   2 tiles, 4               17.9          9.0         10.3        3.8
+//   64 x 64 tiling           21.7         10.6         10.7        5.6
+//                        6144 x 4096  12288 x 4096  24576 x 4096  151936 x 896
+//   1 tile, 16 wavefronts    13.2         19.4         37.4         61.2
+//   2 tiles, 4                9.7         15.4         23.0         32.5
+//   64 x 64 tiling           10.5         12.5         26.3         56.9
+// (one tile reads X from L2 twice as often and fills the chip sooner; the 64 x
+// 64 tiling wins where its tiles fill one round of the CUs.)  SwiGLU, where a
+// workgroup is two groups of kw wavefronts: kw 4 / 2 / the tiling at 4864 x
+// 896 6.1 / 6.2 / 6.4, at 12288 x 4096 28.2 / 27.1 / 27.6.  Above 32 rows the
+// 64 x 64 tiling is faster (64 rows: 4096 x 12288 21.9 against 28.5).
+struct MxSkinny {
+  int nt, kw;
+};
+inline MxSkinny choose_mx_skinny(int M, int N, bool silu) {
+  if (M > 32) return {0, 0};
+  if (silu) return {2, N <= 8192 ? 4 : 2};
+  if (N <= 4096) return {1, 16};
+  if (N > 7168 && N <= 64 * 256) return {0, 0};
+  return {2, 4};
+}
+
 }  // namespace pa

@@ -109,13 +109,10 @@ def test_outputs_stay_in_their_rows(pa):
 
 
 def norm_reference(x, add, w):
+    """The sum as it is stored, and the row's result in 64 bits, of which the
+    kernel's codes are."""
     s = x.double() if add is None else (x.float() + add.float()).to(x.dtype).double()
-    y = s / (s.pow(2).mean(1, keepdim=True) + EPS).sqrt() * w.double()
-    # f32: the squares' sum rounds in a lane's chain of at most max(32, K / 32)
-    # additions and eight more, half of it left by the root; the mean, eps, the
-    # root, the division and three products round once each
-    k = x.shape[1]
-    return s, y, y.abs() * (max(32, k / 32) / 2 + 4 + 8) * 2.0 ** -24
+    return s, s / (s.pow(2).mean(1, keepdim=True) + EPS).sqrt() * w.double()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -126,14 +123,14 @@ def test_rms_norm(pa, rows, cols, dtype, with_add):
     x = hidden_states(g, rows, cols, dtype)
     w = (1 + 0.2 * torch.randn(cols, generator=g, device=DEV)).to(dtype)
     add = hidden_states(g, rows, cols, dtype) if with_add else None
-    s, y, err = norm_reference(x, add, w)
+    s, y = norm_reference(x, add, w)
     before = x.clone()
     total = torch.empty_like(x) if with_add else None
     mx = pa.rms_norm_mx(x, w, EPS, add=add, residual_out=total)
     assert torch.equal(x, before)
     if with_add:
         assert torch.equal(total.double(), s)
-    plain.assert_rounds(mx, y, err)
+    same_as_definition(mx, y)
     # in place: the same sum and the same codes
     mx2 = pa.rms_norm_mx(x, w, EPS, add=add)
     assert torch.equal(mx.codes, mx2.codes)
@@ -143,8 +140,9 @@ def test_rms_norm(pa, rows, cols, dtype, with_add):
 
 def test_rms_norm_special_rows(pa):
     """A row of zeros, one of the smallest values, one with an infinity, one
-    with a NaN, one whose squares overflow: as the formula in f32 has them."""
-    x = torch.ones(5, 256, device=DEV)
+    with a NaN, one whose squares pass f32, a weight that makes a value do so:
+    as the formula has them."""
+    x = torch.ones(6, 256, device=DEV)
     x[0] = 0
     x[1] = 1e-30
     x[2, 7] = float("inf")
@@ -153,11 +151,15 @@ def test_rms_norm_special_rows(pa):
     w = torch.ones(256, device=DEV)
     v = plain.dequantize(pa.rms_norm_mx(x, w, EPS))
     assert (v[0] == 0).all()
-    # 1e-30 / sqrt(eps), as its block's only value: within half a step of 2^-4
+    # 1e-30 / sqrt(eps): within half a step of 2^-4
     assert ((v[1] / 1e-27 - 1).abs() <= 2.0 ** -4).all()
     assert torch.isnan(v[2, 7]) and (torch.cat([v[2, :7], v[2, 8:]]) == 0).all()
     assert torch.isnan(v[3]).all()
-    assert (v[4] == 0).all()  # 1 / sqrt(inf)
+    assert (v[4] == 1).all()
+    w[9] = 2.0 ** 127
+    x[5, 9] = 4
+    v = plain.dequantize(pa.rms_norm_mx(x, w, EPS))
+    assert torch.isnan(v[5, 9]) and (torch.cat([v[5, :9], v[5, 10:]]) > 0.9).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -170,8 +172,8 @@ def test_rms_norm_misaligned(pa, dtype):
         return torch.randn(n + 1, generator=g, device=DEV).to(dtype)[1:]
 
     x, add, w = odd(rows * cols).view(rows, cols), odd(rows * cols).view(rows, cols), odd(cols)
-    s, y, err = norm_reference(x, add, w)
-    plain.assert_rounds(pa.rms_norm_mx(x, w, EPS, add=add), y, err)
+    s, y = norm_reference(x, add, w)
+    same_as_definition(pa.rms_norm_mx(x, w, EPS, add=add), y)
     assert torch.equal(x.double(), s)
 
 

@@ -117,10 +117,23 @@ __global__ __launch_bounds__(256) void quantize_mx_kernel(Layout out, const T* _
   }
 }
 
+// The sum over a row's G lanes: within 16 lanes by lane permutations, across
+// them by shuffles, and for a workgroup per row over its four wavefronts in
+// LDS.
+template <int CTRL>
+__device__ inline double dpp_add(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t o = dpp<CTRL>((uint32_t)u) | (uint64_t)dpp<CTRL>((uint32_t)(u >> 32)) << 32;
+  return v + __builtin_bit_cast(double, o);
+}
 template <int G>
-__device__ inline float row_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+__device__ inline double row_sum(double v, double* red) {
+  v = dpp_add<kDppXor1>(v);
+  v = dpp_add<kDppXor2>(v);
+  v = dpp_add<kDppHalfMirror>(v);
+  v = dpp_add<kDppMirror>(v);
+  v += __shfl_xor(v, 16, 64);
+  v += __shfl_xor(v, 32, 64);
   if constexpr (G == 256) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -129,9 +142,33 @@ __device__ inline float row_sum(float v, float* red) {
   return v;
 }
 
+// v w / rms with r = 1 / rms as a sum of two floats, for a rounding to fewer
+// bits: the f32 nearest to the product (v r, then w, each with its error),
+// moved to the odd float beside it on the side where the product lies if that
+// f32 is even and not the product itself.  The borders between codes are even
+// floats, so the code is that of the product, as if it had not been rounded to
+// f32 in between.
+__device__ inline float scaled_odd(float v, float w, float r, float r_low) {
+#pragma clang fp contract(off)  // q's own rounding is part of q_low
+  const float p = v * r;
+  const float p_low = fmaf(v, r_low, fmaf(v, r, -p));
+  const float q = p * w;
+  const float q_low = fmaf(p_low, w, fmaf(p, w, -q));
+  const float y = q + q_low, low = q_low - (y - q);
+  const int bits = __builtin_bit_cast(int, y);
+  // +1: away from zero
+  const int side = ((__builtin_bit_cast(int, low) ^ bits) >> 31) | 1;
+  constexpr int kFiniteNotZero = 0x198;  // of either sign
+  const bool move = __builtin_amdgcn_classf(low, kFiniteNotZero) && !(bits & 1);
+  return __builtin_bit_cast(float, bits + (move ? side : 0));
+}
+
 // G lanes per row (64: a wavefront, 256: the workgroup), chunk i of lane l is
 // columns 8 (l + G i) ..  C > 0: the row fits C chunks a lane and stays in
-// registers; C = 0: it is read again for the second pass.
+// registers; C = 0: it is read again for the second pass.  The sum of squares
+// is f64 and the scaling exact up to the rounding to codes where f32 leaves it
+// open, so that they are the codes of the formula, whatever the order of the
+// sum (in f32 throughout, 5 of 10^7 fell to the other side of a border).
 template <typename T, int G, int C>
 __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum, const T* residual,
                                                           const T* __restrict__ add,
@@ -139,7 +176,7 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum,
                                                           int hidden, float eps, int near) {
   typedef typename Vec8<T>::V V;
   using E = std::conditional_t<sizeof(T) == 2, __bf16, float>;
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int lane = threadIdx.x % G;
   const int64_t row = first_row(blockIdx.x, 256 / G, near) + threadIdx.x / G;
   if (row >= rows) return;  // a whole wavefront, or at G = 256 the workgroup
@@ -147,7 +184,7 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum,
   const T* x = residual + row * hidden;
   const T* a = add ? add + row * hidden : nullptr;
   T* o = add ? sum + row * hidden : nullptr;
-  float ss = 0.f;
+  double ss = 0.;
   // the row's value: with add the sum, kept in the storage dtype and stored
   auto take = [&](int ch, V& v, const V& av) __attribute__((always_inline)) {
     if (a) {
@@ -156,15 +193,28 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum,
       store8(o, ch, hidden, v);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += (float)v[e] * (float)v[e];
+    for (int e = 0; e < 8; ++e) ss = fma((double)v[e], (double)v[e], ss);
   };
-  auto write = [&](int ch, const V& v, const V& wv, float inv) __attribute__((always_inline)) {
-    // the product with the weight first: exact for bf16
+  float r, r_low;
+  auto finish = [&]() __attribute__((always_inline)) {
+    const double d = rsqrt(row_sum<G>(ss, red) / hidden + (double)eps);
+    r = (float)d;
+    r_low = (float)(d - (double)r);
+  };
+  auto write = [&](int ch, const V& v, const V& wv) __attribute__((always_inline)) {
+    // three roundings, each at most 2^-24, and r's
     float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (float)v[e] * (float)wv[e] * inv;
+    for (int e = 0; e < 8; ++e) y[e] = (float)v[e] * r * (float)wv[e];
     uint32_t dword;
-    *out.code(row, ch) = mx_quantize8(y, dword);
+    bool sure;
+    uint2 codes = mx_quantize8(y, dword, sure);
+    if (!__all(sure)) {  // about 1 of 100 times
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = scaled_odd((float)v[e], (float)wv[e], r, r_low);
+      codes = mx_quantize8(y, dword);
+    }
+    *out.code(row, ch) = codes;
     if (threadIdx.x % 16 == 0) *out.scale(row, ch / 16) = dword;
   };
   if constexpr (C > 0) {
@@ -180,19 +230,19 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum,
 #pragma unroll
     for (int i = 0; i < C; ++i)
       if (lane + G * i < nch) take(lane + G * i, v[i], av[i]);
-    const float inv = 1.0f / sqrtf(row_sum<G>(ss, red) / (float)hidden + eps);
+    finish();
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (lane + G * i < nch) write(lane + G * i, v[i], wv[i], inv);
+      if (lane + G * i < nch) write(lane + G * i, v[i], wv[i]);
   } else {
     for (int ch = lane; ch < nch; ch += G) {
       V v = load8(x, ch, hidden), av;
       if (a) av = load8(a, ch, hidden);
       take(ch, v, av);
     }
-    const float inv = 1.0f / sqrtf(row_sum<G>(ss, red) / (float)hidden + eps);
+    finish();
     for (int ch = lane; ch < nch; ch += G)
-      write(ch, load8<T>(a ? o : x, ch, hidden), load8(w, ch, hidden), inv);
+      write(ch, load8<T>(a ? o : x, ch, hidden), load8(w, ch, hidden));
   }
 }
 

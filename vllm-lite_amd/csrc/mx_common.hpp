@@ -59,19 +59,38 @@ __device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float i
 }
 
 // Eight consecutive columns per lane, a block over 4 lanes, 128 columns over
-// 16 lanes, which all run this.  Returns the lane's codes; dword gets the four
-// scale bytes of the 128 columns (in every lane).
-__device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword) {
+// 16 lanes, which all run this: the largest magnitude of the lane's block, and
+// the four scale bytes of the 128 columns (in every lane) from the lane's own.
+__device__ inline uint32_t mx_block_top8(const float (&y)[8]) {
   uint32_t a = mx_top(y);
   a = max(a, dpp<kDppXor1>(a));
-  a = max(a, dpp<kDppXor2>(a));
-  const uint32_t byte = mx_scale_byte(a);
-  const float inv = mx_inverse(byte);
+  return max(a, dpp<kDppXor2>(a));
+}
+__device__ inline uint32_t mx_scale_dword8(uint32_t byte) {
   uint32_t d = byte << (8 * ((threadIdx.x >> 2) & 3));
   d |= dpp<kDppHalfMirror>(d);
-  d |= dpp<kDppMirror>(d);
-  dword = d;
+  return d | dpp<kDppMirror>(d);
+}
+__device__ inline uint2 mx_codes8(const float (&y)[8], float inv) {
   return uint2{mx_codes4(y[0], y[1], y[2], y[3], inv), mx_codes4(y[4], y[5], y[6], y[7], inv)};
+}
+// Codes and scale bytes of y.
+__device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword) {
+  const uint32_t byte = mx_scale_byte(mx_block_top8(y));
+  dword = mx_scale_dword8(byte);
+  return mx_codes8(y, mx_inverse(byte));
+}
+// The same of values that y has within 2^-21 of their size; sure: whether the
+// lane's codes and scale are theirs all the same, i.e. equal at both ends.
+__device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword, bool& sure) {
+  const uint32_t top = mx_block_top8(y), byte = mx_scale_byte(top);
+  const float inv = mx_inverse(byte);
+  dword = mx_scale_dword8(byte);
+  const uint2 lo = mx_codes8(y, inv * (1.f - 0x1p-21f)), hi = mx_codes8(y, inv * (1.f + 0x1p-21f));
+  // 8 steps of a float are at least 2^-21 of it
+  sure = lo.x == hi.x && lo.y == hi.y &&
+         mx_scale_byte(max(top, 8u) - 8) == mx_scale_byte(top + 8);
+  return lo;
 }
 
 }  // namespace pa

@@ -73,10 +73,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   const int M = p.M, N = p.N, nk = p.steps;
   // Tile order: workgroups are dealt round-robin to the 8 XCDs; XCD i takes
   // the i-th contiguous range of an order that goes through groups of row
-  // tiles (all of them up to 8, so that W is streamed once; else 4), column
-  // tiles outer within a group, so the tiles in flight on an XCD share X and
-  // W rows in its L2.
-  const int group_m = ntm <= 8 ? ntm : 4;
+  // tiles (up to 8, so that W is streamed once), column tiles outer within a
+  // group, so the tiles in flight on an XCD share X and W rows in its L2.
+  const int group_m = min(ntm, 8);
   const int total = ntm * ntn, per_xcd = (total + 7) / 8;
   const int tile = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
   if ((int)(blockIdx.x / 8) >= per_xcd || tile >= total) return;
@@ -365,18 +364,36 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   uint16_t* out = static_cast<uint16_t*>(p.out);
   constexpr int CPRO = BNO / 8;
   if constexpr (!SILU) {
-    if (p.residual)
+    if (p.residual && N % 8 == 0) {
+      // several loads in flight per thread (one at a time took 17 us of a
+      // 256 x 256 tile); those outside the output read its last row or piece
+      constexpr int ITEMS = BM * CPRO / NT, BATCH = ITEMS % 16 == 0 ? 16 : ITEMS % 8 == 0 ? 8 : 1;
+      static_assert(ITEMS * NT == BM * CPRO, "whole batches");
+      for (int i0 = 0; i0 < ITEMS; i0 += BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int i = (i0 + u) * NT + threadIdx.x, r = i / CPRO, cc = i % CPRO * 8;
+          v[u] = *reinterpret_cast<const uint4*>(
+              p.residual + (int64_t)min(m0 + r, M - 1) * N + min(c0 + cc, N - 8));
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int i = (i0 + u) * NT + threadIdx.x;
+          *reinterpret_cast<uint4*>(lds + i / CPRO * ORB + i % CPRO * 16) = v[u];
+        }
+      }
+    } else if (p.residual) {
       for (int i = threadIdx.x; i < BM * CPRO; i += NT) {
         const int r = i / CPRO, cc = i % CPRO * 8;
-        if (m0 + r >= M || c0 + cc >= N) continue;
+        if (m0 + r >= M) continue;
         const uint16_t* src = p.residual + (int64_t)(m0 + r) * N + c0 + cc;
-        uint8_t* dst = lds + r * ORB + cc * 2;
-        if (N % 8 == 0)
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-        else
-          for (int e = 0; e < 8 && c0 + cc + e < N; ++e)
-            reinterpret_cast<uint16_t*>(dst)[e] = src[e];
+        uint16_t* dst = reinterpret_cast<uint16_t*>(lds + r * ORB + cc * 2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + cc + e < N) dst[e] = src[e];
       }
+    }
     for (int i = threadIdx.x; i < BN; i += NT)
       sbias[i] = p.bias && c0 + i < N ? bf16_bits_to_f32(p.bias[c0 + i]) : 0.f;
     __syncthreads();

@@ -669,7 +669,7 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
     return one ? launch_skinny<false, 1, 1, 16>(p, k.kw, s)
                : launch_skinny<false, 2, 1, 16>(p, k.kw, s);
   }
-  switch (choose_mx_tiling(rows, silu ? 2 * out_features : out_features, in_features)) {
+  switch (choose_mx_tiling(rows, (int64_t)out_features * (silu ? 2 : 1), in_features)) {
     case kMx256x256: return launch<2, 2, 4, 4, 1, 2>(p, silu, s);
     case kMx256x128: return launch<4, 2, 2, 2, 1, 3>(p, silu, s);
     case kMx128x128Pair: return launch<2, 2, 2, 2, 1, 2>(p, silu, s);

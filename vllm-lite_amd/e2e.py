@@ -27,6 +27,9 @@ QKV projection with RoPE and the KV write in its epilogue, attention, O, gate|up
 residual adds in the O and down epilogues.  Decode steps after the first are
 one replay each of a captured step that advances the batch by a token on the
 device (pa_batch_advance; the block tables hold the whole generation).
+With weights quantised by Weights.pack_mx() every step runs the decoder block
+in MXFP8 (Engine._forward_mx): half the bytes of the projections' weights, the
+matrix cores at their FP8 rate.
 The norm is chosen explicitly by ModelConfig.norm: "rms" (RMSNorm, what the
 benchmark configuration states) or "layer" (the zero-bias LayerNorm the
 reference's CausalLm constructs for these models,
@@ -88,6 +91,7 @@ class Weights:
         self.wd = [w(h, cfg.inter) for _ in range(cfg.layers)]
         self.norm = torch.ones(h, dtype=dtype, device=device)
         self.packed = None
+        self.mx = None
 
     def pack(self, fold_rms=True):
         """Repacks the weights pa_linear reads (QKV as separate Q and K|V row
@@ -123,6 +127,16 @@ class Weights:
             p["lm_head"] = ops.PackedWeight(self.embed, col_scale=self.norm if fold_rms else None)
         p["rms_folded"] = fold_rms
         self.packed = p
+
+    def pack_mx(self):
+        """Quantises the projections' weights and the tied LM head to MXFP8
+        (ops.MxWeight); engines made with these weights then run in MXFP8.  The
+        row-major tensors stay (the embedding rows are read from them)."""
+        self.mx = {"qkv": [ops.MxWeight(x) for x in self.wqkv],
+                   "o": [ops.MxWeight(x) for x in self.wo],
+                   "gu": [ops.MxWeight(x) for x in self.wgu],
+                   "down": [ops.MxWeight(x) for x in self.wd],
+                   "lm_head": ops.MxWeight(self.embed)}
 
     def nbytes(self):
         """Bytes of the model's weights (row-major; a step reads each once)."""
@@ -173,6 +187,8 @@ class Engine:
     def _logits(self, tokens, logit_rows):
         """forward's logits in the model dtype (bf16)."""
         c, w = self.cfg, self.w
+        if w.mx is not None:
+            return self._forward_mx(tokens, logit_rows)
         t = tokens.shape[0]
         hq, hkv, d = c.heads, c.kv_heads, c.head_dim
         skinny = t <= SKINNY_ROWS
@@ -262,6 +278,36 @@ class Engine:
                 ops.linear(act, w.wd[layer], out=x, add_to_out=True)
         rows = x if logit_rows is None else x[logit_rows].contiguous()
         return ops.linear(rows, pk["lm_head"], rms_eps=c.eps)
+
+    def _norm_mx(self, x, weight):
+        """The configured norm of the rows of x, as MXFP8 rows."""
+        if self.cfg.norm == "rms":
+            return ops.rms_norm_mx(x, weight, self.cfg.eps)
+        return ops.quantize_mx(ops.layer_norm(x, weight, self.cfg.eps))
+
+    def _forward_mx(self, tokens, logit_rows):
+        """_logits with the projections in MXFP8: per layer the norm writes the
+        QKV projection's rows, attention's output is quantised for the O
+        projection, the gate|up projection's SwiGLU epilogue writes the down
+        projection's rows, and O and down add into the residual stream."""
+        c, w, mx = self.cfg, self.w, self.w.mx
+        t = tokens.shape[0]
+        hq, hkv, d = c.heads, c.kv_heads, c.head_dim
+        nq = hq * d
+        x = F.embedding(tokens, w.embed)  # residual stream [T, hidden]
+        for layer in range(c.layers):
+            h = self._norm_mx(x, w.ln1[layer])
+            qkv = ops.linear_mx(h, mx["qkv"][layer], bias=w.bqkv[layer])
+            q = qkv[:, :nq].view(t, hq, d)
+            k = qkv[:, nq:nq + hkv * d].view(t, hkv, d)
+            v = qkv[:, nq + hkv * d:].view(t, hkv, d)
+            attn = self.batch.attention(self.cache, layer, q, k, v, self.inv_freq, self.scale)
+            ops.linear_mx(ops.quantize_mx(attn.view(t, nq)), mx["o"][layer], residual=x, out=x)
+            h = self._norm_mx(x, w.ln2[layer])
+            act = ops.linear_mx(h, mx["gu"][layer], act=ops.ACT_SILU_MUL, mx_out=True)
+            ops.linear_mx(act, mx["down"][layer], residual=x, out=x)
+        rows = x if logit_rows is None else x[logit_rows].contiguous()
+        return ops.linear_mx(self._norm_mx(rows, w.norm), mx["lm_head"])
 
     def generate(self, prompts, max_new):
         """Greedy generation for every prompt (lists of token ids).  Returns

@@ -13,6 +13,7 @@ def lib(pa):
 
 P = C.c_void_p(64)
 ODD = C.c_void_p(65)
+FAR, NEAR = C.c_void_p(1 << 40), C.c_void_p((1 << 40) + 48)
 
 
 def test_sizes(lib):
@@ -41,24 +42,48 @@ def test_quantize_refusals(lib):
     for name in ("codes", "scales", "x"):
         assert quantize(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
         assert quantize(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
+    assert quantize(lib) == -1 and b"overlap" in lib.pa_last_error()
+    assert quantize(lib, codes=FAR, x=NEAR) == -1 and b"overlap" in lib.pa_last_error()
+    assert quantize(lib, scales=FAR, x=NEAR) == -1 and b"overlap" in lib.pa_last_error()
+    assert quantize(lib, codes=FAR, scales=NEAR) == -1 and b"overlap" in lib.pa_last_error()
 
 
-def norm(lib, codes=P, scales=P, sum=P, residual=P, add=P, weight=P, rows=4, hidden=100, dtype=1):
-    return lib.pa_rms_norm_mx(codes, scales, sum, residual, add, weight, rows, hidden, 1e-6, dtype,
-                              None)
+def norm(lib, codes=None, scales=None, sum=None, residual=None, add=None, weight=None, rows=4,
+         hidden=100, dtype=1, **given):
+    """Arrays far apart, but for those given (0: none)."""
+    at = {n: C.c_void_p((i + 1) << 30) for i, n in enumerate(
+        ("codes", "scales", "sum", "residual", "add", "weight"))}
+    for n, v in (("codes", codes), ("scales", scales), ("sum", sum), ("residual", residual),
+                 ("add", add), ("weight", weight)):
+        if v is not None:
+            at[n] = C.c_void_p(v) if v else None
+    return lib.pa_rms_norm_mx(at["codes"], at["scales"], at["sum"], at["residual"], at["add"],
+                              at["weight"], rows, hidden, 1e-6, dtype, None)
 
 
 def test_norm_refusals(lib):
-    assert norm(lib, rows=0, codes=None) == 0
+    assert norm(lib, rows=0, codes=0) == 0
     assert norm(lib, rows=-1) == -1
     assert norm(lib, hidden=0) == -1
     assert norm(lib, dtype=7) == -1
     assert norm(lib, hidden=(1 << 22) + 1) == -3
-    assert norm(lib, sum=None) == -1 and b"needs sum" in lib.pa_last_error()
-    for name in ("codes", "scales", "residual", "weight"):
-        assert norm(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
-    for name in ("codes", "scales", "sum", "residual", "add", "weight"):
-        assert norm(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
+    assert norm(lib, sum=0) == -1 and b"needs sum" in lib.pa_last_error()
+    names = ("codes", "scales", "sum", "residual", "add", "weight")
+    for i, name in enumerate(names):
+        if name not in ("sum", "add"):
+            assert norm(lib, **{name: 0}) == -1 and b"null" in lib.pa_last_error()
+        assert norm(lib, **{name: (1 << 40) + 1}) == -1 and b"aligned" in lib.pa_last_error()
+    # outputs that reach into another array: 4 rows of 100 bf16 are 800 bytes,
+    # of 128 codes 512
+    for out, other in (("codes", "scales"), ("codes", "sum"), ("codes", "residual"),
+                       ("codes", "add"), ("codes", "weight"), ("scales", "sum"),
+                       ("scales", "residual"), ("scales", "add"), ("scales", "weight"),
+                       ("sum", "add"), ("sum", "weight")):
+        assert norm(lib, **{out: 1 << 40, other: (1 << 40) + 48}) == -1, (out, other)
+        assert b"overlap" in lib.pa_last_error()
+    # the sum in place is allowed, a shifted one is not
+    assert norm(lib, sum=1 << 40, residual=(1 << 40) + 16) == -1
+    assert b"overlap" in lib.pa_last_error()
 
 
 def pack(lib, codes=P, scales=P, weight=P, rows=4, cols=100, dtype=1):
@@ -73,6 +98,7 @@ def test_pack_refusals(lib):
     for name in ("codes", "scales", "weight"):
         assert pack(lib, **{name: None}) == -1
         assert pack(lib, **{name: ODD}) == -1
+    assert pack(lib) == -1 and b"overlap" in lib.pa_last_error()
 
 
 def linear(lib, out=P, out_scales=None, x=P, xs=P, w=P, ws=P, bias=None, residual=None, rows=4,
@@ -97,6 +123,14 @@ def test_linear_refusals(lib):
     for name in ("out", "x", "xs", "w", "ws", "bias", "residual"):
         assert linear(lib, **{name: ODD}) == -1 and b"aligned" in lib.pa_last_error()
     assert linear(lib, act=1, out_scales=ODD) == -1
+    # 4 rows of 96 bf16: 768 bytes
+    for name in ("x", "xs", "w", "ws", "bias", "residual"):
+        assert linear(lib, out=FAR, **{name: NEAR}) == -1, name
+        assert b"overlap" in lib.pa_last_error()
+    for name in ("x", "xs", "w", "ws", "out"):
+        assert linear(lib, act=1, out_scales=FAR, **{**{"out": C.c_void_p(1 << 41)},
+                                                     name: NEAR}) == -1, name
+        assert b"overlap" in lib.pa_last_error()
 
 
 def test_wrappers_refuse_host_tensors(pa):

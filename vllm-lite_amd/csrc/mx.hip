@@ -295,7 +295,7 @@ extern "C" size_t pa_mx_row_bytes(int32_t cols) {
   return cols > 0 ? (size_t)mx_steps(cols) * 128 : 0;
 }
 extern "C" size_t pa_mx_scale_bytes(int32_t rows, int32_t cols) {
-  return rows > 0 && cols > 0 ? (size_t)mx_pad_rows(rows) * mx_steps(cols) * 4 : 0;
+  return rows > 0 && cols > 0 ? (size_t)mx_scale_bytes(rows, cols) : 0;
 }
 extern "C" size_t pa_mx_weight_bytes(int32_t rows, int32_t cols) {
   return rows > 0 && cols > 0 ? (size_t)mx_pad_rows(rows) * mx_steps(cols) * 128 : 0;
@@ -315,6 +315,13 @@ extern "C" int32_t pa_quantize_mx(uint8_t* codes, uint8_t* scales, const void* x
   PA_MX_ALIGNED("pa_quantize_mx", codes, scales);
   PA_REQUIRE((uintptr_t)x % dtype_size(dtype) == 0, PA_ERR_INVALID_ARG,
              "pa_quantize_mx: x is not aligned to its elements");
+  {
+    const int64_t nc = (int64_t)rows * mx_steps(cols) * 128, ns = mx_scale_bytes(rows, cols);
+    const int64_t nx = ((rows - 1) * (x_stride ? x_stride : cols) + cols) * (int64_t)dtype_size(dtype);
+    PA_REQUIRE(!mx_overlap(codes, nc, scales, ns) && !mx_overlap(codes, nc, x, nx) &&
+                   !mx_overlap(scales, ns, x, nx),
+               PA_ERR_INVALID_ARG, "pa_quantize_mx: arrays overlap");
+  }
   const RowLayout out{codes, scales, mx_steps(cols), mx_pad_rows(rows)};
   const int64_t stride = x_stride ? x_stride : cols;
   return (dtype == PA_DTYPE_BF16 ? launch_quantize<uint16_t, RowLayout>
@@ -333,6 +340,13 @@ extern "C" int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void
   PA_MX_ALIGNED("pa_linear_mx_pack", codes, scales);
   PA_REQUIRE((uintptr_t)weight % dtype_size(dtype) == 0, PA_ERR_INVALID_ARG,
              "pa_linear_mx_pack: the weight is not aligned to its elements");
+  {
+    const int64_t nc = mx_pad_rows(rows) * mx_steps(cols) * 128, ns = mx_scale_bytes(rows, cols);
+    const int64_t nw = (int64_t)rows * cols * (int64_t)dtype_size(dtype);
+    PA_REQUIRE(!mx_overlap(codes, nc, scales, ns) && !mx_overlap(codes, nc, weight, nw) &&
+                   !mx_overlap(scales, ns, weight, nw),
+               PA_ERR_INVALID_ARG, "pa_linear_mx_pack: arrays overlap");
+  }
   const WeightLayout out{codes, scales, mx_steps(cols)};
   return (dtype == PA_DTYPE_BF16 ? launch_quantize<uint16_t, WeightLayout>
                                  : launch_quantize<float, WeightLayout>)(
@@ -356,6 +370,20 @@ extern "C" int32_t pa_rms_norm_mx(uint8_t* codes, uint8_t* scales, void* sum,
   PA_REQUIRE(((uintptr_t)residual | (uintptr_t)add | (uintptr_t)sum | (uintptr_t)weight) %
                      dtype_size(dtype) == 0,
              PA_ERR_INVALID_ARG, "pa_rms_norm_mx: rows are not aligned to their elements");
+  {
+    const int64_t nc = (int64_t)rows * mx_steps(hidden) * 128, ns = mx_scale_bytes(rows, hidden);
+    const int64_t nw = hidden * (int64_t)dtype_size(dtype), nx = rows * nw;
+    const void* total = add ? sum : nullptr;
+    auto meets = [&](const void* p, int64_t n) {
+      return mx_overlap(p, n, residual, nx) || mx_overlap(p, n, add, nx) ||
+             mx_overlap(p, n, weight, nw);
+    };
+    PA_REQUIRE(!mx_overlap(codes, nc, scales, ns) && !mx_overlap(codes, nc, total, nx) &&
+                   !mx_overlap(scales, ns, total, nx) && !meets(codes, nc) && !meets(scales, ns) &&
+                   !mx_overlap(total, nx, add, nx) && !mx_overlap(total, nx, weight, nw) &&
+                   (total == residual || !mx_overlap(total, nx, residual, nx)),
+               PA_ERR_INVALID_ARG, "pa_rms_norm_mx: arrays overlap");
+  }
   const RowLayout out{codes, scales, mx_steps(hidden), mx_pad_rows(rows)};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PA_DTYPE_BF16)

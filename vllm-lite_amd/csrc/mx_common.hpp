@@ -11,6 +11,14 @@ namespace pa {
 inline int64_t mx_steps(int64_t cols) { return (cols + 127) / 128; }
 inline int64_t mx_pad_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
 constexpr int kMxMaxCols = 1 << 22;
+inline int64_t mx_scale_bytes(int64_t rows, int64_t cols) {
+  return mx_pad_rows(rows) * mx_steps(cols) * 4;
+}
+// Whether n bytes at p and m at q (NULL: none) have any in common.
+inline bool mx_overlap(const void* p, int64_t n, const void* q, int64_t m) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return a && b && (a < b ? b - a < (uintptr_t)n : a - b < (uintptr_t)m);
+}
 
 // Lane permutations within 16 lanes.  Once a value is equal over each aligned
 // group of 4 (8) lanes, the half mirror (mirror) brings the other group's.

@@ -652,6 +652,22 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
              PA_ERR_INVALID_ARG, "pa_linear_mx: scales must be 4-byte aligned");
   PA_REQUIRE((uintptr_t)bias % 2 == 0 && (uintptr_t)residual % 16 == 0, PA_ERR_INVALID_ARG,
              "pa_linear_mx: the residual must be 16-byte aligned, the bias to its elements");
+  {
+    const int64_t wrows = silu ? 2 * (int64_t)out_features : out_features;
+    const int64_t kp = mx_steps(in_features) * 128, nb = (int64_t)rows * out_features * 2;
+    const int64_t no = out_scales ? rows * mx_steps(out_features) * 128 : nb;
+    const int64_t ns = out_scales ? mx_scale_bytes(rows, out_features) : 0;
+    auto meets = [&](const void* q, int64_t n) {
+      return mx_overlap(q, n, x, rows * kp) ||
+             mx_overlap(q, n, x_scales, mx_scale_bytes(rows, in_features)) ||
+             mx_overlap(q, n, weight, mx_pad_rows(wrows) * kp) ||
+             mx_overlap(q, n, weight_scales, mx_scale_bytes(wrows, in_features)) ||
+             mx_overlap(q, n, bias, 2 * (int64_t)out_features);
+    };
+    PA_REQUIRE(!meets(out, no) && !meets(out_scales, ns) && !mx_overlap(out, no, out_scales, ns) &&
+                   (residual == out || !mx_overlap(out, no, residual, nb)),
+               PA_ERR_INVALID_ARG, "pa_linear_mx: out overlaps another array");
+  }
   const MxLinear p{out,      out_scales,
                    x,        x_scales,
                    weight,   weight_scales,

@@ -544,13 +544,14 @@ def _mx_call(fn, device, *args):
         _check(fn, rc)
 
 
-def _mx_dev(device, name, t):
-    if t is not None and (t.device != device or not t.is_contiguous()):
-        raise ValueError(f"{name}: expected a contiguous tensor on {device}")
+def _mx_like(t, shape, dtype, device):
+    return (t.shape == shape and t.dtype == dtype and t.device == device and
+            t.is_contiguous())
 
 
-def _at(t):
-    return None if t is None else t.data_ptr()
+def _mx_refuse(name, t, shape, dtype, device):
+    raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on {device}, "
+                     f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 class MxRows:
@@ -568,8 +569,9 @@ class MxRows:
                              f"not MXFP8 rows of {rows} x {cols}")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda:
             raise ValueError("MXFP8 rows are uint8 device tensors")
-        _mx_dev(codes.device, "codes", codes)
-        _mx_dev(codes.device, "scales", scales)
+        if codes.device != scales.device or not (codes.is_contiguous() and
+                                                 scales.is_contiguous()):
+            raise ValueError("codes and scales must be contiguous, on one device")
 
     @classmethod
     def empty(cls, rows, cols, device="cuda"):
@@ -603,8 +605,9 @@ def quantize_mx(x, out=None):
     if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
         raise ValueError("quantize_mx: rows must have unit stride and not overlap")
     code = _dtype_code(x)
-    out = _mx_out(out, rows, cols, x.device)
-    _mx_call("pa_quantize_mx", x.device, out.codes.data_ptr(), out.scales.data_ptr(),
+    device = x.device
+    out = _mx_out(out, rows, cols, device)
+    _mx_call("pa_quantize_mx", device, out.codes.data_ptr(), out.scales.data_ptr(),
              x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, code)
     return out
 
@@ -612,28 +615,27 @@ def quantize_mx(x, out=None):
 def rms_norm_mx(residual, weight, eps, add=None, residual_out=None, out=None):
     """pa_rms_norm_mx: residual + add (when given; into residual_out, by
     default residual itself), then its RMSNorm as MxRows; [rows, hidden]."""
-    if not residual.is_cuda or residual.dim() != 2:
-        raise ValueError("rms_norm_mx: expected a device tensor [rows, hidden]")
-    rows, hidden = residual.shape
-    if weight.shape != (hidden,) or weight.dtype != residual.dtype:
-        raise ValueError("weight must be [hidden] in the residual dtype")
-    for name, t in (("add", add), ("residual_out", residual_out)):
-        if t is not None and (t.shape != residual.shape or t.dtype != residual.dtype):
-            raise ValueError(f"{name} must match residual")
-    if add is None and residual_out is not None:
-        raise ValueError("residual_out holds the sum with add")
-    if add is not None and residual_out is None:
-        residual_out = residual
-    device = residual.device
-    _mx_dev(device, "residual", residual)
-    _mx_dev(device, "weight", weight)
-    _mx_dev(device, "add", add)
-    _mx_dev(device, "residual_out", residual_out)
+    if not residual.is_cuda or residual.dim() != 2 or not residual.is_contiguous():
+        raise ValueError("rms_norm_mx: expected a contiguous device tensor [rows, hidden]")
+    shape, dtype, device = residual.shape, residual.dtype, residual.device
+    rows, hidden = shape
     code = _dtype_code(residual)
+    total = None
+    if not _mx_like(weight, (hidden,), dtype, device):
+        _mx_refuse("weight", weight, (hidden,), dtype, device)
+    if add is not None:
+        if not _mx_like(add, shape, dtype, device):
+            _mx_refuse("add", add, shape, dtype, device)
+        if residual_out is None:
+            residual_out = residual
+        elif not _mx_like(residual_out, shape, dtype, device):
+            _mx_refuse("residual_out", residual_out, shape, dtype, device)
+        add, total = add.data_ptr(), residual_out.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out holds the sum with add")
     out = _mx_out(out, rows, hidden, device)
-    _mx_call("pa_rms_norm_mx", device, out.codes.data_ptr(), out.scales.data_ptr(),
-             _at(residual_out), residual.data_ptr(), _at(add), weight.data_ptr(), rows, hidden,
-             float(eps), code)
+    _mx_call("pa_rms_norm_mx", device, out.codes.data_ptr(), out.scales.data_ptr(), total,
+             residual.data_ptr(), add, weight.data_ptr(), rows, hidden, eps, code)
     return out
 
 
@@ -665,8 +667,9 @@ class MxWeight:
                 codes.shape != (lib.pa_mx_weight_bytes(rows, cols),) or \
                 scales.shape != (lib.pa_mx_scale_bytes(rows, cols),):
             raise ValueError(f"not the packed MXFP8 codes and scales of {rows} x {cols}")
-        _mx_dev(codes.device, "codes", codes)
-        _mx_dev(codes.device, "scales", scales)
+        if codes.device != scales.device or not (codes.is_contiguous() and
+                                                 scales.is_contiguous()):
+            raise ValueError("codes and scales must be contiguous, on one device")
         return self
 
     def nbytes(self):
@@ -680,33 +683,35 @@ def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_ou
     the one rounding; mx_out (with ACT_SILU_MUL): -> MxRows."""
     if not isinstance(x, MxRows) or not isinstance(weight, MxWeight):
         raise ValueError("linear_mx takes MxRows and an MxWeight")
-    silu = act == ACT_SILU_MUL
-    device, rows = x.codes.device, x.rows
-    n = weight.shape[0] // 2 if silu else weight.shape[0]
-    if weight.shape[1] != x.cols or (silu and weight.shape[0] % 2):
-        raise ValueError(f"weight {weight.shape} does not match x {x.rows} x {x.cols}")
-    if mx_out and not silu:
+    device, rows, k = x.codes.device, x.rows, x.cols
+    n, wk = weight.shape
+    if act == ACT_SILU_MUL:
+        n, odd = divmod(n, 2)
+        if odd:
+            raise ValueError(f"weight {weight.shape} is not a gate|up matrix")
+    elif mx_out:
         raise ValueError("an MXFP8 output needs the SwiGLU epilogue")
-    if weight.codes.device != device:
-        raise ValueError(f"weight on {weight.codes.device}, x on {device}")
-    if bias is not None and (bias.shape != (n,) or bias.dtype != torch.bfloat16):
-        raise ValueError(f"bias must be bf16 {(n,)}")
-    if residual is not None and (residual.shape != (rows, n) or
-                                 residual.dtype != torch.bfloat16):
-        raise ValueError(f"residual must be bf16 {(rows, n)}")
+    if wk != k or weight.codes.device != device:
+        raise ValueError(f"weight {weight.shape} on {weight.codes.device} does not match x "
+                         f"{rows} x {k} on {device}")
+    bf16, shape = torch.bfloat16, (rows, n)
+    if bias is not None:
+        if not _mx_like(bias, (n,), bf16, device):
+            _mx_refuse("bias", bias, (n,), bf16, device)
+        bias = bias.data_ptr()
+    if residual is not None:
+        if not _mx_like(residual, shape, bf16, device):
+            _mx_refuse("residual", residual, shape, bf16, device)
+        residual = residual.data_ptr()
     if mx_out:
         out = _mx_out(out, rows, n, device)
-        data, scales = out.codes, out.scales
+        data, scales = out.codes.data_ptr(), out.scales.data_ptr()
     else:
         if out is None:
-            out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
-        elif out.shape != (rows, n) or out.dtype != torch.bfloat16:
-            raise ValueError(f"out must be bf16 {(rows, n)}")
-        data, scales = out, None
-    _mx_dev(device, "bias", bias)
-    _mx_dev(device, "residual", residual)
-    _mx_dev(device, "out", data)
-    _mx_call("pa_linear_mx", device, data.data_ptr(), _at(scales), x.codes.data_ptr(),
-             x.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), _at(bias),
-             _at(residual), rows, n, x.cols, act)
+            out = torch.empty(shape, dtype=bf16, device=device)
+        elif not _mx_like(out, shape, bf16, device):
+            _mx_refuse("out", out, shape, bf16, device)
+        data, scales = out.data_ptr(), None
+    _mx_call("pa_linear_mx", device, data, scales, x.codes.data_ptr(), x.scales.data_ptr(),
+             weight.codes.data_ptr(), weight.scales.data_ptr(), bias, residual, rows, n, k, act)
     return out

@@ -66,6 +66,14 @@ __device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float i
   return (uint32_t)v;
 }
 
+// silu(g) u = g u / (1 + e^-g) by the exponential and reciprocal instructions
+// (a few units of 2^-24, far below the products' own error): a tile's epilogue
+// runs with one or two wavefronts per SIMD, where expf and the division took
+// 9 us of a 256 x 256 tile.
+__device__ inline float mx_silu_mul(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
+}
+
 // Eight consecutive columns per lane, a block over 4 lanes, 128 columns over
 // 16 lanes, which all run this: the largest magnitude of the lane's block, and
 // the four scale bytes of the 128 columns (in every lane) from the lane's own.

@@ -62,9 +62,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   constexpr int RED = BM * BN * 4 * (KG - 1);
   constexpr int SM0 = S * STAGE > BM * ORB ? S * STAGE : BM * ORB;
   constexpr int SM = SM0 > RED ? SM0 : RED;
-  static_assert(SM + 4 * BN <= 160 * 1024, "LDS");
+  static_assert(SM + 4 * BN + 16 <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[SM];
-  __shared__ float sbias[SILU ? 1 : BN];
+  __shared__ __attribute__((aligned(16))) float sbias[SILU ? 4 : BN];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / GW, wt = wave % GW;
@@ -312,8 +312,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
           const bool real = c0 + (wn * TB + b) * 32 < N;  // N is a multiple of 32
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float gate = acc[a][b][i];
-            const float y = gate / (1.0f + expf(-gate)) * acc[a][b + TB][i];
+            const float y = mx_silu_mul(acc[a][b][i], acc[a][b + TB][i]);
             acc[a][b][i] = real ? y : 0.f;
           }
         }
@@ -394,34 +393,44 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
           if (c0 + cc + e < N) dst[e] = src[e];
       }
     }
-    for (int i = threadIdx.x; i < BN; i += NT)
-      sbias[i] = p.bias && c0 + i < N ? bf16_bits_to_f32(p.bias[c0 + i]) : 0.f;
-    __syncthreads();
+    if (p.bias)
+      for (int i = threadIdx.x; i < BN; i += NT)
+        sbias[i] = c0 + i < N ? bf16_bits_to_f32(p.bias[c0 + i]) : 0.f;
+    if (p.bias || p.residual) __syncthreads();
   }
   // ... the results beside them, rounded once ...
   if (KG == 1 || kg == 0) {
     constexpr int TB = SILU ? TN / 2 : TN;
+    auto stage = [&](auto bias, auto residual) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < TM; ++a)
+      for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TB; ++b)
+        for (int b = 0; b < TB; ++b)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int col = (wn * TB + b) * 32 + 8 * q + 4 * g;
-          uint64_t* at = reinterpret_cast<uint64_t*>(lds + arow[a] * ORB + col * 2);
-          const uint64_t prev = !SILU && p.residual ? *at : 0;
-          uint16_t v[4];
+          for (int q = 0; q < 4; ++q) {
+            const int col = (wn * TB + b) * 32 + 8 * q + 4 * g;
+            uint64_t* at = reinterpret_cast<uint64_t*>(lds + arow[a] * ORB + col * 2);
+            f32x4 y = {acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2],
+                       acc[a][b][4 * q + 3]};
+            if constexpr (decltype(bias)::value) y += *reinterpret_cast<const f32x4*>(sbias + col);
+            if constexpr (decltype(residual)::value) {
+              const uint64_t prev = *at;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = acc[a][b][4 * q + e];
-            if constexpr (!SILU) {
-              y += sbias[col + e];
-              y += bf16_bits_to_f32((uint16_t)(prev >> (16 * e)));
+              for (int e = 0; e < 4; ++e)
+                y[e] += bf16_bits_to_f32((uint16_t)(prev >> (16 * e)));
             }
-            v[e] = f32_to_bf16_bits(y);
+            *at = __builtin_bit_cast(uint64_t, __builtin_convertvector(y, bf16x4));
           }
-          *at = *reinterpret_cast<const uint64_t*>(v);
-        }
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    if constexpr (SILU) {
+      stage(no{}, no{});
+    } else if (!p.residual) {
+      p.bias ? stage(yes{}, no{}) : stage(no{}, no{});
+    } else {
+      p.bias ? stage(yes{}, yes{}) : stage(no{}, yes{});
+    }
   }
   __syncthreads();
   // ... and the rows out, 8 columns per thread at a time
@@ -561,7 +570,7 @@ __global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, 
       const f32x4 up = total(NO + quad / 4, row, quad % 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        y[e] = col < N ? y[e] / (1.0f + expf(-y[e])) * up[e] : 0.f;  // N: a multiple of 32
+        y[e] = col < N ? mx_silu_mul(y[e], up[e]) : 0.f;  // N: a multiple of 32
       if (p.out_scales) {
         // a block is eight consecutive threads' columns
         const float four[4] = {y[0], y[1], y[2], y[3]};

@@ -235,17 +235,20 @@ PRODUCTS = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (3, 64, 128), (7, 100, 129), (1
 # ... and those that reach every kernel and tiling; test_mx_tiling.py holds the
 # rule to these names.
 KERNELS = {
-    (16, 1000, 384): "few rows 1/16", (17, 1000, 384): "few rows 1/16",
-    (9, 4130, 200): "few rows 2/4", (32, 17001, 140): "few rows 2/4",
-    (20, 8010, 260): "64x64", (41, 101, 640): "64x64",
+    (16, 1000, 384): "few rows 1/8", (17, 1000, 384): "few rows 1/8",
+    (33, 1000, 1200): "few rows 1/8", (9, 4130, 200): "few rows 2/4",
+    (32, 17001, 140): "few rows 2/4", (50, 32801, 700): "few rows 2/4",
+    (20, 8010, 260): "64x64", (65, 101, 640): "64x64",
     (618, 2056, 1152): "128x128", (5463, 134, 1100): "128x128",
     (5515, 139, 200): "128x128 pair",
     (1430, 4014, 2000): "256x128", (4669, 1668, 2000): "256x256",
 }
 KERNELS_GATED = {
-    (10, 160, 600): "few rows 2/4", (32, 8224, 140): "few rows 2/2",
-    (53, 128, 900): "64x64", (71, 4352, 2000): "128x128", (80, 4416, 200): "128x128 pair",
-    (652, 4128, 2000): "256x128", (658, 5856, 2000): "256x256",
+    (10, 160, 600): "few rows 2/4", (12, 8224, 140): "few rows 2/2",
+    (32, 8224, 140): "few rows 2/2", (26, 96, 700): "few rows 2/2",
+    (20, 96, 4200): "64x64", (53, 128, 900): "64x64", (71, 4352, 2000): "128x128",
+    (80, 4416, 200): "128x128 pair", (652, 4128, 2000): "256x128",
+    (658, 5856, 2000): "256x256",
 }
 
 

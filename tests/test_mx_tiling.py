@@ -33,12 +33,13 @@ def test_kernels_of_the_gpu_tests(choose):
         assert choose(m, n, k, False) == name, (m, n, k)
     for (m, n, k), name in KERNELS_GATED.items():
         assert choose(m, n, k, True) == name, (m, n, k)
-    assert set(KERNELS.values()) == TILED | {"few rows 1/16", "few rows 2/4"}
+    assert set(KERNELS.values()) == TILED | {"few rows 1/8", "few rows 2/4"}
     assert set(KERNELS_GATED.values()) == TILED | {"few rows 2/4", "few rows 2/2"}
-    # one and two tiles of X rows in each kernel for few rows
-    for table in (KERNELS, KERNELS_GATED):
-        rows = [m for (m, _, _), v in table.items() if v.startswith("few")]
-        assert min(rows) <= 16 < max(rows)
+    # one, two and four tiles of X rows (SwiGLU: one and two)
+    assert {(v, (m > 16) + (m > 32)) for (m, _, _), v in KERNELS.items() if "few" in v} == {
+        (f"few rows {k}", t) for k in ("1/8", "2/4") for t in (0, 1, 2)}
+    assert {(v, int(m > 16)) for (m, _, _), v in KERNELS_GATED.items() if "few" in v} == {
+        ("few rows 2/4", 0), ("few rows 2/2", 0), ("few rows 2/2", 1)}
 
 
 def test_largest_sizes(choose):

@@ -42,5 +42,12 @@ __device__ inline void wait_copies() {
   static_assert(N <= 63, "vmcnt range");
   __builtin_amdgcn_s_waitcnt(0x0070 | (N & 0xF) | ((N >> 4) << 14));
 }
+// Waits until at most N of this wavefront's loads and copies are in flight (no
+// wait for its LDS accesses).
+template <int N>
+__device__ inline void wait_vm() {
+  static_assert(N <= 63, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 0xF) | ((N >> 4) << 14));
+}
 
 }  // namespace pa

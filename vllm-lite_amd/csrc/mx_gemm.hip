@@ -468,19 +468,28 @@ int32_t launch(const MxLinear& p, bool silu, hipStream_t stream) {
 // Few rows (decode steps): the weights' bytes bound the call, so they stream
 // from memory straight to registers.  Yᵀ tiles on
 // v_mfma_scale_f32_16x16x128_f8f6f4: A = a fragment of W (16 rows), B = 16 rows
-// of X (from L2); lane (c, j) = (lane % 16, lane / 16) holds columns 16 j .. + 15
-// and 64 + 16 j .. + 15 of row c of both and the scale byte of columns 32 j ..
-// + 31, and of a product Yᵀ[W row 4 j + r][X row c].  A workgroup computes TG NT
-// W tiles x MT X tiles: TG groups of kw wavefronts, which take NT tiles and an
-// equal share of the K steps each, load a step while they multiply the one
-// before, and sum in LDS, from where every thread finishes four columns of one
-// row.  SILU: one group takes two gate tiles, the other their up tiles, so that
-// a workgroup holds whole blocks of 32 output columns.
-template <bool SILU, int MT, int NT, int MAXW>
-__global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, int kw) {
+// of X; lane (c, j) = (lane % 16, lane / 16) holds columns 16 j .. + 15 and
+// 64 + 16 j .. + 15 of row c of both and the scale byte of columns 32 j .. + 31,
+// and of a product Yᵀ[W row 4 j + r][X row c].  A workgroup computes TG NT W
+// tiles x MT X tiles: TG groups of kw wavefronts, which take NT tiles and an
+// equal share of the K steps each and sum in LDS, from where every thread
+// finishes four columns of one row.  SILU: one group takes two gate tiles, the
+// other their up tiles, so that a workgroup holds whole blocks of 32 output
+// columns.  (Up to KW wavefronts a group: short rows have fewer steps.)
+// A wavefront has the step at hand and the next in flight.  X goes through LDS
+// of the wavefront's own, copied in whole 128-byte lines (loaded as the
+// operands need it, half a line per row and load, L2 served it at half its
+// rate, and 32 rows took 4 us longer than 1 at 896 x 4864).
+template <bool SILU, int MT, int NT, int KW>
+__global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), 4) void mx_skinny_kernel(const MxLinear p,
+                                                                               int kw) {
   static_assert(!SILU || NT == 2, "two gate and two up tiles");
   constexpr int TG = SILU ? 2 : 1, TILES = TG * NT, NO = NT;  // NO: output tiles
-  extern __shared__ f32x4 part[];  // [kw][TILES][MT][64]
+  constexpr int XB = MT * 2048;                               // a step's rows of X
+  constexpr int PART = KW * TILES * MT * 1024;
+  constexpr int SM = KW * TG * 2 * XB > PART ? KW * TG * 2 * XB : PART;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[SM];
+  f32x4* part = reinterpret_cast<f32x4*>(lds);  // [kw][TILES][MT][64], behind the products
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, j = lane >> 4;
@@ -488,31 +497,39 @@ __global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, 
   const int tiles_n = (N + 15) / 16;  // of W (of its gate half)
   const int kp = TG == 1 ? wave : wave % kw, tg = TG == 1 ? 0 : wave / kw;
   const int s0 = (int)((int64_t)kp * nk / kw), s1 = (int)((int64_t)(kp + 1) * nk / kw);
-  const uint8_t *wp[NT], *sp[NT], *xp[MT];
+  const uint8_t *wp[NT], *sp[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     // tiles behind the last read it again
-    const int f = min((int)blockIdx.x * NO + (SILU ? 0 : tg * NT) + t, tiles_n - 1) +
-                  (SILU ? tg * tiles_n : 0);
+    const int f = min((int)blockIdx.x * NO + t, tiles_n - 1) + (SILU ? tg * tiles_n : 0);
     wp[t] = p.w + (int64_t)f * nk * 2048 + lane * 16;
     sp[t] = p.ws + (int64_t)f * nk * 64 + c * 4;
   }
-  int xrow[MT];
+  // rows behind the last are the last again; 16-byte chunks swizzled by the row
+  auto swz = [](int r) -> int { return (r / 2) % 8; };
+  uint32_t xo[2 * MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    xrow[t] = min(16 * t + c, M - 1);  // rows behind the last read it again
-    xp[t] = p.x + (int64_t)xrow[t] * nk * 128 + j * 16;
+  for (int u = 0; u < 2 * MT; ++u) {
+    const int r = u * 8 + lane / 8;
+    xo[u] = (uint32_t)min(r, M - 1) * (uint32_t)(nk * 128) + ((lane % 8) ^ swz(r)) * 16;
   }
+  const uint32_t x0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds +
+                      wave * 2 * XB;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int q = 0; q < MT; ++q) acc[t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Stage {
-    i32x4 w[NT][2], x[MT][2];
+    i32x4 w[NT][2];
     int ws[NT], xs[MT];
   };
-  auto load = [&](int s, Stage& o) __attribute__((always_inline)) {
+  constexpr int FETCHED = 2 * MT + 3 * NT + MT;  // copies and loads of a step
+  auto fetch = [&](int s, int buf, Stage& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2 * MT; ++u)
+      lds_copy16(p.x + (int64_t)s * 128, xo[u],
+                 __builtin_amdgcn_readfirstlane(x0 + buf * XB + u * 1024));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const uint8_t* at = wp[t] + (int64_t)s * 2048;
@@ -521,32 +538,66 @@ __global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, 
       o.ws[t] = *reinterpret_cast<const int*>(sp[t] + (int64_t)s * 64);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const uint8_t* at = xp[t] + (int64_t)s * 128;
-      o.x[t][0] = *reinterpret_cast<const i32x4*>(at);
-      o.x[t][1] = *reinterpret_cast<const i32x4*>(at + 64);
-      o.xs[t] = *reinterpret_cast<const int*>(p.xs + ((int64_t)s * p.pad_m + xrow[t]) * 4);
-    }
+    for (int t = 0; t < MT; ++t)
+      o.xs[t] = *reinterpret_cast<const int*>(
+          p.xs + ((int64_t)s * p.pad_m + min(16 * t + c, M - 1)) * 4);
   };
-  auto multiply = [&](const Stage& o) __attribute__((always_inline)) {
+  // newer: the copies and loads issued after the step's own, all of which have
+  // to be in flight still or done
+  auto multiply = [&](int buf, const Stage& o, auto newer) __attribute__((always_inline)) {
+    wait_vm<decltype(newer)::value>();
+    asm volatile("" ::: "memory");
+    // The scales are used behind the wait only: the compiler moved their
+    // shifts to the loop's head, and waited there for the loads.
+    int ws[NT], xs[MT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      ws[t] = o.ws[t];
+      asm volatile("" : "+v"(ws[t]));
+    }
 #pragma unroll
-      for (int q = 0; q < MT; ++q)
+    for (int q = 0; q < MT; ++q) {
+      xs[q] = o.xs[q];
+      asm volatile("" : "+v"(xs[q]));
+    }
+#pragma unroll
+    for (int q = 0; q < MT; ++q) {
+      const uint8_t* row = lds + wave * 2 * XB + buf * XB + (16 * q + c) * 128;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(row + (j ^ swz(16 * q + c)) * 16);
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(row + ((4 + j) ^ swz(16 * q + c)) * 16);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
         acc[t][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
             __builtin_shufflevector(o.w[t][0], o.w[t][1], 0, 1, 2, 3, 4, 5, 6, 7),
-            __builtin_shufflevector(o.x[q][0], o.x[q][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[t][q], 0,
-            0, 0, o.ws[t] >> (8 * j), 0, o.xs[q] >> (8 * j));
+            __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), acc[t][q], 0, 0, 0,
+            ws[t] >> (8 * j), 0, xs[q] >> (8 * j));
+    }
+    wait_copies<63>();  // the reads are done before the buffer is copied into again
+    asm volatile("" ::: "memory");
   };
+  // No load under a branch that ends before its step is multiplied: the
+  // compiler would wait for all loads in front of every product.
+  using Next = std::integral_constant<int, FETCHED>;
+  using None = std::integral_constant<int, 0>;
   Stage a, b;
-  if (s0 < s1) load(s0, a);
-  for (int s = s0; s < s1; s += 2) {
-    if (s + 1 < s1) load(s + 1, b);
-    multiply(a);
-    if (s + 1 >= s1) break;
-    if (s + 2 < s1) load(s + 2, a);
-    multiply(b);
+  if (s0 < s1) {
+    fetch(s0, 0, a);
+    int s = s0;
+    for (; s + 2 < s1; s += 2) {
+      fetch(s + 1, 1, b);
+      multiply(0, a, Next{});
+      fetch(s + 2, 0, a);
+      multiply(1, b, Next{});
+    }
+    if (s + 1 < s1) {
+      fetch(s + 1, 1, b);
+      multiply(0, a, Next{});
+      multiply(1, b, None{});
+    } else {
+      multiply(0, a, None{});
+    }
   }
+  __syncthreads();  // everyone is done with X
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -613,15 +664,13 @@ __global__ __launch_bounds__(64 * MAXW) void mx_skinny_kernel(const MxLinear p, 
   }
 }
 
-template <bool SILU, int MT, int NT, int MAXW>
-int32_t launch_skinny(const MxLinear& p, int kw, hipStream_t stream) {
-  constexpr int TG = SILU ? 2 : 1;
-  kw = std::min(kw, p.steps);
+template <bool SILU, int MT, int NT, int KW>
+int32_t launch_skinny(const MxLinear& p, hipStream_t stream) {
+  const int kw = std::min(KW, p.steps);
   // an MXFP8 output's padding is written too
   const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
   const dim3 grid((uint32_t)((cols + 16 * NT - 1) / (16 * NT)));
-  const size_t lds = (size_t)kw * TG * NT * MT * 64 * sizeof(f32x4);
-  mx_skinny_kernel<SILU, MT, NT, MAXW><<<grid, 64 * TG * kw, lds, stream>>>(p, kw);
+  mx_skinny_kernel<SILU, MT, NT, KW><<<grid, 64 * (SILU ? 2 : 1) * kw, 0, stream>>>(p, kw);
   return check_launch("pa_linear_mx");
 }
 
@@ -684,15 +733,19 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
                    rows,     out_features,
                    (int)mx_steps(in_features), mx_pad_rows(rows)};
   hipStream_t s = (hipStream_t)stream;
-  if (const MxSkinny k = choose_mx_skinny(rows, out_features, silu); k.kw) {
-    const bool one = rows <= 16;  // one tile of X rows
-    if (silu)
-      return one ? launch_skinny<true, 1, 2, 8>(p, k.kw, s) : launch_skinny<true, 2, 2, 8>(p, k.kw, s);
+  if (const MxSkinny k = choose_mx_skinny(rows, out_features, in_features, silu); k.kw) {
+    const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;  // of X rows
+    if (silu)  // four share K up to 16 rows only
+      return k.kw == 4    ? launch_skinny<true, 1, 2, 4>(p, s)
+             : tiles == 1 ? launch_skinny<true, 1, 2, 2>(p, s)
+                          : launch_skinny<true, 2, 2, 2>(p, s);
     if (k.nt == 2)
-      return one ? launch_skinny<false, 1, 2, 8>(p, k.kw, s)
-                 : launch_skinny<false, 2, 2, 8>(p, k.kw, s);
-    return one ? launch_skinny<false, 1, 1, 16>(p, k.kw, s)
-               : launch_skinny<false, 2, 1, 16>(p, k.kw, s);
+      return tiles == 1   ? launch_skinny<false, 1, 2, 4>(p, s)
+             : tiles == 2 ? launch_skinny<false, 2, 2, 4>(p, s)
+                          : launch_skinny<false, 4, 2, 4>(p, s);
+    return tiles == 1   ? launch_skinny<false, 1, 1, 8>(p, s)
+           : tiles == 2 ? launch_skinny<false, 2, 1, 8>(p, s)
+                        : launch_skinny<false, 4, 1, 8>(p, s);
   }
   switch (choose_mx_tiling(rows, (int64_t)out_features * (silu ? 2 : 1), in_features)) {
     case kMx256x256: return launch<2, 2, 4, 4, 1, 2>(p, silu, s);

@@ -10,14 +10,14 @@ namespace pa {
 // `ns_per_k` for every column of K, the last one `tail` of a round and the rest
 // by how full it is.  Fitted to each tiling's times over 127 shapes (M 40 to
 // 7569, wrows 896 to 24576, K 160 to 12288; rms error 7 to 9%), over which the
-// smallest estimate is the fastest tiling or within 4.6% of it, 0.2% on
+// smallest estimate is the fastest tiling or within 7.5% of it, 0.2% on
 // average.  Measured, us (M x wrows x K):
-//                     333 x 896 x 4864  618 x 6144 x 4096  2048 x 4096 x 4096  7569 x 4096 x 4096
-//   256 x 256               51.8              46.5               48.6                116.8
-//   256 x 128               30.0              28.1               34.7                131.7
-//   128 x 128, pairs        28.2              25.5               36.8                133.3
-//   128 x 128               20.4              21.4               42.7                163.6
-//    64 x  64               12.2              38.3               76.2                270.7
+//                     256 x 4096 x 4096  618 x 6144 x 4096  2048 x 4096 x 4096  7569 x 4096 x 4096
+//   256 x 256               41.9              43.0               45.0                109.0
+//   256 x 128               25.8              27.5               33.9                125.7
+//   128 x 128, pairs        23.8              24.7               35.0                127.4
+//   128 x 128               17.9              19.8               37.8                152.8
+//    64 x  64               11.3              36.0               68.7                255.8
 enum MxTiling { kMx256x256, kMx256x128, kMx128x128Pair, kMx128x128, kMx64x64 };
 inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K) {
   struct Cost {
@@ -47,29 +47,39 @@ inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K) {
 }
 
 // The kernel for few rows: W tiles per wavefront and wavefronts that share K
-// (kw 0: the tiled kernel instead).  Measured at 32 rows, us:
-//   N x K                4096 x 12288  4096 x 4096  896 x 4864  1152 x 896
-//   1 tile, 16 wavefronts    16.4          7.9          8.5        3.8
-//   2 tiles, 4               17.9          9.0         10.3        3.8
-//   64 x 64 tiling           21.7         10.6         10.7        5.6
-//                        6144 x 4096  12288 x 4096  24576 x 4096  151936 x 896
-//   1 tile, 16 wavefronts    13.2         19.4         37.4         61.2
-//   2 tiles, 4                9.7         15.4         23.0         32.5
-//   64 x 64 tiling           10.5         12.5         26.3         56.9
-// (one tile reads X from L2 twice as often and fills the chip sooner; the 64 x
-// 64 tiling wins where its tiles fill one round of the CUs.)  SwiGLU, where a
-// workgroup is two groups of kw wavefronts: kw 4 / 2 / the tiling at 4864 x
-// 896 6.1 / 6.2 / 6.4, at 12288 x 4096 28.2 / 27.1 / 27.6.  Above 32 rows the
-// 64 x 64 tiling is faster (64 rows: 4096 x 12288 21.9 against 28.5).
+// (kw 0: the tiled kernel instead).  Measured, us (rows: N x K):
+//                      32: 896 x 4864  4096 x 4096  4096 x 12288  6144 x 4096
+//   1 tile, 8 wavefronts       6.7         6.7          17.0         10.1
+//   2 tiles, 4                 8.6         7.7          19.6          8.6
+//   64 x 64 tiling            10.5        10.2          21.3         10.2
+//                      32: 8192 x 8192  12288 x 4096  24576 x 4096  151936 x 896
+//   1 tile, 8 wavefronts      19.9          16.8          29.1          59.9
+//   2 tiles, 4                16.9          13.8          21.5          30.8
+//   64 x 64 tiling            16.3          12.2          25.4          52.8
+//                      64: 896 x 4864  4096 x 4096  24576 x 4096  151936 x 896
+//   1 tile, 8 wavefronts       8.7         8.8          45.5         117.1
+//   2 tiles, 4                11.1         9.9          30.7          46.5
+//   64 x 64 tiling            10.6        10.6          28.6          57.2
+// (one tile copies X twice as often and fills the chip sooner; the 64 x 64
+// tiling wins where its tiles fill one round of the CUs.)  SwiGLU, where a
+// workgroup is two groups of kw wavefronts:
+//                   16: 4864 x 896  2048 x 8192  12288 x 4096   32: 4864 x 896  2048 x 8192  12288 x 4096
+//   kw 4                   5.0         16.5          22.2             5.5          20.6          24.9
+//   kw 2                   5.0         18.4          20.5             5.4          21.0          23.4
+//   64 x 64 tiling         5.8         15.9          25.4             5.9          15.8          26.3
 struct MxSkinny {
   int nt, kw;
 };
-inline MxSkinny choose_mx_skinny(int M, int N, bool silu) {
-  if (M > 32) return {0, 0};
-  if (silu) return {2, N <= 8192 ? 4 : 2};
-  if (N <= 4096) return {1, 16};
-  if (N > 7168 && N <= 64 * 256) return {0, 0};
-  return {2, 4};
+inline MxSkinny choose_mx_skinny(int M, int N, int K, bool silu) {
+  constexpr MxSkinny tiled = {0, 0};
+  if (M > (silu ? 32 : 64)) return tiled;
+  if (silu) {
+    if (M > 16 && N <= 8192 && K >= 4096) return tiled;
+    return M <= 16 && N <= 8192 ? MxSkinny{2, 4} : MxSkinny{2, 2};
+  }
+  if (N <= 4096) return {1, 8};
+  if (N > 64 * 512 || (M <= 32 && (N <= 7168 || N > 64 * 256))) return {2, 4};
+  return tiled;
 }
 
 }  // namespace pa

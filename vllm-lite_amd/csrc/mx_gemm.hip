@@ -301,6 +301,30 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     }
     __syncthreads();
   }
+  // 16 bytes of every rs-th row of a staged tile out, `items` of them.  All of a
+  // tile inside the output in batches of LDS reads: under a branch the
+  // compiler reads and stores one by one (43.2 us for 41.6 at 618 x 6144 x 4096
+  // in 256 x 256 tiles).
+  auto rows_out = [&](uint8_t* dst, int64_t dst_step, const uint8_t* src, auto src_step, auto items,
+                      auto rs, int r0) __attribute__((always_inline)) {
+    constexpr int IT = decltype(items)::value, BATCH = IT % 8 == 0 ? 8 : IT;
+    constexpr int SRC = decltype(src_step)::value, R = decltype(rs)::value;
+    if (m0 + BM <= M) {
+#pragma unroll
+      for (int i = 0; i < IT; i += BATCH) {
+        i32x4 v[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          v[u] = *reinterpret_cast<const i32x4*>(src + (i + u) * SRC);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u, dst += dst_step) *reinterpret_cast<i32x4*>(dst) = v[u];
+      }
+    } else {
+      for (int r = r0; r < M - m0; r += R, dst += dst_step, src += SRC)
+        *reinterpret_cast<i32x4*>(dst) = *reinterpret_cast<const i32x4*>(src);
+    }
+  };
   if constexpr (SILU) {
     constexpr int TB = TN / 2;
     // silu(g) u, 0 in the columns behind the last (an MXFP8 output's padding)
@@ -343,49 +367,52 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
       }
       __syncthreads();
       const int pitch = (N + 127) / 128 * 128;
-      uint8_t* out = static_cast<uint8_t*>(p.out);
-      for (int i = threadIdx.x; i < BM * (BNO / 16); i += NT) {
-        const int r = i / (BNO / 16), cc = i % (BNO / 16) * 16;
-        if (m0 + r < M && c0 + cc < pitch)
-          *reinterpret_cast<uint4*>(out + (int64_t)(m0 + r) * pitch + c0 + cc) =
-              *reinterpret_cast<const uint4*>(lds + r * CRB + cc);
-      }
-      for (int i = threadIdx.x; i < BM * NBLK; i += NT) {
-        const int r = i % BM, blk = i / BM, at = c0 / 32 + blk;
-        if (m0 + r < M && at * 32 < pitch)
-          p.out_scales[((at / 4) * p.pad_m + m0 + r) * 4 + at % 4] =
-              lds[BM * CRB + r * NBLK + blk];
-      }
+      constexpr int CPR = BNO / 16, RS = NT / CPR;  // threads of a row, rows per pass
+      constexpr int ITEMS = BM > RS ? BM / RS : 1;
+      static_assert(RS * CPR == NT && BM % std::min(BM, RS) == 0, "whole passes");
+      const int r0 = threadIdx.x / CPR, cc = threadIdx.x % CPR * 16;
+      if (c0 + cc < pitch && r0 < BM)
+        rows_out(static_cast<uint8_t*>(p.out) + (int64_t)(m0 + r0) * pitch + c0 + cc,
+                 (int64_t)RS * pitch, lds + r0 * CRB + cc, std::integral_constant<int, RS * CRB>{},
+                 std::integral_constant<int, ITEMS>{}, std::integral_constant<int, RS>{}, r0);
+      // the blocks of one scale column at once
+      using Bytes = std::conditional_t<NBLK == 4, uint32_t,
+                                       std::conditional_t<NBLK == 2, uint16_t, uint8_t>>;
+      static_assert(sizeof(Bytes) == NBLK, "scale bytes of a tile's row");
+      if (c0 < pitch)
+        for (int r = threadIdx.x; r < min(BM, M - m0); r += NT)
+          *reinterpret_cast<Bytes*>(p.out_scales + ((c0 / 128) * p.pad_m + m0 + r) * 4 +
+                                    c0 / 32 % 4) =
+              *reinterpret_cast<const Bytes*>(lds + BM * CRB + r * NBLK);
       return;
     }
   }
   // bf16 output.  The residual rows and the bias into LDS ...
   uint16_t* out = static_cast<uint16_t*>(p.out);
-  constexpr int CPRO = BNO / 8;
+  // 8 columns a thread at a time, which stay, and RS rows a pass
+  constexpr int CPRO = BNO / 8, RS = NT / CPRO, ITEMS = BM > RS ? BM / RS : 1;
+  static_assert(RS * CPRO == NT && BM % std::min(BM, RS) == 0 && (SILU || RS <= BM),
+                "whole passes");
+  const int r0 = threadIdx.x / CPRO, cc = threadIdx.x % CPRO * 8;
   if constexpr (!SILU) {
     if (p.residual && N % 8 == 0) {
       // several loads in flight per thread (one at a time took 17 us of a
       // 256 x 256 tile); those outside the output read its last row or piece
-      constexpr int ITEMS = BM * CPRO / NT, BATCH = ITEMS % 16 == 0 ? 16 : ITEMS % 8 == 0 ? 8 : 1;
-      static_assert(ITEMS * NT == BM * CPRO, "whole batches");
-      for (int i0 = 0; i0 < ITEMS; i0 += BATCH) {
+      constexpr int BATCH = ITEMS % 16 == 0 ? 16 : ITEMS;
+      const uint16_t* src = p.residual + min(c0 + cc, N - 8);
+#pragma unroll
+      for (int i = 0; i < ITEMS; i += BATCH) {
         uint4 v[BATCH];
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-          const int i = (i0 + u) * NT + threadIdx.x, r = i / CPRO, cc = i % CPRO * 8;
+        for (int u = 0; u < BATCH; ++u)
           v[u] = *reinterpret_cast<const uint4*>(
-              p.residual + (int64_t)min(m0 + r, M - 1) * N + min(c0 + cc, N - 8));
-        }
+              src + (int64_t)min(m0 + r0 + (i + u) * RS, M - 1) * N);
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-          const int i = (i0 + u) * NT + threadIdx.x;
-          *reinterpret_cast<uint4*>(lds + i / CPRO * ORB + i % CPRO * 16) = v[u];
-        }
+        for (int u = 0; u < BATCH; ++u)
+          *reinterpret_cast<uint4*>(lds + (r0 + (i + u) * RS) * ORB + cc * 2) = v[u];
       }
     } else if (p.residual) {
-      for (int i = threadIdx.x; i < BM * CPRO; i += NT) {
-        const int r = i / CPRO, cc = i % CPRO * 8;
-        if (m0 + r >= M) continue;
+      for (int r = r0; r < min(BM, M - m0); r += RS) {
         const uint16_t* src = p.residual + (int64_t)(m0 + r) * N + c0 + cc;
         uint16_t* dst = reinterpret_cast<uint16_t*>(lds + r * ORB + cc * 2);
 #pragma unroll
@@ -403,24 +430,40 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     constexpr int TB = SILU ? TN / 2 : TN;
     auto stage = [&](auto bias, auto residual) __attribute__((always_inline)) {
 #pragma unroll
-      for (int a = 0; a < TM; ++a)
+      for (int b = 0; b < TB; ++b) {
+        const int col = (wn * TB + b) * 32 + 4 * g;
+        f32x4 add[4];
+        if constexpr (decltype(bias)::value)
 #pragma unroll
-        for (int b = 0; b < TB; ++b)
+          for (int q = 0; q < 4; ++q) add[q] = *reinterpret_cast<const f32x4*>(sbias + col + 8 * q);
+        // the LDS reads of two tiles, then their results (with a wait for each
+        // read a 256 x 256 tile took 1 us longer)
+        constexpr int AB = TM < 2 ? 1 : 2;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int col = (wn * TB + b) * 32 + 8 * q + 4 * g;
-            uint64_t* at = reinterpret_cast<uint64_t*>(lds + arow[a] * ORB + col * 2);
+        for (int a0 = 0; a0 < TM; a0 += AB) {
+          uint64_t prev[AB][4];
+          if constexpr (decltype(residual)::value) {
+#pragma unroll
+            for (int u = 0; u < AB * 4; ++u)
+              prev[u / 4][u % 4] = *reinterpret_cast<const uint64_t*>(
+                  lds + arow[a0 + u / 4] * ORB + (col + 8 * (u % 4)) * 2);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int u = 0; u < AB * 4; ++u) {
+            const int a = a0 + u / 4, q = u % 4;
             f32x4 y = {acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2],
                        acc[a][b][4 * q + 3]};
-            if constexpr (decltype(bias)::value) y += *reinterpret_cast<const f32x4*>(sbias + col);
-            if constexpr (decltype(residual)::value) {
-              const uint64_t prev = *at;
+            if constexpr (decltype(bias)::value) y += add[q];
+            if constexpr (decltype(residual)::value)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                y[e] += bf16_bits_to_f32((uint16_t)(prev >> (16 * e)));
-            }
-            *at = __builtin_bit_cast(uint64_t, __builtin_convertvector(y, bf16x4));
+                y[e] += bf16_bits_to_f32((uint16_t)(prev[u / 4][q] >> (16 * e)));
+            *reinterpret_cast<uint64_t*>(lds + arow[a] * ORB + (col + 8 * q) * 2) =
+                __builtin_bit_cast(uint64_t, __builtin_convertvector(y, bf16x4));
           }
+        }
+      }
     };
     using yes = std::true_type;
     using no = std::false_type;
@@ -433,18 +476,17 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     }
   }
   __syncthreads();
-  // ... and the rows out, 8 columns per thread at a time
-  for (int i = threadIdx.x; i < BM * CPRO; i += NT) {
-    const int r = i / CPRO, cc = i % CPRO * 8;
-    const int row = m0 + r, col = c0 + cc;
-    if (row >= M || col >= N) continue;
-    const uint8_t* src = lds + r * ORB + cc * 2;
-    uint16_t* dst = out + (int64_t)row * N + col;
-    if (N % 8 == 0)
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-    else
-      for (int e = 0; e < 8 && col + e < N; ++e)
-        dst[e] = reinterpret_cast<const uint16_t*>(src)[e];
+  // ... and the rows out
+  if (c0 + cc >= N || r0 >= BM) return;
+  uint16_t* dst = out + (int64_t)(m0 + r0) * N + c0 + cc;
+  if (N % 8 == 0) {
+    rows_out(reinterpret_cast<uint8_t*>(dst), (int64_t)RS * N * 2, lds + r0 * ORB + cc * 2,
+             std::integral_constant<int, RS * ORB>{}, std::integral_constant<int, ITEMS>{},
+             std::integral_constant<int, RS>{}, r0);
+  } else {
+    for (int r = r0; r < min(BM, M - m0); r += RS, dst += (int64_t)RS * N)
+      for (int e = 0; e < 8 && c0 + cc + e < N; ++e)
+        dst[e] = reinterpret_cast<const uint16_t*>(lds + r * ORB + cc * 2)[e];
   }
 }
 
@@ -481,8 +523,8 @@ int32_t launch(const MxLinear& p, bool silu, hipStream_t stream) {
 // operands need it, half a line per row and load, L2 served it at half its
 // rate, and 32 rows took 4 us longer than 1 at 896 x 4864).
 template <bool SILU, int MT, int NT, int KW>
-__global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), 4) void mx_skinny_kernel(const MxLinear p,
-                                                                               int kw) {
+__global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_skinny_kernel(
+    const MxLinear p, int kw) {
   static_assert(!SILU || NT == 2, "two gate and two up tiles");
   constexpr int TG = SILU ? 2 : 1, TILES = TG * NT, NO = NT;  // NO: output tiles
   constexpr int XB = MT * 2048;                               // a step's rows of X

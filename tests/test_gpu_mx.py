@@ -238,7 +238,8 @@ KERNELS = {
     (16, 1000, 384): "few rows 1/8", (17, 1000, 384): "few rows 1/8",
     (33, 1000, 1200): "few rows 1/8", (9, 4130, 200): "few rows 2/4",
     (32, 17001, 140): "few rows 2/4", (50, 32801, 700): "few rows 2/4",
-    (20, 8010, 260): "64x64", (65, 101, 640): "64x64",
+    (20, 8010, 260): "64x32", (65, 101, 640): "64x32", (37, 70, 5000): "64x32",
+    (600, 900, 700): "64x64", (130, 5204, 300): "64x64",
     (618, 2056, 1152): "128x128", (5463, 134, 1100): "128x128",
     (5515, 139, 200): "128x128 pair",
     (1430, 4014, 2000): "256x128", (4669, 1668, 2000): "256x256",

@@ -33,7 +33,7 @@ def test_kernels_of_the_gpu_tests(choose):
         assert choose(m, n, k, False) == name, (m, n, k)
     for (m, n, k), name in KERNELS_GATED.items():
         assert choose(m, n, k, True) == name, (m, n, k)
-    assert set(KERNELS.values()) == TILED | {"few rows 1/8", "few rows 2/4"}
+    assert set(KERNELS.values()) == TILED | {"64x32", "few rows 1/8", "few rows 2/4"}
     assert set(KERNELS_GATED.values()) == TILED | {"few rows 2/4", "few rows 2/2"}
     # one, two and four tiles of X rows (SwiGLU: one and two)
     assert {(v, (m > 16) + (m > 32)) for (m, _, _), v in KERNELS.items() if "few" in v} == {
@@ -44,5 +44,5 @@ def test_kernels_of_the_gpu_tests(choose):
 
 def test_largest_sizes(choose):
     """Sizes whose products pass 32 bits."""
-    assert choose(2 ** 31 - 1, 2 ** 24, 4096, False) in TILED
+    assert choose(2 ** 31 - 1, 2 ** 24, 4096, False) in TILED | {"64x32"}
     assert choose(2 ** 31 - 1, 2 ** 24, 2 ** 22, True) in TILED

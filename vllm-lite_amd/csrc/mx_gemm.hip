@@ -51,12 +51,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   constexpr int GW = WM * WN, NT = 64 * GW * KG;
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, BNO = SILU ? BN / 2 : BN;
   constexpr int CA = BM / 8 / GW, CB = BN / 8 / GW;         // 1 KB copies per wavefront
-  constexpr int SC = (BM + BN) / 64, CS = (SC + GW - 1) / GW;  // 256 B copies of scales
+  constexpr int BS = (BN + 63) / 64 * 64;                 // scales of W: 64 rows a copy
+  constexpr int SC = (BM + BS) / 64, CS = (SC + GW - 1) / GW;  // 256 B copies of scales
   constexpr int PER = CA + CB + CS;
-  static_assert(CA * GW * 8 == BM && CB * GW * 8 == BN && BM % 64 == 0 && BN % 64 == 0 &&
-                    (!SILU || (TN % 2 == 0 && (BN / 2) % 16 == 0)),
+  static_assert(CA * GW * 8 == BM && CB * GW * 8 == BN && BM % 64 == 0 && (!SILU || (TN % 2 == 0 && BN % 64 == 0)),
                 "tiles");
-  constexpr int STEP = (BM + BN) * 132, STAGE = KG * STEP;  // codes, then scale dwords
+  constexpr int STEP = (BM + BN) * 128 + (BM + BS) * 4, STAGE = KG * STEP;  // codes, then scale dwords
   constexpr int SX = (BM + BN) * 128, SW = SX + BM * 4;
   constexpr int ORB = BNO * 2 + 16;  // bytes per row of the staged output tile
   constexpr int RED = BM * BN * 4 * (KG - 1);
@@ -391,8 +391,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   uint16_t* out = static_cast<uint16_t*>(p.out);
   // 8 columns a thread at a time, which stay, and RS rows a pass
   constexpr int CPRO = BNO / 8, RS = NT / CPRO, ITEMS = BM > RS ? BM / RS : 1;
-  static_assert(RS * CPRO == NT && BM % std::min(BM, RS) == 0 && (SILU || RS <= BM),
-                "whole passes");
+  static_assert(RS * CPRO == NT && BM % std::min(BM, RS) == 0, "whole passes");
   const int r0 = threadIdx.x / CPRO, cc = threadIdx.x % CPRO * 8;
   if constexpr (!SILU) {
     if (p.residual && N % 8 == 0) {
@@ -409,7 +408,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
               src + (int64_t)min(m0 + r0 + (i + u) * RS, M - 1) * N);
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
-          *reinterpret_cast<uint4*>(lds + (r0 + (i + u) * RS) * ORB + cc * 2) = v[u];
+          if (RS <= BM || r0 < BM)
+            *reinterpret_cast<uint4*>(lds + (r0 + (i + u) * RS) * ORB + cc * 2) = v[u];
       }
     } else if (p.residual) {
       for (int r = r0; r < min(BM, M - m0); r += RS) {
@@ -490,20 +490,17 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   }
 }
 
-template <int WM, int WN, int TM, int TN, int KG, int S>
-int32_t launch(const MxLinear& p, bool silu, hipStream_t stream) {
+template <bool SILU, int WM, int WN, int TM, int TN, int KG, int S>
+int32_t launch(const MxLinear& p, hipStream_t stream) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NT = 64 * WM * WN * KG;
-  const int bno = silu ? BN / 2 : BN;
+  constexpr int BNO = SILU ? BN / 2 : BN;
   // an MXFP8 output's padding is written too
   const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
-  const int64_t ntm = ((int64_t)p.M + BM - 1) / BM, ntn = (cols + bno - 1) / bno;
+  const int64_t ntm = ((int64_t)p.M + BM - 1) / BM, ntn = (cols + BNO - 1) / BNO;
   PA_REQUIRE(ntm * ntn < (1ll << 30), PA_ERR_UNSUPPORTED, "pa_linear_mx: %d x %d outputs", p.M,
              p.N);
   const dim3 grid(8 * (uint32_t)((ntm * ntn + 7) / 8));
-  if (silu)
-    mx_gemm_kernel<true, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
-  else
-    mx_gemm_kernel<false, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
+  mx_gemm_kernel<SILU, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
   return check_launch("pa_linear_mx");
 }
 
@@ -789,11 +786,19 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
            : tiles == 2 ? launch_skinny<false, 2, 1, 8>(p, s)
                         : launch_skinny<false, 4, 1, 8>(p, s);
   }
-  switch (choose_mx_tiling(rows, (int64_t)out_features * (silu ? 2 : 1), in_features)) {
-    case kMx256x256: return launch<2, 2, 4, 4, 1, 2>(p, silu, s);
-    case kMx256x128: return launch<4, 2, 2, 2, 1, 3>(p, silu, s);
-    case kMx128x128Pair: return launch<2, 2, 2, 2, 1, 2>(p, silu, s);
-    case kMx128x128: return launch<2, 2, 2, 2, 1, 4>(p, silu, s);
-    default: return launch<2, 1, 1, 2, 2, 4>(p, silu, s);
+  if (silu) switch (choose_mx_tiling(rows, 2 * (int64_t)out_features, in_features, true)) {
+      case kMx256x256: return launch<true, 2, 2, 4, 4, 1, 2>(p, s);
+      case kMx256x128: return launch<true, 4, 2, 2, 2, 1, 3>(p, s);
+      case kMx128x128Pair: return launch<true, 2, 2, 2, 2, 1, 2>(p, s);
+      case kMx128x128: return launch<true, 4, 2, 1, 2, 1, 3>(p, s);
+      default: return launch<true, 2, 1, 1, 2, 2, 4>(p, s);
+    }
+  switch (choose_mx_tiling(rows, out_features, in_features, false)) {
+    case kMx256x256: return launch<false, 2, 2, 4, 4, 1, 2>(p, s);
+    case kMx256x128: return launch<false, 4, 2, 2, 2, 1, 3>(p, s);
+    case kMx128x128Pair: return launch<false, 2, 2, 2, 2, 1, 2>(p, s);
+    case kMx128x128: return launch<false, 4, 2, 1, 2, 1, 3>(p, s);
+    case kMx64x64: return launch<false, 2, 2, 1, 1, 2, 4>(p, s);
+    default: return launch<false, 2, 1, 1, 1, 2, 4>(p, s);
   }
 }

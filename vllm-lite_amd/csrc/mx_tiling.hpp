@@ -8,31 +8,36 @@ namespace pa {
 // The tilings, and the time each would take: rounds of workgroups over the
 // 256 CUs (two a CU for the pairs of 128 x 128 tiles), each round `us` plus
 // `ns_per_k` for every column of K, the last one `tail` of a round and the rest
-// by how full it is.  Fitted to each tiling's times over 127 shapes (M 40 to
-// 7569, wrows 896 to 24576, K 160 to 12288; rms error 7 to 9%), over which the
-// smallest estimate is the fastest tiling or within 7.5% of it, 0.2% on
-// average.  Measured, us (M x wrows x K):
-//                     256 x 4096 x 4096  618 x 6144 x 4096  2048 x 4096 x 4096  7569 x 4096 x 4096
-//   256 x 256               41.9              43.0               45.0                109.0
-//   256 x 128               25.8              27.5               33.9                125.7
-//   128 x 128, pairs        23.8              24.7               35.0                127.4
-//   128 x 128               17.9              19.8               37.8                152.8
-//    64 x  64               11.3              36.0               68.7                255.8
-enum MxTiling { kMx256x256, kMx256x128, kMx128x128Pair, kMx128x128, kMx64x64 };
-inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K) {
+// by how full it is.  Fitted to each tiling's times over 197 shapes (M 40 to
+// 7569, wrows 896 to 24576, K 160 to 12288; where it is within half as much
+// again of the fastest, rms error 4 to 12%), over which the smallest estimate is
+// the fastest tiling or within 9% of it, 0.2% on average.  Measured, us (M x
+// wrows x K):
+//                         333 x 896 x 4864    256 x 4096 x 4096    618 x 6144 x 4096   2048 x 4096 x 4096   7569 x 4096 x 4096
+//   256 x 256                         47.0                 40.1                 41.5                 44.0                111.1
+//   256 x 128                         29.0                 25.3                 27.2                 33.8                127.5
+//   128 x 128, pairs                  26.7                 23.2                 24.3                 34.4                128.6
+//   128 x 128                         19.3                 17.2                 20.0                 38.4                148.6
+//    64 x  64                         11.3                 10.9                 33.8                 64.0                240.3
+//    64 x  32                          9.7                 15.4                 52.7                103.4                384.2
+// (64 x 32 tiles of SwiGLU would hold half a block of 32 output columns.)
+enum MxTiling { kMx256x256, kMx256x128, kMx128x128Pair, kMx128x128, kMx64x64, kMx64x32 };
+inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K, bool silu) {
   struct Cost {
     MxTiling t;
     int bm, bn, slots;
     double base, us, ns_per_k, tail;
   };
-  static constexpr Cost costs[] = {{kMx256x256, 256, 256, 256, 3.7, 11.1, 11.3, .70},
-                                   {kMx256x128, 256, 128, 256, 1.75, 5.5, 6.87, .68},
-                                   {kMx128x128Pair, 128, 128, 512, 2.0, 4.5, 7.62, .54},
-                                   {kMx128x128, 128, 128, 256, 2.3, 4.1, 4.03, .71},
-                                   {kMx64x64, 64, 64, 256, 1.8, 3.0, 1.65, .85}};
+  static constexpr Cost costs[] = {{kMx256x256, 256, 256, 256, 3.0, 7.3, 11.7, .63},
+                                   {kMx256x128, 256, 128, 256, 1.1, 4.5, 6.99, .64},
+                                   {kMx128x128Pair, 128, 128, 512, 1.8, 3.2, 7.77, .46},
+                                   {kMx128x128, 128, 128, 256, 2.0, 2.5, 4.14, .64},
+                                   {kMx64x64, 64, 64, 256, 1.3, 2.4, 1.66, .86},
+                                   {kMx64x32, 64, 32, 256, 1.6, 1.7, 1.25, .91}};
   MxTiling best = kMx64x64;
   double best_us = 1e300;
   for (const Cost& c : costs) {
+    if (silu && c.t == kMx64x32) continue;
     const int64_t tiles = ((M + (int64_t)c.bm - 1) / c.bm) * ((wrows + c.bn - 1) / c.bn);
     const int64_t rest = tiles % c.slots;
     const double rounds =
@@ -48,21 +53,19 @@ inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K) {
 
 // The kernel for few rows: W tiles per wavefront and wavefronts that share K
 // (kw 0: the tiled kernel instead).  Measured, us (rows: N x K):
-//                      32: 896 x 4864  4096 x 4096  4096 x 12288  6144 x 4096
-//   1 tile, 8 wavefronts       6.7         6.7          17.0         10.1
-//   2 tiles, 4                 8.6         7.7          19.6          8.6
-//   64 x 64 tiling            10.5        10.2          21.3         10.2
-//                      32: 8192 x 8192  12288 x 4096  24576 x 4096  151936 x 896
-//   1 tile, 8 wavefronts      19.9          16.8          29.1          59.9
-//   2 tiles, 4                16.9          13.8          21.5          30.8
-//   64 x 64 tiling            16.3          12.2          25.4          52.8
-//                      64: 896 x 4864  4096 x 4096  24576 x 4096  151936 x 896
-//   1 tile, 8 wavefronts       8.7         8.8          45.5         117.1
-//   2 tiles, 4                11.1         9.9          30.7          46.5
-//   64 x 64 tiling            10.6        10.6          28.6          57.2
-// (one tile copies X twice as often and fills the chip sooner; the 64 x 64
-// tiling wins where its tiles fill one round of the CUs.)  SwiGLU, where a
-// workgroup is two groups of kw wavefronts:
+//                      32: 4096 x 4096  4096 x 12288  6144 x 4096  8192 x 8192  24576 x 4096
+//   1 tile, 8 wavefronts       6.7          16.9         10.1         19.9          28.9
+//   2 tiles, 4                 7.7          19.4          8.4         16.9          21.6
+//   64 x 32 tiling             8.5          17.2          8.8         13.8          25.5
+//   64 x 64 tiling             9.7          20.5          9.7         15.5          24.3
+//                      64: 1152 x 896  4096 x 4096  4096 x 12288  8192 x 8192  151936 x 896
+//   1 tile, 8 wavefronts       3.7          8.8          21.2         27.3         116.7
+//   2 tiles, 4                 4.4          9.9          24.1         20.5          46.4
+//   64 x 32 tiling             4.3          8.8          17.5         14.5          76.0
+//   64 x 64 tiling             4.8         10.0          21.0         15.9          52.7
+// (one tile copies X twice as often and fills the chip sooner; a tiling wins
+// where its tiles fill one round of the CUs.)  SwiGLU, where a workgroup is two
+// groups of kw wavefronts:
 //                   16: 4864 x 896  2048 x 8192  12288 x 4096   32: 4864 x 896  2048 x 8192  12288 x 4096
 //   kw 4                   5.0         16.5          22.2             5.5          20.6          24.9
 //   kw 2                   5.0         18.4          20.5             5.4          21.0          23.4
@@ -71,15 +74,14 @@ struct MxSkinny {
   int nt, kw;
 };
 inline MxSkinny choose_mx_skinny(int M, int N, int K, bool silu) {
-  constexpr MxSkinny tiled = {0, 0};
+  constexpr MxSkinny tiled = {0, 0}, one = {1, 8}, two = {2, 4};
   if (M > (silu ? 32 : 64)) return tiled;
   if (silu) {
     if (M > 16 && N <= 8192 && K >= 4096) return tiled;
     return M <= 16 && N <= 8192 ? MxSkinny{2, 4} : MxSkinny{2, 2};
   }
-  if (N <= 4096) return {1, 8};
-  if (N > 64 * 512 || (M <= 32 && (N <= 7168 || N > 64 * 256))) return {2, 4};
-  return tiled;
+  if (M > 32) return N > 64 * 512 ? two : N <= 4096 && K < 4096 ? one : tiled;
+  return N <= 4096 ? one : N <= 7168 || N > 64 * 256 ? two : tiled;
 }
 
 }  // namespace pa

@@ -199,6 +199,23 @@ def test_pack(pa, n, k, dtype):
     assert not codes[n:].any() and not codes[:, k:].any()
 
 
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 129), (896, 300)])
+def test_from_packed(pa, n, k):
+    """A weight from its packed arrays, whose sizes are the library's."""
+    w = pa.MxWeight(hidden_states(gen(n, k), n, k))
+    lib = pa._lib.load()
+    assert w.codes.numel() == lib.pa_mx_weight_bytes(n, k)
+    assert w.scales.numel() == lib.pa_mx_scale_bytes(n, k)
+    again = pa.MxWeight.from_packed(w.codes, w.scales, n, k)
+    x = pa.quantize_mx(hidden_states(gen(3), 5, k))
+    assert torch.equal(pa.linear_mx(x, again), pa.linear_mx(x, w))
+    for codes, scales, rows, cols in ((w.codes[:-1], w.scales, n, k), (w.codes, w.scales[1:], n, k),
+                                      (w.codes, w.scales, n, k + 128), (w.codes[:0], w.scales[:0], 0, k),
+                                      (w.codes.cpu(), w.scales, n, k), (w.codes.view(torch.int8), w.scales, n, k)):
+        with pytest.raises(ValueError):
+            pa.MxWeight.from_packed(codes, scales, rows, cols)
+
+
 def product(x, w):
     """The product in 64 bits, and what it may be off.  The matrix instructions
     align the (exact) products of 16 consecutive columns to the largest of them

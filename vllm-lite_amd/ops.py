@@ -535,7 +535,7 @@ def _mx_call(fn, device, *args):
     would be most (quantize_mx of 32 rows: 12.7 us with them)."""
     index = device.index
     call = getattr(_lib.load(), fn)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:  # a tensor of `device` exists: CUDA is up
         rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -580,9 +580,11 @@ class MxRows:
             raise ValueError(f"MXFP8 rows of {rows} x {cols}")
         self = cls.__new__(cls)
         kp = -(-cols // 128) * 128
-        self.codes = torch.empty((rows, kp), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((kp // 128, -(-rows // 16) * 16, 4), dtype=torch.uint8,
-                                  device=device)
+        pad = -(-rows // 16) * 16
+        # a microsecond less than torch.empty, of a decode step's call of nine
+        self.codes = torch.empty_strided((rows, kp), (kp, 1), dtype=torch.uint8, device=device)
+        self.scales = torch.empty_strided((kp // 128, pad, 4), (pad * 4, 4, 1),
+                                          dtype=torch.uint8, device=device)
         self.rows, self.cols = rows, cols
         return self
 
@@ -660,12 +662,11 @@ class MxWeight:
     def from_packed(cls, codes, scales, rows, cols):
         """A weight [rows, cols] whose packed codes and scales (flat uint8)
         are at hand, e.g. from a checkpoint."""
-        lib = _lib.load()
         self = cls.__new__(cls)
         self.shape, self.codes, self.scales = (rows, cols), codes, scales
+        size = -(-rows // 16) * 16 * (-(-cols // 128) * 128)  # pa_mx_weight_bytes
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda or \
-                codes.shape != (lib.pa_mx_weight_bytes(rows, cols),) or \
-                scales.shape != (lib.pa_mx_scale_bytes(rows, cols),):
+                rows <= 0 or cols <= 0 or codes.shape != (size,) or scales.shape != (size // 32,):
             raise ValueError(f"not the packed MXFP8 codes and scales of {rows} x {cols}")
         if codes.device != scales.device or not (codes.is_contiguous() and
                                                  scales.is_contiguous()):
@@ -708,7 +709,7 @@ def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_ou
         data, scales = out.codes.data_ptr(), out.scales.data_ptr()
     else:
         if out is None:
-            out = torch.empty(shape, dtype=bf16, device=device)
+            out = torch.empty_strided(shape, (n, 1), dtype=bf16, device=device)
         elif not _mx_like(out, shape, bf16, device):
             _mx_refuse("out", out, shape, bf16, device)
         data, scales = out.data_ptr(), None

@@ -69,7 +69,8 @@ struct WeightLayout {
 // The first of a workgroup's R rows (R a power of two up to 32).  near:
 // workgroups are dealt round-robin to the 8 XCDs; the rows of a group of 32,
 // whose scales share cache lines, then go to one XCD, so that its L2 puts the
-// lines together.
+// lines together.  Norm of rows x 4096 with and without, us: 512 6.5 and 6.6,
+// 2048 15.7 and 16.9, 7569 43.1 and 44.2.
 __device__ inline int64_t first_row(int64_t block, int R, int near) {
   if (!near) return block * R;
   const int64_t i = block / 8;
@@ -84,7 +85,8 @@ inline int64_t row_groups(int64_t rows, int R) {
 // Eight columns per thread, 16 threads per (row, step of 128 columns), a
 // workgroup 2^lg steps of 16 / 2^lg rows at a time, and `times` of these one
 // after another.  Rows `rows` .. `out_rows` are written as zeros (the padding
-// of a weight).
+// of a weight).  Bound by memory: 7569 x 4096 bf16 17.7 us, 5.3 TB/s (a large
+// copy: 5.2); 32 x 896 is a launch, 2.4 us.
 template <typename T, typename Layout>
 __global__ __launch_bounds__(256) void quantize_mx_kernel(Layout out, const T* __restrict__ x,
                                                           int64_t rows, int64_t out_rows, int cols,
@@ -169,6 +171,8 @@ __device__ inline float scaled_odd(float v, float w, float r, float r_low) {
 // is f64 and the scaling exact up to the rounding to codes where f32 leaves it
 // open, so that they are the codes of the formula, whatever the order of the
 // sum (in f32 throughout, 5 of 10^7 fell to the other side of a border).
+// Bound by memory: 7569 x 4096 bf16 with add 43.1 us, 5.1 TB/s (a large copy:
+// 5.2); short of rows, by its latencies: 32 x 896 3.0 us.
 template <typename T, int G, int C>
 __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum, const T* residual,
                                                           const T* __restrict__ add,
@@ -252,8 +256,8 @@ int32_t launch_quantize(const char* what, const Layout& out, const void* x, int6
   int lg = 0;  // as many steps side by side as there are, up to 16
   while (lg < 4 && 1 << lg < out.steps) ++lg;
   const int64_t groups = row_groups(out_rows, 16 >> lg);
-  // many rows: whole rows to a workgroup (7569 x 4096: 20 us, 22 with the steps
-  // over workgroups); few: the steps too
+  // many rows: whole rows to a workgroup (7569 x 4096: 17.7 us, 20.5 with the
+  // steps over workgroups); few: the steps too (512 x 4096: 3.5, 3.7 by rows)
   const int across = (int)((out.steps + (1 << lg) - 1) >> lg);
   const int times = out_rows >= kNearRows ? across : 1;
   quantize_mx_kernel<T, Layout>
@@ -270,16 +274,20 @@ int32_t launch_norm(const RowLayout& out, void* sum, const void* residual, const
       rows >= kNearRows);
   return check_launch("pa_rms_norm_mx");
 }
-template <typename T, typename... Args>
-int32_t launch_norm(const RowLayout& out, const Args&... args) {
-  const int64_t nch = out.steps * 16;  // chunks of 8 columns
-  if (nch <= 64) return launch_norm<T, 64, 1>(out, args...);
-  if (nch <= 128) return launch_norm<T, 64, 2>(out, args...);
-  if (nch <= 256) return launch_norm<T, 256, 1>(out, args...);
-  if (nch <= 512) return launch_norm<T, 256, 2>(out, args...);
-  if (nch <= 1024) return launch_norm<T, 256, 4>(out, args...);
-  if (nch <= 2048) return launch_norm<T, 256, 8>(out, args...);
-  return launch_norm<T, 256, 0>(out, args...);
+// The fewest chunks of 8 columns a lane that hold the row (us, bf16 with add:
+// 2048 x 2048 8.9 in 1 or 2, 9.1 in 4, 10.5 in 8; 64 x 16384 9.4 in 8, 12.4
+// read again).  A wavefront a row up to 512 columns (2048 x 512 4.2, by a
+// workgroup 4.5); up to 1024 where the rows fill the chip many times over (7569
+// x 896 14.9 and 16.0, 2048 x 896 6.3 and 6.0, 32 x 896 3.6 and 3.0).
+template <typename T>
+auto choose_norm(int64_t chunks, int64_t rows) {
+  return chunks <= 64                   ? launch_norm<T, 64, 1>
+         : chunks <= 128 && rows >= 4096 ? launch_norm<T, 64, 2>
+         : chunks <= 256                 ? launch_norm<T, 256, 1>
+         : chunks <= 512                 ? launch_norm<T, 256, 2>
+         : chunks <= 1024                ? launch_norm<T, 256, 4>
+         : chunks <= 2048                ? launch_norm<T, 256, 8>
+                                         : launch_norm<T, 256, 0>;
 }
 
 }  // namespace
@@ -385,8 +393,7 @@ extern "C" int32_t pa_rms_norm_mx(uint8_t* codes, uint8_t* scales, void* sum,
                PA_ERR_INVALID_ARG, "pa_rms_norm_mx: arrays overlap");
   }
   const RowLayout out{codes, scales, mx_steps(hidden), mx_pad_rows(rows)};
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == PA_DTYPE_BF16)
-    return launch_norm<uint16_t>(out, sum, residual, add, weight, (int64_t)rows, hidden, eps, s);
-  return launch_norm<float>(out, sum, residual, add, weight, (int64_t)rows, hidden, eps, s);
+  return (dtype == PA_DTYPE_BF16 ? choose_norm<uint16_t>
+                                 : choose_norm<float>)(out.steps * 16, rows)(
+      out, sum, residual, add, weight, rows, hidden, eps, (hipStream_t)stream);
 }

@@ -45,6 +45,17 @@ struct MxLinear {
 //
 // SILU: the tile's BN weight rows are BN/2 gate rows, then the matching up
 // rows; a wavefront takes TN/2 gate tiles and their up tiles.
+//
+// 256 x 256 tiles read the fewest operand bytes per product, and their four
+// wavefronts, one per SIMD, hold the accumulators in 256 registers each.  Times
+// and rates (normal values): 7569 x 4096 x 4096 113 us, 2250 TFLOP/s; 8192^3
+// 410 us, 2680; gate|up 2048 x 24576 x 4096 with its codes 160 us, 2580 (a
+// library's product alone, one scale per matrix: 103, 381 and 143 us).  Bound
+// by the matrix units' power: on zeros 8192^3 takes 377 us (without the copies
+// 280), on normal values products alone reach 3590 TFLOP/s of the 4700 on
+// zeros.  Fetching lines into L2 ahead of the copies took zeros to 318 us and
+// normal values to 409, at the first two sizes nothing, and is left out.  Fewer
+// tiles than fill the chip: the copies' latency, see mx_tiling.hpp.
 template <bool SILU, int WM, int WN, int TM, int TN, int KG, int S>
 __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLinear p, int ntm,
                                                                     int ntn) {
@@ -309,7 +320,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
                       auto rs, int r0) __attribute__((always_inline)) {
     constexpr int IT = decltype(items)::value, BATCH = IT % 8 == 0 ? 8 : IT;
     constexpr int SRC = decltype(src_step)::value, R = decltype(rs)::value;
-    if (m0 + BM <= M) {
+    if (M - m0 >= BM) {
 #pragma unroll
       for (int i = 0; i < IT; i += BATCH) {
         i32x4 v[BATCH];
@@ -405,7 +416,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
           v[u] = *reinterpret_cast<const uint4*>(
-              src + (int64_t)min(m0 + r0 + (i + u) * RS, M - 1) * N);
+              src + (int64_t)(m0 + min(r0 + (i + u) * RS, M - 1 - m0)) * N);
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
           if (RS <= BM || r0 < BM)

@@ -215,9 +215,9 @@ int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void* weight, i
  * out_scales NULL: out [rows, N] bf16, contiguous, 16-byte aligned, rounded
  * once, from the f32 result.  out_scales given (PA_ACT_SILU_MUL only): the
  * result goes out as MXFP8 rows, codes to out, for the projection after it.
- *   bias [N] or NULL, residual [rows, N] or NULL, bf16, contiguous; residual
- *   may be out itself (the residual stream updated in place), but out overlaps
- *   no other argument.
+ *   bias [N] or NULL, residual [rows, N] (16-byte aligned) or NULL, bf16,
+ *   contiguous; residual may be out itself (the residual stream updated in
+ *   place), but out overlaps no other argument.
  * The sums are f32, over groups of 16 columns whose exact products the matrix
  * instructions align to the group's largest, keeping 13 binary places below
  * its leading one: a result is off by about 2^-14 of its largest products,

@@ -31,9 +31,9 @@ def same_as_definition(mx, y):
     assert torch.equal(torch.nan_to_num(got, 1e9), torch.nan_to_num(v, 1e9))
 
 
-SIZES = [(2500, 130), (2048, 2300), (1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129), (5, 896), (64, 1000),
-         (33, 2048), (7, 2049), (4, 4096), (3, 8200), (2, 12289), (1000, 40), (4099, 96),
-         (4100, 700)]
+SIZES = [(2500, 130), (2048, 2300), (1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129),
+         (5, 896), (64, 1000), (33, 2048), (7, 2049), (4, 4096), (3, 8200), (2, 12289),
+         (1000, 40), (4099, 96), (4100, 700)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -210,9 +210,10 @@ def test_from_packed(pa, n, k):
     again = pa.MxWeight.from_packed(w.codes, w.scales, n, k)
     x = pa.quantize_mx(hidden_states(gen(3), 5, k))
     assert torch.equal(pa.linear_mx(x, again), pa.linear_mx(x, w))
-    for codes, scales, rows, cols in ((w.codes[:-1], w.scales, n, k), (w.codes, w.scales[1:], n, k),
-                                      (w.codes, w.scales, n, k + 128), (w.codes[:0], w.scales[:0], 0, k),
-                                      (w.codes.cpu(), w.scales, n, k), (w.codes.view(torch.int8), w.scales, n, k)):
+    for codes, scales, rows, cols in (
+            (w.codes[:-1], w.scales, n, k), (w.codes, w.scales[1:], n, k),
+            (w.codes, w.scales, n, k + 128), (w.codes[:0], w.scales[:0], 0, k),
+            (w.codes.cpu(), w.scales, n, k), (w.codes.view(torch.int8), w.scales, n, k)):
         with pytest.raises(ValueError):
             pa.MxWeight.from_packed(codes, scales, rows, cols)
 
@@ -372,3 +373,136 @@ def test_linear_scale_range(pa):
     x = pa.quantize_mx(torch.full((3, 160), 2.0 ** 100, device=DEV))
     w = pa.MxWeight(torch.full((20, 160), 2.0 ** -101, device=DEV))
     assert (pa.linear_mx(x, w) == 80).all()
+
+
+@pytest.mark.parametrize("m", [5, 40, 300])
+def test_swiglu_non_finite(pa, m):
+    """NaN and infinite gates and ups in bf16 and as codes: NaN codes in their
+    columns alone, and no part in their block's scale; gates far below zero
+    give zeros."""
+    n, k = 96, 128
+    x = torch.zeros(m, k, device=DEV)
+    x[:, 0] = 1
+    x[1, 1] = 1
+    w = torch.zeros(2 * n, k, device=DEV)
+    w[:n, 0], w[n:, 0] = 2, 3
+    big = 2.0 ** 127
+    w[4, 1], w[n + 9, 1] = float("nan"), float("inf")  # both NaN codes
+    w[40, 1] = -600
+    w[70, 0], w[n + 70, 0] = big, big  # inf in every row
+    xq, wq = pa.quantize_mx(x), pa.MxWeight(w)
+    out = pa.linear_mx(xq, wq, act=pa.ops.ACT_SILU_MUL)
+    y = 2 / (1 + torch.exp(torch.tensor(-2., dtype=torch.float64))).item() * 3
+    plainly = torch.ones(m, n, dtype=torch.bool, device=DEV)
+    plainly[1, 40] = False
+    plainly[:, [4, 9, 70]] = False  # 0 * NaN is NaN: in the rows whose x is 0 too
+    # the constants' own codes (2, 3, 1 are exact), the result's rounding, and
+    # the exponential and reciprocal
+    assert ((out[plainly].double() / y - 1).abs() <= 2.0 ** -8 + 2.0 ** -20).all()
+    assert torch.isnan(out[:, [4, 9]]).all() and (out[1, 40].abs() < 1e-30).all()
+    assert (out[:, 70] == float("inf")).all()
+    mx = pa.linear_mx(xq, wq, act=pa.ops.ACT_SILU_MUL, mx_out=True)
+    v = plain.dequantize(mx)
+    nan = torch.zeros(m, 128, dtype=torch.bool, device=DEV)
+    nan[:, [4, 9, 70]] = True
+    assert torch.equal(torch.isnan(v), nan)
+    assert ((v[:, :n][plainly] / y - 1).abs() <= 2.0 ** -4 + 2.0 ** -20).all()
+    assert v[1, 40].abs() < 1e-2 and not v[:, n:].any()
+
+
+def integers(g, rows, cols, low=-2, high=3):
+    """Small integers: their codes, products and (below 2^24) sums are exact."""
+    return torch.randint(low, high, (rows, cols), generator=g, device=DEV, dtype=torch.int8)
+
+
+def exact_product(x, w):
+    """Of integer matrices, in f64 by columns."""
+    out = torch.zeros(len(x), len(w), dtype=torch.float64, device=DEV)
+    for i in range(0, x.shape[1], 1 << 20):
+        out += x[:, i:i + (1 << 20)].double() @ w[:, i:i + (1 << 20)].double().t()
+    return out
+
+
+@pytest.mark.parametrize("m,n", [(1, 20), (17, 40), (70, 24), (257, 32)])
+def test_longest_rows(pa, m, n):
+    """2^22 columns, the most: quantised, normed and multiplied."""
+    k, g = 1 << 22, gen(m, n)
+    xi, wi = integers(g, m, k), integers(g, n, k)
+    xb = xi.to(torch.bfloat16)
+    x = pa.quantize_mx(xb)
+    ref = exact_product(xi, wi)
+    assert ref.abs().max() < 2 ** 24
+    w = pa.MxWeight(wi.to(torch.bfloat16))
+    assert torch.equal(pa.linear_mx(x, w), ref.to(torch.bfloat16))
+    if m <= 17:
+        one = torch.ones(k, dtype=torch.bfloat16, device=DEV)
+        s = xb.double()
+        same_as_definition(pa.rms_norm_mx(xb, one, EPS),
+                           s / (s.pow(2).mean(-1, keepdim=True) + EPS).sqrt())
+
+
+def test_past_32_bits(pa):
+    """Arrays of more than 2^32 bytes and 2^31 elements: the last rows as in a
+    call of their own."""
+    rows, cols, last = 540_001, 4096, slice(540_001 - 70, 540_001)
+    g = gen(0)
+    x = integers(g, rows, cols, -100, 100).to(torch.bfloat16)
+    q = pa.quantize_mx(x)
+    few = pa.quantize_mx(x[last])
+    assert torch.equal(q.codes[last], few.codes)
+    assert torch.equal(q.scales[:, last], few.scales[:, :70])
+    wt = torch.ones(cols, dtype=torch.bfloat16, device=DEV)
+    add = x[last].clone()
+    few = pa.rms_norm_mx(x[last].contiguous(), wt, EPS)
+    q = pa.rms_norm_mx(x, wt, EPS, out=q)
+    assert torch.equal(q.codes[last], few.codes)
+    assert torch.equal(q.scales[:, last], few.scales[:, :70])
+    assert torch.equal(x[last], add)
+    del q
+    k = 128
+    xi, wi = integers(g, rows, k), integers(g, cols, k)
+    xq, w = pa.quantize_mx(xi.to(torch.bfloat16)), pa.MxWeight(wi.to(torch.bfloat16))
+    out = pa.linear_mx(xq, w, residual=x, out=x)
+    want = exact_product(xi[last], wi) + add.double()
+    assert torch.equal(out[last], want.to(torch.bfloat16))
+    del out, x
+    gu = pa.MxWeight(torch.cat([wi, wi]).to(torch.bfloat16))
+    act = pa.linear_mx(xq, gu, act=pa.ops.ACT_SILU_MUL, mx_out=True)
+    y = exact_product(xi[last], wi)
+    y = y * y / (1 + torch.exp(-y))
+    part = pa.MxRows.empty(70, cols, DEV)
+    part.codes.copy_(act.codes[last])
+    part.scales[:, :70] = act.scales[:, last]
+    plain.assert_rounds(part, y, y.abs() * 16 * 2.0 ** -24)
+
+
+def test_no_rows(pa):
+    x = torch.empty(0, 896, dtype=torch.bfloat16, device=DEV)
+    w = pa.MxWeight(torch.ones(64, 896, device=DEV))
+    one = torch.ones(896, dtype=torch.bfloat16, device=DEV)
+    for rows in (pa.quantize_mx(x), pa.rms_norm_mx(x, one, EPS, add=x.clone())):
+        assert rows.codes.shape == (0, 896) and rows.scales.shape == (7, 0, 4)
+        assert pa.linear_mx(rows, w).shape == (0, 64)
+        assert pa.linear_mx(rows, w, act=pa.ops.ACT_SILU_MUL, mx_out=True).codes.shape == (0, 128)
+
+
+def test_refused_outputs(pa):
+    """Views that the kernels' wide accesses cannot take, and tensors that do
+    not fit."""
+    x = pa.quantize_mx(torch.ones(4, 128, device=DEV))
+    w = pa.MxWeight(torch.ones(64, 128, device=DEV))
+    buf = torch.zeros(4 * 64 + 1, dtype=torch.bfloat16, device=DEV)
+    for bad in (buf[1:].view(4, 64), torch.zeros(4, 65, device=DEV, dtype=torch.bfloat16)[:, :64],
+                torch.zeros(4, 64, device=DEV),
+                torch.zeros(3, 64, device=DEV, dtype=torch.bfloat16)):
+        with pytest.raises((ValueError, RuntimeError)):
+            pa.linear_mx(x, w, out=bad)
+        with pytest.raises((ValueError, RuntimeError)):
+            pa.linear_mx(x, w, residual=bad)
+    with pytest.raises(ValueError):
+        pa.quantize_mx(torch.ones(4, 256, device=DEV), out=x)
+    with pytest.raises(ValueError):
+        pa.quantize_mx(torch.ones(1, 128, device=DEV).expand(4, 128))
+    row = torch.ones(4, 128, device=DEV)
+    with pytest.raises((ValueError, RuntimeError)):  # the sum onto add
+        pa.rms_norm_mx(row, torch.ones(128, device=DEV), EPS, add=row)

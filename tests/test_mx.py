@@ -38,6 +38,7 @@ def test_quantize_refusals(lib):
     assert quantize(lib, dtype=2) == -1 and b"dtype" in lib.pa_last_error()
     assert quantize(lib, stride=99) == -1 and b"overlap" in lib.pa_last_error()
     assert quantize(lib, stride=-100) == -1
+    assert quantize(lib, stride=1 << 61) == -1 and b"stride" in lib.pa_last_error()
     assert quantize(lib, cols=(1 << 22) + 1) == -3
     for name in ("codes", "scales", "x"):
         assert quantize(lib, **{name: None}) == -1 and b"null" in lib.pa_last_error()
@@ -146,3 +147,14 @@ def test_wrappers_refuse_host_tensors(pa):
     with pytest.raises(ValueError):
         pa.MxRows(torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 16, 4, dtype=torch.uint8),
                   4, 64)
+
+
+@pytest.mark.parametrize("rows,cols", [(-1, 64), (1 << 31, 64), (4, 0), (4, (1 << 22) + 1),
+                                       (4, (1 << 32) + 64)])
+def test_wrappers_refuse_sizes(pa, rows, cols):
+    """Before anything is allocated, or cut to 32 bits on its way to the library."""
+    some = torch.zeros(1, dtype=torch.uint8)
+    for make in (lambda: pa.MxRows.empty(rows, cols), lambda: pa.MxRows(some, some, rows, cols),
+                 lambda: pa.MxWeight.from_packed(some, some, rows, cols)):
+        with pytest.raises(ValueError, match=f"{rows} x {cols}"):
+            make()

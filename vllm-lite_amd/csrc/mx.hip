@@ -319,13 +319,15 @@ extern "C" int32_t pa_quantize_mx(uint8_t* codes, uint8_t* scales, const void* x
   PA_REQUIRE(x_stride == 0 || x_stride >= cols, PA_ERR_INVALID_ARG,
              "pa_quantize_mx: rows overlap");
   if (rows == 0) return PA_OK;
+  PA_REQUIRE(x_stride <= INT64_MAX / 8 / rows, PA_ERR_INVALID_ARG, "pa_quantize_mx: bad stride");
   PA_REQUIRE(codes && scales && x, PA_ERR_INVALID_ARG, "pa_quantize_mx: null pointer");
   PA_MX_ALIGNED("pa_quantize_mx", codes, scales);
   PA_REQUIRE((uintptr_t)x % dtype_size(dtype) == 0, PA_ERR_INVALID_ARG,
              "pa_quantize_mx: x is not aligned to its elements");
   {
     const int64_t nc = (int64_t)rows * mx_steps(cols) * 128, ns = mx_scale_bytes(rows, cols);
-    const int64_t nx = ((rows - 1) * (x_stride ? x_stride : cols) + cols) * (int64_t)dtype_size(dtype);
+    const int64_t nx =
+        ((rows - 1) * (x_stride ? x_stride : cols) + cols) * (int64_t)dtype_size(dtype);
     PA_REQUIRE(!mx_overlap(codes, nc, scales, ns) && !mx_overlap(codes, nc, x, nx) &&
                    !mx_overlap(scales, ns, x, nx),
                PA_ERR_INVALID_ARG, "pa_quantize_mx: arrays overlap");

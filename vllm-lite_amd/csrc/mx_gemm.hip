@@ -65,9 +65,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   constexpr int BS = (BN + 63) / 64 * 64;                 // scales of W: 64 rows a copy
   constexpr int SC = (BM + BS) / 64, CS = (SC + GW - 1) / GW;  // 256 B copies of scales
   constexpr int PER = CA + CB + CS;
-  static_assert(CA * GW * 8 == BM && CB * GW * 8 == BN && BM % 64 == 0 && (!SILU || (TN % 2 == 0 && BN % 64 == 0)),
+  static_assert(CA * GW * 8 == BM && CB * GW * 8 == BN && BM % 64 == 0 &&
+                    (!SILU || (TN % 2 == 0 && BN % 64 == 0)),
                 "tiles");
-  constexpr int STEP = (BM + BN) * 128 + (BM + BS) * 4, STAGE = KG * STEP;  // codes, then scale dwords
+  constexpr int STEP = (BM + BN) * 128 + (BM + BS) * 4;  // codes, then scale dwords
+  constexpr int STAGE = KG * STEP;
   constexpr int SX = (BM + BN) * 128, SW = SX + BM * 4;
   constexpr int ORB = BNO * 2 + 16;  // bytes per row of the staged output tile
   constexpr int RED = BM * BN * 4 * (KG - 1);

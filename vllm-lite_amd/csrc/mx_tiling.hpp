@@ -11,15 +11,16 @@ namespace pa {
 // by how full it is.  Fitted to each tiling's times over 197 shapes (M 40 to
 // 7569, wrows 896 to 24576, K 160 to 12288; where it is within half as much
 // again of the fastest, rms error 4 to 12%), over which the smallest estimate is
-// the fastest tiling or within 9% of it, 0.2% on average.  Measured, us (M x
-// wrows x K):
-//                         333 x 896 x 4864    256 x 4096 x 4096    618 x 6144 x 4096   2048 x 4096 x 4096   7569 x 4096 x 4096
-//   256 x 256                         47.0                 40.1                 41.5                 44.0                111.1
-//   256 x 128                         29.0                 25.3                 27.2                 33.8                127.5
-//   128 x 128, pairs                  26.7                 23.2                 24.3                 34.4                128.6
-//   128 x 128                         19.3                 17.2                 20.0                 38.4                148.6
-//    64 x  64                         11.3                 10.9                 33.8                 64.0                240.3
-//    64 x  32                          9.7                 15.4                 52.7                103.4                384.2
+// the fastest tiling or within 9% of it, 0.2% on average.  Measured, us:
+//                   rows:    333    256    618   2048   7569
+//                  wrows:    896   4096   6144   4096   4096
+//                      K:   4864   4096   4096   4096   4096
+//   256 x 256              47.0   40.1   41.5   44.0  111.1
+//   256 x 128              29.0   25.3   27.2   33.8  127.5
+//   128 x 128, pairs       26.7   23.2   24.3   34.4  128.6
+//   128 x 128              19.3   17.2   20.0   38.4  148.6
+//    64 x  64              11.3   10.9   33.8   64.0  240.3
+//    64 x  32               9.7   15.4   52.7  103.4  384.2
 // (64 x 32 tiles of SwiGLU would hold half a block of 32 output columns.)
 enum MxTiling { kMx256x256, kMx256x128, kMx128x128Pair, kMx128x128, kMx64x64, kMx64x32 };
 inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K, bool silu) {
@@ -66,10 +67,14 @@ inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K, bool silu) {
 // (one tile copies X twice as often and fills the chip sooner; a tiling wins
 // where its tiles fill one round of the CUs.)  SwiGLU, where a workgroup is two
 // groups of kw wavefronts:
-//                   16: 4864 x 896  2048 x 8192  12288 x 4096   32: 4864 x 896  2048 x 8192  12288 x 4096
-//   kw 4                   5.0         16.5          22.2             5.5          20.6          24.9
-//   kw 2                   5.0         18.4          20.5             5.4          21.0          23.4
-//   64 x 64 tiling         5.8         15.9          25.4             5.9          15.8          26.3
+//             rows, N x K: 16, 4864 x 896  2048 x 8192  12288 x 4096
+//   kw 4                         5.0          16.5          22.2
+//   kw 2                         5.0          18.4          20.5
+//   64 x 64 tiling               5.8          15.9          25.4
+//                          32, 4864 x 896  2048 x 8192  12288 x 4096
+//   kw 4                         5.5          20.6          24.9
+//   kw 2                         5.4          21.0          23.4
+//   64 x 64 tiling               5.9          15.8          26.3
 struct MxSkinny {
   int nt, kw;
 };

@@ -554,6 +554,13 @@ def _mx_refuse(name, t, shape, dtype, device):
                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def _mx_sizes(rows, cols):
+    """Refuses what the entry points cannot take (int32 rows, 2^22 columns)
+    before ctypes cuts it to 32 bits."""
+    if not 0 <= rows < 1 << 31 or not 0 < cols <= 1 << 22:
+        raise ValueError(f"MXFP8 of {rows} x {cols}")
+
+
 class MxRows:
     """MXFP8 rows [rows, cols]: codes uint8 [rows, Kp] (Kp = cols rounded up to
     128), scales uint8 [Kp / 128, R, 4] (R = rows rounded up to 16), see
@@ -562,6 +569,7 @@ class MxRows:
     __slots__ = ("codes", "scales", "rows", "cols")
 
     def __init__(self, codes, scales, rows, cols):
+        _mx_sizes(rows, cols)
         self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
         kp = -(-cols // 128) * 128
         if codes.shape != (rows, kp) or scales.shape != (kp // 128, -(-rows // 16) * 16, 4):
@@ -576,8 +584,7 @@ class MxRows:
     @classmethod
     def empty(cls, rows, cols, device="cuda"):
         """Rows whose arrays are allocated and not filled."""
-        if rows < 0 or cols <= 0:
-            raise ValueError(f"MXFP8 rows of {rows} x {cols}")
+        _mx_sizes(rows, cols)
         self = cls.__new__(cls)
         kp = -(-cols // 128) * 128
         pad = -(-rows // 16) * 16
@@ -650,6 +657,7 @@ class MxWeight:
             raise ValueError("MxWeight: expected a contiguous device tensor [N, K]")
         lib = _lib.load()
         n, k = self.shape = tuple(weight.shape)
+        _mx_sizes(n, k)
         code = _dtype_code(weight)
         self.codes = torch.empty(lib.pa_mx_weight_bytes(n, k), dtype=torch.uint8,
                                  device=weight.device)
@@ -662,11 +670,12 @@ class MxWeight:
     def from_packed(cls, codes, scales, rows, cols):
         """A weight [rows, cols] whose packed codes and scales (flat uint8)
         are at hand, e.g. from a checkpoint."""
+        _mx_sizes(rows, cols)
         self = cls.__new__(cls)
         self.shape, self.codes, self.scales = (rows, cols), codes, scales
         size = -(-rows // 16) * 16 * (-(-cols // 128) * 128)  # pa_mx_weight_bytes
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda or \
-                rows <= 0 or cols <= 0 or codes.shape != (size,) or scales.shape != (size // 32,):
+                rows == 0 or codes.shape != (size,) or scales.shape != (size // 32,):
             raise ValueError(f"not the packed MXFP8 codes and scales of {rows} x {cols}")
         if codes.device != scales.device or not (codes.is_contiguous() and
                                                  scales.is_contiguous()):

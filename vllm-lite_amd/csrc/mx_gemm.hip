@@ -88,15 +88,15 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   // the i-th contiguous range of an order that goes through groups of row
   // tiles (up to 8, so that W is streamed once), column tiles outer within a
   // group, so the tiles in flight on an XCD share X and W rows in its L2.
-  const int group_m = min(ntm, 8);
-  const int total = ntm * ntn, per_xcd = (total + 7) / 8;
-  const int tile = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-  if ((int)(blockIdx.x / 8) >= per_xcd || tile >= total) return;
-  const int first_m = tile / (group_m * ntn) * group_m;
-  const int gsz = min(group_m, ntm - first_m), in_grp = tile % (group_m * ntn);
-  const int m0 = (first_m + in_grp % gsz) * BM;
-  const int c0 = in_grp / gsz * BNO;  // first output column
-  const int tiles_n = (N + 15) / 16;  // 16-row fragments of W (of its gate half)
+  const uint32_t group_m = min(ntm, 8), group = group_m * (uint32_t)ntn;
+  const uint32_t total = (uint32_t)ntm * ntn, per_xcd = (total + 7) / 8;
+  const uint32_t tile = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= per_xcd || tile >= total) return;
+  const uint32_t first_m = tile / group * group_m, in_grp = tile % group;
+  const uint32_t gsz = min(group_m, ntm - first_m);
+  const int m0 = (int)(first_m + in_grp % gsz) * BM;
+  const int c0 = (int)(in_grp / gsz) * BNO;  // first output column
+  const int tiles_n = (int)((uint32_t)(N + 15) >> 4);  // 16-row fragments of W (of its gate half)
   auto swz = [](int r) -> int { return (r / 2) % 8; };
 
   // This wavefront's copies of a step: scalar bases, 32-bit lane offsets.
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   // the fragment of W that holds row r of the tile
   auto frag = [&](int r) __attribute__((always_inline)) -> int {
     const bool up = SILU && r >= BN / 2;
-    return min((c0 + (up ? r - BN / 2 : r)) / 16, tiles_n - 1) + (up ? tiles_n : 0);
+    return min((c0 + (up ? r - BN / 2 : r)) >> 4, tiles_n - 1) + (up ? tiles_n : 0);
   };
   const uint8_t* wb[CB];  // half a fragment each
 #pragma unroll
@@ -534,7 +534,7 @@ int32_t launch(const MxLinear& p, hipStream_t stream) {
 // rate, and 32 rows took 4 us longer than 1 at 896 x 4864).
 template <bool SILU, int MT, int NT, int KW>
 __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_skinny_kernel(
-    const MxLinear p, int kw) {
+    const MxLinear p, int kw, int share, int more) {
   static_assert(!SILU || NT == 2, "two gate and two up tiles");
   constexpr int TG = SILU ? 2 : 1, TILES = TG * NT, NO = NT;  // NO: output tiles
   constexpr int XB = MT * 2048;                               // a step's rows of X
@@ -546,9 +546,11 @@ __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, j = lane >> 4;
   const int M = p.M, N = p.N, nk = p.steps;
-  const int tiles_n = (N + 15) / 16;  // of W (of its gate half)
-  const int kp = TG == 1 ? wave : wave % kw, tg = TG == 1 ? 0 : wave / kw;
-  const int s0 = (int)((int64_t)kp * nk / kw), s1 = (int)((int64_t)(kp + 1) * nk / kw);
+  const int tiles_n = (int)((uint32_t)(N + 15) >> 4);  // of W (of its gate half)
+  const int tg = TG == 1 || wave < kw ? 0 : 1, kp = wave - tg * kw;
+  // `share` steps each, the first `more` one more (a division here costs as
+  // much as a step)
+  const int s0 = kp * share + min(kp, more), s1 = s0 + share + (kp < more ? 1 : 0);
   const uint8_t *wp[NT], *sp[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -722,7 +724,8 @@ int32_t launch_skinny(const MxLinear& p, hipStream_t stream) {
   // an MXFP8 output's padding is written too
   const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
   const dim3 grid((uint32_t)((cols + 16 * NT - 1) / (16 * NT)));
-  mx_skinny_kernel<SILU, MT, NT, KW><<<grid, 64 * (SILU ? 2 : 1) * kw, 0, stream>>>(p, kw);
+  mx_skinny_kernel<SILU, MT, NT, KW><<<grid, 64 * (SILU ? 2 : 1) * kw, 0, stream>>>(
+      p, kw, p.steps / kw, p.steps % kw);
   return check_launch("pa_linear_mx");
 }
 

@@ -532,6 +532,10 @@ int32_t launch(const MxLinear& p, hipStream_t stream) {
 // of the wavefront's own, copied in whole 128-byte lines (loaded as the
 // operands need it, half a line per row and load, L2 served it at half its
 // rate, and 32 rows took 4 us longer than 1 at 896 x 4864).
+// Bound by the weights' bytes where they are many, and by X's, which every
+// workgroup reads (4096 x 12288: 1 row 11.6 us, 4.3 TB/s, 17 rows 13.8, 32
+// rows 16.8; three steps in flight 11.2, 15.0, 18.1); else by a launch and a
+// few steps' latency (32 x 1152 x 896 3.1 us).
 template <bool SILU, int MT, int NT, int KW>
 __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_skinny_kernel(
     const MxLinear p, int kw, int share, int more) {

@@ -611,13 +611,14 @@ def quantize_mx(x, out=None):
     if not x.is_cuda or x.dim() != 2:
         raise ValueError("quantize_mx: expected a device tensor [rows, cols]")
     rows, cols = x.shape
-    if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
+    pitch, step = x.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and pitch < cols):
         raise ValueError("quantize_mx: rows must have unit stride and not overlap")
     code = _dtype_code(x)
     device = x.device
     out = _mx_out(out, rows, cols, device)
     _mx_call("pa_quantize_mx", device, out.codes.data_ptr(), out.scales.data_ptr(),
-             x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, code)
+             x.data_ptr(), rows, cols, pitch if rows > 1 else cols, code)
     return out
 
 

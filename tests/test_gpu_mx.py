@@ -248,7 +248,8 @@ PRODUCTS = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (3, 64, 128), (7, 100, 129), (1
             (64, 896, 4864), (65, 72, 257), (100, 1001, 1000), (127, 128, 128), (128, 130, 2048),
             (129, 257, 384), (200, 520, 4096), (255, 255, 255), (256, 256, 256), (257, 300, 512),
             (333, 896, 4864), (513, 1025, 130), (618, 2056, 1152), (1025, 640, 896),
-            (2100, 1100, 300), (5000, 900, 160)]
+            (2100, 1100, 300), (5000, 900, 160), (70, 5, 40), (66, 8, 33), (300, 9, 200),
+            (130, 15, 100), (2000, 3, 64), (700, 1031, 96)]
 
 
 # ... and those that reach every kernel and tiling; test_mx_tiling.py holds the

@@ -15,6 +15,9 @@ namespace pa {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// at the alignment of a row of bf16 (the memory takes it whole)
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint64_t u64u __attribute__((aligned(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct MxLinear {
@@ -314,28 +317,24 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
     }
     __syncthreads();
   }
-  // 16 bytes of every rs-th row of a staged tile out, `items` of them.  All of a
-  // tile inside the output in batches of LDS reads: under a branch the
-  // compiler reads and stores one by one (43.2 us for 41.6 at 618 x 6144 x 4096
-  // in 256 x 256 tiles).
+  // 16 bytes of every rs-th row of a staged tile out, `items` of them (of rows
+  // behind M none), in batches of LDS reads, which the asm holds in front of
+  // the branches: behind them the compiler reads and stores one by one (43.2 us
+  // for 41.6 at 618 x 6144 x 4096 in 256 x 256 tiles).
   auto rows_out = [&](uint8_t* dst, int64_t dst_step, const uint8_t* src, auto src_step, auto items,
                       auto rs, int r0) __attribute__((always_inline)) {
     constexpr int IT = decltype(items)::value, BATCH = IT % 8 == 0 ? 8 : IT;
     constexpr int SRC = decltype(src_step)::value, R = decltype(rs)::value;
-    if (M - m0 >= BM) {
 #pragma unroll
-      for (int i = 0; i < IT; i += BATCH) {
-        i32x4 v[BATCH];
+    for (int i = 0; i < IT; i += BATCH) {
+      i32x4 v[BATCH];
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u)
-          v[u] = *reinterpret_cast<const i32x4*>(src + (i + u) * SRC);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int u = 0; u < BATCH; ++u) v[u] = *reinterpret_cast<const i32x4*>(src + (i + u) * SRC);
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u, dst += dst_step) *reinterpret_cast<i32x4*>(dst) = v[u];
-      }
-    } else {
-      for (int r = r0; r < M - m0; r += R, dst += dst_step, src += SRC)
-        *reinterpret_cast<i32x4*>(dst) = *reinterpret_cast<const i32x4*>(src);
+      for (int u = 0; u < BATCH; ++u) asm volatile("" : "+v"(v[u]));
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u, dst += dst_step)
+        if (r0 + (i + u) * R < M - m0) *reinterpret_cast<i32x4u*>(dst) = v[u];
     }
   };
   if constexpr (SILU) {
@@ -407,31 +406,41 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   static_assert(RS * CPRO == NT && BM % std::min(BM, RS) == 0, "whole passes");
   const int r0 = threadIdx.x / CPRO, cc = threadIdx.x % CPRO * 8;
   if constexpr (!SILU) {
-    if (p.residual && N % 8 == 0) {
+    if (p.residual && N >= 8) {
       // several loads in flight per thread (one at a time took 17 us of a
       // 256 x 256 tile); those outside the output read its last row or piece
       constexpr int BATCH = ITEMS % 16 == 0 ? 16 : ITEMS;
-      const uint16_t* src = p.residual + min(c0 + cc, N - 8);
+      const int col = min(c0 + cc, N - 8);
+      const uint16_t* src = p.residual + col;
+      // a piece that ends behind the row: its columns are the last of the 8
+      // that end with it
+      const int shift = min(c0 + cc - col, 7) * 16;
 #pragma unroll
       for (int i = 0; i < ITEMS; i += BATCH) {
-        uint4 v[BATCH];
+        i32x4 v[BATCH];
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
-          v[u] = *reinterpret_cast<const uint4*>(
+          v[u] = *reinterpret_cast<const i32x4u*>(
               src + (int64_t)(m0 + min(r0 + (i + u) * RS, M - 1 - m0)) * N);
+        if (c0 + BNO > N) {
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u) {
+            typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+            u64x2 w = __builtin_bit_cast(u64x2, v[u]);
+            w = shift < 64 ? u64x2{w.x >> shift | (shift ? w.y << (64 - shift) : 0), w.y >> shift}
+                           : u64x2{w.y >> (shift - 64), 0};
+            v[u] = __builtin_bit_cast(i32x4, w);
+          }
+        }
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
           if (RS <= BM || r0 < BM)
-            *reinterpret_cast<uint4*>(lds + (r0 + (i + u) * RS) * ORB + cc * 2) = v[u];
+            *reinterpret_cast<i32x4*>(lds + (r0 + (i + u) * RS) * ORB + cc * 2) = v[u];
       }
     } else if (p.residual) {
-      for (int r = r0; r < min(BM, M - m0); r += RS) {
-        const uint16_t* src = p.residual + (int64_t)(m0 + r) * N + c0 + cc;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(lds + r * ORB + cc * 2);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + cc + e < N) dst[e] = src[e];
-      }
+      for (int i = threadIdx.x; i < min(BM, M - m0) * N; i += NT)
+        *reinterpret_cast<uint16_t*>(lds + i / N * ORB + i % N * 2) =
+            p.residual[(int64_t)m0 * N + i];
     }
     if (p.bias)
       for (int i = threadIdx.x; i < BN; i += NT)
@@ -492,14 +501,18 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void mx_gemm_kernel(const MxLine
   // ... and the rows out
   if (c0 + cc >= N || r0 >= BM) return;
   uint16_t* dst = out + (int64_t)(m0 + r0) * N + c0 + cc;
-  if (N % 8 == 0) {
+  if (c0 + cc + 8 <= N) {
     rows_out(reinterpret_cast<uint8_t*>(dst), (int64_t)RS * N * 2, lds + r0 * ORB + cc * 2,
              std::integral_constant<int, RS * ORB>{}, std::integral_constant<int, ITEMS>{},
              std::integral_constant<int, RS>{}, r0);
-  } else {
-    for (int r = r0; r < min(BM, M - m0); r += RS, dst += (int64_t)RS * N)
-      for (int e = 0; e < 8 && c0 + cc + e < N; ++e)
-        dst[e] = reinterpret_cast<const uint16_t*>(lds + r * ORB + cc * 2)[e];
+  } else {  // the row's last piece
+    for (int r = r0; r < min(BM, M - m0); r += RS, dst += (int64_t)RS * N) {
+      uint16_t v[8];
+      *reinterpret_cast<i32x4*>(v) = *reinterpret_cast<const i32x4*>(lds + r * ORB + cc * 2);
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (c0 + cc + e < N) dst[e] = v[e];
+    }
   }
 }
 
@@ -699,12 +712,11 @@ __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_
     const int64_t at = (int64_t)row * N + col;
     uint16_t* out = static_cast<uint16_t*>(p.out) + at;
     uint16_t prev[4] = {0, 0, 0, 0}, v[4];
-    const bool wide = N % 4 == 0;
-    if (wide && col >= N) continue;
+    if (col >= N) continue;
+    const bool wide = col + 4 <= N;
     if (!SILU && p.residual) {
       if (wide)
-        *reinterpret_cast<uint64_t*>(prev) =
-            *reinterpret_cast<const uint64_t*>(p.residual + at);
+        *reinterpret_cast<uint64_t*>(prev) = *reinterpret_cast<const u64u*>(p.residual + at);
       else
         for (int e = 0; e < 4 && col + e < N; ++e) prev[e] = p.residual[at + e];
     }
@@ -716,7 +728,7 @@ __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_
       v[e] = f32_to_bf16_bits(f);
     }
     if (wide)
-      *reinterpret_cast<uint64_t*>(out) = *reinterpret_cast<const uint64_t*>(v);
+      *reinterpret_cast<u64u*>(out) = *reinterpret_cast<const uint64_t*>(v);
     else
       for (int e = 0; e < 4 && col + e < N; ++e) out[e] = v[e];
   }

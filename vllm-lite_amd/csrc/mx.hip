@@ -22,18 +22,32 @@ struct Vec8<float> {
   typedef float V __attribute__((ext_vector_type(8), aligned(4)));
 };
 
-// Columns 8 ch .. 8 ch + 7 of a row, 0 behind the last.
+// Columns 8 ch .. 8 ch + 7 of a row, 0 behind the last.  A chunk that ends
+// behind the row is the end of the row's last eight elements, moved down:
+// loaded one by one behind a branch, its elements held up the whole wavefront.
 template <typename T>
-__device__ inline typename Vec8<T>::V load8(const T* row, int64_t ch, int cols) {
-  if (8 * ch + 8 <= cols) return *reinterpret_cast<const typename Vec8<T>::V*>(row + 8 * ch);
+__device__ inline typename Vec8<T>::V load8(const T* row, int ch, int cols) {
   typename Vec8<T>::V v = 0;
+  if (cols >= 8) {
+    const int at = min(8 * ch, cols - 8), past = 8 * ch - at;
+    v = *reinterpret_cast<const typename Vec8<T>::V*>(row + at);
+    if (past) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (8 * ch + e < cols) v[e] = Elem<T>::load(row + 8 * ch + e);
+      for (int by = 1; by <= 4; by *= 2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (past & by) v[e] = e + by < 8 ? v[e + by] : 0;
+      if (past >= 8) v = 0;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (8 * ch + e < cols) v[e] = Elem<T>::load(row + 8 * ch + e);
+  }
   return v;
 }
 template <typename T>
-__device__ inline void store8(T* row, int64_t ch, int cols, const typename Vec8<T>::V& v) {
+__device__ inline void store8(T* row, int ch, int cols, const typename Vec8<T>::V& v) {
   if (8 * ch + 8 <= cols) {
     *reinterpret_cast<typename Vec8<T>::V*>(row + 8 * ch) = v;
   } else {

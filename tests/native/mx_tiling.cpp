@@ -6,7 +6,7 @@
 
 int main() {
   static const char* names[] = {"256x256", "256x128", "128x128 pair", "128x128",
-                                "64x64",   "64x32"};
+                                "128x64",  "64x64",   "64x32"};
   int m, n, k, silu;
   while (std::scanf("%d %d %d %d", &m, &n, &k, &silu) == 4) {
     const pa::MxSkinny s = pa::choose_mx_skinny(m, n, k, silu != 0);

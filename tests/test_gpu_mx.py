@@ -260,15 +260,17 @@ KERNELS = {
     (32, 17001, 140): "few rows 2/4", (50, 32801, 700): "few rows 2/4",
     (20, 8010, 260): "64x32", (65, 101, 640): "64x32", (37, 70, 5000): "64x32",
     (600, 900, 700): "64x64", (130, 5204, 300): "64x64",
-    (618, 2056, 1152): "128x128", (5463, 134, 1100): "128x128",
-    (5515, 139, 200): "128x128 pair",
+    (618, 2056, 1152): "128x64", (5463, 134, 1100): "128x64", (5515, 139, 200): "128x64",
+    (999, 4010, 1100): "128x128", (1999, 2054, 900): "128x128 pair",
     (1430, 4014, 2000): "256x128", (4669, 1668, 2000): "256x256",
 }
 KERNELS_GATED = {
     (10, 160, 600): "few rows 2/4", (12, 8224, 140): "few rows 2/2",
     (32, 8224, 140): "few rows 2/2", (26, 96, 700): "few rows 2/2",
-    (20, 96, 4200): "64x64", (53, 128, 900): "64x64", (71, 4352, 2000): "128x128",
-    (80, 4416, 200): "128x128 pair", (652, 4128, 2000): "256x128",
+    (20, 96, 4200): "64x64", (53, 128, 900): "64x64", (71, 4352, 2000): "128x64",
+    (80, 4416, 200): "128x64", (700, 2080, 500): "128x128",
+    (1100, 2080, 300): "128x128 pair",
+    (652, 4128, 2000): "256x128",
     (658, 5856, 2000): "256x256",
 }
 

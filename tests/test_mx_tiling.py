@@ -8,7 +8,7 @@ import pytest
 from test_gpu_mx import KERNELS, KERNELS_GATED
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-TILED = {"64x64", "128x128", "128x128 pair", "256x128", "256x256"}
+TILED = {"64x64", "128x64", "128x128", "128x128 pair", "256x128", "256x256"}
 
 
 @pytest.fixture(scope="module")

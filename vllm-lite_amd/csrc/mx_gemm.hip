@@ -823,6 +823,7 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
       case kMx256x128: return launch<true, 4, 2, 2, 2, 1, 3>(p, s);
       case kMx128x128Pair: return launch<true, 2, 2, 2, 2, 1, 2>(p, s);
       case kMx128x128: return launch<true, 4, 2, 1, 2, 1, 3>(p, s);
+      case kMx128x64: return launch<true, 4, 1, 1, 2, 1, 4>(p, s);
       default: return launch<true, 2, 1, 1, 2, 2, 4>(p, s);
     }
   switch (choose_mx_tiling(rows, out_features, in_features, false)) {
@@ -830,6 +831,7 @@ extern "C" int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x
     case kMx256x128: return launch<false, 4, 2, 2, 2, 1, 3>(p, s);
     case kMx128x128Pair: return launch<false, 2, 2, 2, 2, 1, 2>(p, s);
     case kMx128x128: return launch<false, 4, 2, 1, 2, 1, 3>(p, s);
+    case kMx128x64: return launch<false, 4, 1, 1, 2, 1, 4>(p, s);
     case kMx64x64: return launch<false, 2, 2, 1, 1, 2, 4>(p, s);
     default: return launch<false, 2, 1, 1, 1, 2, 4>(p, s);
   }

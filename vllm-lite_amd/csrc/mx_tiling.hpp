@@ -8,33 +8,43 @@ namespace pa {
 // The tilings, and the time each would take: rounds of workgroups over the
 // 256 CUs (two a CU for the pairs of 128 x 128 tiles), each round `us` plus
 // `ns_per_k` for every column of K, the last one `tail` of a round and the rest
-// by how full it is.  Fitted to each tiling's times over 197 shapes (M 40 to
-// 7569, wrows 896 to 24576, K 160 to 12288; where it is within half as much
-// again of the fastest, rms error 4 to 12%), over which the smallest estimate is
-// the fastest tiling or within 9% of it, 0.2% on average.  Measured, us:
-//                   rows:    333    256    618   2048   7569
-//                  wrows:    896   4096   6144   4096   4096
-//                      K:   4864   4096   4096   4096   4096
-//   256 x 256              47.0   40.1   41.5   44.0  111.1
-//   256 x 128              29.0   25.3   27.2   33.8  127.5
-//   128 x 128, pairs       26.7   23.2   24.3   34.4  128.6
-//   128 x 128              19.3   17.2   20.0   38.4  148.6
-//    64 x  64              11.3   10.9   33.8   64.0  240.3
-//    64 x  32               9.7   15.4   52.7  103.4  384.2
+// by how full it is.  Fitted to each tiling's times over 289 shapes (M 40 to
+// 8192, wrows 256 to 24576, K 160 to 12288; where it is within half as much
+// again of the fastest, rms error 3 to 6%), over which the smallest estimate is
+// the fastest tiling or within 6% of it, 0.1% on average.  Measured, us:
+//                  rows:    333    256    449    618   2048   7569
+//                 wrows:    896   4096   3000   6144   4096   4096
+//                     K:   4864   4096   6200   4096   4096   4096
+//   256 x 256              46.9   39.9   58.5   40.9   43.9  107.1
+//   256 x 128              28.9   25.4   36.0   27.2   34.6  126.0
+//   128 x 128, pairs       26.6   23.2   33.4   24.2   35.6  128.7
+//   128 x 128              19.0   17.6   24.1   20.3   41.7  153.9
+//   128 x  64              14.8   13.5   18.6   25.5   53.8  193.1
+//    64 x  64              10.9   10.7   24.8   34.1   67.7  238.5
+//    64 x  32               9.3   15.2   28.7   51.3  100.5  373.4
 // (64 x 32 tiles of SwiGLU would hold half a block of 32 output columns.)
-enum MxTiling { kMx256x256, kMx256x128, kMx128x128Pair, kMx128x128, kMx64x64, kMx64x32 };
+enum MxTiling {
+  kMx256x256,
+  kMx256x128,
+  kMx128x128Pair,
+  kMx128x128,
+  kMx128x64,
+  kMx64x64,
+  kMx64x32
+};
 inline MxTiling choose_mx_tiling(int M, int64_t wrows, int K, bool silu) {
   struct Cost {
     MxTiling t;
     int bm, bn, slots;
     double base, us, ns_per_k, tail;
   };
-  static constexpr Cost costs[] = {{kMx256x256, 256, 256, 256, 3.0, 7.3, 11.7, .63},
-                                   {kMx256x128, 256, 128, 256, 1.1, 4.5, 6.99, .64},
-                                   {kMx128x128Pair, 128, 128, 512, 1.8, 3.2, 7.77, .46},
-                                   {kMx128x128, 128, 128, 256, 2.0, 2.5, 4.14, .64},
-                                   {kMx64x64, 64, 64, 256, 1.3, 2.4, 1.66, .86},
-                                   {kMx64x32, 64, 32, 256, 1.6, 1.7, 1.25, .91}};
+  static constexpr Cost costs[] = {{kMx256x256, 256, 256, 256, 1.9, 7.7, 11.61, .65},
+                                   {kMx256x128, 256, 128, 256, 0.9, 4.8, 7.10, .61},
+                                   {kMx128x128Pair, 128, 128, 512, 1.8, 3.3, 7.91, .42},
+                                   {kMx128x128, 128, 128, 256, 1.6, 2.7, 4.20, .66},
+                                   {kMx128x64, 128, 64, 256, 1.3, 2.2, 2.64, .82},
+                                   {kMx64x64, 64, 64, 256, 1.6, 1.9, 1.67, .83},
+                                   {kMx64x32, 64, 32, 256, 1.6, 1.6, 1.25, .88}};
   MxTiling best = kMx64x64;
   double best_us = 1e300;
   for (const Cost& c : costs) {

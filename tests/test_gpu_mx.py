@@ -32,7 +32,7 @@ def same_as_definition(mx, y):
 
 
 SIZES = [(2500, 130), (2048, 2300), (1, 1), (1, 32), (3, 31), (2, 33), (16, 128), (17, 129),
-         (5, 896), (64, 1000), (33, 2048), (7, 2049), (4, 4096), (3, 8200), (2, 12289),
+         (5, 896), (64, 1000), (33, 2048), (7, 2049), (4, 4096), (5, 5000), (3, 8200), (2, 12289),
          (1000, 40), (4099, 96), (4100, 700)]
 
 

@@ -289,16 +289,18 @@ int32_t launch_norm(const RowLayout& out, void* sum, const void* residual, const
   return check_launch("pa_rms_norm_mx");
 }
 // The fewest chunks of 8 columns a lane that hold the row (us, bf16 with add:
-// 2048 x 2048 8.9 in 1 or 2, 9.1 in 4, 10.5 in 8; 64 x 16384 9.4 in 8, 12.4
-// read again).  A wavefront a row up to 512 columns (2048 x 512 4.2, by a
-// workgroup 4.5); up to 1024 where the rows fill the chip many times over (7569
-// x 896 14.9 and 16.0, 2048 x 896 6.3 and 6.0, 32 x 896 3.6 and 3.0).
+// 2048 x 2048 8.9 in 1 or 2, 9.1 in 4, 10.5 in 8; 2048 x 6144 21.7 in 3, 22.9 in
+// 4; 64 x 16384 9.4 in 8, 12.4 read again; but 1500 x 12288 33.2 in 8, 38.7 in
+// 6).  A wavefront a row up to 512 columns (2048 x 512 4.2, by a workgroup 4.5);
+// up to 1024 where the rows fill the chip many times over (7569 x 896 14.9 and
+// 16.0, 2048 x 896 6.3 and 6.0, 32 x 896 3.6 and 3.0).
 template <typename T>
 auto choose_norm(int64_t chunks, int64_t rows) {
   return chunks <= 64                   ? launch_norm<T, 64, 1>
          : chunks <= 128 && rows >= 4096 ? launch_norm<T, 64, 2>
          : chunks <= 256                 ? launch_norm<T, 256, 1>
          : chunks <= 512                 ? launch_norm<T, 256, 2>
+         : chunks <= 768                 ? launch_norm<T, 256, 3>
          : chunks <= 1024                ? launch_norm<T, 256, 4>
          : chunks <= 2048                ? launch_norm<T, 256, 8>
                                          : launch_norm<T, 256, 0>;

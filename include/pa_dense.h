@@ -221,7 +221,9 @@ int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void* weight, i
  * The sums are f32, over groups of 16 columns whose exact products the matrix
  * instructions align to the group's largest, keeping 13 binary places below
  * its leading one: a result is off by about 2^-14 of its largest products,
- * well below the bf16 rounding unless terms cancel.
+ * well below the bf16 rounding unless terms cancel.  The scales of an MXFP8
+ * output are those of these results: where a block's largest value lies that
+ * near to a border it may take the neighbouring scale.
  * Any rows, N (with PA_ACT_NONE) and K up to 2^22.  The order of a row's f32
  * sums, and with it the last bit of an output, may depend on rows, N and K
  * (equal calls give equal bits). */

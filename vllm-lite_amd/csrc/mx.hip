@@ -67,6 +67,9 @@ struct RowLayout {
   __device__ uint32_t* scale(int64_t row, int64_t s) const {
     return reinterpret_cast<uint32_t*>(scales) + s * pad_rows + row;
   }
+  RowLayout from(int64_t row) const {
+    return {codes + row * steps * 128, scales + row * 4, steps, pad_rows};
+  }
 };
 struct WeightLayout {
   uint8_t *codes, *scales;
@@ -77,6 +80,9 @@ struct WeightLayout {
   }
   __device__ uint32_t* scale(int64_t row, int64_t s) const {
     return reinterpret_cast<uint32_t*>(scales) + (row / 16 * steps + s) * 16 + row % 16;
+  }
+  WeightLayout from(int64_t row) const {  // row: a multiple of 16
+    return {codes + row / 16 * steps * 2048, scales + row / 16 * steps * 64, steps};
   }
 };
 
@@ -269,24 +275,34 @@ int32_t launch_quantize(const char* what, const Layout& out, const void* x, int6
                         int64_t out_rows, int cols, int64_t stride, hipStream_t s) {
   int lg = 0;  // as many steps side by side as there are, up to 16
   while (lg < 4 && 1 << lg < out.steps) ++lg;
-  const int64_t groups = row_groups(out_rows, 16 >> lg);
   // many rows: whole rows to a workgroup (7569 x 4096: 17.7 us, 20.5 with the
   // steps over workgroups); few: the steps too (512 x 4096: 3.5, 3.7 by rows)
   const int across = (int)((out.steps + (1 << lg) - 1) >> lg);
   const int times = out_rows >= kNearRows ? across : 1;
-  quantize_mx_kernel<T, Layout>
-      <<<dim3((uint32_t)groups, (uint32_t)((across + times - 1) / times)), 256, 0, s>>>(
-          out, (const T*)x, rows, out_rows, cols, stride, lg, times, out_rows >= kNearRows);
-  return check_launch(what);
+  int32_t rc = PA_OK;
+  for (int64_t at = 0; at < out_rows && rc == PA_OK; at += kLaunchRows) {
+    const int64_t n = std::min(kLaunchRows, out_rows - at);
+    const dim3 grid((uint32_t)row_groups(n, 16 >> lg), (uint32_t)((across + times - 1) / times));
+    quantize_mx_kernel<T, Layout><<<grid, 256, 0, s>>>(
+        out.from(at), (const T*)x + at * stride, std::min(rows - at, n), n, cols, stride, lg,
+        times, n >= kNearRows);
+    rc = check_launch(what);
+  }
+  return rc;
 }
 
 template <typename T, int G, int C>
 int32_t launch_norm(const RowLayout& out, void* sum, const void* residual, const void* add,
                     const void* w, int64_t rows, int hidden, float eps, hipStream_t s) {
-  rms_norm_mx_kernel<T, G, C><<<(uint32_t)row_groups(rows, 256 / G), 256, 0, s>>>(
-      out, (T*)sum, (const T*)residual, (const T*)add, (const T*)w, rows, hidden, eps,
-      rows >= kNearRows);
-  return check_launch("pa_rms_norm_mx");
+  int32_t rc = PA_OK;
+  for (int64_t at = 0; at < rows && rc == PA_OK; at += kLaunchRows) {
+    const int64_t n = std::min(kLaunchRows, rows - at), first = at * hidden;
+    rms_norm_mx_kernel<T, G, C><<<(uint32_t)row_groups(n, 256 / G), 256, 0, s>>>(
+        out.from(at), add ? (T*)sum + first : nullptr, (const T*)residual + first,
+        add ? (const T*)add + first : nullptr, (const T*)w, n, hidden, eps, n >= kNearRows);
+    rc = check_launch("pa_rms_norm_mx");
+  }
+  return rc;
 }
 // The fewest chunks of 8 columns a lane that hold the row (us, bf16 with add:
 // 2048 x 2048 8.9 in 1 or 2, 9.1 in 4, 10.5 in 8; 2048 x 6144 21.7 in 3, 22.9 in

@@ -224,7 +224,9 @@ int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void* weight, i
  * well below the bf16 rounding unless terms cancel.  The scales of an MXFP8
  * output are those of these results: where a block's largest value lies that
  * near to a border it may take the neighbouring scale.
- * Any rows, N (with PA_ACT_NONE) and K up to 2^22.  The order of a row's f32
+ * Any rows, N (with PA_ACT_NONE) and K up to 2^22; PA_ERR_UNSUPPORTED where
+ * the outputs' tiles would need 2^32 threads (no such arrays fit a GPU, but for
+ * the last few of 2^31 rows).  The order of a row's f32
  * sums, and with it the last bit of an output, may depend on rows, N and K
  * (equal calls give equal bits). */
 int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x, const uint8_t* x_scales,

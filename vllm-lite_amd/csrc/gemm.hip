@@ -303,10 +303,12 @@ template <int WM, int WN, int TM, int TN, int KG, int BK, int S, typename Off = 
 int32_t launch(const GemmCall& c) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
   const int bno = c.silu ? BN / 2 : BN;
-  const int ntm = (c.M + BM - 1) / BM, ntn = (c.N + bno - 1) / bno;
-  PA_REQUIRE((long long)ntm * ntn < (1ll << 30), PA_ERR_UNSUPPORTED, "pa_linear: %d rows", c.M);
-  const dim3 grid(8 * ((ntm * ntn + 7) / 8));
   constexpr int NT = 64 * WM * WN * KG;
+  const int64_t rows = ((int64_t)c.M + BM - 1) / BM, cols = ((int64_t)c.N + bno - 1) / bno;
+  PA_REQUIRE(rows * cols < (1ll << 30) && grid_fits(rows * cols + 7, NT), PA_ERR_UNSUPPORTED,
+             "pa_linear: %d x %d outputs", c.M, c.N);
+  const int ntm = (int)rows, ntn = (int)cols;
+  const dim3 grid(8 * ((ntm * ntn + 7) / 8));
   if (c.silu)
     gemm_kernel<2, WM, WN, TM, TN, KG, BK, S, Off><<<grid, NT, 0, c.stream>>>(
         c.out, c.x, c.w, nullptr, c.M, c.N, c.K, 0, ntm, ntn);

@@ -523,8 +523,8 @@ int32_t launch(const MxLinear& p, hipStream_t stream) {
   // an MXFP8 output's padding is written too
   const int64_t cols = p.out_scales ? mx_steps(p.N) * 128 : p.N;
   const int64_t ntm = ((int64_t)p.M + BM - 1) / BM, ntn = (cols + BNO - 1) / BNO;
-  PA_REQUIRE(ntm * ntn < (1ll << 30), PA_ERR_UNSUPPORTED, "pa_linear_mx: %d x %d outputs", p.M,
-             p.N);
+  PA_REQUIRE(ntm * ntn < (1ll << 30) && grid_fits(ntm * ntn + 7, NT), PA_ERR_UNSUPPORTED,
+             "pa_linear_mx: %d x %d outputs", p.M, p.N);
   const dim3 grid(8 * (uint32_t)((ntm * ntn + 7) / 8));
   mx_gemm_kernel<SILU, WM, WN, TM, TN, KG, S><<<grid, NT, 0, stream>>>(p, (int)ntm, (int)ntn);
   return check_launch("pa_linear_mx");

@@ -211,9 +211,10 @@ inline size_t dtype_size(int32_t dtype) {
 }
 inline bool dtype_ok(int32_t dtype) { return dtype == PA_DTYPE_F32 || dtype == PA_DTYPE_BF16; }
 
-// Rows a launch, where a row has up to a workgroup of 256 threads.  A launch
-// counts its threads along x in 32 bits: of a grid beyond them the runtime
-// starts a part, and reports success.
+// A launch counts its threads along x in 32 bits: of a grid beyond them the
+// runtime starts a part, and reports success.
+inline bool grid_fits(int64_t groups, int threads) { return groups * threads < (1ll << 32); }
+// Rows a launch, where a row has up to a workgroup of 256 threads.
 constexpr int64_t kLaunchRows = 1 << 23;
 
 // Checks the launch that was just enqueued.

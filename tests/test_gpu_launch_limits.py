@@ -46,3 +46,32 @@ def test_rms_norm_mx(pa, with_add):
     few = pa.rms_norm_mx(base, w, 1e-6, add=add[:PERIOD].clone() if with_add else None)
     assert same_rows(pa.rms_norm_mx(x, w, 1e-6, add=add), few)
     assert repeats(x, base)  # with add the sum, in place
+
+
+@pytest.mark.parametrize("cols", [1032, 1001])  # rows in registers, and read again
+@pytest.mark.parametrize("name", ["rms_norm", "layer_norm"])
+def test_norms(pa, name, cols):
+    base, x = rows_of(cols)
+    w = torch.linspace(0.5, 2, cols, device=DEV).to(torch.bfloat16)
+    norm = getattr(pa, name)
+    add = x.flip(1)
+    few = norm(base, w, 1e-6, add=add[:PERIOD].clone())
+    assert repeats(norm(x, w, 1e-6, add=add), few)
+    assert repeats(x, base)
+
+
+def test_norm_of_wide_rows(pa):
+    """A workgroup per row held in registers."""
+    base, x = rows_of(2056)
+    w = torch.linspace(0.5, 2, 2056, device=DEV).to(torch.bfloat16)
+    few = pa.rms_norm(base, w, 1e-6)
+    assert repeats(pa.rms_norm(x, w, 1e-6, out=x), few)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [24, 17])
+def test_argmax(pa, cols, dtype):
+    """1024 threads per row."""
+    base, x = rows_of(cols, (1 << 22) + 3 * PERIOD)
+    base, x = base.to(dtype), x.to(dtype)
+    assert bool((pa.argmax(x).view(-1, PERIOD) == pa.argmax(base)).all())

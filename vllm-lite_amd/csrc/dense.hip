@@ -923,6 +923,28 @@ constexpr int kGemmKMultiple = 64;  // K the tiled kernel takes: a multiple of t
 
 using namespace pa;
 
+namespace {
+// pa_rms_norm (kLayer false) and pa_layer_norm of rows of T.
+template <typename T, bool kLayer>
+int32_t norm(const char* what, T* out, T* res, const T* add, const T* w, const T* bias,
+             int64_t rows, int hidden, float eps, hipStream_t s) {
+  int32_t rc = PA_OK;
+  for (int64_t at = 0; at < rows && rc == PA_OK; at += kLaunchRows) {
+    const int n = (int)std::min(kLaunchRows, rows - at);
+    T *o = out + at * hidden, *r = res + at * hidden;
+    const T* a = add ? add + at * hidden : nullptr;
+    if (!launch_norm_rows<T, kLayer>(o, r, a, w, bias, n, hidden, eps, s)) {
+      if constexpr (kLayer)
+        layer_norm_kernel<T><<<n, 256, 0, s>>>(o, r, a, w, bias, hidden, eps);
+      else
+        rms_norm_kernel<T><<<n, 256, 0, s>>>(o, r, a, w, hidden, eps);
+    }
+    rc = check_launch(what);
+  }
+  return rc;
+}
+}  // namespace
+
 extern "C" int32_t pa_rms_norm(void* out, void* residual, const void* add, const void* weight,
                                int32_t rows, int32_t hidden, float eps, int32_t dtype,
                                pa_stream_t stream) {
@@ -932,21 +954,12 @@ extern "C" int32_t pa_rms_norm(void* out, void* residual, const void* add, const
   if (rows == 0) return PA_OK;
   PA_REQUIRE(out && residual && weight, PA_ERR_INVALID_ARG, "pa_rms_norm: null pointer");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PA_DTYPE_BF16
-          ? launch_norm_rows<uint16_t, false>(out, residual, add, weight, nullptr, rows, hidden,
-                                              eps, s)
-          : launch_norm_rows<float, false>(out, residual, add, weight, nullptr, rows, hidden, eps,
-                                           s))
-    return check_launch("pa_rms_norm");
   if (dtype == PA_DTYPE_BF16)
-    rms_norm_kernel<uint16_t><<<rows, 256, 0, s>>>((uint16_t*)out, (uint16_t*)residual,
-                                                   (const uint16_t*)add, (const uint16_t*)weight,
-                                                   hidden, eps);
-  else
-    rms_norm_kernel<float><<<rows, 256, 0, s>>>((float*)out, (float*)residual,
-                                                (const float*)add, (const float*)weight, hidden,
-                                                eps);
-  return check_launch("pa_rms_norm");
+    return norm<uint16_t, false>("pa_rms_norm", (uint16_t*)out, (uint16_t*)residual,
+                                 (const uint16_t*)add, (const uint16_t*)weight, nullptr, rows,
+                                 hidden, eps, s);
+  return norm<float, false>("pa_rms_norm", (float*)out, (float*)residual, (const float*)add,
+                            (const float*)weight, nullptr, rows, hidden, eps, s);
 }
 
 extern "C" int32_t pa_layer_norm(void* out, void* residual, const void* add, const void* weight,
@@ -958,19 +971,12 @@ extern "C" int32_t pa_layer_norm(void* out, void* residual, const void* add, con
   if (rows == 0) return PA_OK;
   PA_REQUIRE(out && residual && weight, PA_ERR_INVALID_ARG, "pa_layer_norm: null pointer");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PA_DTYPE_BF16
-          ? launch_norm_rows<uint16_t, true>(out, residual, add, weight, bias, rows, hidden, eps, s)
-          : launch_norm_rows<float, true>(out, residual, add, weight, bias, rows, hidden, eps, s))
-    return check_launch("pa_layer_norm");
   if (dtype == PA_DTYPE_BF16)
-    layer_norm_kernel<uint16_t><<<rows, 256, 0, s>>>(
-        (uint16_t*)out, (uint16_t*)residual, (const uint16_t*)add, (const uint16_t*)weight,
-        (const uint16_t*)bias, hidden, eps);
-  else
-    layer_norm_kernel<float><<<rows, 256, 0, s>>>((float*)out, (float*)residual,
-                                                  (const float*)add, (const float*)weight,
-                                                  (const float*)bias, hidden, eps);
-  return check_launch("pa_layer_norm");
+    return norm<uint16_t, true>("pa_layer_norm", (uint16_t*)out, (uint16_t*)residual,
+                                (const uint16_t*)add, (const uint16_t*)weight,
+                                (const uint16_t*)bias, rows, hidden, eps, s);
+  return norm<float, true>("pa_layer_norm", (float*)out, (float*)residual, (const float*)add,
+                           (const float*)weight, (const float*)bias, rows, hidden, eps, s);
 }
 
 extern "C" int32_t pa_silu_mul(void* out, const void* gate_up, int32_t rows, int32_t inter,
@@ -1211,22 +1217,20 @@ extern "C" int32_t pa_argmax(int64_t* out, const void* logits, int32_t rows, int
   const int esz = dtype == PA_DTYPE_BF16 ? 2 : 4;
   const bool vec = (uintptr_t)logits % 16 == 0 && (row_stride * esz) % 16 == 0 &&
                    (cols * esz) % 16 == 0;
-  if (dtype == PA_DTYPE_BF16) {
-    if (vec)
-      argmax_kernel<uint16_t, 8><<<rows, kArgmaxThreads, 0, s>>>(out, (const uint16_t*)logits,
-                                                                 cols, row_stride);
+  constexpr int64_t kRows = kLaunchRows * 256 / kArgmaxThreads;
+  int32_t rc = PA_OK;
+  for (int64_t at = 0; at < rows && rc == PA_OK; at += kRows) {
+    const int n = (int)std::min(kRows, rows - at);
+    auto go = [&](auto kernel, auto* x) {
+      kernel<<<n, kArgmaxThreads, 0, s>>>(out + at, x + at * row_stride, cols, row_stride);
+    };
+    if (dtype == PA_DTYPE_BF16)
+      go(vec ? argmax_kernel<uint16_t, 8> : argmax_kernel<uint16_t, 1>, (const uint16_t*)logits);
     else
-      argmax_kernel<uint16_t, 1><<<rows, kArgmaxThreads, 0, s>>>(out, (const uint16_t*)logits,
-                                                                 cols, row_stride);
-  } else {
-    if (vec)
-      argmax_kernel<float, 4><<<rows, kArgmaxThreads, 0, s>>>(out, (const float*)logits, cols,
-                                                              row_stride);
-    else
-      argmax_kernel<float, 1><<<rows, kArgmaxThreads, 0, s>>>(out, (const float*)logits, cols,
-                                                              row_stride);
+      go(vec ? argmax_kernel<float, 4> : argmax_kernel<float, 1>, (const float*)logits);
+    rc = check_launch("pa_argmax");
   }
-  return check_launch("pa_argmax");
+  return rc;
 }
 
 extern "C" int32_t pa_linear_rope_cache(void* out, const void* x, const void* weight,

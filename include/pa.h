@@ -12,6 +12,8 @@
  *    "host".  The caller owns all memory; the stateless entry points
  *    allocate nothing.  Work is enqueued on `stream` (NULL = the default
  *    stream); nothing synchronises unless stated.
+ *    Calls whose launch would pass 2^32 threads (2^24 tokens or sequences and
+ *    more in some) return PA_ERR_UNSUPPORTED.
  *  - Return value: PA_OK (0) or a negative pa_status.  No entry point aborts,
  *    throws or unwinds; pa_last_error() gives a message for the calling
  *    thread's most recent failure.

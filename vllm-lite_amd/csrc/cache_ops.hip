@@ -522,15 +522,18 @@ int32_t launch_write_token(void* k_cache, void* v_cache, const void* key, const 
 
 namespace {
 template <typename Ids>
-void launch_read(const void* k_cache, const void* v_cache, int32_t dtype, const Ids& ids,
-                 int seq_len, int H, int D, int num_blocks, void* out_k, void* out_v,
-                 hipStream_t s) {
+int32_t launch_read(const char* what, const void* k_cache, const void* v_cache, int32_t dtype, const Ids& ids,
+                    int seq_len, int H, int D, int num_blocks, void* out_k, void* out_v,
+                    hipStream_t s) {
+  // less than a block: by token, which waits for one round trip (write + read
+  // of one token 18.1 us against 18.5 by block)
+  const bool by_block = seq_len >= kBlock && D <= kReadMaxD && H <= 65535;
+  const int64_t groups = by_block ? ((int64_t)seq_len + kBlock - 1) / kBlock : seq_len;
+  PA_REQUIRE(grid_fits(groups, 256), PA_ERR_UNSUPPORTED, "%s: %d tokens", what, seq_len);
   auto go = [&](auto elem) {
     using T = decltype(elem);
-    // less than a block: by token, which waits for one round trip (write + read
-    // of one token 18.1 us against 18.5 by block)
-    if (seq_len >= kBlock && D <= kReadMaxD && H <= 65535)
-      read_kv_block_kernel<T, Ids><<<dim3((seq_len + kBlock - 1) / kBlock, H), 256, 0, s>>>(
+    if (by_block)
+      read_kv_block_kernel<T, Ids><<<dim3((uint32_t)groups, H), 256, 0, s>>>(
           (const T*)k_cache, (const T*)v_cache, ids, seq_len, H, D, num_blocks, (T*)out_k,
           (T*)out_v);
     else
@@ -541,6 +544,7 @@ void launch_read(const void* k_cache, const void* v_cache, int32_t dtype, const 
     go(uint16_t{});
   else
     go(float{});
+  return check_launch(what);
 }
 }  // namespace
 
@@ -549,13 +553,10 @@ int32_t launch_read_kv_small(const void* k_cache, const void* v_cache, int32_t d
                              int num_blocks, void* out_k, void* out_v, hipStream_t stream) {
   auto go = [&](auto v) {
     for (int i = 0; i < n_ids && i < (int)(sizeof(v.id) / sizeof(v.id[0])); ++i) v.id[i] = ids[i];
-    launch_read(k_cache, v_cache, dtype, v, seq_len, H, D, num_blocks, out_k, out_v, stream);
+    return launch_read("read_kv", k_cache, v_cache, dtype, v, seq_len, H, D, num_blocks, out_k,
+                       out_v, stream);
   };
-  if (n_ids <= kFewIds)
-    go(SmallIds<kFewIds>{});
-  else
-    go(SmallIds<kSmallIds>{});
-  return check_launch("read_kv");
+  return n_ids <= kFewIds ? go(SmallIds<kFewIds>{}) : go(SmallIds<kSmallIds>{});
 }
 
 int32_t launch_block_hash_replay(const void* k_cache, const void* key, int32_t dtype, int H,
@@ -563,6 +564,7 @@ int32_t launch_block_hash_replay(const void* k_cache, const void* key, int32_t d
                                  const int32_t* task_beg, const int32_t* tok,
                                  const int32_t* off, uint64_t* hashes, hipStream_t stream) {
   if (num_tasks == 0) return PA_OK;
+  PA_REQUIRE_GRID("write_kv", num_tasks);
   if (dtype == PA_DTYPE_BF16)
     block_hash_replay_kernel<uint16_t><<<num_tasks, 256, 0, stream>>>(
         (const uint16_t*)k_cache, (const uint16_t*)key, H, D, task_block, task_beg, tok, off,
@@ -606,8 +608,10 @@ extern "C" int32_t pa_reshape_and_cache(const void* key, const void* value, void
                    ((uintptr_t)value % 16) == 0 && ((uintptr_t)k_cache % 16) == 0;
   const dim3 grid(num_tokens), block(256);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 wgrid((num_tokens + kBlock - 1) / kBlock, num_kv_heads);
   if (vec && head_dim <= 512 && ((uintptr_t)v_cache % 16) == 0) {
+    const int64_t groups = ((int64_t)num_tokens + kBlock - 1) / kBlock;
+    PA_REQUIRE_GRID("pa_reshape_and_cache", groups);
+    const dim3 wgrid((uint32_t)groups, num_kv_heads);
     if (dtype == PA_DTYPE_BF16)
       cache_write_kernel<uint16_t, uint16_t><<<wgrid, block, 0, s>>>(
           (const uint16_t*)key, (const uint16_t*)value, (uint16_t*)k_cache, (uint16_t*)v_cache,
@@ -619,6 +623,7 @@ extern "C" int32_t pa_reshape_and_cache(const void* key, const void* value, void
           num_tokens, num_kv_heads, head_dim, num_slots, key_stride, value_stride, nullptr);
     return check_launch("pa_reshape_and_cache");
   }
+  PA_REQUIRE_GRID("pa_reshape_and_cache", num_tokens);
   if (dtype == PA_DTYPE_BF16) {
     auto* kc = (uint16_t*)k_cache;
     auto* vc = (uint16_t*)v_cache;
@@ -673,7 +678,9 @@ int32_t reshape_and_cache_fp8_impl(const void* key, const void* value, uint8_t* 
   if (vec && head_dim <= 512 && ((uintptr_t)v_cache % 16) == 0 && ((uintptr_t)key % 16) == 0 &&
       ((uintptr_t)value % 16) == 0 && (key_stride * es) % 16 == 0 &&
       (value_stride * es) % 16 == 0) {
-    const dim3 wgrid((num_tokens + kBlock - 1) / kBlock, num_kv_heads);
+    const int64_t groups = ((int64_t)num_tokens + kBlock - 1) / kBlock;
+    PA_REQUIRE_GRID("pa_reshape_and_cache_fp8", groups);
+    const dim3 wgrid((uint32_t)groups, num_kv_heads);
     if (src_dtype == PA_DTYPE_BF16)
       cache_write_kernel<uint16_t, uint8_t><<<wgrid, block, 0, s>>>(
           (const uint16_t*)key, (const uint16_t*)value, k_cache, v_cache, slot_mapping,
@@ -684,6 +691,7 @@ int32_t reshape_and_cache_fp8_impl(const void* key, const void* value, uint8_t* 
           num_kv_heads, head_dim, num_slots, key_stride, value_stride, flags);
     return check_launch("pa_reshape_and_cache_fp8");
   }
+  PA_REQUIRE_GRID("pa_reshape_and_cache_fp8", num_tokens);
 #define PA_LAUNCH_Q(T, V)                                                                    \
   reshape_and_cache_fp8_kernel<T, V><<<grid, block, 0, s>>>(                                 \
       (const T*)key, (const T*)value, k_cache, v_cache, slot_mapping, num_kv_heads, head_dim, \
@@ -740,6 +748,7 @@ extern "C" int32_t pa_slot_mapping(const int32_t* block_tables, int32_t max_bloc
   if (num_seqs == 0 || num_tokens == 0) return PA_OK;
   PA_REQUIRE(block_tables && positions && cu_seq_tokens && slot_mapping, PA_ERR_INVALID_ARG,
              "pa_slot_mapping: null pointer");
+  PA_REQUIRE_GRID("pa_slot_mapping", num_seqs);
   slot_mapping_kernel<<<num_seqs, 256, 0, (hipStream_t)stream>>>(
       block_tables, max_blocks_per_seq, positions, cu_seq_tokens, num_tokens, slot_mapping);
   return check_launch("pa_slot_mapping");
@@ -760,13 +769,13 @@ extern "C" int32_t pa_read_kv(const void* k_cache, const void* v_cache, const in
   PA_REQUIRE(k_cache && v_cache && block_ids && out_k && out_v, PA_ERR_INVALID_ARG,
              "pa_read_kv: null pointer");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PA_DTYPE_FP8_E4M3)
-    read_kv_fp8_kernel<<<seq_len, 256, 0, s>>>(
-        (const uint8_t*)k_cache, (const uint8_t*)v_cache, block_ids, num_kv_heads, head_dim,
-        num_blocks, (float*)out_k, (float*)out_v);
-  else
-    launch_read(k_cache, v_cache, dtype, block_ids, seq_len, num_kv_heads, head_dim, num_blocks,
-                out_k, out_v, s);
+  if (dtype != PA_DTYPE_FP8_E4M3)
+    return launch_read("pa_read_kv", k_cache, v_cache, dtype, block_ids, seq_len, num_kv_heads,
+                       head_dim, num_blocks, out_k, out_v, s);
+  PA_REQUIRE_GRID("pa_read_kv", seq_len);
+  read_kv_fp8_kernel<<<seq_len, 256, 0, s>>>(
+      (const uint8_t*)k_cache, (const uint8_t*)v_cache, block_ids, num_kv_heads, head_dim,
+      num_blocks, (float*)out_k, (float*)out_v);
   return check_launch("pa_read_kv");
 }
 
@@ -779,6 +788,7 @@ extern "C" int32_t pa_block_hash(const float* k_cache, const int32_t* block_ids,
   if (n == 0) return PA_OK;
   PA_REQUIRE(k_cache && block_ids && hashes, PA_ERR_INVALID_ARG, "pa_block_hash: null pointer");
   const int64_t per_block = (int64_t)num_kv_heads * kBlock * head_dim;
+  PA_REQUIRE_GRID("pa_block_hash", n);
   block_hash_kernel<<<n, 256, 0, (hipStream_t)stream>>>(k_cache, block_ids, per_block, num_blocks,
                                                         hashes);
   return check_launch("pa_block_hash");

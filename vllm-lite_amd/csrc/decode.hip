@@ -1717,6 +1717,8 @@ int32_t decode_impl(void* out, const void* q, const void* k_cache, const void* v
       merge_waves > 1 && (np > 1 || plan.part_len > kPart / 2) ? 0 : plan.part_len;
   PA_REQUIRE(np <= 1024, PA_ERR_UNSUPPORTED,
              "pa_decode: context of %d tokens needs %d > 1024 partitions", max_context_len, np);
+  PA_REQUIRE(np == 1 || grid_fits((int64_t)num_seqs * num_heads, 256), PA_ERR_UNSUPPORTED,
+             "pa_decode: %d sequences in partitions", num_seqs);
   float* ws_o = nullptr;
   float* ws_ml = nullptr;
   if (plan.ws_bytes) {

@@ -229,6 +229,12 @@ inline int32_t check_launch(const char* what) {
 
 }  // namespace pa
 
+// A workgroup of 256 threads for each of n things: see grid_fits.
+#define PA_REQUIRE_GRID(what, n)                                               \
+  PA_REQUIRE(::pa::grid_fits((n), 256), PA_ERR_UNSUPPORTED,                    \
+             what ": %lld workgroups of 256 threads (less than 2^32 in all)",  \
+             (long long)(n))
+
 #define PA_REQUIRE(cond, code, ...) \
   do {                              \
     if (!(cond)) {                  \

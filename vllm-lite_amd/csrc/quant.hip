@@ -94,6 +94,7 @@ int32_t launch_quant_write(float* k_cache, float* v_cache, float* scales, const 
                            const int32_t* task_beg, const int32_t* tok, const int32_t* off,
                            uint64_t* hashes, hipStream_t stream) {
   if (num_tasks == 0) return PA_OK;
+  PA_REQUIRE_GRID("quantised write_kv", num_tasks);
   quant_write_kernel<<<num_tasks, 256, 0, stream>>>(k_cache, v_cache, scales, k, v, H, D,
                                                     task_block, task_beg, tok, off, hashes);
   return check_launch("quantised write_kv");
@@ -103,6 +104,7 @@ int32_t launch_quant_read(const float* k_cache, const float* v_cache, const floa
                           const int32_t* block_ids, int seq_len, int H, int D, float* out_k,
                           float* out_v, hipStream_t stream) {
   if (seq_len == 0) return PA_OK;
+  PA_REQUIRE_GRID("quantised read_kv", seq_len);
   quant_read_kernel<<<seq_len, 256, 0, stream>>>(k_cache, v_cache, scales, block_ids, H, D, out_k,
                                                  out_v);
   return check_launch("quantised read_kv");

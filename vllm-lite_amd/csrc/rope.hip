@@ -274,7 +274,8 @@ extern "C" int32_t pa_rope_reshape_and_cache(void* q, int64_t q_stride, const vo
   if (tiled) {
     // columns of workgroups over the heads: about four workgroups per CU, at
     // least one head pass each
-    const int tiles = (num_tokens + kTileTokens - 1) / kTileTokens;
+    const int tiles = (int)(((int64_t)num_tokens + kTileTokens - 1) / kTileTokens);
+    PA_REQUIRE_GRID("pa_rope_reshape_and_cache", tiles);
     const int at_once = 256 / (kTileTokens * head_dim / 16);
     const int rot = (num_heads + num_kv_heads + at_once - 1) / at_once;
     const int want = std::max(1, 1024 / tiles);
@@ -290,7 +291,10 @@ extern "C" int32_t pa_rope_reshape_and_cache(void* q, int64_t q_stride, const vo
           (float*)q, q_stride, (const float*)key, key_stride, (const float*)value, value_stride,
           (float*)k_cache, (float*)v_cache, slot_mapping, positions, inv_freq, num_tokens,
           num_heads, num_kv_heads, head_dim, num_slots, rot_cols);
-  } else if (dtype == PA_DTYPE_BF16)
+    return check_launch("pa_rope_reshape_and_cache");
+  }
+  PA_REQUIRE_GRID("pa_rope_reshape_and_cache", num_tokens);
+  if (dtype == PA_DTYPE_BF16)
     rope_cache_kernel<uint16_t><<<num_tokens, 256, 0, s>>>(
         (uint16_t*)q, q_stride, (const uint16_t*)key, key_stride, (const uint16_t*)value,
         value_stride, (uint16_t*)k_cache, (uint16_t*)v_cache, slot_mapping, positions, inv_freq,

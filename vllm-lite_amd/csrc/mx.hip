@@ -164,33 +164,31 @@ __device__ inline double row_sum(double v, double* red) {
   return v;
 }
 
-// v w / rms with r = 1 / rms as a sum of two floats, for a rounding to fewer
-// bits: the f32 nearest to the product (v r, then w, each with its error),
-// moved to the odd float beside it on the side where the product lies if that
-// f32 is even and not the product itself.  The borders between codes are even
-// floats, so the code is that of the product, as if it had not been rounded to
-// f32 in between.
-__device__ inline float scaled_odd(float v, float w, float r, float r_low) {
-#pragma clang fp contract(off)  // q's own rounding is part of q_low
-  const float p = v * r;
-  const float p_low = fmaf(v, r_low, fmaf(v, r, -p));
-  const float q = p * w;
-  const float q_low = fmaf(p_low, w, fmaf(p, w, -q));
-  const float y = q + q_low, low = q_low - (y - q);
+// v w / rms with d = 1 / rms, for a rounding to fewer bits: the f32 nearest to
+// the product (v w is exact in f64, and d's error and the product's are 2^-52 of
+// it), moved to the odd float beside it on the side where the product lies if
+// that f32 is even and not the product itself.  The borders between codes are
+// even floats, so the code is that of the product, as if it had not been rounded
+// to f32 in between.
+__device__ inline float scaled_odd(float v, float w, double d) {
+  const double q = (double)v * (double)w * d;
+  const float y = (float)q;
+  const double low = q - (double)y;
   const int bits = __builtin_bit_cast(int, y);
   // +1: away from zero
-  const int side = ((__builtin_bit_cast(int, low) ^ bits) >> 31) | 1;
+  const int side = (((int)(__builtin_bit_cast(uint64_t, low) >> 32) ^ bits) >> 31) | 1;
   constexpr int kFiniteNotZero = 0x198;  // of either sign
-  const bool move = __builtin_amdgcn_classf(low, kFiniteNotZero) && !(bits & 1);
+  const bool move = __builtin_amdgcn_class(low, kFiniteNotZero) && !(bits & 1);
   return __builtin_bit_cast(float, bits + (move ? side : 0));
 }
 
 // G lanes per row (64: a wavefront, 256: the workgroup), chunk i of lane l is
 // columns 8 (l + G i) ..  C > 0: the row fits C chunks a lane and stays in
 // registers; C = 0: it is read again for the second pass.  The sum of squares
-// is f64 and the scaling exact up to the rounding to codes where f32 leaves it
-// open, so that they are the codes of the formula, whatever the order of the
-// sum (in f32 throughout, 5 of 10^7 fell to the other side of a border).
+// and, where f32 leaves a code open, the scaling are f64, so that they are the
+// codes of the formula, whatever the order of the sum, unless it lies within
+// hidden 2^-53 of a border between codes (in f32 throughout, 5 of 10^7 fell to
+// the other side).
 // Bound by memory: 7569 x 4096 bf16 with add 43.1 us, 5.1 TB/s (a large copy:
 // 5.2); short of rows, by its latencies: 32 x 896 3.0 us.
 template <typename T, int G, int C>
@@ -219,23 +217,35 @@ __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum,
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fma((double)v[e], (double)v[e], ss);
   };
-  float r, r_low;
+  double d;
+  float r;
+  bool usual;  // r 2^kMxUp has all its bits
   auto finish = [&]() __attribute__((always_inline)) {
-    const double d = rsqrt(row_sum<G>(ss, red) / hidden + (double)eps);
-    r = (float)d;
-    r_low = (float)(d - (double)r);
+    d = rsqrt(row_sum<G>(ss, red) / hidden + (double)eps);
+    r = (float)(d * __builtin_ldexp(1., kMxUp));
+    usual = r >= 0x1p-126f && r < __builtin_inff();
   };
   auto write = [&](int ch, const V& v, const V& wv) __attribute__((always_inline)) {
-    // three roundings, each at most 2^-24, and r's
+    // 2^kMxUp times the values: three roundings, r's among them, each at most
+    // 2^-24 where v r and the values are normal floats.  So they are wherever a
+    // code is not zero, if the block's largest value is at least 2^-40: such
+    // values are above 2^-59, and v r, with any weight, above 2^(kMxUp - 187).
     float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = (float)v[e] * r * (float)wv[e];
-    uint32_t dword;
+    uint32_t dword, top;
     bool sure;
-    uint2 codes = mx_quantize8(y, dword, sure);
-    if (!__all(sure)) {  // about 1 of 100 times
+    uint2 codes = mx_quantize8_up(y, dword, top, sure);
+    constexpr uint32_t kSmall = (127u + kMxUp - 40) << 23;
+    if (__any(top < kSmall)) {  // zeros are exact
+      bool zero = true;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = scaled_odd((float)v[e], (float)wv[e], r, r_low);
+      for (int e = 0; e < 8; ++e) zero = zero && (float)v[e] == 0.f;
+      sure = sure && (top >= kSmall || zero);
+    }
+    if (!__all(sure && usual)) {  // about 1 of 100 times
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = scaled_odd((float)v[e], (float)wv[e], d);
       codes = mx_quantize8(y, dword);
     }
     *out.code(row, ch) = codes;

@@ -31,12 +31,14 @@ constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirr
 // The largest finite magnitude of N values, as the bits of a float (0 if none
 // is finite).  A maximum of floats finds it wherever all are finite; a NaN or
 // an infinity among them shows in the maximum, or (a quiet NaN) is passed over.
+// finite: whether none shows in the wavefront's maxima.
 template <int N>
-__device__ inline uint32_t mx_top(const float (&y)[N]) {
+__device__ inline uint32_t mx_top(const float (&y)[N], bool& finite) {
   float m = 0.f;
 #pragma unroll
   for (int e = 0; e < N; ++e) m = fmaxf(m, __builtin_fabsf(y[e]));
-  if (__any(!(m < __builtin_inff()))) {
+  finite = !__any(!(m < __builtin_inff()));
+  if (!finite) {
     uint32_t a = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -46,6 +48,11 @@ __device__ inline uint32_t mx_top(const float (&y)[N]) {
     return a;
   }
   return __builtin_bit_cast(uint32_t, m);
+}
+template <int N>
+__device__ inline uint32_t mx_top(const float (&y)[N]) {
+  bool finite;
+  return mx_top(y, finite);
 }
 // The scale byte of a block whose largest finite magnitude has bits a: with
 // a = 1.m 2^x, a <= 448 2^e = 1.75 2^(8 + e) asks for e >= x - 8, and one more
@@ -77,8 +84,8 @@ __device__ inline float mx_silu_mul(float g, float u) {
 // Eight consecutive columns per lane, a block over 4 lanes, 128 columns over
 // 16 lanes, which all run this: the largest magnitude of the lane's block, and
 // the four scale bytes of the 128 columns (in every lane) from the lane's own.
-__device__ inline uint32_t mx_block_top8(const float (&y)[8]) {
-  uint32_t a = mx_top(y);
+__device__ inline uint32_t mx_block_top8(const float (&y)[8], bool& finite) {
+  uint32_t a = mx_top(y, finite);
   a = max(a, dpp<kDppXor1>(a));
   return max(a, dpp<kDppXor2>(a));
 }
@@ -92,20 +99,31 @@ __device__ inline uint2 mx_codes8(const float (&y)[8], float inv) {
 }
 // Codes and scale bytes of y.
 __device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword) {
-  const uint32_t byte = mx_scale_byte(mx_block_top8(y));
+  bool finite;
+  const uint32_t byte = mx_scale_byte(mx_block_top8(y, finite));
   dword = mx_scale_dword8(byte);
   return mx_codes8(y, mx_inverse(byte));
 }
-// The same of values that y has within 2^-21 of their size; sure: whether the
-// lane's codes and scale are theirs all the same, i.e. equal at both ends.
-__device__ inline uint2 mx_quantize8(const float (&y)[8], uint32_t& dword, bool& sure) {
-  const uint32_t top = mx_block_top8(y), byte = mx_scale_byte(top);
-  const float inv = mx_inverse(byte);
+// The same of values of which y has 2^kMxUp times, within 2^-21 of their size;
+// top: mx_block_top8 of y; sure: whether the lane's codes and scale are theirs
+// all the same, i.e. equal at both ends (never where a y of the wavefront is not
+// finite, as times 2^kMxUp it may not be).
+constexpr int kMxUp = 64;
+__device__ inline uint2 mx_quantize8_up(const float (&y)[8], uint32_t& dword, uint32_t& top,
+                                        bool& sure) {
+  bool finite;
+  top = mx_block_top8(y, finite);
+  auto scale_byte = [](uint32_t a) __attribute__((always_inline)) {
+    const uint32_t x = (a + 0x1FFFFFu) >> 23;
+    return x > 8 + kMxUp ? x - (8 + kMxUp) : 0;
+  };
+  const uint32_t byte = scale_byte(top);  // up to 183, as top is finite
+  const float inv = __builtin_bit_cast(float, (254u - kMxUp - byte) << 23);
   dword = mx_scale_dword8(byte);
   const uint2 lo = mx_codes8(y, inv * (1.f - 0x1p-21f)), hi = mx_codes8(y, inv * (1.f + 0x1p-21f));
   // 8 steps of a float are at least 2^-21 of it
-  sure = lo.x == hi.x && lo.y == hi.y &&
-         mx_scale_byte(max(top, 8u) - 8) == mx_scale_byte(top + 8);
+  sure = finite && lo.x == hi.x && lo.y == hi.y &&
+         scale_byte(max(top, 8u) - 8) == scale_byte(top + 8);
   return lo;
 }
 

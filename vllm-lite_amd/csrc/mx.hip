@@ -314,22 +314,26 @@ int32_t launch_norm(const RowLayout& out, void* sum, const void* residual, const
   }
   return rc;
 }
-// The fewest chunks of 8 columns a lane that hold the row (us, bf16 with add:
-// 2048 x 2048 8.9 in 1 or 2, 9.1 in 4, 10.5 in 8; 2048 x 6144 21.7 in 3, 22.9 in
-// 4; 64 x 16384 9.4 in 8, 12.4 read again; but 1500 x 12288 33.2 in 8, 38.7 in
-// 6).  A wavefront a row up to 512 columns (2048 x 512 4.2, by a workgroup 4.5);
-// up to 1024 where the rows fill the chip many times over (7569 x 896 14.9 and
-// 16.0, 2048 x 896 6.3 and 6.0, 32 x 896 3.6 and 3.0).
+// The fewest chunks of 8 columns a lane that hold the row (us with add, bf16 and
+// f32: 2048 x 4096 16.0 and 26.5 in 2, 17.6 and 26.4 in 4, 17.9 and 27.7 in 8;
+// 2048 x 6144 22.8 and 37.6 in 3, 23.5 and 37.1 in 4; 64 x 16384 10.3 and 10.1 in
+// 8, 14.0 and 13.7 read again; but 1500 x 12288 33.8 and 56.0 in 8, 40.7 and 54.4
+// in 6).  A wavefront a row up to 512 columns (7569 x 256 7.8 and 8.8, by a
+// workgroup 10.3 and 11.8; 2048 x 512 4.7 and 5.8, by one 4.9 and 5.5); in bf16 up
+// to 1024 where the rows fill the chip many times over (7569 x 896 15.1, by one
+// 16.4; 2048 x 896 6.3 and 6.2, 32 x 896 3.7 and 3.2), in f32 not (7569 x 896 22.5,
+// by one 20.6; 7569 x 640 17.9 and 17.8).
 template <typename T>
 auto choose_norm(int64_t chunks, int64_t rows) {
-  return chunks <= 64                   ? launch_norm<T, 64, 1>
-         : chunks <= 128 && rows >= 4096 ? launch_norm<T, 64, 2>
-         : chunks <= 256                 ? launch_norm<T, 256, 1>
-         : chunks <= 512                 ? launch_norm<T, 256, 2>
-         : chunks <= 768                 ? launch_norm<T, 256, 3>
-         : chunks <= 1024                ? launch_norm<T, 256, 4>
-         : chunks <= 2048                ? launch_norm<T, 256, 8>
-                                         : launch_norm<T, 256, 0>;
+  if constexpr (sizeof(T) == 2)
+    if (chunks > 64 && chunks <= 128 && rows >= 4096) return launch_norm<T, 64, 2>;
+  return chunks <= 64     ? launch_norm<T, 64, 1>
+         : chunks <= 256  ? launch_norm<T, 256, 1>
+         : chunks <= 512  ? launch_norm<T, 256, 2>
+         : chunks <= 768  ? launch_norm<T, 256, 3>
+         : chunks <= 1024 ? launch_norm<T, 256, 4>
+         : chunks <= 2048 ? launch_norm<T, 256, 8>
+                          : launch_norm<T, 256, 0>;
 }
 
 }  // namespace

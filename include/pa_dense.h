@@ -219,11 +219,16 @@ int32_t pa_linear_mx_pack(uint8_t* codes, uint8_t* scales, const void* weight, i
  *   contiguous; residual may be out itself (the residual stream updated in
  *   place), but out overlaps no other argument.
  * The sums are f32, over groups of 16 columns whose exact products the matrix
- * instructions align to the group's largest, keeping 13 binary places below
- * its leading one: a result is off by about 2^-14 of its largest products,
- * well below the bf16 rounding unless terms cancel.  The scales of an MXFP8
- * output are those of these results: where a block's largest value lies that
- * near to a border it may take the neighbouring scale.
+ * instructions align to the group's largest, cutting them off (towards zero) 13
+ * binary places below its leading one.  A product loses less than 2^-13 of the
+ * group's largest, so a group is off by less than 2^-9 of it and a result by
+ * less than the sum of that over the K / 16 groups.  The losses have the signs of
+ * the products: where these are mixed they add up as the root of their squares
+ * (normal values, K 896 to 16384: 2^-16 of the result's root mean square, well
+ * below the bf16 rounding unless terms cancel).  silu is off by up to (1.5 |g| +
+ * 8) 2^-24 of it and 0 below -87.3, where it is less than 2^-119.  The scales of
+ * an MXFP8 output are those of these results: where a block's largest value lies
+ * that near to a border it may take the neighbouring scale.
  * Any rows, N (with PA_ACT_NONE) and K up to 2^22; PA_ERR_UNSUPPORTED where
  * the outputs' tiles would need 2^32 threads (no such arrays fit a GPU, but for
  * the last few of 2^31 rows).  The order of a row's f32

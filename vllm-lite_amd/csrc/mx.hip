@@ -8,6 +8,9 @@
 #include "pa_internal.hpp"
 #include "../../include/pa_dense.h"
 
+// Times here are a call's on the device, calls in a row, over sets of operands
+// that together pass the last-level cache.
+
 namespace pa {
 namespace {
 
@@ -89,8 +92,8 @@ struct WeightLayout {
 // The first of a workgroup's R rows (R a power of two up to 32).  near:
 // workgroups are dealt round-robin to the 8 XCDs; the rows of a group of 32,
 // whose scales share cache lines, then go to one XCD, so that its L2 puts the
-// lines together.  Norm of rows x 4096 with and without, us: 512 6.5 and 6.6,
-// 2048 15.7 and 16.9, 7569 43.1 and 44.2.
+// lines together.  Norm of rows x 4096 with and without, us: 512 6.7 and 6.7,
+// 2048 16.0 and 17.2, 7569 43.6 and 45.8.
 __device__ inline int64_t first_row(int64_t block, int R, int near) {
   if (!near) return block * R;
   const int64_t i = block / 8;
@@ -105,8 +108,8 @@ inline int64_t row_groups(int64_t rows, int R) {
 // Eight columns per thread, 16 threads per (row, step of 128 columns), a
 // workgroup 2^lg steps of 16 / 2^lg rows at a time, and `times` of these one
 // after another.  Rows `rows` .. `out_rows` are written as zeros (the padding
-// of a weight).  Bound by memory: 7569 x 4096 bf16 17.7 us, 5.3 TB/s (a large
-// copy: 5.2); 32 x 896 is a launch, 2.4 us.
+// of a weight).  Bound by memory: 7569 x 4096 bf16 20.3 us, 4.6 TB/s, f32 30.4 us,
+// 5.1 TB/s (a large copy: 5.2); 32 x 896 is a launch, 2.5 us.
 template <typename T, typename Layout>
 __global__ __launch_bounds__(256) void quantize_mx_kernel(Layout out, const T* __restrict__ x,
                                                           int64_t rows, int64_t out_rows, int cols,
@@ -189,8 +192,10 @@ __device__ inline float scaled_odd(float v, float w, double d) {
 // codes of the formula, whatever the order of the sum, unless it lies within
 // hidden 2^-53 of a border between codes (in f32 throughout, 5 of 10^7 fell to
 // the other side).
-// Bound by memory: 7569 x 4096 bf16 with add 43.1 us, 5.1 TB/s (a large copy:
-// 5.2); short of rows, by its latencies: 32 x 896 3.0 us.
+// Bound by memory: 7569 x 4096 with add, bf16 45 us, 4.9 TB/s, f32 80 us, 5.1
+// TB/s, f32 without 33 us, 4.8 TB/s (a large copy: 5.2); short of rows, by its
+// latencies: 32 x 896 3.0 us, with add 3.2.  bf16 without add, where a byte takes
+// the most arithmetic: 25.4 us, 3.7 TB/s.
 template <typename T, int G, int C>
 __global__ __launch_bounds__(256) void rms_norm_mx_kernel(RowLayout out, T* sum, const T* residual,
                                                           const T* __restrict__ add,
@@ -285,7 +290,7 @@ int32_t launch_quantize(const char* what, const Layout& out, const void* x, int6
                         int64_t out_rows, int cols, int64_t stride, hipStream_t s) {
   int lg = 0;  // as many steps side by side as there are, up to 16
   while (lg < 4 && 1 << lg < out.steps) ++lg;
-  // many rows: whole rows to a workgroup (7569 x 4096: 17.7 us, 20.5 with the
+  // many rows: whole rows to a workgroup (7569 x 4096: 20.1 us, 21.4 with the
   // steps over workgroups); few: the steps too (512 x 4096: 3.5, 3.7 by rows)
   const int across = (int)((out.steps + (1 << lg) - 1) >> lg);
   const int times = out_rows >= kNearRows ? across : 1;

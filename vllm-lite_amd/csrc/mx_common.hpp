@@ -73,10 +73,12 @@ __device__ inline uint32_t mx_codes4(float a, float b, float c, float d, float i
   return (uint32_t)v;
 }
 
-// silu(g) u = g u / (1 + e^-g) by the exponential and reciprocal instructions
-// (a few units of 2^-24, far below the products' own error): a tile's epilogue
-// runs with one or two wavefronts per SIMD, where expf and the division took
-// 9 us of a 256 x 256 tile.
+// silu(g) u = g u / (1 + e^-g) by the exponential and reciprocal instructions: a
+// tile's epilogue runs with one or two wavefronts per SIMD, where expf and the
+// division took 9 us of a 256 x 256 tile.  Off by (1.5 |g| + 8) 2^-24 of it at
+// most: e^-g is exp2 of the rounded g log2(e), so its error grows with |g| (2^-17
+// at -87).  Below -87.3 the reciprocal is below the normal floats, and the result
+// 0.
 __device__ inline float mx_silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
 }

@@ -1,6 +1,8 @@
 // pa_linear_mx: Y[M, N] = X[M, K] · W[N, K]ᵀ on MXFP8 rows and weights
 // (layouts: include/pa_dense.h), a tiled GEMM on the scaled matrix
-// instructions.
+// instructions.  Times here are a call's on the device, calls in a row, over sets
+// of operands that together pass the last-level cache (large products: three
+// sets).
 #include <algorithm>
 #include <type_traits>
 
@@ -50,12 +52,13 @@ struct MxLinear {
 // rows; a wavefront takes TN/2 gate tiles and their up tiles.
 //
 // 256 x 256 tiles read the fewest operand bytes per product, and their four
-// wavefronts, one per SIMD, hold the accumulators in 256 registers each.  Times
-// and rates (normal values): 7569 x 4096 x 4096 113 us, 2250 TFLOP/s; 8192^3
-// 410 us, 2680; gate|up 2048 x 24576 x 4096 with its codes 160 us, 2580 (a
-// library's product alone, one scale per matrix: 103, 381 and 143 us).  Bound
-// by the matrix units' power: on zeros 8192^3 takes 377 us (without the copies
-// 280), on normal values products alone reach 3590 TFLOP/s of the 4700 on
+// wavefronts, one per SIMD, hold the accumulators in 256 registers each (and
+// three that only the epilogues read in scratch).  Times and rates (normal
+// values): 7569 x 4096 x 4096 112 us, 2270 TFLOP/s, with the residual 123, in
+// place 117; 8192^3 412 us, 2670; gate|up 2048 x 24576 x 4096 with its codes 166
+// us, 2480, in bf16 169 (a library's product alone, one scale per matrix: 103, 381
+// and 143 us).  Bound by the matrix units' power: on zeros 8192^3 takes 375 us
+// (without the copies 280), on normal values products alone reach 3590 TFLOP/s of the 4700 on
 // zeros.  Fetching lines into L2 ahead of the copies took zeros to 318 us and
 // normal values to 409, at the first two sizes nothing, and is left out.  Fewer
 // tiles than fill the chip: the copies' latency, see mx_tiling.hpp.
@@ -545,10 +548,11 @@ int32_t launch(const MxLinear& p, hipStream_t stream) {
 // of the wavefront's own, copied in whole 128-byte lines (loaded as the
 // operands need it, half a line per row and load, L2 served it at half its
 // rate, and 32 rows took 4 us longer than 1 at 896 x 4864).
-// Bound by the weights' bytes where they are many, and by X's, which every
-// workgroup reads (4096 x 12288: 1 row 11.6 us, 4.3 TB/s, 17 rows 13.8, 32
-// rows 16.8; three steps in flight 11.2, 15.0, 18.1); else by a launch and a
-// few steps' latency (32 x 1152 x 896 3.1 us).
+// Bound by the weights' bytes where they are many (1 x 151936 x 896 22.9 us, 6.1
+// TB/s), and by X's, which every workgroup reads (4096 x 12288: 1 row 11.7 us, 4.4
+// TB/s, 17 rows 14.1, 32 rows 17.2; three steps in flight 3% less for 1 row, 8%
+// more for 17 and 32; 32 x 151936 x 896 30.4, 64 rows 44.8); else by a launch and a
+// few steps' latency (32 x 1152 x 896 3.4 us, with the bias 3.7).
 template <bool SILU, int MT, int NT, int KW>
 __global__ __launch_bounds__(64 * KW * (SILU ? 2 : 1), MT == 4 ? 2 : 4) void mx_skinny_kernel(
     const MxLinear p, int kw, int share, int more) {

@@ -64,3 +64,17 @@ def test_decode(pa, dtype, seqs, heads):
     assert lib.pa_decode(out, q, k, v, tables, 1 << 12, lens, 1 << 16, seqs, heads, 1, 64, 1 << 20,
                          1., ws, 1 << 62, dtype, None) == UNSUPPORTED
     assert b"in partitions" in lib.pa_last_error()
+
+
+@pytest.mark.parametrize("dtype,head_dim,max_q", [(0, 64, 1 << 26), (0, 24, 1 << 26),
+                                                  (1, 256, 1 << 26), (1, 40, 2 ** 31 - 1),
+                                                  (2, 40, 1 << 26), (1, 64, 2 ** 31 - 1),
+                                                  (1, 128, 2 ** 31 - 1)])
+def test_prefill(pa, dtype, head_dim, max_q):
+    """A bound on the rows of a sequence that no launch holds (the tiled kernels:
+    over enough sequences and heads)."""
+    lib = pa._lib.load()
+    out, q, k, v, tables, cu, past = FAR
+    assert lib.pa_prefill(out, q, k, v, tables, 16, cu, past, 64, 1000, max_q, 8, 8, head_dim,
+                          1 << 20, 1., dtype, None) == UNSUPPORTED
+    assert b"too large" in lib.pa_last_error()

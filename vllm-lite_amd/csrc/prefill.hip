@@ -1348,6 +1348,9 @@ int32_t prefill_impl(void* out, const void* q, const void* k_cache, const void* 
                          (uintptr_t)v_cache) % 16 == 0 &&
                         q_row % 4 == 0 && num_seqs <= 65535 &&
                         (long long)num_kv_heads * ((num_heads / num_kv_heads + 3) / 4) <= 65535;
+  // the other kernels' most threads per row of q (prefill_generic_kernel's)
+  PA_REQUIRE(tiled || grid_fits(max_q_len, 64), PA_ERR_UNSUPPORTED,
+             "pa_prefill: launch too large");
   if (tiled) {
     const int G = num_heads / num_kv_heads;
     const int HW = G < 4 ? G : 4;
@@ -1359,7 +1362,7 @@ int32_t prefill_impl(void* out, const void* q, const void* k_cache, const void* 
       constexpr int KG = decltype(kgc)::value;
       using TC = decltype(cache);
       const int TT = 16 * NT * (W / KG / 4) * (4 / HW);
-      const int tiles_per_seq = (max_q_len + TT - 1) / TT;
+      const int tiles_per_seq = (int)(((int64_t)max_q_len + TT - 1) / TT);
       const long long total = (long long)num_seqs * num_kv_heads * head_groups * tiles_per_seq;
       PA_REQUIRE(total < (1ll << 31) / 8, PA_ERR_UNSUPPORTED, "pa_prefill: launch too large");
       const int per_xcd = (int)((total + 7) / 8);

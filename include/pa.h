@@ -333,6 +333,87 @@ int32_t pa_prefill_quantized(void* out, const void* q, const float* k_cache, con
                              int32_t head_dim, int32_t num_blocks, float scale,
                              pa_stream_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* The int8 cache                                                         */
+/* ---------------------------------------------------------------------- */
+
+/* A cache of one byte an element that keeps 7 to 8 bits of precision: codes int8
+ * in the block layouts above (K [NB, Hkv, 16, D], V [NB, Hkv, D, 16]) and a scale
+ * byte for each (block, kv head) of each, k_scales / v_scales [NB, Hkv] uint8.  A
+ * value is code * 2^(byte - 127); scale bytes are 1 to 254 (0 reads as scale 0).
+ * No counterpart in the reference, whose quantised cache keeps int8 values in f32
+ * with one scale for a block's K, V and heads (pa_kv_cache_create_quantized).
+ * q and out are bf16, head_dim is 32, 64, 96, 128, 192 or 256
+ * (PA_ERR_UNSUPPORTED for others), code arrays are 16-byte aligned. */
+
+/* Appends tokens to their sequences' blocks.  Sequence s owns rows
+ * cu_seq_tokens[s] .. cu_seq_tokens[s + 1] - 1 (n of them) and has
+ * context_lens[s] tokens with them: row i is position
+ * context_lens[s] - n + i, in block block_tables[s][position / 16].  For each
+ * touched block and kv head, of K and of V by themselves:
+ *   a = the largest |x| among the call's finite values there
+ *   e = the least integer >= -126 with a <= 127 * 2^e
+ *   if the block's token 0 is not among the call's: its scale may not shrink,
+ *     e = max(e, byte - 127), and where that is more, the codes of the tokens
+ *     before the call's become code * 2^(byte - 127 - e), rounded
+ *   codes = x * 2^-e, rounded; NaN gives 0, infinities +-127
+ * all to nearest, ties to even.  A call that writes a block's token 0 starts the
+ * block afresh, whatever it held.  Codes behind the call's last token stay.
+ *   key, value    [T, Hkv, D] of dtype (PA_DTYPE_F32 or PA_DTYPE_BF16) with token
+ *                 strides in elements (0 = contiguous), any alignment
+ *   q, inv_freq   both or neither: query heads q [T, num_heads, D] of dtype, token
+ *                 stride q_stride, rotated in place, and keys rotated before they
+ *                 are quantised, as pa_rope_reshape_and_cache does (angle_i =
+ *                 position * inv_freq[i] in f32; inv_freq [D / 2] f32)
+ *   max_tokens    host upper bound of a sequence's n: of longer ones the rows
+ *                 behind it are not written
+ * Tokens whose table entry is missing or outside [0, num_blocks) write nothing (q
+ * is still rotated); sequences with context_lens[s] < n neither.  cu_seq_tokens
+ * outside [0, num_tokens] are clamped on the device.  A block is written by one
+ * sequence of a call: what two that share one leave there is unspecified. */
+int32_t pa_append_int8(int8_t* k_cache, int8_t* v_cache, uint8_t* k_scales, uint8_t* v_scales,
+                       const void* key, int64_t key_stride, const void* value,
+                       int64_t value_stride, void* q, int64_t q_stride, const float* inv_freq,
+                       const int32_t* block_tables, int32_t max_blocks_per_seq,
+                       const int32_t* cu_seq_tokens, const int32_t* context_lens,
+                       int32_t num_seqs, int32_t num_tokens, int32_t max_tokens,
+                       int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t num_blocks, int32_t dtype, pa_stream_t stream);
+
+/* pa_read_kv of an int8 cache: the first seq_len tokens of one sequence as f32
+ * values, out_k / out_v [seq_len, Hkv, D].  Any head_dim. */
+int32_t pa_read_kv_int8(const int8_t* k_cache, const int8_t* v_cache, const uint8_t* k_scales,
+                        const uint8_t* v_scales, const int32_t* block_ids, int32_t n_ids,
+                        int32_t seq_len, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t num_blocks, float* out_k, float* out_v, pa_stream_t stream);
+
+/* Bytes of workspace pa_decode_int8 needs for these sizes (0: none). */
+size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t max_context_len);
+
+/* pa_decode over an int8 cache, arguments and conventions as there (any number of
+ * query heads per kv head; calls that may overlap need workspaces of their own).
+ * The scores are exact products of the codes with q rounded to 15 bits of its
+ * row's largest value, probabilities times the V scale are rounded to bf16, sums
+ * are f32.  A query row with a NaN or an infinity gives NaN. */
+int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
+                       const uint8_t* k_scales, const uint8_t* v_scales,
+                       const int32_t* block_tables, int32_t max_blocks_per_seq,
+                       const int32_t* context_lens, int32_t max_context_len, int32_t num_seqs,
+                       int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t num_blocks, float scale, void* workspace, size_t workspace_bytes,
+                       pa_stream_t stream);
+
+/* pa_prefill over an int8 cache, arguments and conventions as there, arithmetic as
+ * pa_decode_int8. */
+int32_t pa_prefill_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
+                        const uint8_t* k_scales, const uint8_t* v_scales,
+                        const int32_t* block_tables, int32_t max_blocks_per_seq,
+                        const int32_t* cu_q_lens, const int32_t* past_lens, int32_t num_seqs,
+                        int32_t total_q, int32_t max_q_len, int32_t num_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, float scale,
+                        pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,15 +10,21 @@ raises.
 from . import _lib
 from .ops import (
     BLOCK_SIZE,
+    Int8Cache,
     MxRows,
     MxWeight,
     PaError,
+    append_int8,
     argmax,
     block_hash,
     decode,
+    decode_int8,
+    decode_int8_workspace_size,
     decode_workspace_size,
     prefill,
+    prefill_int8,
     read_kv,
+    read_kv_int8,
     reshape_and_cache,
     reshape_and_cache_fp8,
     rope_inv_freq,
@@ -36,17 +42,23 @@ from .kv_cache import PagedKvCache, StepBatch
 
 __all__ = [
     "BLOCK_SIZE",
+    "Int8Cache",
     "MxRows",
     "MxWeight",
     "PaError",
     "PagedKvCache",
     "StepBatch",
+    "append_int8",
     "argmax",
     "block_hash",
     "decode",
+    "decode_int8",
+    "decode_int8_workspace_size",
     "decode_workspace_size",
     "prefill",
+    "prefill_int8",
     "read_kv",
+    "read_kv_int8",
     "reshape_and_cache",
     "reshape_and_cache_fp8",
     "rope_inv_freq",

@@ -52,6 +52,14 @@ SIGNATURES = {
                                    _i32, _i32, _f32, _p, _sz, _p]),
     "pa_prefill_quantized": (_i32, [_p, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32,
                                     _i32, _i32, _i32, _f32, _p]),
+    "pa_append_int8": (_i32, [_p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i32, _p, _p,
+                              _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
+    "pa_read_kv_int8": (_i32, [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "pa_decode_int8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "pa_decode_int8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32,
+                              _i32, _f32, _p, _sz, _p]),
+    "pa_prefill_int8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32,
+                               _i32, _i32, _i32, _f32, _p]),
     "pa_kv_cache_create_quantized": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_p)]),
     "pa_kv_cache_is_quantized": (_i32, [_p]),
     "pa_kv_cache_scales_ptr": (_p, [_p, _i32]),

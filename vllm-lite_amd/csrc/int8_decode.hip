@@ -1,0 +1,245 @@
+// Single-token attention over the int8 cache (pa_decode_int8).
+//
+// A workgroup of NW wavefronts takes part_len tokens of one sequence for up to 16
+// query heads of one kv head; its wavefronts share them in steps of 64 tokens and
+// merge through LDS.  Contexts of several parts leave a result for each in the
+// workspace, which a second launch merges.
+// Bound by memory: every code is read once, for all heads of its group.
+#include <algorithm>
+
+#include "int8_wave.hpp"
+#include "pa_internal.hpp"
+
+namespace pa {
+namespace {
+
+constexpr int kStep = 4 * kBlock;  // tokens a step
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void decode_int8_kernel(
+    uint16_t* __restrict__ out, const uint16_t* __restrict__ q, int64_t q_row,
+    const int8_t* __restrict__ kc, const int8_t* __restrict__ vc, const uint8_t* __restrict__ ks,
+    const uint8_t* __restrict__ vs, const int32_t* __restrict__ tables, int mbs,
+    const int32_t* __restrict__ context_lens, int Hq, int Hkv, int G, int head_groups,
+    int num_blocks, float scale_log2, int num_parts, int part_len, float* __restrict__ ws_o,
+    float* __restrict__ ws_ml) {
+  constexpr int DT = D / 16;
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = blockIdx.x, seq = blockIdx.z;
+  const int kvh = blockIdx.y / head_groups, h0 = (blockIdx.y % head_groups) * 16;
+  const int heads = min(G - h0, 16);  // query heads of this workgroup
+  const int64_t row0 = (int64_t)seq * Hq + kvh * G + h0;
+  Int8Query<D> qv;
+  int8_query<D>(c < heads ? q + (int64_t)seq * q_row + (int64_t)(kvh * G + h0 + c) * D : nullptr,
+                j, scale_log2, qv);
+  const int ctx = min(context_lens[seq], mbs * kBlock);
+  const int begin = part * part_len, end = min(ctx, begin + part_len);
+  if (begin >= end && part > 0) return;  // (part 0 of an empty context writes zeros)
+  // this wavefront's steps
+  const int steps = max(0, (end - begin + kStep - 1) / kStep);
+  const int s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
+  const int32_t* tab = tables + (int64_t)seq * mbs;
+  const Int8Blocks<D> blocks{kc, vc, ks, vs, Hkv, kvh};
+  Int8State<D> S;
+  S.init();
+  int32_t ids = -1;
+  for (int s = s0; s < s1; ++s) {
+    const int b = (begin + s * kStep) / kBlock;  // the step's first block
+    // lane t holds the id of block t of the next 16 steps
+    const int ahead = (s - s0) % 16;
+    if (ahead == 0) ids = b + lane < mbs ? tab[b + lane] : -1;
+    int id[4];
+    bool whole = true;
+    int lim = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      id[g] = __builtin_amdgcn_readlane(ids, 4 * ahead + g);
+      const bool ok = id[g] >= 0 && id[g] < num_blocks;
+      const int n = ok ? min(max(end - (b + g) * kBlock, 0), kBlock) : 0;
+      if (!ok) id[g] = 0;
+      whole = whole && n == kBlock;
+      lim = g == j ? n : lim;
+    }
+    Int8Step<D> st;
+    blocks.load(id, c, j, st);
+    int8_step<D>(st, qv, whole, lim, S);
+  }
+  float lsum = S.lsum;
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  // The wavefronts' results meet in LDS.
+  __shared__ float so[NW][16][D];
+  __shared__ float sml[NW][16][2];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    *reinterpret_cast<f32x4*>(&so[wave][c][16 * dt + 4 * j]) = S.o[dt];
+  if (j == 0) {
+    sml[wave][c][0] = S.m;
+    sml[wave][c][1] = lsum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * D; i += 64 * NW) {
+    const int h = i / D, d = i % D;
+    float m = kInt8NoMax;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, sml[w][h][0]);
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float a = __builtin_amdgcn_exp2f(sml[w][h][0] - m);
+      num += a * so[w][h][d];
+      den += a * sml[w][h][1];
+    }
+    if (num_parts == 1) {
+      // den is 0 for a row without keys; NaN goes through
+      out[row0 * D + i] = f32_to_bf16_bits(den != 0.f ? num / den : 0.f);
+    } else {
+      const int64_t at = (row0 + h) * num_parts + part;
+      ws_o[at * D + d] = num;
+      if (d == 0) {
+        ws_ml[2 * at] = m;
+        ws_ml[2 * at + 1] = den;
+      }
+    }
+  }
+}
+
+// Merges the parts of one (sequence, query head).
+__global__ __launch_bounds__(256) void decode_int8_merge_kernel(
+    uint16_t* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
+    const int32_t* __restrict__ context_lens, int Hq, int D, int num_parts, int part_len,
+    int mbs) {
+  const int64_t row = blockIdx.x;
+  const int ctx = min(context_lens[row / Hq], mbs * kBlock);
+  const int np = min(num_parts, (max(ctx, 1) + part_len - 1) / part_len);
+  const float* ml = ws_ml + 2 * row * num_parts;
+  const float* o = ws_o + row * num_parts * D;
+  float m = kInt8NoMax;
+  for (int p = 0; p < np; ++p) m = fmaxf(m, ml[2 * p]);
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  float num = 0.f, den = 0.f;
+  for (int p = 0; p < np; ++p) {
+    const float a = __builtin_amdgcn_exp2f(ml[2 * p] - m);
+    num += a * o[(int64_t)p * D + d];
+    den += a * ml[2 * p + 1];
+  }
+  out[row * D + d] = f32_to_bf16_bits(den != 0.f ? num / den : 0.f);
+}
+
+// Tokens of a part for a launch over contexts of up to max_ctx tokens.
+struct Int8Plan {
+  int part_len, parts;
+};
+Int8Plan plan_of(int num_seqs, int num_heads, int num_kv_heads, int max_ctx) {
+  const int groups = (num_heads / num_kv_heads + 15) / 16;
+  const long long pairs = (long long)num_seqs * num_kv_heads * groups;
+  int len = 4096;
+  while (len > 256 && pairs * ((max_ctx + len - 1) / len) < 512) len /= 2;
+  if (len >= max_ctx) len = std::max(kStep, (max_ctx + kStep - 1) / kStep * kStep);
+  return {len, std::max(1, (int)(((long long)max_ctx + len - 1) / len))};
+}
+
+}  // namespace
+}  // namespace pa
+
+using namespace pa;
+
+extern "C" size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads,
+                                                int32_t num_kv_heads, int32_t head_dim,
+                                                int32_t max_context_len) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
+      head_dim <= 0 || max_context_len <= 0)
+    return 0;
+  const Int8Plan p = plan_of(num_seqs, num_heads, num_kv_heads, max_context_len);
+  return p.parts == 1 ? 0
+                      : (size_t)num_seqs * num_heads * p.parts * (head_dim + 2) * sizeof(float);
+}
+
+namespace pa {
+int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_t* k_cache,
+                            const int8_t* v_cache, const uint8_t* k_scales,
+                            const uint8_t* v_scales, const int32_t* block_tables,
+                            int32_t max_blocks_per_seq, const int32_t* context_lens,
+                            int32_t max_context_len, int32_t num_seqs, int32_t num_heads,
+                            int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, float scale,
+                            void* workspace, size_t workspace_bytes, hipStream_t s) {
+  clear_error();
+  PA_REQUIRE(num_seqs >= 0 && num_heads > 0 && num_kv_heads > 0 && head_dim > 0 &&
+                 num_blocks > 0 && max_blocks_per_seq > 0 && max_context_len >= 0,
+             PA_ERR_INVALID_ARG, "pa_decode_int8: bad sizes");
+  PA_REQUIRE(num_heads % num_kv_heads == 0, PA_ERR_INVALID_ARG,
+             "pa_decode_int8: num_heads %d not a multiple of num_kv_heads %d", num_heads,
+             num_kv_heads);
+  PA_REQUIRE((int64_t)max_blocks_per_seq * kBlock >= max_context_len &&
+                 (int64_t)max_blocks_per_seq * kBlock < (1ll << 31) - 4096,
+             PA_ERR_OUT_OF_BOUNDS,
+             "pa_decode_int8: max_context_len %d, block table of %d blocks", max_context_len,
+             max_blocks_per_seq);
+  PA_REQUIRE(int8_head_dim(head_dim), PA_ERR_UNSUPPORTED, "pa_decode_int8: head_dim %d", head_dim);
+  if (num_seqs == 0 || max_context_len == 0) return PA_OK;
+  PA_REQUIRE(out && q && k_cache && v_cache && k_scales && v_scales && block_tables &&
+                 context_lens,
+             PA_ERR_INVALID_ARG, "pa_decode_int8: null pointer");
+  if (q_row == 0) q_row = (int64_t)num_heads * head_dim;
+  PA_REQUIRE(q_row >= (int64_t)num_heads * head_dim, PA_ERR_INVALID_ARG,
+             "pa_decode_int8: q row stride %lld below num_heads * head_dim", (long long)q_row);
+  PA_REQUIRE(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (uintptr_t)q % 4 == 0 &&
+                 q_row % 2 == 0 && (uintptr_t)out % 2 == 0,
+             PA_ERR_INVALID_ARG, "pa_decode_int8: caches not 16-byte or q not 4-byte aligned");
+  const int G = num_heads / num_kv_heads, head_groups = (G + 15) / 16;
+  const Int8Plan plan = plan_of(num_seqs, num_heads, num_kv_heads, max_context_len);
+  const int np = plan.parts;
+  PA_REQUIRE(num_seqs <= 65535 && (long long)num_kv_heads * head_groups <= 65535 &&
+                 (long long)num_blocks * num_kv_heads < (1ll << 32) && grid_fits(np, 512) &&
+                 grid_fits((int64_t)num_seqs * num_heads, 256),
+             PA_ERR_UNSUPPORTED, "pa_decode_int8: launch too large");
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
+  if (np > 1) {
+    const size_t rows = (size_t)num_seqs * num_heads * np;
+    const size_t need = rows * (head_dim + 2) * sizeof(float);
+    PA_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 4 == 0,
+               PA_ERR_WORKSPACE, "pa_decode_int8: workspace of %zu bytes needed, %zu given", need,
+               workspace ? workspace_bytes : 0);
+    ws_o = (float*)workspace;
+    ws_ml = ws_o + rows * head_dim;
+  }
+  const dim3 grid(np, num_kv_heads * head_groups, num_seqs);
+#define PA_LAUNCH_DECODE_INT8(DD)                                                              \
+  decode_int8_kernel<DD, (DD <= 128 ? 8 : 4)><<<grid, 64 * (DD <= 128 ? 8 : 4), 0, s>>>(       \
+      (uint16_t*)out, (const uint16_t*)q, q_row, k_cache, v_cache, k_scales, v_scales,         \
+      block_tables, max_blocks_per_seq, context_lens, num_heads, num_kv_heads, G, head_groups, \
+      num_blocks, scale * kInt8Log2e, np, plan.part_len, ws_o, ws_ml)
+  switch (head_dim) {
+    case 32: PA_LAUNCH_DECODE_INT8(32); break;
+    case 64: PA_LAUNCH_DECODE_INT8(64); break;
+    case 96: PA_LAUNCH_DECODE_INT8(96); break;
+    case 128: PA_LAUNCH_DECODE_INT8(128); break;
+    case 192: PA_LAUNCH_DECODE_INT8(192); break;
+    default: PA_LAUNCH_DECODE_INT8(256); break;
+  }
+#undef PA_LAUNCH_DECODE_INT8
+  int32_t rc = check_launch("pa_decode_int8");
+  if (rc != PA_OK || np == 1) return rc;
+  decode_int8_merge_kernel<<<num_seqs * num_heads, 256, 0, s>>>(
+      (uint16_t*)out, ws_o, ws_ml, context_lens, num_heads, head_dim, np, plan.part_len,
+      max_blocks_per_seq);
+  return check_launch("pa_decode_int8 merge");
+}
+}  // namespace pa
+
+extern "C" int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache,
+                                  const int8_t* v_cache, const uint8_t* k_scales,
+                                  const uint8_t* v_scales, const int32_t* block_tables,
+                                  int32_t max_blocks_per_seq, const int32_t* context_lens,
+                                  int32_t max_context_len, int32_t num_seqs, int32_t num_heads,
+                                  int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
+                                  float scale, void* workspace, size_t workspace_bytes,
+                                  pa_stream_t stream) {
+  return decode_int8_strided(out, q, 0, k_cache, v_cache, k_scales, v_scales, block_tables,
+                             max_blocks_per_seq, context_lens, max_context_len, num_seqs,
+                             num_heads, num_kv_heads, head_dim, num_blocks, scale, workspace,
+                             workspace_bytes, (hipStream_t)stream);
+}

@@ -1,0 +1,237 @@
+// Attention of one wavefront over an int8 cache: 16 query rows (the columns of the
+// matrix instructions) against a run of 16-token blocks, four blocks a step.
+//
+// Lanes (lane = 16 j + c):
+//   Sᵀ = K·Qᵀ on v_mfma_i32_16x16x64_i8, the codes as they lie in memory.  The
+//     query row is a fixed-point number of 15 bits, 2^e (128 hi + lo), hi and lo
+//     int8, so a score is 128 K·hi + K·lo in exact 32-bit integers; what is rounded
+//     is q alone, by at most 2^-14 of the row's largest (bf16 would round the scaled
+//     q by 2^-9 of each value).  Tile kk's row 4 g + r is token 4 kk + r of block g: the
+//     lane (c, j) receives query c's scores of block j, token 4 kk + r in x[4 kk + r],
+//     and the block's K scale is one factor a lane.
+//   Oᵀ += Vᵀ·Pᵀ on v_mfma_f32_16x16x32_bf16: a lane loads the 16 tokens of dim
+//     16 dt + c of block j (16 bytes of the token-minor block), and holds their
+//     probabilities already.  The codes become bf16 exactly; the V scale goes into
+//     the probability, which is rounded to bf16 with it (2^-9 of each).
+// All loads are 16 bytes a lane.
+#pragma once
+
+#include "int8_common.hpp"
+
+namespace pa {
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kInt8Log2e = 1.4426950408889634f;
+// "No maximum yet": below any score, and m - m is 0.
+constexpr float kInt8NoMax = -3.0e38f;
+
+// Four int8 codes of w as floats, and pairs of those as bf16 (exact: the low half
+// of such a float is 0).
+__device__ inline uint32_t codes_bf16x2(uint32_t w, int at) {
+  const float a = (float)(int8_t)(w >> (8 * at));
+  const float b = (float)(int8_t)(w >> (8 * at + 8));
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a),
+                               0x07060302u);
+}
+__device__ inline bf16x8 codes_bf16x8(uint32_t lo, uint32_t hi) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  const u32x4_t r = {codes_bf16x2(lo, 0), codes_bf16x2(lo, 2), codes_bf16x2(hi, 0),
+                     codes_bf16x2(hi, 2)};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+template <int D>
+struct Int8Query {
+  static constexpr int KS = (D + 63) / 64;  // reduction steps of 64 dims
+  i32x4 hi[KS], lo[KS];
+  float factor;  // of a score: scale * log2(e) * 2^e; NaN for a row that is not finite
+};
+
+// The 16-byte chunk of a K row that reduction step s reads in lane group j; a chunk
+// past the row (dims not a multiple of 64) reads another, against zeros.
+template <int D>
+__device__ inline int int8_chunk(int s, int j) {
+  const int ch = 4 * s + j;
+  return D % 64 == 0 || ch < D / 16 ? ch : ch - 2;
+}
+
+// Splits the query row at `row` (null: zeros), dims as int8_chunk says; the lanes
+// of a column hold the row's parts.
+template <int D>
+__device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, Int8Query<D>& q) {
+  constexpr int KS = Int8Query<D>::KS;
+  float x[KS][16];
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const bool on = row && (D % 64 == 0 || 4 * s + j < D / 16);
+    uint4 w[2] = {uint4{0, 0, 0, 0}, uint4{0, 0, 0, 0}};
+    if (on) {
+      struct __attribute__((aligned(4))) Half {  // rows of any 4-byte alignment
+        uint32_t v[8];
+      };
+      const Half h = *reinterpret_cast<const Half*>(row + 16 * (4 * s + j));
+      w[0] = uint4{h.v[0], h.v[1], h.v[2], h.v[3]};
+      w[1] = uint4{h.v[4], h.v[5], h.v[6], h.v[7]};
+    }
+    const uint32_t d[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[s][i] = bf16_bits_to_f32((uint16_t)(d[i / 2] >> (16 * (i & 1))));
+      const float m = fabsf(x[s][i]);
+      bad |= !(m < INFINITY);
+      amax = fmaxf(amax, m);
+    }
+  }
+  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+  int worse = bad;
+  worse |= __shfl_xor(worse, 16, 64);
+  worse |= __shfl_xor(worse, 32, 64);
+  // |x| 2^-e < 2^14 - 64: the largest is m 2^b, m < 2, so e = b - 13 gives less than
+  // 2^14 and hi at most 128 where m is near 2; e = b - 12 there
+  const uint32_t u = __builtin_bit_cast(uint32_t, amax);
+  int e = (int)(u >> 23) - 127 - 13 + ((u & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
+  e = max(e, -140);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    uint32_t hw[4], lw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hw[i] = lw[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int n = worse ? 0 : (int)rintf(ldexpf(x[s][i], -e));
+      const int hi = (n + 64) >> 7, lo = n - 128 * hi;
+      hw[i / 4] |= (uint32_t)(uint8_t)hi << (8 * (i & 3));
+      lw[i / 4] |= (uint32_t)(uint8_t)lo << (8 * (i & 3));
+    }
+    q.hi[s] = i32x4{(int)hw[0], (int)hw[1], (int)hw[2], (int)hw[3]};
+    q.lo[s] = i32x4{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
+  }
+  q.factor = worse ? __builtin_nanf("") : ldexpf(scale_log2, e);
+}
+
+// A wavefront's online softmax: o unnormalised, m in the log2 domain, lsum this
+// lane's share of the denominator.
+template <int D>
+struct Int8State {
+  f32x4 o[D / 16];
+  float m, lsum;
+  __device__ void init() {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = kInt8NoMax;
+    lsum = 0.f;
+  }
+};
+
+// What a step of four blocks brings in.
+template <int D>
+struct Int8Step {
+  static constexpr int KS = Int8Query<D>::KS;
+  i32x4 k[4][KS];
+  i32x4 v[D / 16];
+  uint32_t kb, vb;  // scale bytes of block j
+};
+
+template <int D>
+struct Int8Blocks {
+  const int8_t* kc;
+  const int8_t* vc;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int Hkv, kvh;
+  // Loads the step whose four blocks' ids (in the pool) are id[g].
+  __device__ inline void load(const int (&id)[4], int c, int j, Int8Step<D>& st) const {
+    const int g = c >> 2;
+    const uint32_t kid = g < 2 ? (g ? id[1] : id[0]) : (g == 2 ? id[2] : id[3]);
+    const uint32_t vid = j < 2 ? (j ? id[1] : id[0]) : (j == 2 ? id[2] : id[3]);
+    const uint32_t kslice = kid * (uint32_t)Hkv + kvh, vslice = vid * (uint32_t)Hkv + kvh;
+    const int8_t* kr = kc + (uint64_t)kslice * (kBlock * D) + (c & 3) * D;
+    const int8_t* vr = vc + (uint64_t)vslice * (kBlock * D) + c * kBlock;
+    st.kb = ks[vslice];
+    st.vb = vs[vslice];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int s = 0; s < Int8Step<D>::KS; ++s)
+        st.k[kk][s] = __builtin_nontemporal_load(
+            reinterpret_cast<const i32x4*>(kr + 4 * kk * D + 16 * int8_chunk<D>(s, j)));
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+      st.v[dt] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vr + dt * 16 * kBlock));
+  }
+};
+
+// One step into the softmax.  lim: tokens of block j (this lane's scores) that
+// query c attends, 16 where `whole` (wavefront-uniform).
+template <int D>
+__device__ inline void int8_step(const Int8Step<D>& st, const Int8Query<D>& q, bool whole, int lim,
+                                 Int8State<D>& S) {
+  constexpr int KS = Int8Query<D>::KS;
+  i32x4 a[4];
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) a[kk] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      a[kk] = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.k[kk][s], q.hi[s], a[kk], 0, 0, 0);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[kk][r] <<= 7;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      a[kk] = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.k[kk][s], q.lo[s], a[kk], 0, 0, 0);
+  // blocks that are not attended may hold any bytes
+  const bool none = !whole && lim <= 0;
+  const float f = ldexpf(q.factor, none ? 0 : (int)st.kb - 127);
+  const int ev = none ? 0 : (int)st.vb - 127;
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = (float)a[i >> 2][i & 3] * f;
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i >= lim) x[i] = -INFINITY;
+  }
+  float bm = x[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) bm = fmaxf(bm, x[i]);
+  // the maximum stays until a score passes it by 2^8
+  if (__builtin_amdgcn_ballot_w64(bm > S.m + 8.0f)) {
+    bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+    bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+    const float mn = fmaxf(S.m, bm);
+    const float r = __builtin_amdgcn_exp2f(S.m - mn);
+    S.m = mn;
+    S.lsum *= r;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) S.o[dt] *= r;
+  }
+  const float fv = ldexpf(1.f, ev);
+  bf16x8 p0, p1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float p = __builtin_amdgcn_exp2f(x[i] - S.m);
+    S.lsum += p;
+    if (i < 8)
+      p0[i] = (__bf16)(p * fv);
+    else
+      p1[i - 8] = (__bf16)(p * fv);
+  }
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) {
+    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        codes_bf16x8(st.v[dt][0], st.v[dt][1]), p0, S.o[dt], 0, 0, 0);
+    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        codes_bf16x8(st.v[dt][2], st.v[dt][3]), p1, S.o[dt], 0, 0, 0);
+  }
+}
+
+}  // namespace pa

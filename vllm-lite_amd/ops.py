@@ -726,3 +726,162 @@ def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_ou
     _mx_call("pa_linear_mx", device, data, scales, x.codes.data_ptr(), x.scales.data_ptr(),
              weight.codes.data_ptr(), weight.scales.data_ptr(), bias, residual, rows, n, k, act)
     return out
+
+
+# ---- the int8 cache (pa.h) --------------------------------------------------
+
+
+class Int8Cache:
+    """One layer's int8 cache: codes k int8 [NB, H, 16, D] and v int8
+    [NB, H, D, 16], scale bytes k_scales and v_scales uint8 [NB, H]; a value is
+    code * 2^(byte - 127), see pa.h.  Int8Cache.empty makes a zeroed one."""
+
+    __slots__ = ("k", "v", "k_scales", "v_scales", "num_blocks", "num_kv_heads", "head_dim")
+
+    def __init__(self, k, v, k_scales, v_scales):
+        if k.dim() != 4 or k.shape[2] != BLOCK_SIZE:
+            raise ValueError("k must be [NB, H, 16, D]")
+        nb, h, _, d = k.shape
+        device = k.device
+        if not k.is_cuda:
+            raise ValueError("an int8 cache is on the device")
+        for name, t, shape, dtype in (("k", k, (nb, h, BLOCK_SIZE, d), torch.int8),
+                                      ("v", v, (nb, h, d, BLOCK_SIZE), torch.int8),
+                                      ("k_scales", k_scales, (nb, h), torch.uint8),
+                                      ("v_scales", v_scales, (nb, h), torch.uint8)):
+            if not _mx_like(t, shape, dtype, device):
+                _mx_refuse(name, t, shape, dtype, device)
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.num_blocks, self.num_kv_heads, self.head_dim = nb, h, d
+
+    @classmethod
+    def empty(cls, num_blocks, num_kv_heads, head_dim, device="cuda"):
+        """A zeroed cache."""
+        def zeros(*shape, dtype=torch.int8):
+            return torch.zeros(shape, dtype=dtype, device=device)
+
+        nb, h, d = num_blocks, num_kv_heads, head_dim
+        return cls(zeros(nb, h, BLOCK_SIZE, d), zeros(nb, h, d, BLOCK_SIZE),
+                   zeros(nb, h, dtype=torch.uint8), zeros(nb, h, dtype=torch.uint8))
+
+    def _ptrs(self):
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scales.data_ptr(),
+                self.v_scales.data_ptr())
+
+
+def _int8_index(name, t, shape, device):
+    if not _mx_like(t, shape, torch.int32, device):
+        _mx_refuse(name, t, shape, torch.int32, device)
+    return t.data_ptr()
+
+
+def _int8_tables(block_tables, device):
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [num_seqs, max_blocks_per_seq]")
+    _int8_index("block_tables", block_tables, block_tables.shape, device)
+    return block_tables.shape
+
+
+def append_int8(cache, key, value, block_tables, cu_seq_tokens, context_lens, max_tokens, q=None,
+                inv_freq=None):
+    """pa_append_int8: quantises key / value [T, H, D] (bf16 or f32, rows that may
+    be strided views) into the cache's blocks.  Sequence s owns rows
+    cu_seq_tokens[s] .. [s + 1] and has context_lens[s] tokens with them
+    (block_tables [B, MBS], cu_seq_tokens [B + 1], context_lens [B], int32);
+    max_tokens: the most of any sequence.  With inv_freq (f32 [D / 2]), q
+    [T, Hq, D] is rotated in place and the keys on their way."""
+    device, h, d = cache.k.device, cache.num_kv_heads, cache.head_dim
+    b, mbs = _int8_tables(block_tables, device)
+    t = key.shape[0]
+    code = _dtype_code(key)
+    if (q is None) != (inv_freq is None):
+        raise ValueError("q is rotated with inv_freq: both or neither")
+    hq = 0 if q is None else q.shape[1] if q.dim() == 3 else 0
+    for name, x, heads in (("key", key, h), ("value", value, h), ("q", q, hq)):
+        if x is None:
+            continue
+        if x.shape != (t, heads, d) or heads == 0 or x.dtype != key.dtype or x.device != device:
+            raise ValueError(f"{name}: expected {key.dtype} [{t}, {heads or 'Hq'}, {d}] on "
+                             f"{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        if not _rows_ok(x, heads, d):
+            raise ValueError(f"{name}: rows must be contiguous [H, D], not overlapping")
+    if inv_freq is not None and not _mx_like(inv_freq, (d // 2,), torch.float32, device):
+        _mx_refuse("inv_freq", inv_freq, (d // 2,), torch.float32, device)
+    _mx_call("pa_append_int8", device, *cache._ptrs(), key.data_ptr(),
+             key.stride(0) if t > 1 else 0, value.data_ptr(), value.stride(0) if t > 1 else 0,
+             None if q is None else q.data_ptr(), 0 if q is None or t <= 1 else q.stride(0),
+             None if inv_freq is None else inv_freq.data_ptr(), block_tables.data_ptr(), mbs,
+             _int8_index("cu_seq_tokens", cu_seq_tokens, (b + 1,), device),
+             _int8_index("context_lens", context_lens, (b,), device), b, t, max_tokens, hq, h, d,
+             cache.num_blocks, code)
+
+
+def read_kv_int8(cache, block_ids, seq_len):
+    """pa_read_kv_int8: one sequence's first seq_len tokens as f32 (k, v)
+    [seq_len, H, D]; block_ids int32."""
+    device = cache.k.device
+    if block_ids.dim() != 1:
+        raise ValueError("block_ids must be one-dimensional")
+    ids = _int8_index("block_ids", block_ids, block_ids.shape, device)
+    shape = (seq_len, cache.num_kv_heads, cache.head_dim)
+    out_k, out_v = (torch.empty(shape, dtype=torch.float32, device=device) for _ in range(2))
+    _mx_call("pa_read_kv_int8", device, *cache._ptrs(), ids, block_ids.shape[0], seq_len,
+             cache.num_kv_heads, cache.head_dim, cache.num_blocks, out_k.data_ptr(),
+             out_v.data_ptr())
+    return out_k, out_v
+
+
+def decode_int8_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len):
+    return _lib.load().pa_decode_int8_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim,
+                                                     max_context_len)
+
+
+def _int8_q(q, cache, out):
+    device = cache.k.device
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError("q must be [rows, Hq, D]")
+    if not _mx_like(q, q.shape, torch.bfloat16, device):
+        _mx_refuse("q", q, q.shape, torch.bfloat16, device)
+    if out is None:
+        return torch.empty_like(q)
+    if not _mx_like(out, q.shape, torch.bfloat16, device):
+        _mx_refuse("out", out, q.shape, torch.bfloat16, device)
+    return out
+
+
+def decode_int8(q, cache, block_tables, context_lens, max_context_len, scale=None, out=None,
+                workspace=None):
+    """pa_decode_int8: q [B, Hq, D] bf16 -> out [B, Hq, D]."""
+    device, d = cache.k.device, cache.head_dim
+    out = _int8_q(q, cache, out)
+    n, hq, _ = q.shape
+    b, mbs = _int8_tables(block_tables, device)
+    if b != n:
+        raise ValueError(f"block_tables of {b} sequences, q of {n}")
+    lens = _int8_index("context_lens", context_lens, (b,), device)
+    if workspace is None:
+        need = decode_int8_workspace_size(b, hq, cache.num_kv_heads, d, max_context_len)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {device}")
+    _mx_call("pa_decode_int8", device, out.data_ptr(), q.data_ptr(), *cache._ptrs(),
+             block_tables.data_ptr(), mbs, lens, max_context_len, b, hq, cache.num_kv_heads, d,
+             cache.num_blocks, 1.0 / math.sqrt(d) if scale is None else scale,
+             None if workspace is None else workspace.data_ptr(),
+             0 if workspace is None else workspace.numel() * workspace.element_size())
+    return out
+
+
+def prefill_int8(q, cache, block_tables, cu_q_lens, past_lens, max_q_len, scale=None, out=None):
+    """pa_prefill_int8: q [total_q, Hq, D] bf16 -> out [total_q, Hq, D]."""
+    device, d = cache.k.device, cache.head_dim
+    out = _int8_q(q, cache, out)
+    n, hq, _ = q.shape
+    b, mbs = _int8_tables(block_tables, device)
+    _mx_call("pa_prefill_int8", device, out.data_ptr(), q.data_ptr(), *cache._ptrs(),
+             block_tables.data_ptr(), mbs, _int8_index("cu_q_lens", cu_q_lens, (b + 1,), device),
+             _int8_index("past_lens", past_lens, (b,), device), b, n, max_q_len, hq,
+             cache.num_kv_heads, d, cache.num_blocks,
+             1.0 / math.sqrt(d) if scale is None else scale)
+    return out

@@ -247,6 +247,40 @@ int32_t pa_linear_mx(void* out, uint8_t* out_scales, const uint8_t* x, const uin
 int32_t pa_argmax(int64_t* out, const void* logits, int32_t rows, int32_t cols,
                   int64_t row_stride, int32_t dtype, pa_stream_t stream);
 
+/* Draws a token from each row of a logit matrix.  With the row's settings T =
+ * temperature, k = top_k, p = top_p, m = min_p and u = uniform, x its logits and
+ * M the largest:
+ *   w_i = exp((x_i - M) / T): 1 where x_i = M (also +inf), 0 for -inf; NaN is no
+ *         value and never drawn
+ *   top-k (0 < k < cols): the k largest are kept, of equal ones the first
+ *   top-p (p < 1): of those, in descending order (equal ones by index), the
+ *         shortest run whose weights sum to p times the sum of all of them or
+ *         more; one at least
+ *   min-p (m > 0): of those the ones with w_i >= m, and the largest
+ *   out[r] = the first kept i, in the order of the columns, whose weights up to
+ *         and with it sum to more than u times the sum of all kept
+ * T not above 0: the argmax of pa_argmax.  A row without a value above -inf gives
+ * 0.  u is in [0, 1): below 0 and NaN count as 0, 1 and more draw the last.
+ *   uniform [rows] f32; temperature, top_p, min_p [rows] f32 and top_k [rows]
+ *   int32, each may be NULL (1, off, off, off); all device
+ *   logits  [rows, cols] of dtype with row_stride elements between rows (0 =
+ *           cols), rows at any element; cols up to 2^22, rows up to 65535
+ *   out     [rows] int64 (device)
+ * Weights are formed in f64 and summed exactly in units of 2^-(62 - b), b =
+ * max(1, ceil(log2 cols)), of the largest: the draw is that of the formula but for
+ * borders closer than a few of those times cols, and does not depend on the order
+ * of anything.
+ * workspace: pa_sample_workspace_size() bytes, 16-byte aligned, with any contents;
+ * calls that may overlap need workspaces of their own.
+ * The reference samples on the host (crates/core/src/sampling.rs). */
+int32_t pa_sample(int64_t* out, const void* logits, const float* uniform,
+                  const float* temperature, const int32_t* top_k, const float* top_p,
+                  const float* min_p, int32_t rows, int32_t cols, int64_t row_stride,
+                  void* workspace, size_t workspace_bytes, int32_t dtype, pa_stream_t stream);
+
+/* Workspace bytes of pa_sample. */
+size_t pa_sample_workspace_size(int32_t rows);
+
 #ifdef __cplusplus
 }
 #endif

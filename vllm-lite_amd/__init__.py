@@ -35,6 +35,8 @@ from .ops import (
     rms_norm,
     rms_norm_mx,
     rope_reshape_and_cache,
+    sample,
+    sample_workspace_size,
     silu_mul,
     slot_mapping,
 )
@@ -69,6 +71,8 @@ __all__ = [
     "rms_norm",
     "rms_norm_mx",
     "rope_reshape_and_cache",
+    "sample",
+    "sample_workspace_size",
     "silu_mul",
     "slot_mapping",
 ]

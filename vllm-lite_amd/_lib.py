@@ -45,6 +45,8 @@ SIGNATURES = {
     "pa_linear_mx_pack": (_i32, [_p, _p, _p, _i32, _i32, _i32, _p]),
     "pa_linear_mx": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p]),
     "pa_argmax": (_i32, [_p, _p, _i32, _i32, _i64, _i32, _p]),
+    "pa_sample": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i64, _p, _sz, _i32, _p]),
+    "pa_sample_workspace_size": (_sz, [_i32]),
     "pa_linear_rope_cache": (_i32, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
                                     _p, _p, _p, _p, _p, _i32, _i32, _p]),
     "pa_linear_pack_qkv": (_i32, [_p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]),

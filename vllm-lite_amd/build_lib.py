@@ -14,7 +14,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpa.so")
 SOURCES = ["cache_ops.hip", "decode.hip", "prefill.hip", "rope.hip", "quant.hip", "dense.hip",
            "gemm.hip", "mx.hip", "mx_gemm.hip", "int8_cache.hip", "int8_decode.hip",
-           "int8_prefill.hip", "kv_cache.cpp", "batch.cpp"]
+           "int8_prefill.hip", "sample.hip", "kv_cache.cpp", "batch.cpp"]
 ARCH = os.environ.get("PA_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

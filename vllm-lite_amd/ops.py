@@ -394,6 +394,54 @@ def argmax(logits, out=None):
     return out
 
 
+def sample_workspace_size(rows):
+    return _lib.load().pa_sample_workspace_size(rows)
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None,
+           workspace=None):
+    """pa_sample: token ids drawn from logit rows [rows, vocab] (bf16 or f32, unit
+    stride along the vocab) with the uniform numbers `uniform` (f32 [rows], in
+    [0, 1)) -> int64 [rows].  temperature, top_p, min_p (f32 [rows]) and top_k
+    (int32 [rows]): each row's settings, None for 1, off, off, off; a temperature
+    of 0 is the argmax.  workspace: sample_workspace_size(rows) bytes (uint8)."""
+    if not logits.is_cuda:
+        raise ValueError("sample: expected a device tensor")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("sample: logits must be [rows, vocab] with unit column stride")
+    rows, cols = logits.shape
+    device = logits.device
+    code = _dtype_code(logits)
+    if not 0 < cols <= 1 << 22 or rows > 65535:
+        raise ValueError(f"sample: {rows} rows of {cols} (at most 65535 of 2^22)")
+    if rows > 1 and logits.stride(0) < cols:
+        logits = logits.contiguous()  # rows that overlap (e.g. an expanded view)
+    ptrs = []
+    for name, t, dtype in (("uniform", uniform, torch.float32),
+                           ("temperature", temperature, torch.float32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        if t is None and name != "uniform":
+            ptrs.append(None)
+            continue
+        if t is None or not _mx_like(t, (rows,), dtype, device):
+            raise ValueError(f"{name}: expected a contiguous {dtype} tensor [{rows}] on {device}")
+        ptrs.append(t.data_ptr())
+    if out is None:
+        out = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)
+    elif not _mx_like(out, (rows,), torch.int64, device):
+        _mx_refuse("out", out, (rows,), torch.int64, device)
+    if workspace is None:
+        workspace = torch.empty_strided((sample_workspace_size(rows),), (1,), dtype=torch.uint8,
+                                        device=device)
+    elif workspace.device != device or workspace.dtype != torch.uint8 or \
+            not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous uint8 tensor on {device}")
+    _mx_call("pa_sample", device, out.data_ptr(), logits.data_ptr(), *ptrs, rows, cols,
+             logits.stride(0) if rows > 1 else cols, workspace.data_ptr(), workspace.numel(), code)
+    return out
+
+
 ACT_NONE, ACT_SILU_MUL = 0, 1
 LINEAR_RMS_IN, LINEAR_ADD_OUT = 1, 2
 

@@ -50,7 +50,14 @@ typedef struct ihipStream_t* pa_stream_t; /* same type as hipStream_t */
 
 #define PA_BLOCK_SIZE 16
 
-typedef enum pa_dtype { PA_DTYPE_F32 = 0, PA_DTYPE_BF16 = 1, PA_DTYPE_FP8_E4M3 = 2 } pa_dtype;
+/* PA_DTYPE_INT8: what pa_kv_cache_dtype says of an int8 cache (below), which has
+ * entry points of its own. */
+typedef enum pa_dtype {
+  PA_DTYPE_F32 = 0,
+  PA_DTYPE_BF16 = 1,
+  PA_DTYPE_FP8_E4M3 = 2,
+  PA_DTYPE_INT8 = 3
+} pa_dtype;
 
 typedef enum pa_status {
   PA_OK = 0,

@@ -51,6 +51,19 @@ int32_t pa_kv_cache_is_quantized(const pa_kv_cache* cache);
 /* Device f32 [num_blocks] block scales of one layer (NULL unless quantised). */
 float* pa_kv_cache_scales_ptr(pa_kv_cache* cache, int32_t layer);
 
+/* An int8 cache (pa.h) for num_layers layers, zero-filled: codes and scale bytes of
+ * each layer.  It is written by pa_batch_attention (or pa_append_int8 on its
+ * arrays), which take bf16; pa_kv_cache_read_kv returns its values as f32, and the
+ * writes of single tokens and runs, with their block hashes, are not for it
+ * (PA_ERR_UNSUPPORTED).  pa_kv_cache_dtype is PA_DTYPE_INT8.  No counterpart in the
+ * reference. */
+int32_t pa_kv_cache_create_int8(int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t num_blocks, pa_kv_cache** out);
+/* Device uint8 [num_blocks, num_kv_heads] scale bytes of one layer's K / V (NULL
+ * unless an int8 cache). */
+uint8_t* pa_kv_cache_key_scales_ptr(pa_kv_cache* cache, int32_t layer);
+uint8_t* pa_kv_cache_value_scales_ptr(pa_kv_cache* cache, int32_t layer);
+
 /* Accessors (tensor_store/layout.rs:15-44). */
 int32_t pa_kv_cache_num_layers(const pa_kv_cache* cache);
 int32_t pa_kv_cache_num_blocks(const pa_kv_cache* cache);
@@ -205,6 +218,8 @@ int32_t pa_batch_qkv_rope_cache(pa_batch* batch, pa_kv_cache* cache, int32_t lay
  *   [T, Hkv, D], each with a token stride in elements (0 = contiguous; q, k
  *   and v may be views of one fused QKV projection output), inv_freq [D/2]
  *   device f32 or NULL, scale = attn_factor / sqrt(D).
+ * On an int8 cache (pa_kv_cache_create_int8; q, key and value bf16) the write is
+ * pa_append_int8 and the attention pa_decode_int8 or pa_prefill_int8.
  * key == value == NULL (and inv_freq NULL): the step's K / V are already in
  * the cache and q is final (pa_batch_qkv_rope_cache ran); attention only.
  * Allocates (once, grown on demand) the decode workspace; a call that would

@@ -83,6 +83,16 @@ def test_workspace_size(lib):
     assert parts > 0 and parts % (32 * 130 * 4) == 0
 
 
+def test_kv_cache_create_rejects_bad_sizes(lib):
+    h = C.c_void_p()
+    assert lib.pa_kv_cache_create_int8(0, 2, 64, 4, C.byref(h)) == -1
+    assert lib.pa_kv_cache_create_int8(1, 2, 64, -4, C.byref(h)) == -1
+    assert lib.pa_kv_cache_create_int8(1, 2, 64, 4, None) == -1
+    assert lib.pa_kv_cache_create(1, 2, 64, 4, 3, C.byref(h)) == -1  # not by its dtype
+    assert not h.value
+    assert lib.pa_kv_cache_key_scales_ptr(None, 0) is None
+
+
 def test_wrappers_refuse(pa):
     cpu = [torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2, 64, 16, dtype=torch.int8),
            torch.zeros(4, 2, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)]

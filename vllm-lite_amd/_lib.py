@@ -63,6 +63,9 @@ SIGNATURES = {
     "pa_prefill_int8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32,
                                _i32, _i32, _i32, _f32, _p]),
     "pa_kv_cache_create_quantized": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_p)]),
+    "pa_kv_cache_create_int8": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_p)]),
+    "pa_kv_cache_key_scales_ptr": (_p, [_p, _i32]),
+    "pa_kv_cache_value_scales_ptr": (_p, [_p, _i32]),
     "pa_kv_cache_is_quantized": (_i32, [_p]),
     "pa_kv_cache_scales_ptr": (_p, [_p, _i32]),
     "pa_rope_reshape_and_cache": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i32,

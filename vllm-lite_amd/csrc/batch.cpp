@@ -323,9 +323,22 @@ extern "C" int32_t pa_batch_attention(pa_batch* b, pa_kv_cache* cache, int32_t l
   PA_REQUIRE(key || !inv_freq, PA_ERR_INVALID_ARG,
              "pa_batch_attention: inv_freq without key / value (rotated where written)");
   const int64_t* slots = (const int64_t*)b->slots.ptr;
+  const bool int8 = dtype == PA_DTYPE_INT8;
+  auto* kc8 = (int8_t*)kc;
+  auto* vc8 = (int8_t*)vc;
+  uint8_t* ks8 = pa_kv_cache_key_scales_ptr(cache, layer);
+  uint8_t* vs8 = pa_kv_cache_value_scales_ptr(cache, layer);
   int32_t rc = PA_OK;
   if (!key) {
     // the step's K / V were written by pa_batch_qkv_rope_cache
+  } else if (int8) {
+    // (positions from the context lengths, which pa_batch_advance moves on)
+    rc = pa_append_int8(kc8, vc8, ks8, vs8, key, key_stride, value, value_stride,
+                        inv_freq ? q : nullptr, q_stride, inv_freq,
+                        (const int32_t*)b->tables.ptr, b->max_blocks,
+                        (const int32_t*)b->cu_q.ptr, (const int32_t*)b->ctx_lens.ptr, b->num_seqs,
+                        b->num_tokens, b->max_q, num_heads, hkv, d, b->num_blocks, PA_DTYPE_BF16,
+                        stream);
   } else if (inv_freq) {
     rc = pa_rope_reshape_and_cache(q, q_stride, key, key_stride, value, value_stride, kc, vc,
                                    slots, (const int64_t*)b->positions.ptr, inv_freq,
@@ -348,7 +361,9 @@ extern "C" int32_t pa_batch_attention(pa_batch* b, pa_kv_cache* cache, int32_t l
     // 768 tokens took 20 us more per step than in one workgroup each).
     const int usual_ctx = b->capacity > 0 ? b->capacity - b->capacity / 4 : 0;
     const size_t need = std::max<size_t>(
-        pa_decode_workspace_size(b->num_seqs, num_heads, d, max_ctx), 256);
+        int8 ? pa_decode_int8_workspace_size(b->num_seqs, num_heads, hkv, d, max_ctx)
+             : pa_decode_workspace_size(b->num_seqs, num_heads, d, max_ctx),
+        256);
     if (need > b->workspace.bytes) {
       // growing frees and allocates, which a stream capture cannot record
       hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -360,11 +375,23 @@ extern "C" int32_t pa_batch_attention(pa_batch* b, pa_kv_cache* cache, int32_t l
                  need);
       if ((rc = b->workspace.ensure(need))) return rc;
     }
+    if (int8)
+      return pa::decode_int8_strided(out, q, q_stride, kc8, vc8, ks8, vs8,
+                                     (const int32_t*)b->tables.ptr, b->max_blocks,
+                                     (const int32_t*)b->ctx_lens.ptr, max_ctx, b->num_seqs,
+                                     num_heads, hkv, d, b->num_blocks, scale, b->workspace.ptr,
+                                     b->workspace.bytes, (hipStream_t)stream);
     return pa::decode_strided(out, q, q_stride, kc, vc, (const int32_t*)b->tables.ptr,
                               b->max_blocks, (const int32_t*)b->ctx_lens.ptr, max_ctx, usual_ctx,
                               b->num_seqs, num_heads, hkv, d, b->num_blocks, scale,
                               b->workspace.ptr, b->workspace.bytes, dtype, stream);
   }
+  if (int8)
+    return pa::prefill_int8_strided(out, q, q_stride, kc8, vc8, ks8, vs8,
+                                    (const int32_t*)b->tables.ptr, b->max_blocks,
+                                    (const int32_t*)b->cu_q.ptr, (const int32_t*)b->past.ptr,
+                                    b->num_seqs, b->num_tokens, b->max_q, num_heads, hkv, d,
+                                    b->num_blocks, scale, (hipStream_t)stream);
   return pa::prefill_strided(out, q, q_stride, kc, vc, (const int32_t*)b->tables.ptr,
                              b->max_blocks, (const int32_t*)b->cu_q.ptr,
                              (const int32_t*)b->past.ptr, b->num_seqs, b->num_tokens, b->max_q,
@@ -385,6 +412,8 @@ extern "C" int32_t pa_batch_qkv_rope_cache(pa_batch* b, pa_kv_cache* cache, int3
   PA_REQUIRE(pa_kv_cache_num_blocks(cache) == b->num_blocks, PA_ERR_INVALID_ARG,
              "pa_batch_qkv_rope_cache: batch prepared for %d blocks, cache has %d",
              b->num_blocks, pa_kv_cache_num_blocks(cache));
+  PA_REQUIRE(pa_kv_cache_dtype(cache) != PA_DTYPE_INT8, PA_ERR_UNSUPPORTED,
+             "pa_batch_qkv_rope_cache: an int8 cache is written by pa_batch_attention");
   const int hkv = pa_kv_cache_num_heads(cache), d = pa_kv_cache_head_dim(cache);
   PA_REQUIRE(num_heads > 0 && num_heads % hkv == 0, PA_ERR_INVALID_ARG,
              "pa_batch_qkv_rope_cache: num_heads %d not a multiple of num_kv_heads %d",

@@ -23,6 +23,8 @@ struct pa_kv_cache {
   bool quantized = false;
   std::vector<void*> key, value;
   std::vector<float*> scales;  // quantised caches: [num_blocks] per layer
+  // int8 caches: scale bytes [num_blocks, num_heads] per layer, K's then V's
+  std::vector<uint8_t*> int8_scales;
   // The reference's per-layer block-hash map (tensor_store/mod.rs:42):
   // hash of a K block after a token was written -> the block's id.
   std::vector<std::unordered_map<uint64_t, int64_t>> block_hashes;
@@ -197,15 +199,11 @@ int32_t scatter(pa_kv_cache* c, int layer, const std::vector<int64_t>& slots, co
   return PA_OK;
 }
 
-}  // namespace
-
-extern "C" int32_t pa_kv_cache_create(int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
-                                      int32_t num_blocks, int32_t dtype, pa_kv_cache** out) {
+int32_t create(int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
+               int32_t dtype, pa_kv_cache** out) {
   pa::clear_error();
   PA_REQUIRE(out, PA_ERR_INVALID_ARG, "pa_kv_cache_create: null out");
   *out = nullptr;
-  PA_REQUIRE(pa::dtype_ok(dtype), PA_ERR_INVALID_ARG, "pa_kv_cache_create: unknown dtype %d",
-             dtype);
   PA_REQUIRE(num_layers > 0 && num_kv_heads > 0 && head_dim > 0 && num_blocks > 0,
              PA_ERR_INVALID_ARG, "pa_kv_cache_create: sizes must be positive");
   auto* c = new pa_kv_cache();
@@ -233,6 +231,22 @@ extern "C" int32_t pa_kv_cache_create(int32_t num_layers, int32_t num_kv_heads, 
   return PA_OK;
 }
 
+// The writes of single tokens and runs do not take int8 caches.
+#define PA_REQUIRE_NOT_INT8(what, c)                                     \
+  PA_REQUIRE((c)->dtype != PA_DTYPE_INT8, PA_ERR_UNSUPPORTED,            \
+             what ": an int8 cache is written by pa_batch_attention or pa_append_int8")
+
+}  // namespace
+
+extern "C" int32_t pa_kv_cache_create(int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t num_blocks, int32_t dtype, pa_kv_cache** out) {
+  pa::clear_error();
+  if (out) *out = nullptr;
+  PA_REQUIRE(!out || pa::dtype_ok(dtype), PA_ERR_INVALID_ARG,
+             "pa_kv_cache_create: unknown dtype %d", dtype);
+  return create(num_layers, num_kv_heads, head_dim, num_blocks, dtype, out);
+}
+
 extern "C" int32_t pa_kv_cache_create_quantized(int32_t num_layers, int32_t num_kv_heads,
                                                 int32_t head_dim, int32_t num_blocks,
                                                 pa_kv_cache** out) {
@@ -258,8 +272,31 @@ extern "C" int32_t pa_kv_cache_create_quantized(int32_t num_layers, int32_t num_
   return PA_OK;
 }
 
+extern "C" int32_t pa_kv_cache_create_int8(int32_t num_layers, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t num_blocks,
+                                           pa_kv_cache** out) {
+  // the codes as one-byte arrays, then the scales
+  int32_t rc = create(num_layers, num_kv_heads, head_dim, num_blocks, PA_DTYPE_INT8, out);
+  if (rc != PA_OK) return rc;
+  pa_kv_cache* c = *out;
+  const size_t bytes = (size_t)num_blocks * num_kv_heads;
+  for (int i = 0; i < 2 * num_layers; ++i) {
+    uint8_t* sp = nullptr;
+    if (hipMalloc(&sp, bytes) != hipSuccess || hipMemset(sp, 0, bytes) != hipSuccess) {
+      if (sp) (void)hipFree(sp);
+      pa_kv_cache_destroy(c);
+      *out = nullptr;
+      pa::set_error("pa_kv_cache_create_int8: allocating the scales failed");
+      return PA_ERR_HIP;
+    }
+    c->int8_scales.push_back(sp);
+  }
+  return PA_OK;
+}
+
 extern "C" void pa_kv_cache_destroy(pa_kv_cache* c) {
   if (!c) return;
+  for (uint8_t* p : c->int8_scales) (void)hipFree(p);
   for (void* p : c->key) (void)hipFree(p);
   for (void* p : c->value) (void)hipFree(p);
   for (float* p : c->scales) (void)hipFree(p);
@@ -283,6 +320,17 @@ extern "C" float* pa_kv_cache_scales_ptr(pa_kv_cache* c, int32_t layer) {
   return (c && c->quantized && layer >= 0 && layer < c->num_layers) ? c->scales[layer] : nullptr;
 }
 
+extern "C" uint8_t* pa_kv_cache_key_scales_ptr(pa_kv_cache* c, int32_t layer) {
+  return (c && c->dtype == PA_DTYPE_INT8 && layer >= 0 && layer < c->num_layers)
+             ? c->int8_scales[2 * layer]
+             : nullptr;
+}
+extern "C" uint8_t* pa_kv_cache_value_scales_ptr(pa_kv_cache* c, int32_t layer) {
+  return (c && c->dtype == PA_DTYPE_INT8 && layer >= 0 && layer < c->num_layers)
+             ? c->int8_scales[2 * layer + 1]
+             : nullptr;
+}
+
 extern "C" void* pa_kv_cache_key_ptr(pa_kv_cache* c, int32_t layer) {
   return (c && layer >= 0 && layer < c->num_layers) ? c->key[layer] : nullptr;
 }
@@ -295,6 +343,7 @@ extern "C" int32_t pa_kv_cache_write_kv(pa_kv_cache* c, int32_t layer, int64_t b
                                         pa_stream_t stream) {
   pa::clear_error();
   PA_REQUIRE(c && k && v, PA_ERR_INVALID_ARG, "write_kv: null argument");
+  PA_REQUIRE_NOT_INT8("write_kv", c);
   PA_REQUIRE(layer >= 0 && layer < c->num_layers, PA_ERR_OUT_OF_BOUNDS,
              "layer_idx %d out of bounds for %d layers", layer, c->num_layers);
   PA_REQUIRE(block_id >= 0 && block_id < c->num_blocks, PA_ERR_OUT_OF_BOUNDS,
@@ -323,6 +372,7 @@ extern "C" int32_t pa_kv_cache_write_kv_batch(pa_kv_cache* c, int32_t layer, int
                                               int32_t num_tokens, pa_stream_t stream) {
   pa::clear_error();
   PA_REQUIRE(c && k && v, PA_ERR_INVALID_ARG, "write_kv_batch: null argument");
+  PA_REQUIRE_NOT_INT8("write_kv_batch", c);
   PA_REQUIRE(layer >= 0 && layer < c->num_layers, PA_ERR_OUT_OF_BOUNDS,
              "layer_idx %d out of bounds for %d layers", layer, c->num_layers);
   PA_REQUIRE(num_tokens >= 0 && block_id >= 0 && block_id < c->num_blocks && token_offset >= 0,
@@ -357,6 +407,7 @@ extern "C" int32_t pa_kv_cache_write_prefill_kv(pa_kv_cache* c, int32_t layer,
   pa::clear_error();
   PA_REQUIRE(c && k && v && (block_ids || n_ids == 0), PA_ERR_INVALID_ARG,
              "write_prefill_kv: null argument");
+  PA_REQUIRE_NOT_INT8("write_prefill_kv", c);
   PA_REQUIRE(layer >= 0 && layer < c->num_layers, PA_ERR_OUT_OF_BOUNDS,
              "layer_idx %d out of bounds for %d layers", layer, c->num_layers);
   PA_REQUIRE(num_tokens >= 0, PA_ERR_INVALID_ARG, "write_prefill_kv: negative token count");
@@ -399,7 +450,8 @@ extern "C" int32_t pa_kv_cache_read_kv(pa_kv_cache* c, int32_t layer, const int6
   }
   hipStream_t s = (hipStream_t)stream;
   int32_t rc = PA_OK;
-  if (!c->quantized && used <= pa::kSmallIds) {
+  const bool int8 = c->dtype == PA_DTYPE_INT8;
+  if (!c->quantized && !int8 && used <= pa::kSmallIds) {
     // the ids go in the kernel arguments: no upload.  Only the shortest reads
     // return before the stream has run them (as the header says).
     rc = pa::launch_read_kv_small(c->key[layer], c->value[layer], c->dtype, ids.data(), used, n,
@@ -417,6 +469,11 @@ extern "C" int32_t pa_kv_cache_read_kv(pa_kv_cache* c, int32_t layer, const int6
     rc = pa::launch_quant_read((const float*)c->key[layer], (const float*)c->value[layer],
                                c->scales[layer], (const int32_t*)d_ids, n, c->num_heads,
                                c->head_dim, (float*)out_k, (float*)out_v, s);
+  else if (int8)
+    rc = pa_read_kv_int8((const int8_t*)c->key[layer], (const int8_t*)c->value[layer],
+                         c->int8_scales[2 * layer], c->int8_scales[2 * layer + 1],
+                         (const int32_t*)d_ids, used, n, c->num_heads, c->head_dim, c->num_blocks,
+                         (float*)out_k, (float*)out_v, stream);
   else
     rc = pa_read_kv(c->key[layer], c->value[layer], (const int32_t*)d_ids, used, n, c->num_heads,
                     c->head_dim, c->num_blocks, out_k, out_v, c->dtype, stream);

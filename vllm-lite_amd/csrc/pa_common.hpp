@@ -207,7 +207,9 @@ void set_error(const char* fmt, ...);
 void clear_error();
 
 inline size_t dtype_size(int32_t dtype) {
-  return dtype == PA_DTYPE_BF16 ? 2 : dtype == PA_DTYPE_FP8_E4M3 ? 1 : 4;
+  return dtype == PA_DTYPE_BF16 ? 2
+         : dtype == PA_DTYPE_FP8_E4M3 || dtype == PA_DTYPE_INT8 ? 1
+                                                               : 4;
 }
 inline bool dtype_ok(int32_t dtype) { return dtype == PA_DTYPE_F32 || dtype == PA_DTYPE_BF16; }
 

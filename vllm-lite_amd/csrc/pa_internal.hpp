@@ -64,4 +64,23 @@ PA_HIDDEN int32_t prefill_strided(void* out, const void* q, int64_t q_row, const
                                   int32_t head_dim, int32_t num_blocks, float scale,
                                   int32_t dtype, hipStream_t stream);
 
+// pa_decode_int8 / pa_prefill_int8 with q rows q_row elements apart (0: contiguous).
+PA_HIDDEN int32_t decode_int8_strided(void* out, const void* q, int64_t q_row,
+                                      const int8_t* k_cache, const int8_t* v_cache,
+                                      const uint8_t* k_scales, const uint8_t* v_scales,
+                                      const int32_t* block_tables, int32_t max_blocks_per_seq,
+                                      const int32_t* context_lens, int32_t max_context_len,
+                                      int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, int32_t num_blocks, float scale,
+                                      void* workspace, size_t workspace_bytes,
+                                      hipStream_t stream);
+PA_HIDDEN int32_t prefill_int8_strided(void* out, const void* q, int64_t q_row,
+                                       const int8_t* k_cache, const int8_t* v_cache,
+                                       const uint8_t* k_scales, const uint8_t* v_scales,
+                                       const int32_t* block_tables, int32_t max_blocks_per_seq,
+                                       const int32_t* cu_q_lens, const int32_t* past_lens,
+                                       int32_t num_seqs, int32_t total_q, int32_t max_q_len,
+                                       int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                       int32_t num_blocks, float scale, hipStream_t stream);
+
 }  // namespace pa

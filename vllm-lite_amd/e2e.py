@@ -146,17 +146,52 @@ class Weights:
         return sum(t.numel() * t.element_size() for t in ts)
 
 
-class Engine:
-    """Batched greedy generation over one paged KV cache."""
+@dataclasses.dataclass
+class Sampling:
+    """How a request's tokens are drawn (ops.sample's settings)."""
+    temperature: float = 1.0  # 0: the largest logit
+    top_k: int = 0            # 0: off
+    top_p: float = 1.0
+    min_p: float = 0.0
 
-    def __init__(self, cfg, weights, num_blocks, device="cuda", graph=True):
+
+class Sampler:
+    """The settings of a batch's requests on the device, and the uniform numbers
+    of all its steps, from `seed` alone."""
+
+    def __init__(self, settings, steps, seed, device):
+        def column(name, dtype):
+            return torch.tensor([getattr(s, name) for s in settings], dtype=dtype, device=device)
+
+        self.settings = dict(temperature=column("temperature", torch.float32),
+                             top_k=column("top_k", torch.int32),
+                             top_p=column("top_p", torch.float32),
+                             min_p=column("min_p", torch.float32))
+        g = torch.Generator(device=device).manual_seed(seed)
+        self.uniform = torch.rand(steps, len(settings), generator=g, device=device)
+        self.workspace = torch.empty(ops.sample_workspace_size(len(settings)), dtype=torch.uint8,
+                                     device=device)
+
+    def __call__(self, logits, step):
+        """The tokens of step `step` (an index, or an int64 tensor [1] in a
+        captured step)."""
+        u = self.uniform[step]
+        return ops.sample(logits, u.view(-1), workspace=self.workspace, **self.settings)
+
+
+class Engine:
+    """Batched generation over one paged KV cache, greedy or sampled."""
+
+    def __init__(self, cfg, weights, num_blocks, device="cuda", graph=True,
+                 kv_dtype=torch.bfloat16):
         """graph: capture one decode step's forward in a HIP graph and replay
         it for the following steps (the batch is re-prepared on the host
-        before every replay; see StepBatch.set_capacity)."""
+        before every replay; see StepBatch.set_capacity).  kv_dtype torch.int8:
+        an int8 KV cache with a scale per block and head, at half the bytes."""
         self.cfg, self.w, self.device = cfg, weights, torch.device(device)
         self.graph = graph
         self.cache = PagedKvCache(cfg.layers, cfg.kv_heads, cfg.head_dim, num_blocks,
-                                  torch.bfloat16, device)
+                                  kv_dtype, device)
         self.batch = StepBatch()
         self.inv_freq = torch.from_numpy(ops.rope_inv_freq(cfg.head_dim, cfg.rope_theta)).to(
             self.device)
@@ -179,10 +214,11 @@ class Engine:
         in a decode step)."""
         return self._logits(tokens, logit_rows).float()
 
-    def next_tokens(self, tokens, logit_rows):
-        """Greedy next token of each row of logit_rows (int64 [R]): pa_argmax
-        over the bf16 logits, argmax_logits's rule."""
-        return ops.argmax(self._logits(tokens, logit_rows))
+    def next_tokens(self, tokens, logit_rows, sampler=None, step=0):
+        """Next token of each row of logit_rows (int64 [R]): pa_argmax over the
+        bf16 logits, argmax_logits's rule, or drawn by the Sampler."""
+        logits = self._logits(tokens, logit_rows)
+        return ops.argmax(logits) if sampler is None else sampler(logits, step)
 
     def _logits(self, tokens, logit_rows):
         """forward's logits in the model dtype (bf16)."""
@@ -254,7 +290,7 @@ class Engine:
         nq = hq * d
         x = F.embedding(tokens, w.embed)  # residual stream [T, hidden]
         for layer in range(c.layers):
-            if "qkv_rope" in pk:
+            if "qkv_rope" in pk and self.cache.dtype == torch.bfloat16:
                 # one QKV projection with RoPE and the KV write in its
                 # epilogue; attention reads q as a strided view of its rows
                 qkv = self.batch.qkv_rope_cache(self.cache, layer, x, pk["qkv_rope"][layer],
@@ -309,11 +345,20 @@ class Engine:
         rows = x if logit_rows is None else x[logit_rows].contiguous()
         return ops.linear_mx(self._norm_mx(rows, w.norm), mx["lm_head"])
 
-    def generate(self, prompts, max_new):
-        """Greedy generation for every prompt (lists of token ids).  Returns
-        (generated ids [B, max_new] on the host, {"prefill_s", "decode_s"})."""
+    def generate(self, prompts, max_new, sampling=None, seed=0):
+        """Generation for every prompt (lists of token ids): greedy, or with
+        sampling (a Sampling for all, or a list of one for each prompt), its
+        random numbers from seed.  Returns (generated ids [B, max_new] on the
+        host, {"prefill_s", "decode_s"})."""
         b = len(prompts)
         lens = [len(p) for p in prompts]
+        sampler = None
+        if sampling is not None:
+            if isinstance(sampling, Sampling):
+                sampling = [sampling] * b
+            if len(sampling) != b:
+                raise ValueError(f"{len(sampling)} sampling settings for {b} prompts")
+            sampler = Sampler(sampling, max_new, seed, self.device)
         blocks = []
         for n in lens:
             need = (n + max_new + 15) // 16
@@ -327,7 +372,7 @@ class Engine:
             tokens = torch.tensor([x for p in prompts for x in p], dtype=torch.int64,
                                   device=self.device)
             last = torch.tensor([sum(lens[:i + 1]) - 1 for i in range(b)], device=self.device)
-            nxt = self.next_tokens(tokens, last)
+            nxt = self.next_tokens(tokens, last, sampler, 0)
             out = [nxt]
             torch.cuda.synchronize(self.device)
             t1 = time.perf_counter()
@@ -340,7 +385,7 @@ class Engine:
                     # eager (also the warm-up of every launch the graph records)
                     self.batch.prepare(self.cache, [1] * b, [n + step - 1 for n in lens],
                                        blocks)
-                    nxt = self.next_tokens(nxt, rows)
+                    nxt = self.next_tokens(nxt, rows, sampler, step)
                     out.append(nxt)
                     continue
                 if graph is None:
@@ -356,7 +401,7 @@ class Engine:
                     graph = torch.cuda.CUDAGraph()
                     with torch.cuda.graph(graph):
                         self.batch.advance(self.cache)
-                        static_out = self.next_tokens(static_tok, rows)
+                        static_out = self.next_tokens(static_tok, rows, sampler, row)
                         static_tok.copy_(static_out)
                         hist.index_copy_(0, row, static_out[None])
                         row.add_(1)

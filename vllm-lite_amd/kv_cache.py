@@ -13,7 +13,7 @@ from array import array
 import torch
 
 from . import _lib
-from .ops import BLOCK_SIZE, PaError, _DTYPES, _check
+from .ops import BLOCK_SIZE, Int8Cache, PaError, _DTYPES, _check
 
 _DT_BACK = {v: k for k, v in _DTYPES.items()}
 
@@ -35,7 +35,10 @@ def _i64_array(xs):
 
 class PagedKvCache:
     """quantized=True mirrors PagedKvCache::new(..., quantized = true): an f32
-    cache of int8 values with one scale per block (re-quantised per write)."""
+    cache of int8 values with one scale per block (re-quantised per write).
+    dtype torch.int8: one-byte codes with a scale per block and kv head
+    (pa_kv_cache_create_int8), written by StepBatch.attention from bf16; read_kv
+    returns its values as f32."""
 
     def __init__(self, num_layers, num_heads, head_dim, num_blocks, dtype=torch.float32,
                  device="cuda", quantized=False):
@@ -44,6 +47,9 @@ class PagedKvCache:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.dtype = dtype
+        # of the payloads: q, K and V of an int8 cache are bf16, read_kv's f32
+        int8 = dtype == torch.int8
+        self.step_dtype = torch.bfloat16 if int8 else dtype
         self.num_heads = num_heads
         self.head_dim = head_dim
         h = C.c_void_p()
@@ -51,7 +57,10 @@ class PagedKvCache:
             raise ValueError("quantised caches are f32")
         self.quantized = quantized
         with torch.cuda.device(self.device):
-            if quantized:
+            if int8:
+                _check("pa_kv_cache_create_int8", self._lib.pa_kv_cache_create_int8(
+                    num_layers, num_heads, head_dim, num_blocks, C.byref(h)))
+            elif quantized:
                 _check("pa_kv_cache_create_quantized", self._lib.pa_kv_cache_create_quantized(
                     num_layers, num_heads, head_dim, num_blocks, C.byref(h)))
             else:
@@ -106,10 +115,23 @@ class PagedKvCache:
 
         return torch.as_tensor(_Buf(), device=self.device).view(torch.float32)
 
-    def _layer_tensor(self, ptr, shape):
+    def int8(self, layer):
+        """One layer's arrays as an Int8Cache (int8 caches only)."""
+        if self.dtype != torch.int8:
+            raise ValueError("not an int8 cache")
+        shape = (self.num_blocks(), self.num_heads)
+        return Int8Cache(
+            self.key_cache(layer), self.value_cache(layer),
+            self._layer_tensor(self._lib.pa_kv_cache_key_scales_ptr(self._h, layer), shape,
+                               torch.uint8),
+            self._layer_tensor(self._lib.pa_kv_cache_value_scales_ptr(self._h, layer), shape,
+                               torch.uint8))
+
+    def _layer_tensor(self, ptr, shape, dtype=None):
         if not ptr:
             raise PaError("pa_kv_cache layer", -2, "layer out of bounds")
-        es = torch.empty(0, dtype=self.dtype).element_size()
+        dtype = dtype or self.dtype
+        es = torch.empty(0, dtype=dtype).element_size()
         n = 1
         for s in shape:
             n *= s
@@ -122,7 +144,7 @@ class PagedKvCache:
             __cuda_array_interface__ = iface
 
         raw = torch.as_tensor(_Buf(), device=self.device)
-        return raw.view(self.dtype).view(shape)
+        return raw.view(dtype).view(shape)
 
     # reference operations ------------------------------------------------
     def _stream(self):
@@ -133,7 +155,7 @@ class PagedKvCache:
         (buffer.rs:139-165, :42-67): same shape, trailing dims [H, D], and
         the expected token count; returns contiguous tensors and T."""
         for x in (k, v):
-            if x.device != self.device or x.dtype != self.dtype:
+            if x.device != self.device or x.dtype != self.step_dtype:
                 raise ValueError("payload must be a device tensor in the cache dtype")
         if tuple(k.shape) != tuple(v.shape):
             raise ValueError(f"k and v must have same dimensions, got {tuple(k.shape)} vs "
@@ -173,7 +195,8 @@ class PagedKvCache:
         """PagedKvCache::read_kv (buffer.rs:273-339) -> (k, v) [n, H, D]."""
         ids, n_ids = _i64_array(block_ids)
         cover = min(seq_len, n_ids * BLOCK_SIZE) if n_ids and seq_len > 0 else 0
-        out_k = torch.empty(cover, self.num_heads, self.head_dim, dtype=self.dtype,
+        out_k = torch.empty(cover, self.num_heads, self.head_dim,
+                            dtype=torch.float32 if self.dtype == torch.int8 else self.dtype,
                             device=self.device)
         out_v = torch.empty_like(out_k)
         n = C.c_int32(0)
@@ -305,9 +328,9 @@ class StepBatch:
         for x in (q, key, value):
             if x is None:
                 continue
-            if x.dtype != cache.dtype or x.device != cache.device or x.stride(2) != 1 or \
+            if x.dtype != cache.step_dtype or x.device != cache.device or x.stride(2) != 1 or \
                     x.stride(1) != d or (t > 1 and x.stride(0) < x.shape[1] * d):
-                raise ValueError("q / key / value rows must be [H, D] in the cache dtype, "
+                raise ValueError(f"q / key / value rows must be [H, D] in {cache.step_dtype}, "
                                  "token rows not overlapping")
         if inv_freq is not None and (inv_freq.dtype != torch.float32 or
                                      inv_freq.shape != (d // 2,)):

@@ -6,6 +6,7 @@
 // workspace, which a second launch merges.
 // Bound by memory: every code is read once, for all heads of its group.
 #include <algorithm>
+#include <type_traits>
 
 #include "int8_wave.hpp"
 #include "pa_internal.hpp"
@@ -15,8 +16,13 @@ namespace {
 
 constexpr int kStep = 4 * kBlock;  // tokens a step
 
+// Each wavefront takes every NW-th step of the part, so that its block ids are known
+// before the context length is.  The next step's K is loaded where this one's has
+// become scores, its V where this one's has been multiplied: a step is always on its
+// way, in one set of registers.
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) void decode_int8_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 16 ? 4 : D == 256 ? 1 : 2))) void
+decode_int8_kernel(
     uint16_t* __restrict__ out, const uint16_t* __restrict__ q, int64_t q_row,
     const int8_t* __restrict__ kc, const int8_t* __restrict__ vc, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, const int32_t* __restrict__ tables, int mbs,
@@ -30,53 +36,84 @@ __global__ __launch_bounds__(64 * NW) void decode_int8_kernel(
   const int kvh = blockIdx.y / head_groups, h0 = (blockIdx.y % head_groups) * 16;
   const int heads = min(G - h0, 16);  // query heads of this workgroup
   const int64_t row0 = (int64_t)seq * Hq + kvh * G + h0;
+  const int begin = part * part_len;
+  const int32_t* tab = tables + (int64_t)seq * mbs;
+  // Lane t holds block t % 4 of the wavefront's step t / 4, for 16 steps.
+  auto load_ids = [&](int step) -> int32_t {
+    const int b = (begin + (wave + (step + lane / 4) * NW) * kStep) / kBlock + lane % 4;
+    return b < mbs ? tab[b] : -1;
+  };
+  int32_t ids = load_ids(0);
+  const int ctx = min(context_lens[seq], mbs * kBlock);
+  const int end = min(ctx, begin + part_len);
+  if (begin >= end && part > 0) return;  // (part 0 of an empty context writes zeros)
+  const Int8Blocks<D> blocks{kc, vc, ks, vs, Hkv, kvh};
+  const int left = end - begin - wave * kStep;  // tokens from this wavefront's first step on
+  const int steps = left > 0 ? (left + NW * kStep - 1) / (NW * kStep) : 0;
+  // a step's blocks, in the pool, and how much of block j there is
+  struct Place {
+    int kid, vid, lim;
+    bool whole;
+  };
+  auto place = [&](int step) -> Place {
+    const int at = 4 * (step % 16);
+    Place p{__shfl(ids, at + (c >> 2), 64), __shfl(ids, at + j, 64), 0, false};
+    const bool ok = p.vid >= 0 && p.vid < num_blocks;
+    const int t0 = begin + (wave + step * NW) * kStep + j * kBlock;
+    p.lim = ok ? min(max(end - t0, 0), kBlock) : 0;
+    p.whole = __builtin_amdgcn_ballot_w64(p.lim < kBlock) == 0;
+    if (!ok) p.vid = 0;
+    if (p.kid < 0 || p.kid >= num_blocks) p.kid = 0;
+    return p;
+  };
+  Int8Keys<D> k;
+  Int8Values<D> v;
+  Place now{};
+  if (steps > 0) {
+    now = place(0);
+    blocks.load_keys(now.kid, now.vid, c, j, k);
+    blocks.load_values(now.vid, c, v);
+  }
   Int8Query<D> qv;
   int8_query<D>(c < heads ? q + (int64_t)seq * q_row + (int64_t)(kvh * G + h0 + c) * D : nullptr,
                 j, scale_log2, qv);
-  const int ctx = min(context_lens[seq], mbs * kBlock);
-  const int begin = part * part_len, end = min(ctx, begin + part_len);
-  if (begin >= end && part > 0) return;  // (part 0 of an empty context writes zeros)
-  // this wavefront's steps
-  const int steps = max(0, (end - begin + kStep - 1) / kStep);
-  const int s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
-  const int32_t* tab = tables + (int64_t)seq * mbs;
-  const Int8Blocks<D> blocks{kc, vc, ks, vs, Hkv, kvh};
   Int8State<D> S;
   S.init();
-  int32_t ids = -1;
-  for (int s = s0; s < s1; ++s) {
-    const int b = (begin + s * kStep) / kBlock;  // the step's first block
-    // lane t holds the id of block t of the next 16 steps
-    const int ahead = (s - s0) % 16;
-    if (ahead == 0) ids = b + lane < mbs ? tab[b + lane] : -1;
-    int id[4];
-    bool whole = true;
-    int lim = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      id[g] = __builtin_amdgcn_readlane(ids, 4 * ahead + g);
-      const bool ok = id[g] >= 0 && id[g] < num_blocks;
-      const int n = ok ? min(max(end - (b + g) * kBlock, 0), kBlock) : 0;
-      if (!ok) id[g] = 0;
-      whole = whole && n == kBlock;
-      lim = g == j ? n : lim;
+  auto step = [&](int s, auto more) {
+    i32x4 a[4];
+    bf16x8 p0, p1;
+    int8_scores<D>(k, qv, a);
+    const uint32_t kscale = k.scale;
+    Place next = now;
+    if constexpr (decltype(more)::value) {
+      if ((s + 1) % 16 == 0) ids = load_ids(s + 1);
+      next = place(s + 1);
+      blocks.load_keys(next.kid, next.vid, c, j, k);
     }
-    Int8Step<D> st;
-    blocks.load(id, c, j, st);
-    int8_step<D>(st, qv, whole, lim, S);
-  }
+    __builtin_amdgcn_sched_barrier(0);
+    int8_softmax<D>(a, kscale, v.scale, qv.factor, now.whole, now.lim, S, p0, p1);
+    __builtin_amdgcn_sched_barrier(0);
+    int8_output<D>(v, p0, p1, S);
+    if constexpr (decltype(more)::value) blocks.load_values(next.vid, c, v);
+    now = next;
+  };
+  for (int s = 0; s + 1 < steps; ++s) step(s, std::true_type{});
+  if (steps > 0) step(steps - 1, std::false_type{});
   float lsum = S.lsum;
   lsum += __shfl_xor(lsum, 16, 64);
   lsum += __shfl_xor(lsum, 32, 64);
-  // The wavefronts' results meet in LDS.
-  __shared__ float so[NW][16][D];
+  // The wavefronts' results meet in LDS (rows 4 floats apart in the banks).
+  constexpr int P = D + 4;
+  __shared__ __attribute__((aligned(16))) float so[NW][16][P];
   __shared__ float sml[NW][16][2];
+  if (c < heads) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-    *reinterpret_cast<f32x4*>(&so[wave][c][16 * dt + 4 * j]) = S.o[dt];
-  if (j == 0) {
-    sml[wave][c][0] = S.m;
-    sml[wave][c][1] = lsum;
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<f32x4*>(&so[wave][c][16 * dt + 4 * j]) = S.o[dt];
+    if (j == 0) {
+      sml[wave][c][0] = S.m;
+      sml[wave][c][1] = lsum;
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < heads * D; i += 64 * NW) {
@@ -105,40 +142,76 @@ __global__ __launch_bounds__(64 * NW) void decode_int8_kernel(
   }
 }
 
-// Merges the parts of one (sequence, query head).
-__global__ __launch_bounds__(256) void decode_int8_merge_kernel(
+// Merges the parts of one (sequence, query head), one wavefront for each: their
+// (m, l) a lane each, 64 at a time, then their outputs eight loads at a time.
+template <int DL>
+__global__ __launch_bounds__(64) void decode_int8_merge_kernel(
     uint16_t* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
     const int32_t* __restrict__ context_lens, int Hq, int D, int num_parts, int part_len,
     int mbs) {
   const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float2* ml = reinterpret_cast<const float2*>(ws_ml) + row * num_parts;
+  const float* o = ws_o + row * num_parts * D;
+  float2 mine = ml[min(lane, num_parts - 1)];  // (parts without keys are not written)
   const int ctx = min(context_lens[row / Hq], mbs * kBlock);
   const int np = min(num_parts, (max(ctx, 1) + part_len - 1) / part_len);
-  const float* ml = ws_ml + 2 * row * num_parts;
-  const float* o = ws_o + row * num_parts * D;
-  float m = kInt8NoMax;
-  for (int p = 0; p < np; ++p) m = fmaxf(m, ml[2 * p]);
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  float num = 0.f, den = 0.f;
-  for (int p = 0; p < np; ++p) {
-    const float a = __builtin_amdgcn_exp2f(ml[2 * p] - m);
-    num += a * o[(int64_t)p * D + d];
-    den += a * ml[2 * p + 1];
+  float M = kInt8NoMax, num[DL], den = 0.f;
+#pragma unroll
+  for (int x = 0; x < DL; ++x) num[x] = 0.f;
+  for (int p0 = 0; p0 < np; p0 += 64) {
+    if (p0 > 0) mine = ml[min(p0 + lane, num_parts - 1)];
+    const bool on = p0 + lane < np;
+    float m = on ? mine.x : kInt8NoMax;
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    m = fmaxf(m, M);
+    const float keep = __builtin_amdgcn_exp2f(M - m);
+    M = m;
+    const float w = on ? __builtin_amdgcn_exp2f(mine.x - m) : 0.f;
+    float l = on ? w * mine.y : 0.f;
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) l += __shfl_xor(l, s, 64);
+    den = den * keep + l;
+#pragma unroll
+    for (int x = 0; x < DL; ++x) num[x] *= keep;
+    const int n = min(64, np - p0);
+    for (int p = 0; p < n; p += 8) {
+      float v[8][DL];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int x = 0; x < DL; ++x)
+          v[u][x] = lane + 64 * x < D ? o[(int64_t)(p0 + min(p + u, n - 1)) * D + lane + 64 * x]
+                                      : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (p + u < n) {
+          const float a = __builtin_bit_cast(
+              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), p + u));
+#pragma unroll
+          for (int x = 0; x < DL; ++x) num[x] += a * v[u][x];
+        }
+      }
+    }
   }
-  out[row * D + d] = f32_to_bf16_bits(den != 0.f ? num / den : 0.f);
+#pragma unroll
+  for (int x = 0; x < DL; ++x)
+    if (lane + 64 * x < D)
+      out[row * D + lane + 64 * x] = f32_to_bf16_bits(den != 0.f ? num[x] / den : 0.f);
 }
 
-// Tokens of a part for a launch over contexts of up to max_ctx tokens.
+// How a launch over contexts of up to max_ctx tokens is cut.
 struct Int8Plan {
-  int part_len, parts;
+  int waves, part_len, parts;
 };
-Int8Plan plan_of(int num_seqs, int num_heads, int num_kv_heads, int max_ctx) {
+Int8Plan plan_of(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_ctx) {
   const int groups = (num_heads / num_kv_heads + 15) / 16;
   const long long pairs = (long long)num_seqs * num_kv_heads * groups;
   int len = 4096;
   while (len > 256 && pairs * ((max_ctx + len - 1) / len) < 512) len /= 2;
   if (len >= max_ctx) len = std::max(kStep, (max_ctx + kStep - 1) / kStep * kStep);
-  return {len, std::max(1, (int)(((long long)max_ctx + len - 1) / len))};
+  return {head_dim <= 192 ? 8 : 4, len, std::max(1, (int)(((long long)max_ctx + len - 1) / len))};
 }
 
 }  // namespace
@@ -152,7 +225,7 @@ extern "C" size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_he
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
       head_dim <= 0 || max_context_len <= 0)
     return 0;
-  const Int8Plan p = plan_of(num_seqs, num_heads, num_kv_heads, max_context_len);
+  const Int8Plan p = plan_of(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len);
   return p.parts == 1 ? 0
                       : (size_t)num_seqs * num_heads * p.parts * (head_dim + 2) * sizeof(float);
 }
@@ -189,7 +262,7 @@ int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_
                  q_row % 2 == 0 && (uintptr_t)out % 2 == 0,
              PA_ERR_INVALID_ARG, "pa_decode_int8: caches not 16-byte or q not 4-byte aligned");
   const int G = num_heads / num_kv_heads, head_groups = (G + 15) / 16;
-  const Int8Plan plan = plan_of(num_seqs, num_heads, num_kv_heads, max_context_len);
+  const Int8Plan plan = plan_of(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len);
   const int np = plan.parts;
   PA_REQUIRE(num_seqs <= 65535 && (long long)num_kv_heads * head_groups <= 65535 &&
                  (long long)num_blocks * num_kv_heads < (1ll << 32) && grid_fits(np, 512) &&
@@ -200,18 +273,27 @@ int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_
   if (np > 1) {
     const size_t rows = (size_t)num_seqs * num_heads * np;
     const size_t need = rows * (head_dim + 2) * sizeof(float);
-    PA_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 4 == 0,
+    PA_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0,
                PA_ERR_WORKSPACE, "pa_decode_int8: workspace of %zu bytes needed, %zu given", need,
                workspace ? workspace_bytes : 0);
     ws_o = (float*)workspace;
     ws_ml = ws_o + rows * head_dim;
   }
   const dim3 grid(np, num_kv_heads * head_groups, num_seqs);
-#define PA_LAUNCH_DECODE_INT8(DD)                                                              \
-  decode_int8_kernel<DD, (DD <= 128 ? 8 : 4)><<<grid, 64 * (DD <= 128 ? 8 : 4), 0, s>>>(       \
+#define PA_LAUNCH_DECODE_INT8_NW(DD, NW)                                                       \
+  decode_int8_kernel<DD, NW><<<grid, 64 * NW, 0, s>>>(                                         \
       (uint16_t*)out, (const uint16_t*)q, q_row, k_cache, v_cache, k_scales, v_scales,         \
       block_tables, max_blocks_per_seq, context_lens, num_heads, num_kv_heads, G, head_groups, \
       num_blocks, scale * kInt8Log2e, np, plan.part_len, ws_o, ws_ml)
+#define PA_LAUNCH_DECODE_INT8(DD)                          \
+  do {                                                     \
+    if (DD == 256 || plan.waves == 4)                      \
+      PA_LAUNCH_DECODE_INT8_NW(DD, 4);                     \
+    else if (DD > 64 || plan.waves == 8)                   \
+      PA_LAUNCH_DECODE_INT8_NW(DD, (DD == 256 ? 4 : 8));   \
+    else                                                   \
+      PA_LAUNCH_DECODE_INT8_NW(DD, (DD > 64 ? 4 : 16));    \
+  } while (0)
   switch (head_dim) {
     case 32: PA_LAUNCH_DECODE_INT8(32); break;
     case 64: PA_LAUNCH_DECODE_INT8(64); break;
@@ -221,11 +303,20 @@ int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_
     default: PA_LAUNCH_DECODE_INT8(256); break;
   }
 #undef PA_LAUNCH_DECODE_INT8
+#undef PA_LAUNCH_DECODE_INT8_NW
   int32_t rc = check_launch("pa_decode_int8");
   if (rc != PA_OK || np == 1) return rc;
-  decode_int8_merge_kernel<<<num_seqs * num_heads, 256, 0, s>>>(
-      (uint16_t*)out, ws_o, ws_ml, context_lens, num_heads, head_dim, np, plan.part_len,
-      max_blocks_per_seq);
+  auto merge = [&](auto kernel) {
+    kernel<<<num_seqs * num_heads, 64, 0, s>>>((uint16_t*)out, ws_o, ws_ml, context_lens,
+                                               num_heads, head_dim, np, plan.part_len,
+                                               max_blocks_per_seq);
+  };
+  if (head_dim <= 64)
+    merge(decode_int8_merge_kernel<1>);
+  else if (head_dim <= 128)
+    merge(decode_int8_merge_kernel<2>);
+  else
+    merge(decode_int8_merge_kernel<4>);
   return check_launch("pa_decode_int8 merge");
 }
 }  // namespace pa

@@ -46,21 +46,22 @@ __global__ __launch_bounds__(64 * kPrefillWaves) void prefill_int8_kernel(
   for (int s = 0; s < steps; ++s) {
     const int b = 4 * s;
     if (s % 16 == 0) ids = b + lane < mbs ? tab[b + lane] : -1;
-    int id[4];
-    bool whole = (s + 1) * kStep <= past + r0 + 1;
-    int lim = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      id[g] = __builtin_amdgcn_readlane(ids, 4 * (s % 16) + g);
-      const bool ok = id[g] >= 0 && id[g] < num_blocks;
-      const int n = ok ? min(max(mine - (b + g) * kBlock, 0), kBlock) : 0;
-      if (!ok) id[g] = 0;
-      whole = whole && ok;
-      lim = g == j ? n : lim;
-    }
-    Int8Step<D> st;
-    blocks.load(id, c, j, st);
-    int8_step<D>(st, qv, whole, lim, S);
+    const int at = 4 * (s % 16);
+    int kid = __shfl(ids, at + (c >> 2), 64), vid = __shfl(ids, at + j, 64);
+    const bool ok = vid >= 0 && vid < num_blocks;
+    const int lim = ok ? min(max(mine - (b + j) * kBlock, 0), kBlock) : 0;
+    const bool whole = __builtin_amdgcn_ballot_w64(lim < kBlock) == 0;
+    if (!ok) vid = 0;
+    if (kid < 0 || kid >= num_blocks) kid = 0;
+    Int8Keys<D> k;
+    Int8Values<D> v;
+    blocks.load_keys(kid, vid, c, j, k);
+    blocks.load_values(vid, c, v);
+    i32x4 a[4];
+    bf16x8 p0, p1;
+    int8_scores<D>(k, qv, a);
+    int8_softmax<D>(a, k.scale, v.scale, qv.factor, whole, lim, S, p0, p1);
+    int8_output<D>(v, p0, p1, S);
   }
   float lsum = S.lsum;
   lsum += __shfl_xor(lsum, 16, 64);

@@ -35,6 +35,9 @@ __device__ inline uint32_t codes_bf16x2(uint32_t w, int at) {
                                0x07060302u);
 }
 __device__ inline bf16x8 codes_bf16x8(uint32_t lo, uint32_t hi) {
+  // the words as they are: the compiler would carry bytes in registers of their own
+  // from the loads to here
+  asm("" : "+v"(lo), "+v"(hi));
   typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
   const u32x4_t r = {codes_bf16x2(lo, 0), codes_bf16x2(lo, 2), codes_bf16x2(hi, 0),
                      codes_bf16x2(hi, 2)};
@@ -61,35 +64,29 @@ __device__ inline int int8_chunk(int s, int j) {
 template <int D>
 __device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, Int8Query<D>& q) {
   constexpr int KS = Int8Query<D>::KS;
-  float x[KS][16];
-  float amax = 0.f;
-  bool bad = false;
+  uint32_t raw[KS][8];  // pairs of bf16
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const bool on = row && (D % 64 == 0 || 4 * s + j < D / 16);
-    uint4 w[2] = {uint4{0, 0, 0, 0}, uint4{0, 0, 0, 0}};
-    if (on) {
-      struct __attribute__((aligned(4))) Half {  // rows of any 4-byte alignment
-        uint32_t v[8];
-      };
-      const Half h = *reinterpret_cast<const Half*>(row + 16 * (4 * s + j));
-      w[0] = uint4{h.v[0], h.v[1], h.v[2], h.v[3]};
-      w[1] = uint4{h.v[4], h.v[5], h.v[6], h.v[7]};
-    }
-    const uint32_t d[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+    struct __attribute__((aligned(4))) Half {  // rows of any 4-byte alignment
+      uint32_t v[8];
+    };
+    Half h{};
+    if (on) h = *reinterpret_cast<const Half*>(row + 16 * (4 * s + j));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[s][i] = bf16_bits_to_f32((uint16_t)(d[i / 2] >> (16 * (i & 1))));
-      const float m = fabsf(x[s][i]);
-      bad |= !(m < INFINITY);
-      amax = fmaxf(amax, m);
-    }
+    for (int i = 0; i < 8; ++i) raw[s][i] = h.v[i];
   }
-  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-  int worse = bad;
-  worse |= __shfl_xor(worse, 16, 64);
-  worse |= __shfl_xor(worse, 32, 64);
+  // the largest of |x| as integers: NaN and infinities are above the rest
+  uint32_t top = 0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      top = max(top, max(raw[s][i] & 0x7FFFu, (raw[s][i] >> 16) & 0x7FFFu));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+  const bool worse = top >= 0x7F80u;
+  const float amax = bf16_bits_to_f32((uint16_t)top);
   // |x| 2^-e < 2^14 - 64: the largest is m 2^b, m < 2, so e = b - 13 gives less than
   // 2^14 and hi at most 128 where m is near 2; e = b - 12 there
   const uint32_t u = __builtin_bit_cast(uint32_t, amax);
@@ -102,7 +99,8 @@ __device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, 
     for (int i = 0; i < 4; ++i) hw[i] = lw[i] = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int n = worse ? 0 : (int)rintf(ldexpf(x[s][i], -e));
+      const float x = bf16_bits_to_f32((uint16_t)(raw[s][i / 2] >> (16 * (i & 1))));
+      const int n = worse ? 0 : (int)rintf(ldexpf(x, -e));
       const int hi = (n + 64) >> 7, lo = n - 128 * hi;
       hw[i / 4] |= (uint32_t)(uint8_t)hi << (8 * (i & 3));
       lw[i / 4] |= (uint32_t)(uint8_t)lo << (8 * (i & 3));
@@ -127,13 +125,17 @@ struct Int8State {
   }
 };
 
-// What a step of four blocks brings in.
+// A step of four blocks: this lane's rows of K and V, and block j's scale bytes.
 template <int D>
-struct Int8Step {
+struct Int8Keys {
   static constexpr int KS = Int8Query<D>::KS;
   i32x4 k[4][KS];
+  uint32_t scale;
+};
+template <int D>
+struct Int8Values {
   i32x4 v[D / 16];
-  uint32_t kb, vb;  // scale bytes of block j
+  uint32_t scale;
 };
 
 template <int D>
@@ -143,35 +145,33 @@ struct Int8Blocks {
   const uint8_t* ks;
   const uint8_t* vs;
   int Hkv, kvh;
-  // Loads the step whose four blocks' ids (in the pool) are id[g].
-  __device__ inline void load(const int (&id)[4], int c, int j, Int8Step<D>& st) const {
-    const int g = c >> 2;
-    const uint32_t kid = g < 2 ? (g ? id[1] : id[0]) : (g == 2 ? id[2] : id[3]);
-    const uint32_t vid = j < 2 ? (j ? id[1] : id[0]) : (j == 2 ? id[2] : id[3]);
-    const uint32_t kslice = kid * (uint32_t)Hkv + kvh, vslice = vid * (uint32_t)Hkv + kvh;
-    const int8_t* kr = kc + (uint64_t)kslice * (kBlock * D) + (c & 3) * D;
-    const int8_t* vr = vc + (uint64_t)vslice * (kBlock * D) + c * kBlock;
-    st.kb = ks[vslice];
-    st.vb = vs[vslice];
+  // Load a step: kid the id of block c / 4 (whose K rows this lane loads), vid that
+  // of block j, both in the pool.
+  __device__ inline void load_keys(int kid, int vid, int c, int j, Int8Keys<D>& st) const {
+    const uint32_t slice = (uint32_t)kid * (uint32_t)Hkv + kvh;
+    const int8_t* kr = kc + (uint64_t)slice * (kBlock * D) + (c & 3) * D;
+    st.scale = ks[(uint32_t)vid * (uint32_t)Hkv + kvh];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int s = 0; s < Int8Step<D>::KS; ++s)
+      for (int s = 0; s < Int8Keys<D>::KS; ++s)
         st.k[kk][s] = __builtin_nontemporal_load(
             reinterpret_cast<const i32x4*>(kr + 4 * kk * D + 16 * int8_chunk<D>(s, j)));
+  }
+  __device__ inline void load_values(int vid, int c, Int8Values<D>& st) const {
+    const uint32_t slice = (uint32_t)vid * (uint32_t)Hkv + kvh;
+    const int8_t* vr = vc + (uint64_t)slice * (kBlock * D) + c * kBlock;
+    st.scale = vs[slice];
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt)
       st.v[dt] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(vr + dt * 16 * kBlock));
   }
 };
 
-// One step into the softmax.  lim: tokens of block j (this lane's scores) that
-// query c attends, 16 where `whole` (wavefront-uniform).
+// The step's scores as integers.
 template <int D>
-__device__ inline void int8_step(const Int8Step<D>& st, const Int8Query<D>& q, bool whole, int lim,
-                                 Int8State<D>& S) {
+__device__ inline void int8_scores(const Int8Keys<D>& st, const Int8Query<D>& q, i32x4 (&a)[4]) {
   constexpr int KS = Int8Query<D>::KS;
-  i32x4 a[4];
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) a[kk] = i32x4{0, 0, 0, 0};
 #pragma unroll
@@ -188,10 +188,19 @@ __device__ inline void int8_step(const Int8Step<D>& st, const Int8Query<D>& q, b
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
       a[kk] = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.k[kk][s], q.lo[s], a[kk], 0, 0, 0);
+}
+
+// The scores into the softmax: the probabilities times the V scale, in bf16.  lim:
+// tokens of block j (this lane's scores) that query c attends, 16 where `whole`
+// (wavefront-uniform).
+template <int D>
+__device__ inline void int8_softmax(const i32x4 (&a)[4], uint32_t kscale, uint32_t vscale,
+                                    float factor, bool whole, int lim, Int8State<D>& S, bf16x8& p0,
+                                    bf16x8& p1) {
   // blocks that are not attended may hold any bytes
   const bool none = !whole && lim <= 0;
-  const float f = ldexpf(q.factor, none ? 0 : (int)st.kb - 127);
-  const int ev = none ? 0 : (int)st.vb - 127;
+  const float f = ldexpf(factor, none ? 0 : (int)kscale - 127);
+  const float fv = scale_of(none ? 127 : vscale);
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = (float)a[i >> 2][i & 3] * f;
@@ -214,8 +223,6 @@ __device__ inline void int8_step(const Int8Step<D>& st, const Int8Query<D>& q, b
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) S.o[dt] *= r;
   }
-  const float fv = ldexpf(1.f, ev);
-  bf16x8 p0, p1;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float p = __builtin_amdgcn_exp2f(x[i] - S.m);
@@ -225,12 +232,20 @@ __device__ inline void int8_step(const Int8Step<D>& st, const Int8Query<D>& q, b
     else
       p1[i - 8] = (__bf16)(p * fv);
   }
+}
+
+// The probabilities' product with the values.
+template <int D>
+__device__ inline void int8_output(const Int8Values<D>& st, const bf16x8& p0, const bf16x8& p1,
+                                   Int8State<D>& S) {
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) {
     S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
         codes_bf16x8(st.v[dt][0], st.v[dt][1]), p0, S.o[dt], 0, 0, 0);
     S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
         codes_bf16x8(st.v[dt][2], st.v[dt][3]), p1, S.o[dt], 0, 0, 0);
+    // (all the conversions first would take four times the values' registers)
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 

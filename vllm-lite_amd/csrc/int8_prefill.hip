@@ -1,8 +1,23 @@
 // Chunked causal attention over the int8 cache (pa_prefill_int8).
 //
-// A wavefront takes 16 query rows of one head against the keys up to their own,
-// straight from the cache.
+// A workgroup takes ROWS query rows of one sequence and kv head, a row being one
+// (token, query head of the group), numbered token by token, so any group fills it.
+// Keys come in tiles of KT (whole blocks): every thread loads its 16-byte pieces of
+// the codes two tiles ahead into registers and writes them as bf16 (exact) into one
+// of three LDS buffers, once for all wavefronts, whose steps of 32 keys then only
+// read matrix operands.
+//   Sᵀ = K·Qᵀ on v_mfma_f32_16x16x32_bf16, codes by the query as it is: exact
+//     products.  A lane's eight scores of a step are of one block, so its scale (times
+//     the softmax's) and the row's running maximum are one multiply-add.
+//   Oᵀ += Vᵀ·Pᵀ, codes by probabilities that carry the V scale: its exponent goes
+//     into the exponential's argument.  The denominators are one more product, of the
+//     same probabilities by 2^-exponent (exact).
+// The next step's score products are issued among this step's exponentials.  The
+// maximum is kept until a score passes it by 2^8.
+// KG = 2: half the wavefronts take the first 32 keys of each tile, half the second,
+// for launches of few rows; their results meet in LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "int8_wave.hpp"
 #include "pa_internal.hpp"
@@ -10,74 +25,577 @@
 namespace pa {
 namespace {
 
-constexpr int kStep = 4 * kBlock;  // keys a step
-constexpr int kPrefillWaves = 4;
+constexpr int kMaxSeqs = 256;  // whose tiles a launch numbers through
+
+// Rows of sequence s in q, clamped to what the caller's arrays hold.
+struct Rows {
+  int begin, len, past;
+};
+__device__ inline Rows rows_of(const int32_t* __restrict__ cu_q,
+                               const int32_t* __restrict__ past_lens, int s, int total_q,
+                               int max_q) {
+  const int begin = min(max(cu_q[s], 0), total_q);
+  const int end = min(max(cu_q[s + 1], begin), total_q);
+  return {begin, min(end - begin, max_q), max(past_lens[s], 0)};
+}
+
+template <int V>
+using IC = std::integral_constant<int, V>;
+
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+struct PrefillArgs {
+  uint16_t* out;
+  const uint16_t* q;
+  int64_t q_row;
+  const int8_t* kc;
+  const int8_t* vc;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  const int32_t* tables;
+  const int32_t* cu_q;
+  const int32_t* past_lens;
+  int mbs, Hq, Hkv, G, num_blocks, B, total_q, max_q, tiles_per_seq;
+  float scale_log2;
+};
 
 template <int D>
-__global__ __launch_bounds__(64 * kPrefillWaves) void prefill_int8_kernel(
-    uint16_t* __restrict__ out, const uint16_t* __restrict__ q, int64_t q_row,
-    const int8_t* __restrict__ kc, const int8_t* __restrict__ vc, const uint8_t* __restrict__ ks,
-    const uint8_t* __restrict__ vs, const int32_t* __restrict__ tables, int mbs,
-    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ past_lens, int Hq, int Hkv,
-    int G, int num_blocks, float scale_log2, int total_q, int max_q) {
-  constexpr int DT = D / 16;
-  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y, kvh = head / G, seq = blockIdx.z;
-  const int q_begin = min(max(cu_q[seq], 0), total_q);
-  const int len = min(min(max(cu_q[seq + 1], q_begin), total_q) - q_begin, max_q);
-  const int past = max(past_lens[seq], 0);
-  const int r0 = (blockIdx.x * kPrefillWaves + wave) * 16;
-  if (r0 >= len) return;
-  const int row = r0 + c;
-  Int8Query<D> qv;
-  int8_query<D>(row < len ? q + (int64_t)(q_begin + row) * q_row + (int64_t)head * D : nullptr, j,
-                scale_log2, qv);
-  // keys in all, and of this lane's row
-  const int64_t cap = (int64_t)mbs * kBlock;
-  const int end = (int)min((int64_t)past + min(len, r0 + 16), cap);
-  const int mine = (int)min((int64_t)past + row + 1, cap);
-  const int32_t* tab = tables + (int64_t)seq * mbs;
-  const Int8Blocks<D> blocks{kc, vc, ks, vs, Hkv, kvh};
-  Int8State<D> S;
-  S.init();
-  int32_t ids = -1;
-  const int steps = (end + kStep - 1) / kStep;
-  for (int s = 0; s < steps; ++s) {
-    const int b = 4 * s;
-    if (s % 16 == 0) ids = b + lane < mbs ? tab[b + lane] : -1;
-    const int at = 4 * (s % 16);
-    int kid = __shfl(ids, at + (c >> 2), 64), vid = __shfl(ids, at + j, 64);
-    const bool ok = vid >= 0 && vid < num_blocks;
-    const int lim = ok ? min(max(mine - (b + j) * kBlock, 0), kBlock) : 0;
-    const bool whole = __builtin_amdgcn_ballot_w64(lim < kBlock) == 0;
-    if (!ok) vid = 0;
-    if (kid < 0 || kid >= num_blocks) kid = 0;
-    Int8Keys<D> k;
-    Int8Values<D> v;
-    blocks.load_keys(kid, vid, c, j, k);
-    blocks.load_values(vid, c, v);
-    i32x4 a[4];
-    bf16x8 p0, p1;
-    int8_scores<D>(k, qv, a);
-    int8_softmax<D>(a, k.scale, v.scale, qv.factor, whole, lim, S, p0, p1);
-    int8_output<D>(v, p0, p1, S);
+constexpr int key_tile() {  // keys a tile: three buffers of K and V fit LDS
+  return D <= 128 ? 64 : 32;
+}
+
+template <int D, int NT, int W, int KG>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 4))) void
+prefill_int8_kernel(const PrefillArgs a) {
+  constexpr int KS = D / 32;  // reduction steps of the scores
+  constexpr int DT = D / 16;  // tiles of the output
+  constexpr int KT = key_tile<D>(), NB = KT / kBlock;
+  constexpr int NBUF = 3;
+  constexpr int SPT = KT / 32 / KG;  // a wavefront's steps a tile
+  static_assert(SPT >= 1, "a step for every group of wavefronts");
+  constexpr int ROWS = 16 * NT * (W / KG);
+  constexpr int T = 64 * W;
+  // LDS rows are an odd number of 16-byte chunks, so that the 16 lanes of an operand
+  // read (consecutive rows) meet different banks
+  constexpr int KROW = D * 2 + 16, VROW = KT * 2 + 16;
+  constexpr int PIECES = 2 * KT * D / 16;  // 16-byte pieces of a tile, K's then V's
+  constexpr int PPT = (PIECES + T - 1) / T;
+  struct Tiles {
+    uint8_t k[NBUF][KT * KROW], v[NBUF][D * VROW];
+  };
+  __shared__ __attribute__((aligned(16))) Tiles lds;
+  // of a tile's blocks: the factor of their scores, the exponent of their V scale,
+  // and 2^-exponent as a pair of bf16
+  __shared__ float s_factor[NBUF][NB], s_exp[NBUF][NB];
+  __shared__ uint32_t s_one[NBUF][NB];
+  __shared__ int rank_seq[kMaxSeqs], rank_begin[kMaxSeqs], rank_len[kMaxSeqs],
+      rank_past[kMaxSeqs], rank_tile0[kMaxSeqs], rank_of[kMaxSeqs], tile0_of[kMaxSeqs];
+  __shared__ int tiles_in_all;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, j = lane >> 4;
+  const int G = a.G, B = a.B;
+  auto tiles_of = [&](int len) -> int { return (len * G + ROWS - 1) / ROWS; };
+
+  // Work items: ROWS rows of a sequence for one kv head.  The sequences' tiles are
+  // numbered through, those with the most keys first and within one the later
+  // (longer) tiles first, by ranks and prefix sums formed in LDS (up to kMaxSeqs
+  // sequences; beyond, tiles_per_seq for each in index order).  A kv head's items go
+  // to one XCD, or to its share of them, whose L2 then holds its K and V; an XCD's
+  // workgroups take its items in rounds, forth and back, which pairs long and short
+  // ones.
+  const bool compact = B <= kMaxSeqs;
+  if (compact) {
+    for (int b = tid; b < B; b += T) rank_of[b] = tile0_of[b] = 0;
+    __syncthreads();
+    for (int o0 = 0; o0 < B; o0 += 64) {
+      const Rows ro = rows_of(a.cu_q, a.past_lens, min(o0 + lane, B - 1), a.total_q, a.max_q);
+      const int okey = ro.past + ro.len, otiles = tiles_of(ro.len), n = min(B - o0, 64);
+      for (int b0 = 0; b0 < B; b0 += 64) {
+        const int b = b0 + lane;
+        int key = okey;
+        if (b0 != o0) {
+          const Rows r = rows_of(a.cu_q, a.past_lens, min(b, B - 1), a.total_q, a.max_q);
+          key = r.past + r.len;
+        }
+        int rank = 0, before = 0;
+        for (int i = wave; i < n; i += W) {
+          const int ko = __builtin_amdgcn_readlane(okey, i);
+          const bool first = ko > key || (ko == key && o0 + i < b);
+          rank += first;
+          before += first ? __builtin_amdgcn_readlane(otiles, i) : 0;
+        }
+        if (b < B && rank > 0) {
+          atomicAdd(&rank_of[b], rank);
+          atomicAdd(&tile0_of[b], before);
+        }
+      }
+    }
+    __syncthreads();
+    for (int b = tid; b < B; b += T) {
+      const Rows r = rows_of(a.cu_q, a.past_lens, b, a.total_q, a.max_q);
+      const int rank = rank_of[b], before = tile0_of[b];
+      rank_seq[rank] = b;
+      rank_begin[rank] = r.begin;
+      rank_len[rank] = r.len;
+      rank_past[rank] = r.past;
+      rank_tile0[rank] = before;
+      if (rank == B - 1) tiles_in_all = before + tiles_of(r.len);
+    }
+    __syncthreads();
   }
-  float lsum = S.lsum;
-  lsum += __shfl_xor(lsum, 16, 64);
-  lsum += __shfl_xor(lsum, 32, 64);
-  if (row >= len) return;
-  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-  uint16_t* o = out + ((int64_t)(q_begin + row) * Hq + head) * D + 4 * j;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    struct __attribute__((aligned(8))) W {
-      uint16_t v[4];
-    } w;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) w.v[r] = f32_to_bf16_bits(S.o[dt][r] * inv);
-    *reinterpret_cast<W*>(o + 16 * dt) = w;
+  const int nq = compact ? tiles_in_all : B * a.tiles_per_seq;  // tiles a kv head
+  const int xcd = (int)(blockIdx.x % 8), nslot = (int)(gridDim.x / 8), slot = (int)(blockIdx.x / 8);
+  // the XCD's item i is tile (t0 + i * dt) % nq of head g0 + (t0 + i * dt) / nq
+  int g0 = 0, t0 = 0, dt_items = 1, items;
+  const int Hkv = a.Hkv;
+  if (Hkv == 1 || Hkv == 2 || Hkv == 4 || Hkv == 8) {
+    const int sh = Hkv == 1 ? 3 : Hkv == 2 ? 2 : Hkv == 4 ? 1 : 0;
+    dt_items = 1 << sh;
+    g0 = xcd >> sh;
+    t0 = xcd & (dt_items - 1);
+    items = t0 < nq ? (nq - t0 + dt_items - 1) >> sh : 0;
+  } else {
+    const int total = Hkv * nq, per_xcd = (total + 7) / 8;
+    t0 = min(total, xcd * per_xcd);
+    items = min(total, t0 + per_xcd) - t0;
   }
+
+  auto process = [&](int item) {
+    int kvh = g0, qt = t0 + item * dt_items;
+    if (qt >= nq) {
+      kvh += qt / nq;
+      qt %= nq;
+    }
+    __syncthreads();  // every wavefront is done with the previous item's LDS
+    int seq, tile;
+    Rows qr;
+    if (compact) {
+      int r = -1;  // the last rank whose tiles begin at or before this one
+      for (int b0 = 0; b0 < B; b0 += 64)
+        r += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
+            b0 + lane < B && rank_tile0[min(b0 + lane, B - 1)] <= qt));
+      seq = __builtin_amdgcn_readfirstlane(rank_seq[r]);
+      qr.begin = __builtin_amdgcn_readfirstlane(rank_begin[r]);
+      qr.len = __builtin_amdgcn_readfirstlane(rank_len[r]);
+      qr.past = __builtin_amdgcn_readfirstlane(rank_past[r]);
+      tile = tiles_of(qr.len) - 1 - (qt - __builtin_amdgcn_readfirstlane(rank_tile0[r]));
+    } else {
+      seq = qt / a.tiles_per_seq;
+      tile = a.tiles_per_seq - 1 - qt % a.tiles_per_seq;
+      qr = rows_of(a.cu_q, a.past_lens, seq, a.total_q, a.max_q);
+    }
+    const int rows = qr.len * G, past = qr.past;
+    if (tile * ROWS >= rows) return;  // uniform over the workgroup
+    const int last_token = (min(rows, (tile + 1) * ROWS) - 1) / G;
+    const int64_t cap = (int64_t)a.mbs * kBlock;
+    const int key_end = (int)min((int64_t)past + last_token + 1, cap);
+    const int n_kt = (key_end + KT - 1) / KT;
+    const int nblk = (key_end + kBlock - 1) / kBlock;
+    const int32_t* tab = a.tables + (int64_t)seq * a.mbs;
+
+    // KG = 2: wavefronts W / 2 .. take the second 32 keys of every tile
+    const int kgrp = KG == 2 ? wave / (W / 2) : 0, wt = KG == 2 ? wave % (W / 2) : wave;
+    const int r0 = tile * ROWS + wt * 16 * NT;  // first row of this wavefront
+    const bool active = r0 < rows;
+
+    // ---- staging: this thread's pieces of a tile
+    // Piece i < KT D / 16 is chunk i % (D / 16) of key i / (D / 16); the others are
+    // dim i' % D of block i' / D.  Blocks behind the last and ids outside the pool
+    // read block 0.
+    int32_t next_id[PPT];  // of the tile to load next
+    auto load_ids = [&](int kt) {
+#pragma unroll
+      for (int n = 0; n < PPT; ++n) {
+        const int i = tid + n * T;
+        const int b = i < PIECES / 2 ? i / (D / 16) / kBlock : (i - PIECES / 2) / D;
+        const int32_t id = tab[min(kt * NB + min(b, NB - 1), nblk - 1)];
+        next_id[n] = id >= 0 && id < a.num_blocks ? id : 0;
+      }
+    };
+    i32x4 raw[PPT];
+    uint32_t raw_k = 0, raw_v = 0;  // threads below NB: block tid's scale bytes
+    auto load_tile = [&](int kt) {
+#pragma unroll
+      for (int n = 0; n < PPT; ++n) {
+        const int i = tid + n * T;
+        const uint64_t slice = (uint64_t)((uint32_t)next_id[n] * (uint32_t)Hkv + kvh) * (kBlock * D);
+        if (PIECES % T != 0 && i >= PIECES) continue;
+        if (i < PIECES / 2) {
+          raw[n] = *reinterpret_cast<const i32x4*>(a.kc + slice + (i % (kBlock * D / 16)) * 16);
+        } else {
+          raw[n] = *reinterpret_cast<const i32x4*>(a.vc + slice + ((i - PIECES / 2) % D) * 16);
+        }
+      }
+      if (tid < NB) {
+        const int32_t id = tab[min(kt * NB + tid, nblk - 1)];
+        const uint32_t s = (uint32_t)(id >= 0 && id < a.num_blocks ? id : 0) * (uint32_t)Hkv + kvh;
+        raw_k = a.ks[s];
+        raw_v = a.vs[s];
+      }
+    };
+    auto write_tile = [&](int buf) {
+#pragma unroll
+      for (int n = 0; n < PPT; ++n) {
+        const int i = tid + n * T;
+        if (PIECES % T != 0 && i >= PIECES) continue;
+        uint8_t* to;
+        if (i < PIECES / 2) {
+          // key 32 s + 8 g + 4 kk + r sits at row 32 s + 16 kk + 4 g + r: the lanes of
+          // an operand read take consecutive rows
+          const int key = i / (D / 16), ch = i % (D / 16);
+          const int r = (key & ~31) + ((key >> 2) & 1) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+          to = &lds.k[buf][r * KROW + ch * 32];
+        } else {
+          const int v = i - PIECES / 2;
+          to = &lds.v[buf][(v % D) * VROW + (v / D) * 32];
+        }
+        reinterpret_cast<bf16x8*>(to)[0] = codes_bf16x8(raw[n][0], raw[n][1]);
+        reinterpret_cast<bf16x8*>(to)[1] = codes_bf16x8(raw[n][2], raw[n][3]);
+      }
+      if (tid < NB) {
+        // (a scale of 0, and what no scale is, only occurs in blocks never written)
+        const int ev = raw_v == 0 || raw_v > 253 ? 0 : (int)raw_v - 127;
+        s_factor[buf][tid] = fabsf(a.scale_log2) * scale_of(raw_k);
+        s_exp[buf][tid] = (float)ev;
+        s_one[buf][tid] = (uint32_t)(127 - ev) * 0x00800080u;
+      }
+    };
+    // LDS writes done, then a barrier; loads to registers stay in flight.
+    auto barrier = [&]() __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+
+    // ---- the query rows, and the table's ids
+    load_ids(0);
+    load_tile(0);
+    bf16x8 qv[NT][KS];
+    int pos[NT];  // the lane's rows' positions
+    const uint16_t flip = a.scale_log2 < 0.f ? 0x8000 : 0;  // a negative scale, by the query
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = r0 + 16 * nt + c, rc = min(row, rows - 1);
+      const int token = rc / G, h = rc - token * G;
+      pos[nt] = past + token;
+      const uint16_t* qp =
+          a.q + (int64_t)(qr.begin + token) * a.q_row + (int64_t)(kvh * G + h) * D + 8 * j;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        struct __attribute__((aligned(4))) Piece {  // rows of any 4-byte alignment
+          uint32_t v[4];
+        };
+        const Piece p = *reinterpret_cast<const Piece*>(qp + 32 * s);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = row < rows ? p.v[i] ^ (flip * 0x10001u) : 0;
+        typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        qv[nt][s] = __builtin_bit_cast(bf16x8, u32x4_t{w[0], w[1], w[2], w[3]});
+      }
+    }
+    int bad = 0;
+    for (int b = tid; b < nblk; b += T) {
+      const int32_t id = tab[b];
+      bad |= id < 0 || id >= a.num_blocks ? 1 : 0;
+    }
+    const bool bad_ids = __syncthreads_or(bad) != 0;
+    f32x4 o[NT][DT];
+    f32x4 lacc[NT];  // denominators
+    float nm[NT];    // minus the rows' maxima
+    float raise = 8.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      nm[nt] = 0.f;
+      lacc[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[nt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // tiles 0 and 1 into LDS, tile 2 on its way
+    write_tile(0);
+    if (n_kt > 1) {
+      load_ids(1);
+      load_tile(1);
+      write_tile(1);
+    }
+    if (n_kt > 2) {
+      load_ids(2);
+      load_tile(2);
+      if (n_kt > 3) load_ids(3);
+    }
+    barrier();
+
+    auto qk_load = [&](int buf, int st, bf16x8 (&ka)[2][KS]) __attribute__((always_inline)) {
+      const uint8_t* row = &lds.k[buf][(st * 32 + c) * KROW + j * 16];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          ka[kk][s] = *reinterpret_cast<const bf16x8*>(row + kk * 16 * KROW + s * 64);
+    };
+    f32x4 S0[NT][2], S1[NT][2];
+    {
+      bf16x8 ka[2][KS];
+      qk_load(0, kgrp, ka);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          S0[nt][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+            S0[nt][kk] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[kk][s], qv[nt][s], S0[nt][kk], 0, 0, 0);
+        }
+    }
+
+    // One step of 32 keys (step `st` of tile kt, in buffer buf): the softmax of S
+    // (computed before), this step's products with V among the next step's scores.
+    // LAST: the tile's last step of this wavefront, which begins with the boundary.
+    auto step = [&](int buf, int st, auto last, int kt, f32x4 (&S)[NT][2], f32x4 (&Sn)[NT][2]) {
+      constexpr bool LAST = decltype(last)::value;
+      const int next = buf == NBUF - 1 ? 0 : buf + 1;
+      const int free_buf = buf == 0 ? NBUF - 1 : buf - 1;
+      bf16x8 va[DT];
+      {
+        const uint8_t* row = &lds.v[buf][c * VROW + st * 64 + j * 16];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          va[dt] = *reinterpret_cast<const bf16x8*>(row + dt * 16 * VROW);
+      }
+      const int blk = 2 * st + (j >> 1);  // the lane's block of the tile
+      const float factor = s_factor[buf][blk], ev = s_exp[buf][blk];
+      const uint32_t one = s_one[buf][blk];
+      bf16x8 ka[2][KS];
+      if constexpr (LAST) {
+        // The next tile is in LDS (written a boundary ago), the one before this is
+        // free.  Past the last tile the operands read here are never used.
+        if (kt + 1 < n_kt) {
+          barrier();
+          if (kt + 2 < n_kt) write_tile(free_buf);
+          if (kt + 3 < n_kt) {
+            load_tile(kt + 3);
+            if (kt + 4 < n_kt) load_ids(kt + 4);
+          }
+          asm volatile("" ::: "memory");
+        }
+        qk_load(next, kgrp, ka);
+      } else {
+        qk_load(buf, st + 1, ka);
+      }
+      float f = factor;
+      float add[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) add[nt] = nm[nt];
+      {
+        const int kb = kt * KT + st * 32;
+        const bool tail = kt * KT + KT > key_end || bad_ids;
+        if (tail || kb + 31 > past + r0 / G) {
+          // keys behind the last, in blocks outside the pool or above a row's
+          // diagonal: the scores are finished here
+          int end = key_end;
+          if (bad_ids) {
+            const int b = kt * NB + blk;
+            const int32_t id = b < nblk ? tab[b] : -1;
+            end = id >= 0 && id < a.num_blocks ? key_end : 0;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int key = kb + 8 * j + i;
+              const float x = __builtin_fmaf(S[nt][i >> 2][i & 3], f, nm[nt]);
+              S[nt][i >> 2][i & 3] = key >= end || key > pos[nt] ? -INFINITY : x;
+            }
+            add[nt] = 0.f;
+          }
+          f = 1.f;
+        }
+        float lm[NT];
+        bool need = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float m0 = max3(S[nt][0][0], S[nt][0][1], S[nt][0][2]);
+          const float m1 = max3(S[nt][0][3], S[nt][1][0], S[nt][1][1]);
+          lm[nt] = __builtin_fmaf(max3(m0, m1, max3(S[nt][1][2], S[nt][1][3], S[nt][1][3])), f,
+                                  add[nt]);
+          need |= lm[nt] > raise;
+        }
+        // A row's first step with keys sets its maximum exactly: step 0, or the first
+        // that ids outside the pool do not mask (its denominator is 0 until then).
+        const bool first = kt == 0 && (SPT == 1 || st == 0);
+        if (__builtin_expect(first || __builtin_amdgcn_ballot_w64(need) != 0, 0)) {
+          raise = 8.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float bm = lm[nt];
+            bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+            bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+            const bool none = first || lacc[nt][0] == 0.f;
+            const bool masked = !(bm > -INFINITY);
+            if (none && masked) raise = -INFINITY;
+            const float delta = none ? (masked ? 0.f : bm) : fmaxf(bm, 0.f);
+            nm[nt] -= delta;
+            add[nt] -= delta;
+            if (!first) {
+              const float r = none ? 1.f : __builtin_amdgcn_exp2f(-delta);
+              lacc[nt] *= r;
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= r;
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) add[nt] += ev;
+      }
+      {
+        constexpr int NQK = 2 * KS * NT;  // next-step score products
+        constexpr int NEXP = 8 * NT;      // exponentials a lane
+        constexpr int EPM = (NEXP + NQK - 1) / NQK;
+        float pv[NT][8];
+#pragma unroll
+        for (int g = 0; g < NQK; ++g) {
+          const int s = g / (2 * NT), q_ = g % (2 * NT), nt_ = q_ / 2, kk = q_ % 2;
+          Sn[nt_][kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              ka[kk][s], qv[nt_][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : Sn[nt_][kk], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < EPM; ++e) {
+            const int x = g * EPM + e;
+            if (x < NEXP) {
+              const int nt = x / 8, i = x % 8;
+              pv[nt][i] =
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(S[nt][i >> 2][i & 3], f, add[nt]));
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NQK; ++g) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x002, EPM, 0);  // VALU
+          __builtin_amdgcn_sched_group_barrier(0x400, EPM, 0);  // transcendental
+        }
+        bf16x8 pb[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pb[nt][i] = (__bf16)pv[nt][i];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            o[nt][dt] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt], pb[nt], o[nt][dt], 0, 0, 0);
+        typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4_t{one, one, one, one});
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          lacc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[nt], lacc[nt], 0, 0, 0);
+      }
+    };
+
+    for (int kt = 0, buf = 0; kt < n_kt; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1) {
+      if constexpr (SPT == 2) {
+        step(buf, 0, std::false_type{}, kt, S0, S1);
+        step(buf, 1, std::true_type{}, kt, S1, S0);
+      } else {
+        step(buf, kgrp, std::true_type{}, kt, S0, S1);
+        if (++kt == n_kt) break;
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
+        step(buf, kgrp, std::true_type{}, kt, S1, S0);
+      }
+    }
+
+    if constexpr (KG == 2) {
+      // The two groups' results, in the tiles' space.  A group that saw no key of a
+      // row (l = 0) drops out.
+      static_assert(W / 2 * NT * (DT * 1024 + 512) <= (int)sizeof(Tiles), "space");
+      float* mo = reinterpret_cast<float*>(&lds);
+      float* mml = mo + W / 2 * NT * DT * 256;
+      __syncthreads();
+      if (kgrp == 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            *reinterpret_cast<f32x4*>(mo + ((wt * NT + nt) * DT + dt) * 256 + lane * 4) =
+                o[nt][dt];
+          *reinterpret_cast<float2*>(mml + ((wt * NT + nt) * 64 + lane) * 2) =
+              float2{-nm[nt], lacc[nt][0]};
+        }
+      }
+      __syncthreads();
+      if (kgrp == 1) return;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 ml = *reinterpret_cast<const float2*>(mml + ((wt * NT + nt) * 64 + lane) * 2);
+        const float ma = lacc[nt][0] != 0.f ? -nm[nt] : kInt8NoMax;
+        const float mb = ml.y != 0.f ? ml.x : kInt8NoMax;
+        const float mx = fmaxf(ma, mb);
+        const float fa = __builtin_amdgcn_exp2f(ma - mx), fb = __builtin_amdgcn_exp2f(mb - mx);
+        lacc[nt] = lacc[nt] * fa + ml.y * fb;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          o[nt][dt] = o[nt][dt] * fa + *reinterpret_cast<const f32x4*>(
+                                           mo + ((wt * NT + nt) * DT + dt) * 256 + lane * 4) * fb;
+      }
+    }
+
+    if (!active) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = r0 + 16 * nt + c;
+      if (row >= rows) continue;
+      const int token = row / G, h = row - token * G;
+      const float l = lacc[nt][0];
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      uint16_t* to = a.out + ((int64_t)(qr.begin + token) * a.Hq + kvh * G + h) * D + 4 * j;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        struct __attribute__((aligned(8))) Four {
+          uint16_t v[4];
+        } w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w.v[r] = f32_to_bf16_bits(o[nt][dt][r] * inv);
+        *reinterpret_cast<Four*>(to + 16 * dt) = w;
+      }
+    }
+  };
+  for (int r = 0; r * nslot < items; ++r) {
+    const int item = r * nslot + ((r & 1) ? nslot - 1 - slot : slot);
+    if (item < items) process(item);
+  }
+}
+
+int compute_units() {
+  static const int cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+      n = 256;
+    return std::max(n, 8);
+  }();
+  return cus;
+}
+
+template <int D, int NT, int W, int KG>
+int32_t launch(const PrefillArgs& args, int num_seqs, hipStream_t s) {
+  PrefillArgs a = args;
+  constexpr int ROWS = 16 * NT * (W / KG);
+  a.tiles_per_seq = (int)(((int64_t)a.max_q * a.G + ROWS - 1) / ROWS);
+  const long long total = (long long)num_seqs * a.Hkv * a.tiles_per_seq;
+  PA_REQUIRE(total < (1ll << 31) / 8 && (int64_t)a.max_q * a.G < (1ll << 31) - ROWS,
+             PA_ERR_UNSUPPORTED, "pa_prefill_int8: launch too large");
+  const int per_xcd = (int)((total + 7) / 8);
+  // a multiple of the 8 XCDs, about one workgroup per CU
+  const dim3 grid(8 * std::max(1, std::min(per_xcd, compute_units() / 8)));
+  prefill_int8_kernel<D, NT, W, KG><<<grid, 64 * W, 0, s>>>(a);
+  return PA_OK;
 }
 
 }  // namespace
@@ -108,27 +626,43 @@ int32_t prefill_int8_strided(void* out, const void* q, int64_t q_row, const int8
                  q_row % 2 == 0 && (uintptr_t)out % 8 == 0,
              PA_ERR_INVALID_ARG,
              "pa_prefill_int8: caches not 16-byte, q not 4-byte or out not 8-byte aligned");
-  PA_REQUIRE((int64_t)max_blocks_per_seq * kBlock < (1ll << 31) - 4096 && num_heads <= 65535 &&
-                 num_seqs <= 65535 && (long long)num_blocks * num_kv_heads < (1ll << 32) &&
-                 grid_fits(((int64_t)max_q_len + 63) / 64, 256),
+  PA_REQUIRE((int64_t)max_blocks_per_seq * kBlock < (1ll << 31) - 4096 &&
+                 (long long)num_blocks * num_kv_heads < (1ll << 32),
              PA_ERR_UNSUPPORTED, "pa_prefill_int8: launch too large");
-  const int rows = 16 * kPrefillWaves;
-  const dim3 grid(((int64_t)max_q_len + rows - 1) / rows, num_heads, num_seqs);
   const int G = num_heads / num_kv_heads;
-#define PA_LAUNCH_PREFILL_INT8(DD)                                                             \
-  prefill_int8_kernel<DD><<<grid, 64 * kPrefillWaves, 0, s>>>(                                 \
-      (uint16_t*)out, (const uint16_t*)q, q_row, k_cache, v_cache, k_scales, v_scales,         \
-      block_tables, max_blocks_per_seq, cu_q_lens, past_lens, num_heads, num_kv_heads, G,      \
-      num_blocks, scale * kInt8Log2e, total_q, max_q_len)
+  const PrefillArgs a{(uint16_t*)out, (const uint16_t*)q, q_row, k_cache, v_cache, k_scales,
+                      v_scales, block_tables, cu_q_lens, past_lens, max_blocks_per_seq, num_heads,
+                      num_kv_heads, G, num_blocks, num_seqs, total_q, max_q_len, 0,
+                      scale * kInt8Log2e};
+  // Rows a workgroup: an item's time is its keys times the time a tile takes, and a
+  // launch's items share the CUs; the lengths are on the device, so the items are
+  // counted from the totals.
+  auto cost = [&](int rows, double per_tile) -> double {
+    const double tiles = std::max((double)num_seqs, (double)total_q * G / rows + 0.5 * num_seqs);
+    return per_tile * std::max(1., 0.65 / 256 * tiles * num_kv_heads);
+  };
+  const double c256 = cost(256, 1.), c128 = cost(128, 0.7), c64 = cost(64, 0.53);
+  auto narrow = [&](auto dc) -> int32_t {
+    constexpr int DD = decltype(dc)::value;
+    if (c256 <= c128 && c256 <= c64) return launch<DD, 2, 8, 1>(a, num_seqs, s);
+    if (c128 <= c64) return launch<DD, 2, 8, 2>(a, num_seqs, s);
+    return launch<DD, 1, 8, 2>(a, num_seqs, s);
+  };
+  auto wide = [&](auto dc) -> int32_t {
+    constexpr int DD = decltype(dc)::value;
+    if (c128 <= c64) return launch<DD, 2, 4, 1>(a, num_seqs, s);
+    return launch<DD, 1, 4, 1>(a, num_seqs, s);
+  };
+  int32_t rc;
   switch (head_dim) {
-    case 32: PA_LAUNCH_PREFILL_INT8(32); break;
-    case 64: PA_LAUNCH_PREFILL_INT8(64); break;
-    case 96: PA_LAUNCH_PREFILL_INT8(96); break;
-    case 128: PA_LAUNCH_PREFILL_INT8(128); break;
-    case 192: PA_LAUNCH_PREFILL_INT8(192); break;
-    default: PA_LAUNCH_PREFILL_INT8(256); break;
+    case 32: rc = narrow(IC<32>{}); break;
+    case 64: rc = narrow(IC<64>{}); break;
+    case 96: rc = narrow(IC<96>{}); break;
+    case 128: rc = narrow(IC<128>{}); break;
+    case 192: rc = wide(IC<192>{}); break;
+    default: rc = wide(IC<256>{}); break;
   }
-#undef PA_LAUNCH_PREFILL_INT8
+  if (rc != PA_OK) return rc;
   return check_launch("pa_prefill_int8");
 }
 }  // namespace pa

@@ -2,30 +2,29 @@
 //
 // A workgroup takes ROWS query rows of one sequence and kv head, a row being one
 // (token, query head of the group), numbered token by token, so any group fills it.
-// Keys come in tiles of KT (whole blocks): every thread loads its 16-byte pieces of
-// the codes two tiles ahead into registers and writes them as bf16 (exact) into one
-// of three LDS buffers, once for all wavefronts, whose steps of 32 keys then only
-// read matrix operands.
+// Keys come in tiles of KT (whole blocks).  Their codes are copied HBM -> LDS four
+// tiles ahead; two tiles ahead every wavefront writes the pieces that it copied itself
+// (so no barrier stands between) as bf16, exact, into one of three buffers of matrix
+// operands, once for all wavefronts.
 //   Sᵀ = K·Qᵀ on v_mfma_f32_16x16x32_bf16, codes by the query as it is: exact
-//     products.  A lane's eight scores of a step are of one block, so its scale (times
-//     the softmax's) and the row's running maximum are one multiply-add.
+//     products.  A lane's eight scores of a step of 32 keys are of one block: the
+//     softmax's and the block's scale and the row's running maximum are one
+//     multiply-add of a score.
 //   Oᵀ += Vᵀ·Pᵀ, codes by probabilities that carry the V scale: its exponent goes
 //     into the exponential's argument.  The denominators are one more product, of the
-//     same probabilities by 2^-exponent (exact).
-// The next step's score products are issued among this step's exponentials.  The
-// maximum is kept until a score passes it by 2^8.
+//     same probabilities (as rounded) by 2^-exponent, exact.
+// The maximum is kept until a score passes it by 2^8.
 // KG = 2: half the wavefronts take the first 32 keys of each tile, half the second,
 // for launches of few rows; their results meet in LDS.
 #include <algorithm>
 #include <type_traits>
 
 #include "int8_wave.hpp"
+#include "lds_copy.hpp"
 #include "pa_internal.hpp"
 
 namespace pa {
 namespace {
-
-constexpr int kMaxSeqs = 256;  // whose tiles a launch numbers through
 
 // Rows of sequence s in q, clamped to what the caller's arrays hold.
 struct Rows {
@@ -68,30 +67,40 @@ constexpr int key_tile() {  // keys a tile: three buffers of K and V fit LDS
   return D <= 128 ? 64 : 32;
 }
 
+template <int D>
+constexpr int max_seqs() {  // whose tiles a launch numbers through, beside the tiles in LDS
+  return D <= 192 ? 256 : 128;
+}
+
 template <int D, int NT, int W, int KG>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 4))) void
 prefill_int8_kernel(const PrefillArgs a) {
   constexpr int KS = D / 32;  // reduction steps of the scores
   constexpr int DT = D / 16;  // tiles of the output
   constexpr int KT = key_tile<D>(), NB = KT / kBlock;
-  constexpr int NBUF = 3;
   constexpr int SPT = KT / 32 / KG;  // a wavefront's steps a tile
   static_assert(SPT >= 1, "a step for every group of wavefronts");
+  // EARLY: operands are read ahead (K two steps, V one), where the tiles are there and
+  // the registers too.
+  constexpr bool EARLY = SPT == 2;
+  constexpr int NBUF = 3;  // operand buffers; tile kt + 2 is written during tile kt
   constexpr int ROWS = 16 * NT * (W / KG);
   constexpr int T = 64 * W;
-  // LDS rows are an odd number of 16-byte chunks, so that the 16 lanes of an operand
-  // read (consecutive rows) meet different banks
-  constexpr int KROW = D * 2 + 16, VROW = KT * 2 + 16;
+  // LDS rows of 2 mod 4 16-byte chunks: an operand read (16 rows, 4 chunks of each)
+  // runs at 248 bytes a clock, at 128 with an odd number and at 32 with rows of 256
+  // bytes
+  constexpr int KROW = D * 2 + 32, VROW = KT * 2 + 32;
+  static_assert(KROW / 16 % 4 == 2 && VROW / 16 % 4 == 2, "LDS rows");
   constexpr int PIECES = 2 * KT * D / 16;  // 16-byte pieces of a tile, K's then V's
-  constexpr int PPT = (PIECES + T - 1) / T;
+  constexpr int CHUNKS = PIECES / 64;      // of a wavefront's copy instruction
+  constexpr int PPT = (CHUNKS + W - 1) / W;
+  constexpr int GT = 64 / NB;  // tiles whose blocks' ids and scales 64 lanes hold
   struct Tiles {
     uint8_t k[NBUF][KT * KROW], v[NBUF][D * VROW];
   };
   __shared__ __attribute__((aligned(16))) Tiles lds;
-  // of a tile's blocks: the factor of their scores, the exponent of their V scale,
-  // and 2^-exponent as a pair of bf16
-  __shared__ float s_factor[NBUF][NB], s_exp[NBUF][NB];
-  __shared__ uint32_t s_one[NBUF][NB];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage[2][PIECES * 16];
+  constexpr int kMaxSeqs = max_seqs<D>();
   __shared__ int rank_seq[kMaxSeqs], rank_begin[kMaxSeqs], rank_len[kMaxSeqs],
       rank_past[kMaxSeqs], rank_tile0[kMaxSeqs], rank_of[kMaxSeqs], tile0_of[kMaxSeqs];
   __shared__ int tiles_in_all;
@@ -204,66 +213,78 @@ prefill_int8_kernel(const PrefillArgs a) {
     const int r0 = tile * ROWS + wt * 16 * NT;  // first row of this wavefront
     const bool active = r0 < rows;
 
-    // ---- staging: this thread's pieces of a tile
-    // Piece i < KT D / 16 is chunk i % (D / 16) of key i / (D / 16); the others are
-    // dim i' % D of block i' / D.  Blocks behind the last and ids outside the pool
-    // read block 0.
-    int32_t next_id[PPT];  // of the tile to load next
-    auto load_ids = [&](int kt) {
+    // ---- the blocks' ids and scales: lane t holds those of block t of a group of GT
+    // tiles.  Blocks behind the last and ids outside the pool read block 0.
+    auto load_ids = [&](int group) -> int32_t {
+      return tab[min(group * 64 + lane, nblk - 1)];
+    };
+    auto in_pool = [&](int32_t id) -> int32_t { return id >= 0 && id < a.num_blocks ? id : 0; };
+    int32_t ids = in_pool(load_ids(0)), ids_next = load_ids(1);  // of the tiles copied
+    uint32_t ksc, vsc, ksc_next, vsc_next;                       // of the tiles computed
+    {
+      const uint32_t s = (uint32_t)ids * (uint32_t)Hkv + kvh;
+      ksc = a.ks[s];
+      vsc = a.vs[s];
+      ksc_next = ksc;
+      vsc_next = vsc;
+    }
+    // ---- staging: wavefront w copies and writes pieces 64 (w + n W) + lane.  Piece
+    // i < KT D / 16 is chunk i % (D / 16) of key i / (D / 16); the others are dim i' % D
+    // of block i' / D.
+    auto copy_tile = [&](int kt) {
+      if (kt % GT == 0 && kt > 0) {
+        ids = in_pool(ids_next);
+        ids_next = load_ids(kt / GT + 1);
+        const uint32_t s = (uint32_t)ids * (uint32_t)Hkv + kvh;
+        ksc_next = a.ks[s];
+        vsc_next = a.vs[s];
+      }
 #pragma unroll
       for (int n = 0; n < PPT; ++n) {
-        const int i = tid + n * T;
-        const int b = i < PIECES / 2 ? i / (D / 16) / kBlock : (i - PIECES / 2) / D;
-        const int32_t id = tab[min(kt * NB + min(b, NB - 1), nblk - 1)];
-        next_id[n] = id >= 0 && id < a.num_blocks ? id : 0;
+        const int ch = wave + n * W;
+        if (CHUNKS % W != 0 && ch >= CHUNKS) continue;
+        const bool is_k = ch < CHUNKS / 2;
+        const int i = (is_k ? ch : ch - CHUNKS / 2) * 64 + lane;
+        const uint32_t id = __shfl(ids, kt % GT * NB + i / D, 64);
+        const uint64_t off =
+            (uint64_t)(id * (uint32_t)Hkv + kvh) * (kBlock * D) + (uint32_t)(i % D) * 16;
+        const uint32_t to = (uint32_t)(uintptr_t)(
+            __attribute__((address_space(3))) uint8_t*)&stage[kt & 1][ch * 1024];
+        lds_copy16((const uint8_t*)(is_k ? a.kc : a.vc), off,
+                   __builtin_amdgcn_readfirstlane(to));
       }
     };
-    i32x4 raw[PPT];
-    uint32_t raw_k = 0, raw_v = 0;  // threads below NB: block tid's scale bytes
-    auto load_tile = [&](int kt) {
+    // Waits for this wavefront's copies of a tile, those of the next one (`more`) in
+    // flight, and writes the tile's operands.
+    auto write_tile = [&](int kt, int buf, bool more) {
+      if (!more)
+        wait_vm<0>();
+      else if (CHUNKS % W == 0 || wave + (PPT - 1) * W < CHUNKS)
+        wait_vm<PPT>();
+      else
+        wait_vm<PPT - 1>();
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int n = 0; n < PPT; ++n) {
-        const int i = tid + n * T;
-        const uint64_t slice = (uint64_t)((uint32_t)next_id[n] * (uint32_t)Hkv + kvh) * (kBlock * D);
-        if (PIECES % T != 0 && i >= PIECES) continue;
-        if (i < PIECES / 2) {
-          raw[n] = *reinterpret_cast<const i32x4*>(a.kc + slice + (i % (kBlock * D / 16)) * 16);
-        } else {
-          raw[n] = *reinterpret_cast<const i32x4*>(a.vc + slice + ((i - PIECES / 2) % D) * 16);
-        }
-      }
-      if (tid < NB) {
-        const int32_t id = tab[min(kt * NB + tid, nblk - 1)];
-        const uint32_t s = (uint32_t)(id >= 0 && id < a.num_blocks ? id : 0) * (uint32_t)Hkv + kvh;
-        raw_k = a.ks[s];
-        raw_v = a.vs[s];
-      }
-    };
-    auto write_tile = [&](int buf) {
-#pragma unroll
-      for (int n = 0; n < PPT; ++n) {
-        const int i = tid + n * T;
-        if (PIECES % T != 0 && i >= PIECES) continue;
+        const int ch = wave + n * W;
+        if (CHUNKS % W != 0 && ch >= CHUNKS) continue;
+        const bool is_k = ch < CHUNKS / 2;
+        const int i = (is_k ? ch : ch - CHUNKS / 2) * 64 + lane;
+        const i32x4 raw = *reinterpret_cast<const i32x4*>(&stage[kt & 1][ch * 1024 + lane * 16]);
         uint8_t* to;
-        if (i < PIECES / 2) {
+        if (is_k) {
           // key 32 s + 8 g + 4 kk + r sits at row 32 s + 16 kk + 4 g + r: the lanes of
           // an operand read take consecutive rows
-          const int key = i / (D / 16), ch = i % (D / 16);
+          const int key = i / (D / 16), x = i % (D / 16);
           const int r = (key & ~31) + ((key >> 2) & 1) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
-          to = &lds.k[buf][r * KROW + ch * 32];
+          to = &lds.k[buf][r * KROW + x * 32];
         } else {
-          const int v = i - PIECES / 2;
-          to = &lds.v[buf][(v % D) * VROW + (v / D) * 32];
+          to = &lds.v[buf][(i % D) * VROW + (i / D) * 32];
         }
-        reinterpret_cast<bf16x8*>(to)[0] = codes_bf16x8(raw[n][0], raw[n][1]);
-        reinterpret_cast<bf16x8*>(to)[1] = codes_bf16x8(raw[n][2], raw[n][3]);
-      }
-      if (tid < NB) {
-        // (a scale of 0, and what no scale is, only occurs in blocks never written)
-        const int ev = raw_v == 0 || raw_v > 253 ? 0 : (int)raw_v - 127;
-        s_factor[buf][tid] = fabsf(a.scale_log2) * scale_of(raw_k);
-        s_exp[buf][tid] = (float)ev;
-        s_one[buf][tid] = (uint32_t)(127 - ev) * 0x00800080u;
+        bf16x8 first, second;
+        codes_bf16x16(raw, first, second);
+        reinterpret_cast<bf16x8*>(to)[0] = first;
+        reinterpret_cast<bf16x8*>(to)[1] = second;
       }
     };
     // LDS writes done, then a barrier; loads to registers stay in flight.
@@ -275,11 +296,11 @@ prefill_int8_kernel(const PrefillArgs a) {
     };
 
     // ---- the query rows, and the table's ids
-    load_ids(0);
-    load_tile(0);
+    copy_tile(0);
+    if (n_kt > 1) copy_tile(1);
     bf16x8 qv[NT][KS];
     int pos[NT];  // the lane's rows' positions
-    const uint16_t flip = a.scale_log2 < 0.f ? 0x8000 : 0;  // a negative scale, by the query
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0;  // a negative scale, by the query
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = r0 + 16 * nt + c, rc = min(row, rows - 1);
@@ -295,7 +316,7 @@ prefill_int8_kernel(const PrefillArgs a) {
         const Piece p = *reinterpret_cast<const Piece*>(qp + 32 * s);
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = row < rows ? p.v[i] ^ (flip * 0x10001u) : 0;
+        for (int i = 0; i < 4; ++i) w[i] = row < rows ? p.v[i] ^ flip : 0;
         typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
         qv[nt][s] = __builtin_bit_cast(bf16x8, u32x4_t{w[0], w[1], w[2], w[3]});
       }
@@ -308,113 +329,114 @@ prefill_int8_kernel(const PrefillArgs a) {
     const bool bad_ids = __syncthreads_or(bad) != 0;
     f32x4 o[NT][DT];
     f32x4 lacc[NT];  // denominators
-    float nm[NT];    // minus the rows' maxima
-    float raise = 8.0f;
+    float nm[NT];    // minus the rows' maxima; INFINITY: none yet
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      nm[nt] = 0.f;
+      nm[nt] = INFINITY;
       lacc[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[nt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // tiles 0 and 1 into LDS, tile 2 on its way
-    write_tile(0);
+    // the first two tiles' operands, the next two on their way
+    write_tile(0, 0, n_kt > 1);
+    if (n_kt > 2) copy_tile(2);
     if (n_kt > 1) {
-      load_ids(1);
-      load_tile(1);
-      write_tile(1);
-    }
-    if (n_kt > 2) {
-      load_ids(2);
-      load_tile(2);
-      if (n_kt > 3) load_ids(3);
+      write_tile(1, 1, n_kt > 2);
+      if (n_kt > 3) copy_tile(3);
     }
     barrier();
 
-    auto qk_load = [&](int buf, int st, bf16x8 (&ka)[2][KS]) __attribute__((always_inline)) {
-      const uint8_t* row = &lds.k[buf][(st * 32 + c) * KROW + j * 16];
+    f32x4 S[NT][2];
+    bf16x8 ka[2][KS], va[DT], pb[NT];
+    auto qk_load = [&](int buf, int st) __attribute__((always_inline)) {
+      const uint8_t* p = &lds.k[buf][(st * 32 + c) * KROW + j * 16];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int s = 0; s < KS; ++s)
-          ka[kk][s] = *reinterpret_cast<const bf16x8*>(row + kk * 16 * KROW + s * 64);
+          ka[kk][s] = *reinterpret_cast<const bf16x8*>(p + kk * 16 * KROW + s * 64);
     };
-    f32x4 S0[NT][2], S1[NT][2];
-    {
-      bf16x8 ka[2][KS];
-      qk_load(0, kgrp, ka);
+    auto v_load = [&](int buf, int st) __attribute__((always_inline)) {
+      const uint8_t* p = &lds.v[buf][c * VROW + st * 64 + j * 16];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int dt = 0; dt < DT; ++dt)
+        va[dt] = *reinterpret_cast<const bf16x8*>(p + dt * 16 * VROW);
+    };
+    auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          S0[nt][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
-            S0[nt][kk] =
-                __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[kk][s], qv[nt][s], S0[nt][kk], 0, 0, 0);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+            S[nt][kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                ka[kk][s], qv[nt][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[nt][kk], 0, 0, 0);
+    };
+    auto next_buf = [](int buf, int n) -> int { return buf + n >= NBUF ? buf + n - NBUF : buf + n; };
+    qk_load(0, kgrp);
+    scores();
+    if constexpr (EARLY) {
+      qk_load(0, 1);
+      v_load(0, 0);
     }
+    const int last_pos = past + (min(rows, r0 + 16 * NT) - 1) / G;  // of this wavefront's rows
+    const float scale = fabsf(a.scale_log2);
 
-    // One step of 32 keys (step `st` of tile kt, in buffer buf): the softmax of S
-    // (computed before), this step's products with V among the next step's scores.
-    // LAST: the tile's last step of this wavefront, which begins with the boundary.
-    auto step = [&](int buf, int st, auto last, int kt, f32x4 (&S)[NT][2], f32x4 (&Sn)[NT][2]) {
-      constexpr bool LAST = decltype(last)::value;
-      const int next = buf == NBUF - 1 ? 0 : buf + 1;
-      const int free_buf = buf == 0 ? NBUF - 1 : buf - 1;
-      bf16x8 va[DT];
-      {
-        const uint8_t* row = &lds.v[buf][c * VROW + st * 64 + j * 16];
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          va[dt] = *reinterpret_cast<const bf16x8*>(row + dt * 16 * VROW);
-      }
-      const int blk = 2 * st + (j >> 1);  // the lane's block of the tile
-      const float factor = s_factor[buf][blk], ev = s_exp[buf][blk];
-      const uint32_t one = s_one[buf][blk];
-      bf16x8 ka[2][KS];
-      if constexpr (LAST) {
-        // The next tile is in LDS (written a boundary ago), the one before this is
-        // free.  Past the last tile the operands read here are never used.
-        if (kt + 1 < n_kt) {
-          barrier();
-          if (kt + 2 < n_kt) write_tile(free_buf);
-          if (kt + 3 < n_kt) {
-            load_tile(kt + 3);
-            if (kt + 4 < n_kt) load_ids(kt + 4);
-          }
-          asm volatile("" ::: "memory");
+    // During tile kt: this wavefront's share of the tile two on, and the copies of the
+    // one four on.
+    auto prepare = [&](int kt, int buf) __attribute__((always_inline)) {
+      if (kt + 2 >= n_kt) return;
+      write_tile(kt + 2, next_buf(buf, 2), kt + 3 < n_kt);
+      if (kt + 4 < n_kt) copy_tile(kt + 4);
+    };
+    // A step of 32 keys, step `st` of tile kt (in buffer buf): probabilities of S, the
+    // next S, the products with V, the operands of the steps after.  A tile's first
+    // step begins with a barrier: behind it the next tile is in LDS, written during the
+    // one before, and the buffer of that one is free.
+    auto step = [&](int buf, int st, auto first_, int kt) {
+      constexpr bool FIRST = decltype(first_)::value;
+      const int kb = kt * KT + st * 32;
+      const bool live = active && kb <= last_pos;
+      if (FIRST && kt > 0) {
+        if (kt % GT == 0) {
+          ksc = ksc_next;
+          vsc = vsc_next;
         }
-        qk_load(next, kgrp, ka);
-      } else {
-        qk_load(buf, st + 1, ka);
+        barrier();
       }
-      float f = factor;
-      float add[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) add[nt] = nm[nt];
-      {
-        const int kb = kt * KT + st * 32;
+      if (live) {
+        if constexpr (!EARLY) {
+          qk_load(next_buf(buf, 1), kgrp);
+          v_load(buf, st);
+        }
+        // the scales of the lane's block: a K scale of 2^(byte - 127); the V scale's
+        // exponent (0 for a byte that no scale is, in blocks never written)
+        const int at = kt % GT * NB + 2 * st;
+        const uint32_t k0 = __builtin_amdgcn_readlane(ksc, at),
+                       k1 = __builtin_amdgcn_readlane(ksc, at + 1),
+                       v0 = __builtin_amdgcn_readlane(vsc, at),
+                       v1 = __builtin_amdgcn_readlane(vsc, at + 1);
+        const uint32_t vb = j & 2 ? v1 : v0;
+        float f = scale * scale_of(j & 2 ? k1 : k0);
+        const int e = vb == 0 || vb > 253 ? 0 : (int)vb - 127;
+        const uint32_t one = (uint32_t)(127 - e) * 0x00800080u;
         const bool tail = kt * KT + KT > key_end || bad_ids;
         if (tail || kb + 31 > past + r0 / G) {
-          // keys behind the last, in blocks outside the pool or above a row's
-          // diagonal: the scores are finished here
+          // keys behind the last, in blocks outside the pool or above a row's diagonal
           int end = key_end;
           if (bad_ids) {
-            const int b = kt * NB + blk;
+            const int b = kt * NB + 2 * st + (j >> 1);
             const int32_t id = b < nblk ? tab[b] : -1;
             end = id >= 0 && id < a.num_blocks ? key_end : 0;
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int key = kb + 8 * j + i;
-              const float x = __builtin_fmaf(S[nt][i >> 2][i & 3], f, nm[nt]);
+              const float x = S[nt][i >> 2][i & 3] * f;
               S[nt][i >> 2][i & 3] = key >= end || key > pos[nt] ? -INFINITY : x;
             }
-            add[nt] = 0.f;
-          }
           f = 1.f;
         }
         float lm[NT];
@@ -423,68 +445,40 @@ prefill_int8_kernel(const PrefillArgs a) {
         for (int nt = 0; nt < NT; ++nt) {
           const float m0 = max3(S[nt][0][0], S[nt][0][1], S[nt][0][2]);
           const float m1 = max3(S[nt][0][3], S[nt][1][0], S[nt][1][1]);
-          lm[nt] = __builtin_fmaf(max3(m0, m1, max3(S[nt][1][2], S[nt][1][3], S[nt][1][3])), f,
-                                  add[nt]);
-          need |= lm[nt] > raise;
+          lm[nt] = max3(m0, m1, max3(S[nt][1][2], S[nt][1][3], S[nt][1][3])) * f;
+          // (a row without keys so far has nm = inf: any score passes, and -inf + inf
+          // does not)
+          need |= lm[nt] + nm[nt] > 8.0f;
         }
-        // A row's first step with keys sets its maximum exactly: step 0, or the first
-        // that ids outside the pool do not mask (its denominator is 0 until then).
-        const bool first = kt == 0 && (SPT == 1 || st == 0);
-        if (__builtin_expect(first || __builtin_amdgcn_ballot_w64(need) != 0, 0)) {
-          raise = 8.0f;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(need) != 0, 0)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float bm = lm[nt];
-            bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-            bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-            const bool none = first || lacc[nt][0] == 0.f;
-            const bool masked = !(bm > -INFINITY);
-            if (none && masked) raise = -INFINITY;
-            const float delta = none ? (masked ? 0.f : bm) : fmaxf(bm, 0.f);
-            nm[nt] -= delta;
-            add[nt] -= delta;
-            if (!first) {
-              const float r = none ? 1.f : __builtin_amdgcn_exp2f(-delta);
-              lacc[nt] *= r;
+            float top = fmaxf(lm[nt], -nm[nt]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float r = nm[nt] == INFINITY ? 1.f : __builtin_amdgcn_exp2f(-nm[nt] - top);
+            nm[nt] = -top;
+            lacc[nt] *= r;
 #pragma unroll
-              for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= r;
-            }
+            for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= r;
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) add[nt] += ev;
-      }
-      {
-        constexpr int NQK = 2 * KS * NT;  // next-step score products
-        constexpr int NEXP = 8 * NT;      // exponentials a lane
-        constexpr int EPM = (NEXP + NQK - 1) / NQK;
-        float pv[NT][8];
+        for (int nt = 0; nt < NT; ++nt) {
+          const float shift = (nm[nt] == INFINITY ? 0.f : nm[nt]) + (float)e;
 #pragma unroll
-        for (int g = 0; g < NQK; ++g) {
-          const int s = g / (2 * NT), q_ = g % (2 * NT), nt_ = q_ / 2, kk = q_ % 2;
-          Sn[nt_][kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              ka[kk][s], qv[nt_][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : Sn[nt_][kk], 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < EPM; ++e) {
-            const int x = g * EPM + e;
-            if (x < NEXP) {
-              const int nt = x / 8, i = x % 8;
-              pv[nt][i] =
-                  __builtin_amdgcn_exp2f(__builtin_fmaf(S[nt][i >> 2][i & 3], f, add[nt]));
-            }
-          }
+          for (int i = 0; i < 8; ++i)
+            pb[nt][i] = (__bf16)__builtin_amdgcn_exp2f(
+                __builtin_fmaf(S[nt][i >> 2][i & 3], f, shift));
         }
-#pragma unroll
-        for (int g = 0; g < NQK; ++g) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // MFMA
-          __builtin_amdgcn_sched_group_barrier(0x002, EPM, 0);  // VALU
-          __builtin_amdgcn_sched_group_barrier(0x400, EPM, 0);  // transcendental
-        }
-        bf16x8 pb[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pb[nt][i] = (__bf16)pv[nt][i];
+        // between the softmax and the products, which the other wavefront of this SIMD
+        // runs meanwhile: 347 us where 371 at the step's end, 397 behind the scores and
+        // 293 without the writes (4 x 1024-2048 tokens on 0-4096, 32 / 8 heads of 128)
+        if constexpr (FIRST) prepare(kt, buf);
+        __builtin_amdgcn_s_setprio(1);
+        scores();
+        // (past the last tile what is read here is never used)
+        if constexpr (EARLY) qk_load(next_buf(buf, 1), st);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -496,24 +490,20 @@ prefill_int8_kernel(const PrefillArgs a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           lacc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[nt], lacc[nt], 0, 0, 0);
+        if constexpr (EARLY) v_load(FIRST ? buf : next_buf(buf, 1), 1 - st);
       }
+      __builtin_amdgcn_s_setprio(0);
+      if (FIRST && !live) prepare(kt, buf);
     };
 
-    for (int kt = 0, buf = 0; kt < n_kt; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1) {
-      if constexpr (SPT == 2) {
-        step(buf, 0, std::false_type{}, kt, S0, S1);
-        step(buf, 1, std::true_type{}, kt, S1, S0);
-      } else {
-        step(buf, kgrp, std::true_type{}, kt, S0, S1);
-        if (++kt == n_kt) break;
-        buf = buf == NBUF - 1 ? 0 : buf + 1;
-        step(buf, kgrp, std::true_type{}, kt, S1, S0);
-      }
+    for (int kt = 0, buf = 0; kt < n_kt; ++kt, buf = next_buf(buf, 1)) {
+      step(buf, SPT == 2 ? 0 : kgrp, std::true_type{}, kt);
+      if constexpr (SPT == 2) step(buf, 1, std::false_type{}, kt);
     }
 
     if constexpr (KG == 2) {
       // The two groups' results, in the tiles' space.  A group that saw no key of a
-      // row (l = 0) drops out.
+      // row (nm = inf) drops out.
       static_assert(W / 2 * NT * (DT * 1024 + 512) <= (int)sizeof(Tiles), "space");
       float* mo = reinterpret_cast<float*>(&lds);
       float* mml = mo + W / 2 * NT * DT * 256;
@@ -534,11 +524,11 @@ prefill_int8_kernel(const PrefillArgs a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float2 ml = *reinterpret_cast<const float2*>(mml + ((wt * NT + nt) * 64 + lane) * 2);
-        const float ma = lacc[nt][0] != 0.f ? -nm[nt] : kInt8NoMax;
-        const float mb = ml.y != 0.f ? ml.x : kInt8NoMax;
-        const float mx = fmaxf(ma, mb);
-        const float fa = __builtin_amdgcn_exp2f(ma - mx), fb = __builtin_amdgcn_exp2f(mb - mx);
-        lacc[nt] = lacc[nt] * fa + ml.y * fb;
+        const float m = -nm[nt], mx = fmaxf(m, ml.x);
+        const float fa = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+        const float fb = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+        // (a row of NaN has no maximum, but sums of NaN)
+        lacc[nt][0] = lacc[nt][0] * fa + ml.y * fb;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
           o[nt][dt] = o[nt][dt] * fa + *reinterpret_cast<const f32x4*>(
@@ -636,22 +626,27 @@ int32_t prefill_int8_strided(void* out, const void* q, int64_t q_row, const int8
                       scale * kInt8Log2e};
   // Rows a workgroup: an item's time is its keys times the time a tile takes, and a
   // launch's items share the CUs; the lengths are on the device, so the items are
-  // counted from the totals.
+  // counted from the totals.  us for 256 / 128 / 64 rows: 4 prompts of 2048, 32 / 8
+  // heads of 128, 182 / 245 / 397; one of 2048 79 / 65 / 102; one of 512 on 1024
+  // 61 / 45 / 40; 64 x 16 on 500 48 / 38 / 39; 1624 tokens of two, 24 / 4 heads of 96,
+  // 100 / 74 / 94; one of 333, 14 / 2 heads of 64, 16 / 12 / 10.  (128 rows as two groups of keys,
+  // 72, 48 and 47 where 65, 45 and 38; 64 rows of one group 135, 51 and 45.)
   auto cost = [&](int rows, double per_tile) -> double {
     const double tiles = std::max((double)num_seqs, (double)total_q * G / rows + 0.5 * num_seqs);
     return per_tile * std::max(1., 0.65 / 256 * tiles * num_kv_heads);
   };
-  const double c256 = cost(256, 1.), c128 = cost(128, 0.7), c64 = cost(64, 0.53);
+  const double c256 = cost(256, 1.), c128 = cost(128, 0.72), c64 = cost(64, 0.62);
   auto narrow = [&](auto dc) -> int32_t {
     constexpr int DD = decltype(dc)::value;
     if (c256 <= c128 && c256 <= c64) return launch<DD, 2, 8, 1>(a, num_seqs, s);
-    if (c128 <= c64) return launch<DD, 2, 8, 2>(a, num_seqs, s);
+    if (c128 <= c64) return launch<DD, 1, 8, 1>(a, num_seqs, s);
     return launch<DD, 1, 8, 2>(a, num_seqs, s);
   };
+  // (the registers of the wide heads hold 16 rows a wavefront: 134 us where four
+  // wavefronts of 32 rows took 199, 700 tokens on 1000 and 300, 16 / 4 heads of 256)
   auto wide = [&](auto dc) -> int32_t {
     constexpr int DD = decltype(dc)::value;
-    if (c128 <= c64) return launch<DD, 2, 4, 1>(a, num_seqs, s);
-    return launch<DD, 1, 4, 1>(a, num_seqs, s);
+    return launch<DD, 1, 8, 1>(a, num_seqs, s);
   };
   int32_t rc;
   switch (head_dim) {

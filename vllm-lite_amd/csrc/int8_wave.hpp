@@ -34,14 +34,15 @@ __device__ inline uint32_t codes_bf16x2(uint32_t w, int at) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a),
                                0x07060302u);
 }
-__device__ inline bf16x8 codes_bf16x8(uint32_t lo, uint32_t hi) {
+__device__ inline void codes_bf16x16(i32x4 w, bf16x8& lo, bf16x8& hi) {
   // the words as they are: the compiler would carry bytes in registers of their own
   // from the loads to here
-  asm("" : "+v"(lo), "+v"(hi));
+  asm("" : "+v"(w));
   typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-  const u32x4_t r = {codes_bf16x2(lo, 0), codes_bf16x2(lo, 2), codes_bf16x2(hi, 0),
-                     codes_bf16x2(hi, 2)};
-  return __builtin_bit_cast(bf16x8, r);
+  lo = __builtin_bit_cast(bf16x8, u32x4_t{codes_bf16x2(w[0], 0), codes_bf16x2(w[0], 2),
+                                          codes_bf16x2(w[1], 0), codes_bf16x2(w[1], 2)});
+  hi = __builtin_bit_cast(bf16x8, u32x4_t{codes_bf16x2(w[2], 0), codes_bf16x2(w[2], 2),
+                                          codes_bf16x2(w[3], 0), codes_bf16x2(w[3], 2)});
 }
 
 template <int D>
@@ -240,10 +241,10 @@ __device__ inline void int8_output(const Int8Values<D>& st, const bf16x8& p0, co
                                    Int8State<D>& S) {
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) {
-    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-        codes_bf16x8(st.v[dt][0], st.v[dt][1]), p0, S.o[dt], 0, 0, 0);
-    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-        codes_bf16x8(st.v[dt][2], st.v[dt][3]), p1, S.o[dt], 0, 0, 0);
+    bf16x8 lo, hi;
+    codes_bf16x16(st.v[dt], lo, hi);
+    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p0, S.o[dt], 0, 0, 0);
+    S.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p1, S.o[dt], 0, 0, 0);
     // (all the conversions first would take four times the values' registers)
     __builtin_amdgcn_sched_barrier(0);
   }

@@ -10,12 +10,12 @@
 //
 // Nothing is sorted.  What top-k and top-p keep of a row is all above a threshold
 // value and the first `ties` tokens equal to it:
-//   1  sample_max_kernel    the row's largest and least logit, in slices
-//   2  sample_hist_kernel   counts and weights of 2048 equal intervals of the logits
-//   3  sample_pick_kernel   the values in the interval where a threshold lies
-//   4  sample_draw_kernel   the threshold among those values (radix selection),
-//                           the kept weight of every slice, and, in the last
-//                           workgroup of the row, the token
+//   1  sample_max_kernel    the row's largest and least logit
+//   2  sample_hist_kernel   counts and weights of 512 equal intervals of the logits
+//   3  sample_pick_kernel   the values in the intervals in which the thresholds lie
+//   4  sample_draw_kernel   the threshold among those values (radix selection), the
+//                           kept weight of every wavefront's run of tokens and, in the
+//                           row's last workgroup, the token
 // 2 and 3 only where the call gives top_k or top_p; rows that do not use them pass
 // through.  Each kernel reads the logits once, in workgroups of a slice of a row.
 #include <algorithm>
@@ -28,11 +28,14 @@
 namespace pa {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kBins = 2048;
-constexpr int kMaxSlices = 64;
+constexpr int kThreads = 1024;
+constexpr int kWaves = kThreads / 64;
+constexpr int kBins = 512;
+constexpr int kWorkgroups = 512;  // of a launch where its rows allow: two a CU
+constexpr int kMaxSlices = 16;
+constexpr int kLaneParts = kMaxSlices * kThreads / 64 / 64;  // of a row, to a wavefront
 constexpr int kListMax = 4096;  // values that step 3 collects; more are read from the row again
-constexpr int kDigits = 11;     // bits a round of the selection
+constexpr int kDigits = 9;      // bits a round of the selection
 
 // What a row has in the workspace.
 struct Stats {  // of a slice
@@ -40,16 +43,22 @@ struct Stats {  // of a slice
   int at;  // of the first largest
   int pad;
 };
-struct Part {  // of a slice: what is kept of it
+struct Part {  // of a wavefront's run: what is kept of it
   unsigned long long mass;
   unsigned int ties, pad;
 };
 struct Row {
   Stats stats[kMaxSlices];
-  Part part[kMaxSlices];
   unsigned long long mass[kBins];
   unsigned int count[kBins];
   unsigned int list[kListMax];
+  // Top-k's threshold is in interval kb (kBins: none, fewer values than k): `above`
+  // values and the weight `least` come before it.
+  unsigned long long above, least;
+  // Top-p's, where all that top-k may leave has it in one interval: that (else kBins),
+  // and the weight before it.
+  unsigned long long before;
+  int kb, pb;
   unsigned int listed, arrived, pad[2];
 };
 
@@ -63,8 +72,9 @@ struct Args {
   const float* top_p;
   const float* min_p;
   Row* rows;
-  int cols, slices, per;  // per: 16-byte chunks a slice
-  int shift;              // weights in units of 2^-shift
+  Part* parts;  // of (row, slice, wavefront)
+  int cols, slices;
+  int shift;  // weights in units of 2^-shift, at most 51
 };
 
 __device__ const double kPow[16] = {  // 2^(-i / 16)
@@ -77,7 +87,8 @@ __device__ const double kPow[16] = {  // 2^(-i / 16)
 struct Settings {
   float max, min;       // of the row; min of the values above -inf
   float t, p;
-  double rate, least;   // 1 / T; min_p
+  double top;           // max
+  double rate, least;   // of y = 16 (max - x) / (T ln 2): the factor, and min-p's bound
   int k;
   bool greedy, by_k, by_p;
   float range, step;    // intervals: of d = max - x up to range, step a unit
@@ -93,42 +104,45 @@ __device__ inline float value_of(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// exp(-z) 2^shift to the nearest integer, z >= 0: 2^(-n / 16) from the table, n the
-// nearest to 16 z / ln 2, and the series of the exponential for the rest (below
-// 0.022, to the sixth power).
-__device__ inline unsigned long long fixed_exp(double z, int shift, const double* pow16) {
+// The weight of a value in units of 2^-shift: exp(-z), z = (max - x) / T, to the nearest
+// integer.  y = 16 z / ln 2 = n - f with n whole and |f| <= 1/2: exp(-z) =
+// 2^(-n / 16) 2^(f / 16), the one from the table, the other the series of the
+// exponential to the sixth power (its rest below 2^-51).  Both roundings to integers
+// are additions of a number whose unit is 1 in f64, so shift is at most 51.
+constexpr double kUnit = 0x1.8p+52, kWhole = 0x1p+52;
+__device__ inline unsigned long long weigh(double y, int shift, const double* pow16) {
 #pragma clang fp contract(off)  // a value's weight is the same in every kernel
-  const double y = z * 0x1.71547652b82fep+4;
-  if (!(y < 16.0 * 64.0)) return 0;
-  const double n = __builtin_rint(y);
-  const double r = (n - y) * 0x1.62e42fefa39efp-5;
-  double s = 1.0 / 720;
-  s = __builtin_fma(s, r, 1.0 / 120);
-  s = __builtin_fma(s, r, 1.0 / 24);
-  s = __builtin_fma(s, r, 1.0 / 6);
-  s = __builtin_fma(s, r, 0.5);
-  s = __builtin_fma(s, r, 1.0);
-  s = __builtin_fma(s, r, 1.0);
-  const int i = (int)n;
-  const double w = __builtin_amdgcn_ldexp(s * pow16[i & 15], shift - (i >> 4));
-  return (unsigned long long)__builtin_rint(w);
+  const double m = y + kUnit;
+  const double f = (m - kUnit) - y;
+  const uint32_t n = (uint32_t)__builtin_bit_cast(unsigned long long, m);
+  constexpr double c = 0x1.62e42fefa39efp-5;  // ln 2 / 16
+  double s = c * c * c * c * c * c / 720;
+  s = __builtin_fma(s, f, c * c * c * c * c / 120);
+  s = __builtin_fma(s, f, c * c * c * c / 24);
+  s = __builtin_fma(s, f, c * c * c / 6);
+  s = __builtin_fma(s, f, c * c / 2);
+  s = __builtin_fma(s, f, c);
+  s = __builtin_fma(s, f, 1.0);
+  const unsigned long long p = __builtin_bit_cast(unsigned long long, pow16[n & 15]) +
+                               ((unsigned long long)(uint32_t)(shift - (int)(n >> 4)) << 52);
+  const double w = __builtin_fma(s, __builtin_bit_cast(double, p), kWhole);
+  return y < 16.0 * 64.0 ? __builtin_bit_cast(unsigned long long, w) & 0xFFFFFFFFFFFFFull : 0;
 }
-
-// The weight of a value (a value at the largest: exactly 1).
+// (a value at the largest, which may be infinite: exactly 1)
 __device__ inline unsigned long long weight_of(float x, const Settings& s, int shift,
                                                const double* pow16) {
 #pragma clang fp contract(off)
-  if (x == s.max) return 1ull << shift;
-  return fixed_exp(((double)s.max - (double)x) * s.rate, shift, pow16);
+  const unsigned long long w = weigh((s.top - (double)x) * s.rate, shift, pow16);
+  return x == s.max ? 1ull << shift : w;
 }
-// The weight if min-p keeps it, else 0.  The test is on w = exp(-z) itself: z in f64
+// The weight if min-p keeps it, else 0.  The test is on exp(-z) itself: z in f64
 // against -ln(min_p).
 __device__ inline unsigned long long kept_weight(float x, const Settings& s, int shift,
                                                  const double* pow16) {
 #pragma clang fp contract(off)
-  if (x == s.max) return 1ull << shift;
-  const double z = ((double)s.max - (double)x) * s.rate;
-  return z <= s.least ? fixed_exp(z, shift, pow16) : 0;
+  const double y = (s.top - (double)x) * s.rate;
+  const unsigned long long w = y <= s.least ? weigh(y, shift, pow16) : 0;
+  return x == s.max ? 1ull << shift : w;
 }
 
 // The interval of a value, -1 outside (weights there are 0).
@@ -149,34 +163,45 @@ __device__ inline Settings settings_of(const Args& a, int row) {
   s.greedy = !(s.t > 0.f);
   s.by_k = !s.greedy && s.k > 0 && s.k < a.cols;
   s.by_p = !s.greedy && s.p < 1.f;
-  s.rate = 1.0 / (double)s.t;
-  s.least = m > 0.f ? -log((double)m) : (double)INFINITY;
+  constexpr double k = 0x1.71547652b82fep+4;  // 16 / ln 2
+  s.rate = k / (double)s.t;
+  s.least = m > 0.f ? -log((double)m) * k : (double)INFINITY;
   return s;
 }
 
-// The row's extremes from its slices (all threads; `red` of 2 floats).
-__device__ inline void extremes(const Row& row, int slices, Settings& s, float* red) {
-  if (threadIdx.x < 64) {
-    float mx = -INFINITY, mn = INFINITY;
-    if ((int)threadIdx.x < slices) {
-      mx = row.stats[threadIdx.x].max;
-      mn = row.stats[threadIdx.x].min;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-      mn = fminf(mn, __shfl_xor(mn, o, 64));
-    }
-    if (threadIdx.x == 0) {
-      red[0] = mx;
-      red[1] = mn;
-    }
-  }
-  __syncthreads();
-  s.max = red[0];
-  s.min = red[1];
-  // Weights end at exp(-(shift + 1) ln 2), shift <= 62: d / T <= 44.
-  s.range = fminf(44.f * s.t, s.max - s.min);
+// What a wavefront's lanes give, joined by f: `none` for lanes that give nothing.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t dpp(uint32_t v, uint32_t none = 0) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ inline uint32_t lane_of(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <typename F>
+__device__ inline uint32_t wave_join(uint32_t v, uint32_t none, F f) {
+  v = f(v, dpp<0x111, 0xF>(v, none));  // within 16 lanes, with 1, 2, 4 and 8 before
+  v = f(v, dpp<0x112, 0xF>(v, none));
+  v = f(v, dpp<0x114, 0xF>(v, none));
+  v = f(v, dpp<0x118, 0xF>(v, none));
+  v = f(v, dpp<0x142, 0xA>(v, none));  // the first and third sixteen's, with the next
+  v = f(v, dpp<0x143, 0xC>(v, none));  // the first half's, with the second
+  return lane_of(v, 63);
+}
+
+// The row's extremes from its slices.
+__device__ inline void extremes(const Row& row, int slices, Settings& s) {
+  const Stats& mine = row.stats[min((int)(threadIdx.x & 63), slices - 1)];
+  auto f32 = [](uint32_t v) { return __builtin_bit_cast(float, v); };
+  auto u32 = [](float v) { return __builtin_bit_cast(uint32_t, v); };
+  s.max = f32(wave_join(u32(mine.max), u32(-INFINITY), [&](uint32_t a, uint32_t b) {
+    return u32(fmaxf(f32(a), f32(b)));
+  }));
+  s.min = f32(wave_join(u32(mine.min), u32(INFINITY), [&](uint32_t a, uint32_t b) {
+    return u32(fminf(f32(a), f32(b)));
+  }));
+  s.top = (double)s.max;
+  // Weights end at exp(-(shift + 1) ln 2), shift <= 51: d / T <= 36.1.
+  s.range = fminf(37.f * s.t, s.max - s.min);
   s.step = s.range > 0.f ? kBins / s.range : 0.f;
 }
 
@@ -226,73 +251,137 @@ __device__ inline void Chunks<float>::load(int chunk, float (&x)[4]) const {
   }
 }
 
-// f(value) for each value of this workgroup's slice.
-template <typename T, typename F>
-__device__ inline void each_of_slice(const Args& a, int row, int slice, F f) {
-  const Chunks<T> c(a, row);
-  const int end = min(c.count, (slice + 1) * a.per);
-  for (int ch = slice * a.per + threadIdx.x; ch < end; ch += kThreads) {
-    float x[Chunks<T>::E];
-    c.load(ch, x);
-#pragma unroll
-    for (int i = 0; i < Chunks<T>::E; ++i) f(x[i], c.index(ch, i));
+// The run of chunks of part `part` of a row (a wavefront's: slice by slice, wavefront by
+// wavefront), lane by lane in turn: whole 64s, evenly.  The first chunks are on their
+// way from construction on, the next while these are used.
+template <typename T>
+struct Run {
+  static constexpr int E = Chunks<T>::E;
+  Chunks<T> c;
+  int at, end;
+  float next[E];
+  __device__ Run(const Args& a, int row, int part) : c(a, row) {
+    const uint32_t units = (c.count + 63) / 64, parts = a.slices * kWaves;  // 2^16 x 2^8
+    at = (int)(units * part / parts) * 64 + (threadIdx.x & 63);
+    end = min((int)(units * (part + 1) / parts) * 64, c.count);
+    if (at < end) c.load(at, next);
   }
-}
+  // f(x, chunk) for each chunk's values
+  template <typename F>
+  __device__ void each(F f) {
+    while (at < end) {
+      float x[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = next[i];
+      const int now = at;
+      at += 64;
+      if (at < end) c.load(at, next);
+      f(x, now);
+    }
+  }
+};
 
-// The sum of the values of the threads before this one; total of all.
+// The running sums of a wavefront's values, lane by lane (the last lane's: the total),
+// of 64 and 32 bits.
+template <int CTRL, int ROWS>
+__device__ inline unsigned long long dpp(unsigned long long v) {
+  return (unsigned long long)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 |
+         dpp<CTRL, ROWS>((uint32_t)v);
+}
+__device__ inline unsigned long long lane_of(unsigned long long v, int lane) {
+  return (unsigned long long)lane_of((uint32_t)(v >> 32), lane) << 32 |
+         lane_of((uint32_t)v, lane);
+}
 template <typename V>
-__device__ inline V scan_before(V v, V* red, V& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  V incl = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V up = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += up;
-  }
-  __syncthreads();
-  if (lane == 63) red[wave] = incl;
-  __syncthreads();
-  V before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += red[w];
-    total += red[w];
-  }
-  return before + incl - v;
+__device__ inline V wave_scan(V v) {
+  v += dpp<0x111, 0xF>(v);  // within 16 lanes, from 1, 2, 4 and 8 before
+  v += dpp<0x112, 0xF>(v);
+  v += dpp<0x114, 0xF>(v);
+  v += dpp<0x118, 0xF>(v);
+  v += dpp<0x142, 0xA>(v);  // the first and third sixteen's total, to the next
+  v += dpp<0x143, 0xC>(v);  // the first half's, to the second
+  return v;
 }
-
-// Where the running sum of n = kBins entries first reaches `want` (1 or more): its
-// index and the sum before it; index kBins where it does not.  All threads.
+template <typename V>
+__device__ inline V wave_sum(V v) {
+  return lane_of(wave_scan(v), 63);
+}
+// Where the running sum of the kBins entries at h first reaches `want` (1 or more): its
+// index and the sum before it; index kBins and the total where it does not.  By a
+// wavefront; a lane has 8 entries in turn (read from memory as they are, from LDS in
+// the order of slot(), in which 64 lanes read 64 neighbours).
+constexpr int kLaneBins = kBins / 64;
+__device__ inline int slot(int entry) { return entry % kLaneBins * 64 + entry / kLaneBins; }
 struct Cross {
   int at;
   unsigned long long before;
 };
 template <typename V>
-__device__ inline Cross cross(const V* h, unsigned long long want, unsigned long long* red,
-                              Cross* found, unsigned long long& total) {
-  constexpr int N = kBins / kThreads;
-  V v[N];
-  unsigned long long sum = 0;
+struct Entries {
+  V v[kLaneBins];
+  unsigned long long sum, before, total;
+  __device__ explicit Entries(const V* h, bool slots = false) {
+    const int lane = threadIdx.x & 63;
+    sum = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = h[threadIdx.x * N + i];
-    sum += v[i];
+    for (int i = 0; i < kLaneBins; ++i) {
+      v[i] = h[slots ? i * 64 + lane : lane * kLaneBins + i];
+      sum += v[i];
+    }
+    before = wave_scan(sum);
+    total = lane_of(before, 63);
+    before -= sum;
   }
-  unsigned long long run = scan_before(sum, red, total);
-  if (threadIdx.x == 0) *found = Cross{kBins, total};
-  __syncthreads();
-  if (run < want && want <= run + sum) {
+  __device__ Cross cross(unsigned long long want) const {
+    const unsigned long long here =
+        __builtin_amdgcn_ballot_w64(before < want && want <= before + sum);
+    if (here == 0) return Cross{kBins, total};
+    const int lane = __builtin_ctzll(here);
+    unsigned long long run = before, from = 0;
+    int at = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (run < want && want <= run + v[i]) *found = Cross{(int)threadIdx.x * N + i, run};
+    for (int i = 0; i < kLaneBins; ++i) {
+      if (run < want && want <= run + v[i]) {
+        at = i;
+        from = run;
+      }
       run += v[i];
     }
+    return Cross{lane * kLaneBins + (int)lane_of((unsigned int)at, lane), lane_of(from, lane)};
   }
+  // the sum before entry b, and with it
+  __device__ unsigned long long upto(int b, bool with) const {
+    unsigned long long s = 0;
+#pragma unroll
+    for (int i = 0; i < kLaneBins; ++i) {
+      const int at = (threadIdx.x & 63) * kLaneBins + i;
+      if (at < b || (with && at == b)) s += v[i];
+    }
+    return wave_sum(s);
+  }
+};
+
+// The sum over all threads (with two barriers).
+__device__ inline unsigned long long sum_of(unsigned long long v, unsigned long long* red) {
+  v = wave_sum(v);
   __syncthreads();
-  const Cross c = *found;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return c;
+  return wave_sum((threadIdx.x & 63) < kWaves ? red[threadIdx.x & 63] : 0ull);
+}
+
+// What wavefronts of a row leave for its last workgroup is written and read as
+// agent-scope atomics, which pass by the XCDs' L2s, and every wavefront waits until its
+// own are done before the barrier in front of the count.  (So nothing lies dirty in an
+// L2 and nothing stale there: releasing and acquiring fences of whole L2s, by every
+// wavefront, took 70 us for 512 workgroups.)
+template <typename V>
+__device__ inline void put(V* p, V v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V>
+__device__ inline V get(const V* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ceil(f w) for 0 < f < 1, at least 1; floor(f w), below w.  Exact: f has 24 bits.
@@ -321,17 +410,9 @@ __device__ inline unsigned long long share_down(float f, unsigned long long w) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x;
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
   Row& r = a.rows[row];
-  float mx = -INFINITY, mn = INFINITY;
-  int at = INT_MAX;
-  each_of_slice<T>(a, row, slice, [&](float x, int i) {
-    if (x > mx) {
-      mx = x;
-      at = i;
-    }
-    if (x > -INFINITY) mn = fminf(mn, x);
-  });
+  Run<T> run(a, row, slice * kWaves + wave);
   // what the next kernels add to
   if (a.top_k || a.top_p) {
     for (int b = slice * kThreads + threadIdx.x; b < kBins; b += a.slices * kThreads) {
@@ -340,7 +421,19 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
     }
   }
   if (slice == 0 && threadIdx.x == 0) r.listed = r.arrived = 0;
-  __shared__ Stats red[kThreads / 64];
+  float mx = -INFINITY, mn = INFINITY;
+  int at = INT_MAX;
+  run.each([&](const auto& x, int chunk) {
+#pragma unroll
+    for (int i = 0; i < Chunks<T>::E; ++i) {
+      if (x[i] > mx) {
+        mx = x[i];
+        at = run.c.index(chunk, i);
+      }
+      if (x[i] > -INFINITY) mn = fminf(mn, x[i]);
+    }
+  });
+  __shared__ Stats red[kWaves];
   auto join = [&](float ox, float on, int oat) {
     if (ox > mx || (ox == mx && oat < at)) {
       mx = ox;
@@ -351,35 +444,40 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
     join(__shfl_xor(mx, o, 64), __shfl_xor(mn, o, 64), __shfl_xor(at, o, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = Stats{mx, mn, at, 0};
+  if ((threadIdx.x & 63) == 0) red[wave] = Stats{mx, mn, at, 0};
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 64; ++w) join(red[w].max, red[w].min, red[w].at);
+    for (int w = 1; w < kWaves; ++w) join(red[w].max, red[w].min, red[w].at);
     r.stats[slice] = Stats{mx, mn, at, 0};
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x;
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
   Settings s = settings_of(a, row);
   if (!s.by_k && !s.by_p) return;
   __shared__ unsigned long long mass[kBins];
   __shared__ unsigned int count[kBins];
   __shared__ double pow16[16];
-  __shared__ float red[2];
   Row& r = a.rows[row];
+  Run<T> run(a, row, slice * kWaves + wave);
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     mass[b] = 0;
     count[b] = 0;
   }
   if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  extremes(r, a.slices, s, red);
-  each_of_slice<T>(a, row, slice, [&](float x, int) {
-    const int b = bin_of(x, s);
-    if (b < 0) return;
-    if (s.by_k) atomicAdd(&count[b], 1u);
-    if (s.by_p) atomicAdd(&mass[b], weight_of(x, s, a.shift, pow16));
+  extremes(r, a.slices, s);
+  if (s.max == -INFINITY) return;
+  __syncthreads();
+  run.each([&](const auto& x, int) {
+#pragma unroll
+    for (int i = 0; i < Chunks<T>::E; ++i) {
+      const int b = bin_of(x[i], s);
+      if (b < 0) continue;
+      if (s.by_k) atomicAdd(&count[b], 1u);
+      if (s.by_p) atomicAdd(&mass[b], weight_of(x[i], s, a.shift, pow16));
+    }
   });
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
@@ -388,67 +486,79 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
   }
 }
 
-// Where the thresholds lie, as far as the intervals tell: top-k's is in interval kb
-// (kBins: none, fewer values than k), before it `above` values.  All threads.
-struct Found {
-  int kb;
-  unsigned long long above;
-};
-__device__ inline Found find_k(const Row& r, const Settings& s, unsigned long long* red,
-                               Cross* found) {
-  if (!s.by_k) return Found{kBins, 0};
-  unsigned long long total;
-  const Cross c = cross(r.count, (unsigned long long)s.k, red, found, total);
-  return Found{c.at, c.before};
-}
-
-// Sum of the intervals' weights before interval b.
-__device__ inline unsigned long long mass_before(const Row& r, int b, unsigned long long* red) {
-  unsigned long long v = 0, total;
-  for (int i = threadIdx.x; i < b; i += kThreads) v += r.mass[i];
-  scan_before(v, red, total);
-  return total;
-}
-
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x;
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
   Settings s = settings_of(a, row);
   if (!s.by_k && !s.by_p) return;
-  __shared__ unsigned long long red[kThreads / 64];
-  __shared__ Cross found;
-  __shared__ float ext[2];
+  __shared__ uint32_t list[kListMax];
+  __shared__ unsigned int n, at;
+  __shared__ int bins[3];
   Row& r = a.rows[row];
-  extremes(r, a.slices, s, ext);
-  const Found f = find_k(r, s, red, &found);
-  int lo = kBins, hi = -1;  // top-p's interval is one of these
-  if (s.by_p) {
-    // the weight that top-k leaves lies between that before its interval and that
-    // with all of it
-    const unsigned long long least = mass_before(r, f.kb, red);
-    const unsigned long long most = least + (f.kb < kBins ? r.mass[f.kb] : 0);
-    unsigned long long total;
-    lo = min(cross(r.mass, share_up(s.p, least), red, &found, total).at, f.kb);
-    hi = min(cross(r.mass, share_up(s.p, most), red, &found, total).at, f.kb);
+  Run<T> run(a, row, slice * kWaves + wave);
+  extremes(r, a.slices, s);
+  if (s.max == -INFINITY) return;
+  // the intervals of the thresholds: k's, and p's first and last possible
+  if (wave == 0) {
+    Cross k{kBins, 0};
+    if (s.by_k) k = Entries<unsigned int>(r.count).cross((unsigned long long)s.k);
+    Cross p{kBins, 0};
+    int lo = kBins, hi = -1;
+    unsigned long long least = 0;
+    if (s.by_p) {
+      // the weight that top-k leaves lies between that before its interval and that
+      // with all of it
+      const Entries<unsigned long long> m(r.mass);
+      least = k.at == kBins ? m.total : m.upto(k.at, false);
+      p = m.cross(share_up(s.p, least));
+      lo = min(p.at, k.at);
+      hi = k.at == kBins ? lo : min(m.cross(share_up(s.p, m.upto(k.at, true))).at, k.at);
+    }
+    if (threadIdx.x == 0) {
+      n = 0;
+      bins[0] = k.at;
+      bins[1] = lo;
+      bins[2] = hi;
+      if (slice == 0) {
+        r.kb = k.at;
+        r.above = k.before;
+        r.least = least;
+        r.pb = lo == hi && p.at == lo ? lo : kBins;
+        r.before = p.before;
+      }
+    }
   }
-  each_of_slice<T>(a, row, slice, [&](float x, int) {
-    const int b = bin_of(x, s);
-    if (b >= 0 && (b == f.kb || (b >= lo && b <= hi))) {
-      const unsigned int at = atomicAdd(&r.listed, 1u);
-      if (at < kListMax) r.list[at] = key_of(x);
+  __syncthreads();
+  const int kb = bins[0], lo = bins[1], hi = bins[2];
+  run.each([&](const auto& x, int) {
+#pragma unroll
+    for (int i = 0; i < Chunks<T>::E; ++i) {
+      const int b = bin_of(x[i], s);
+      if (b >= 0 && (b == kb || (b >= lo && b <= hi))) {
+        const unsigned int to = atomicAdd(&n, 1u);
+        if (to < kListMax) list[to] = key_of(x[i]);
+      }
     }
   });
+  __syncthreads();
+  if (n == 0) return;
+  if (threadIdx.x == 0) at = atomicAdd(&r.listed, n);
+  __syncthreads();
+  if (at >= kListMax) return;
+  const unsigned int room = min(n, kListMax - at);
+  for (unsigned int i = threadIdx.x; i < room; i += kThreads) r.list[at + i] = list[i];
 }
 
-// The largest value v of the interval `bin` so that the values >= v weigh `want` or
-// more (each 1, or its weight), and the sum of those above it.  Rounds of kDigits
-// bits from the highest in which the interval's keys differ.  `each(f)` calls f(key)
-// for the candidates.
+// The largest value v among the candidates so that those >= v weigh `want` or more
+// (each 1, or its weight), and the sum of those above it.  Rounds of kDigits bits from
+// the highest in which the keys differ to the lowest (values of 16 bits need few).
+// `each(f)` calls f(key) for a thread's candidates.  A round's histogram is one of
+// three: while it is filled the next is cleared, which the round before last read, so
+// one barrier a round will do; every wavefront finds the digit for itself.
 struct Select {
-  unsigned long long hist[kBins];
-  unsigned long long red[kThreads / 64];
-  Cross found;
-  uint32_t lo, hi;
+  unsigned long long hist[3][kBins];
+  unsigned long long red[kWaves];
+  uint32_t ones, zeros;  // bits that some key has set, and clear
 };
 struct Threshold {
   uint32_t key;
@@ -456,65 +566,73 @@ struct Threshold {
 };
 template <typename Each, typename Weight>
 __device__ inline Threshold select(Each each, Weight weight, unsigned long long want, Select& l) {
-  if (threadIdx.x == 0) {
-    l.lo = 0xFFFFFFFFu;
-    l.hi = 0;
-  }
-  __syncthreads();
-  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+  uint32_t ones = 0, zeros = 0;
   each([&](uint32_t key) {
-    lo = min(lo, key);
-    hi = max(hi, key);
+    ones |= key;
+    zeros |= ~key;
   });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
-  }
+  auto either = [](uint32_t a, uint32_t b) { return a | b; };
+  ones = wave_join(ones, 0, either);
+  zeros = wave_join(zeros, 0, either);
+  __syncthreads();  // the last use of l
+  if (threadIdx.x == 0) l.ones = l.zeros = 0;
+  if (threadIdx.x < kBins) l.hist[0][threadIdx.x] = 0;
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) {
-    atomicMin(&l.lo, lo);
-    atomicMax(&l.hi, hi);
+    atomicOr(&l.ones, ones);
+    atomicOr(&l.zeros, zeros);
   }
   __syncthreads();
-  lo = l.lo;
-  hi = l.hi;
-  int left = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);  // bits still open
-  Threshold t{hi, 0};
-  while (left > 0) {
-    const int shift = max(left - kDigits, 0);
+  ones = l.ones;
+  zeros = l.zeros;
+  const uint32_t differ = ones & zeros;
+  Threshold t{ones & ~differ, 0};
+  if (differ == 0) return t;
+  const int stop = __builtin_ctz(differ);
+  int left = 32 - __builtin_clz(differ);  // bits still open
+  // below `stop` the keys agree
+  for (int round = 0; left > stop; ++round) {
+    const int shift = max(left - kDigits, stop);
     const uint32_t digits = (1u << (left - shift)) - 1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) l.hist[b] = 0;
-    __syncthreads();
+    unsigned long long* h = l.hist[round % 3];
+    if (threadIdx.x < kBins) l.hist[(round + 1) % 3][threadIdx.x] = 0;
     each([&](uint32_t key) {
       if (left == 32 || (key >> left) == (t.key >> left))
-        atomicAdd(&l.hist[digits - ((key >> shift) & digits)], weight(key));
+        atomicAdd(&h[slot((int)(digits - ((key >> shift) & digits)))], weight(key));
     });
     __syncthreads();
-    unsigned long long total;
-    const Cross c = cross(l.hist, want, l.red, &l.found, total);
+    const Cross c = Entries<unsigned long long>(h, true).cross(want);
     const uint32_t digit = c.at < kBins ? digits - c.at : 0;  // (always found: want <= the sum)
-    t.key = (t.key & ~((digits << shift) | ((1u << shift) - 1))) | (digit << shift);
+    t.key = (t.key & ~(digits << shift)) | (digit << shift);
     if (c.at < kBins) {
       t.above += c.before;
       want -= c.before;
     }
     left = shift;
   }
-  __syncthreads();
   return t;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x;
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void
+sample_draw_kernel(const Args a) {
+  const int row = blockIdx.y, slice = blockIdx.x, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Settings s = settings_of(a, row);
   Row& r = a.rows[row];
-  __shared__ float ext[2];
   __shared__ double pow16[16];
   __shared__ Select l;
-  __shared__ unsigned int last;
-  extremes(r, a.slices, s, ext);
+  Run<T> run(a, row, slice * kWaves + wave);
+  constexpr int kMine = kListMax / kThreads;
+  unsigned int listed = 0;
+  uint32_t mine[kMine];
+  if (s.by_k || s.by_p) {
+    listed = r.listed;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) mine[i] = r.list[i * kThreads + threadIdx.x];
+  }
+  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
+  extremes(r, a.slices, s);
   if (s.greedy || s.max == -INFINITY) {
     // the first largest; 0 where nothing is above -inf
     if (slice == 0 && threadIdx.x == 0) {
@@ -525,21 +643,23 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const Args a) {
     }
     return;
   }
-  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
   __syncthreads();
   // Kept: the values above `cut` and the first `ties` at it.
   uint32_t cut = 0;
   unsigned long long ties = 0;
   if (s.by_k || s.by_p) {
-    // the values of interval b, from the list or, where that overflowed, the row
-    const unsigned int listed = r.listed;
+    // the values of interval b, from the list (a thread's few in registers) or, where
+    // that overflowed, the row
+    int bins[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      bins[i] = i * kThreads + threadIdx.x < listed ? bin_of(value_of(mine[i]), s) : -1;
     auto values = [&](int b) {
       return [&, b](auto f) {
         if (listed <= kListMax) {
-          for (unsigned int i = threadIdx.x; i < listed; i += kThreads) {
-            const uint32_t key = r.list[i];
-            if (bin_of(value_of(key), s) == b) f(key);
-          }
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (bins[i] == b) f(mine[i]);
         } else {
           const Chunks<T> c(a, row);
           for (int ch = threadIdx.x; ch < c.count; ch += kThreads) {
@@ -553,130 +673,151 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const Args a) {
       };
     };
     auto weight = [&](uint32_t key) { return weight_of(value_of(key), s, a.shift, pow16); };
-    const Found f = find_k(r, s, l.red, &l.found);
-    unsigned long long total = 0;
-    if (f.kb < kBins) {
-      const unsigned long long want = (unsigned long long)s.k - f.above;
-      const Threshold t = select(values(f.kb), [](uint32_t) { return 1ull; }, want, l);
+    const int kb = r.kb;
+    unsigned long long total = r.least;
+    if (kb < kBins) {
+      const unsigned long long want = (unsigned long long)s.k - r.above;
+      const Threshold t = select(values(kb), [](uint32_t) { return 1ull; }, want, l);
       cut = t.key;
       ties = want - t.above;
       if (s.by_p) {
-        unsigned long long mine = 0, sum;
-        values(f.kb)([&](uint32_t key) { mine += key > cut ? weight(key) : 0; });
-        scan_before(mine, l.red, sum);
-        total = mass_before(r, f.kb, l.red) + sum + ties * weight(cut);
+        unsigned long long above = 0;
+        values(kb)([&](uint32_t key) { above += key > cut ? weight(key) : 0; });
+        total += sum_of(above, l.red) + ties * weight(cut);
       }
-    } else if (s.by_p) {
-      total = mass_before(r, kBins, l.red);
     }
     if (s.by_p) {
       const unsigned long long want = share_up(s.p, total);
-      unsigned long long all;
-      const Cross c = cross(r.mass, want, l.red, &l.found, all);
+      Cross c{r.pb, r.before};
+      if (c.at == kBins) c = Entries<unsigned long long>(r.mass).cross(want);
       const Threshold t = select(values(c.at), weight, want - c.before, l);
       cut = t.key;
       const unsigned long long w = max(weight(cut), 1ull);
       ties = (want - c.before - t.above + w - 1) / w;
     }
   }
-  // The slice's share.
+  // What is kept of the wavefront's run.
   unsigned long long mass = 0;
   unsigned int equal = 0;
-  each_of_slice<T>(a, row, slice, [&](float x, int) {
-    const uint32_t key = key_of(x);
-    if (key > cut) mass += kept_weight(x, s, a.shift, pow16);
-    equal += cut && key == cut;
-  });
-  unsigned long long mass_all;
-  unsigned int equal_all;
-  scan_before(mass, l.red, mass_all);
-  scan_before(equal, (unsigned int*)&l.hist[0], equal_all);
-  // The last workgroup of the row to get here has every slice's share: written
-  // through by agent-scope stores before a releasing count, read behind an acquiring
-  // fence.
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(&r.part[slice].mass, mass_all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(&r.part[slice].ties, equal_all, __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(&r.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-           (unsigned int)a.slices - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  const unsigned long long even = cut ? kept_weight(value_of(cut), s, a.shift, pow16) : 0;
-  unsigned long long part = 0;
-  unsigned int eq = 0;
-  if ((int)threadIdx.x < a.slices) {
-    part = __hip_atomic_load(&r.part[threadIdx.x].mass, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
-    eq = __hip_atomic_load(&r.part[threadIdx.x].ties, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  // of n tokens at the threshold with `before` of them in front, those that are kept
-  auto tied = [&](unsigned long long before, unsigned long long n) -> unsigned long long {
-    return before >= ties ? 0 : min(n, ties - before);
-  };
-  unsigned long long all, dummy;
-  unsigned long long eq_before = scan_before((unsigned long long)eq, l.red, dummy);
-  part += tied(eq_before, eq) * even;
-  const unsigned long long part_before = scan_before(part, l.red, all);
-  // the first kept token with a running sum above uniform * the total
-  const unsigned long long target = share_down(a.uniform[row], all);
-  __shared__ int in_slice;
-  __shared__ unsigned long long from, eq_from;
-  __syncthreads();
-  if (part_before <= target && target < part_before + part) {
-    in_slice = threadIdx.x;
-    from = part_before;
-    eq_from = eq_before;
-  }
-  __syncthreads();
-  // its slice, each thread a run of chunks
-  const Chunks<T> c(a, row);
-  const int begin = in_slice * a.per, end = min(c.count, begin + a.per);
-  const int run = (end - begin + kThreads - 1) / kThreads;
-  const int c0 = min(end, begin + (int)threadIdx.x * run), c1 = min(end, c0 + run);
-  mass = 0;
-  equal = 0;
-  for (int ch = c0; ch < c1; ++ch) {
-    float x[Chunks<T>::E];
-    c.load(ch, x);
+  run.each([&](const auto& x, int) {
 #pragma unroll
     for (int i = 0; i < Chunks<T>::E; ++i) {
       const uint32_t key = key_of(x[i]);
       if (key > cut) mass += kept_weight(x[i], s, a.shift, pow16);
       equal += cut && key == cut;
     }
+  });
+  mass = wave_sum(mass);
+  equal = wave_sum(equal);
+  Part* parts = a.parts + (int64_t)row * a.slices * kWaves;
+  if (lane == 0) {
+    put(&parts[slice * kWaves + wave].mass, mass);
+    put(&parts[slice * kWaves + wave].ties, equal);
   }
-  eq_before = eq_from + scan_before((unsigned long long)equal, l.red, dummy);
-  mass += tied(eq_before, equal) * even;
-  unsigned long long sum = from + scan_before(mass, l.red, dummy);
-  if (sum <= target && target < sum + mass) {
-    bool done = false;
-    for (int ch = c0; ch < c1 && !done; ++ch) {
-      float x[Chunks<T>::E];
-      c.load(ch, x);
-      for (int i = 0; i < Chunks<T>::E && !done; ++i) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (wave != 0) return;
+  unsigned int arrived = 0;
+  if (lane == 0)
+    arrived = __hip_atomic_fetch_add(&r.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (lane_of(arrived, 0) != (unsigned int)a.slices - 1) return;
+  // The row's last workgroup has every part; its first wavefront draws.
+  const unsigned long long even = cut ? kept_weight(value_of(cut), s, a.shift, pow16) : 0;
+  // of n tokens at the threshold with `before` of them in front, the weight of those kept
+  auto tied = [&](unsigned long long before, unsigned int n) -> unsigned long long {
+    return before >= ties ? 0 : min((unsigned long long)n, ties - before) * even;
+  };
+  const int count = a.slices * kWaves, each = (count + 63) / 64;
+  unsigned long long m[kLaneParts], eq = 0, sum = 0;
+  unsigned int n_eq[kLaneParts];
+#pragma unroll
+  for (int i = 0; i < kLaneParts; ++i) {
+    const int at = lane * each + i;
+    const bool there = i < each && at < count;
+    m[i] = there ? get(&parts[at].mass) : 0;
+    n_eq[i] = there ? get(&parts[at].ties) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kLaneParts; ++i) eq += n_eq[i];
+  unsigned long long eq_run = wave_scan(eq) - eq;
+#pragma unroll
+  for (int i = 0; i < kLaneParts; ++i) {
+    m[i] += tied(eq_run, n_eq[i]);
+    sum += m[i];
+    eq_run += n_eq[i];
+  }
+  eq_run -= eq;
+  const unsigned long long upto = wave_scan(sum);
+  // the first kept token with a running sum above uniform * the total
+  const unsigned long long target = share_down(a.uniform[row], lane_of(upto, 63));
+  unsigned long long from = upto - sum;
+  const unsigned long long hit =
+      __builtin_amdgcn_ballot_w64(from <= target && target < upto);
+  const int holder = hit ? __builtin_ctzll(hit) : 0;
+  int part = lane * each;
+#pragma unroll
+  for (int i = 0; i < kLaneParts - 1; ++i) {
+    const bool past = part == lane * each + i && i + 1 < each && target >= from + m[i];
+    part += past;
+    from += past ? m[i] : 0;
+    eq_run += past ? n_eq[i] : 0;
+  }
+  part = min((int)lane_of((uint32_t)part, holder), count - 1);
+  from = lane_of(from, holder);
+  eq_run = lane_of(eq_run, holder);
+  // its chunks, 64 at a time
+  const Run<T> chosen(a, row, part);
+  for (int c0 = chosen.at - lane; c0 < chosen.end; c0 += 64) {
+    const bool have = c0 + lane < chosen.end;
+    float x[Chunks<T>::E];
+    unsigned long long w[Chunks<T>::E];
+    unsigned int n = 0;
+    mass = 0;
+    if (have) {
+      chosen.c.load(c0 + lane, x);
+#pragma unroll
+      for (int i = 0; i < Chunks<T>::E; ++i) {
         const uint32_t key = key_of(x[i]);
-        if (key > cut) {
-          sum += kept_weight(x[i], s, a.shift, pow16);
-        } else if (cut && key == cut) {
-          if (eq_before < ties) sum += even;
-          ++eq_before;
+        w[i] = key > cut ? kept_weight(x[i], s, a.shift, pow16) : 0;
+        mass += w[i];
+        n += cut && key == cut;
+      }
+    }
+    const unsigned int n_upto = wave_scan(n);
+    unsigned long long before_eq = eq_run + (n_upto - n);
+    mass += tied(before_eq, n);
+    const unsigned long long m_upto = wave_scan(mass);
+    unsigned long long at = from + (m_upto - mass);
+    const bool mine = at <= target && target < at + mass;
+    if (mine) {
+      int token = 0;
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < Chunks<T>::E; ++i) {
+        if (cut && key_of(x[i]) == cut) {
+          w[i] = tied(before_eq, 1);
+          ++before_eq;
         }
-        if (sum > target) {
-          a.out[row] = c.index(ch, i);
+        at += w[i];
+        if (!done && at > target) {
+          token = chosen.c.index(c0 + lane, i);
           done = true;
         }
       }
+      a.out[row] = token;
     }
+    if (__builtin_amdgcn_ballot_w64(mine) != 0) return;
+    from += lane_of(m_upto, 63);
+    eq_run += lane_of(n_upto, 63);
   }
 }
 
-int slices_of(int rows, int cols, int es) {
-  const int chunks = (int)(((int64_t)cols * es + 15) / 16) + 1;
-  const int most = std::max(1, std::min(kMaxSlices, chunks / kThreads));
-  return std::max(1, std::min(most, (512 + rows - 1) / std::max(rows, 1)));
+// Slices of a row: workgroups of 1024 threads, two a CU, a chunk a thread or more.
+int most_slices(int rows) {
+  return std::max(1, std::min(kMaxSlices, kWorkgroups / std::max(rows, 1)));
+}
+int slices_of(int rows, int chunks) {
+  return std::max(1, std::min(most_slices(rows), (chunks + kThreads - 1) / kThreads));
 }
 
 }  // namespace
@@ -685,7 +826,7 @@ int slices_of(int rows, int cols, int es) {
 using namespace pa;
 
 extern "C" size_t pa_sample_workspace_size(int32_t rows) {
-  return rows > 0 ? (size_t)rows * sizeof(Row) : 0;
+  return rows > 0 ? (size_t)rows * (sizeof(Row) + most_slices(rows) * kWaves * sizeof(Part)) : 0;
 }
 
 extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* uniform,
@@ -709,12 +850,12 @@ extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* unif
   PA_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
              PA_ERR_WORKSPACE, "pa_sample: workspace of %zu bytes (16-byte aligned) needed, %zu given",
              need, workspace ? workspace_bytes : 0);
-  const int slices = slices_of(rows, cols, es);
   const int chunks = (int)(((int64_t)cols * es + 15) / 16) + 1;
+  const int slices = slices_of(rows, chunks);
   int bits = 1;
   while ((1 << bits) < cols) ++bits;
   const Args a{out, logits, row_stride, uniform, temperature, top_k, top_p, min_p, (Row*)workspace,
-               cols, slices, (chunks + slices - 1) / slices, 62 - bits};
+               (Part*)((Row*)workspace + rows), cols, slices, std::min(62 - bits, 51)};
   const dim3 grid(slices, rows);
   hipStream_t s = (hipStream_t)stream;
 #define PA_LAUNCH_SAMPLE(KERNEL)                                                   \

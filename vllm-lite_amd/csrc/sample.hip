@@ -12,10 +12,11 @@
 // value and the first `ties` tokens equal to it:
 //   1  sample_max_kernel    the row's largest and least logit
 //   2  sample_hist_kernel   counts and weights of 512 equal intervals of the logits
-//   3  sample_pick_kernel   the values in the intervals in which the thresholds lie
-//   4  sample_draw_kernel   the threshold among those values (radix selection), the
-//                           kept weight of every wavefront's run of tokens and, in the
-//                           row's last workgroup, the token
+//   3  sample_pick_kernel   the values in the intervals in which the thresholds lie, and
+//                           (in the row's last workgroup) the thresholds among them, by
+//                           radix selection
+//   4  sample_draw_kernel   the kept weight of every wavefront's run of tokens and, in
+//                           the row's last workgroup, the token
 // 2 and 3 only where the call gives top_k or top_p; rows that do not use them pass
 // through.  Each kernel reads the logits once, in workgroups of a slice of a row.
 #include <algorithm>
@@ -28,11 +29,11 @@
 namespace pa {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 512;
-constexpr int kWorkgroups = 512;  // of a launch where its rows allow: two a CU
-constexpr int kMaxSlices = 16;
+constexpr int kWorkgroups = 1024;  // of a launch where its rows allow: four a CU
+constexpr int kMaxSlices = 32;
 constexpr int kLaneParts = kMaxSlices * kThreads / 64 / 64;  // of a row, to a wavefront
 constexpr int kListMax = 4096;  // values that step 3 collects; more are read from the row again
 constexpr int kDigits = 9;      // bits a round of the selection
@@ -52,14 +53,9 @@ struct Row {
   unsigned long long mass[kBins];
   unsigned int count[kBins];
   unsigned int list[kListMax];
-  // Top-k's threshold is in interval kb (kBins: none, fewer values than k): `above`
-  // values and the weight `least` come before it.
-  unsigned long long above, least;
-  // Top-p's, where all that top-k may leave has it in one interval: that (else kBins),
-  // and the weight before it.
-  unsigned long long before;
-  int kb, pb;
-  unsigned int listed, arrived, pad[2];
+  uint32_t cut;  // kept: the values above `cut` and the first `ties` at it
+  unsigned long long ties;
+  unsigned int listed, arrived[2];
 };
 
 struct Args {
@@ -92,6 +88,7 @@ struct Settings {
   int k;
   bool greedy, by_k, by_p;
   float range, step;    // intervals: of d = max - x up to range, step a unit
+  __device__ bool narrows() const { return (by_k || by_p) && max > -INFINITY; }
 };
 
 // The order of the values as unsigned integers (0 stands for no value: NaN).
@@ -188,21 +185,25 @@ __device__ inline uint32_t wave_join(uint32_t v, uint32_t none, F f) {
   return lane_of(v, 63);
 }
 
-// The row's extremes from its slices.
-__device__ inline void extremes(const Row& row, int slices, Settings& s) {
-  const Stats& mine = row.stats[min((int)(threadIdx.x & 63), slices - 1)];
+// The row's settings and, from its slices, extremes: formed by the first wavefront (a
+// CU's wavefronts share its issue slots), for all behind the next barrier.
+__device__ inline void prepare(const Args& a, int row, Settings& to) {
+  if (threadIdx.x >= 64) return;
+  Settings s = settings_of(a, row);
+  const Stats& mine = a.rows[row].stats[min((int)threadIdx.x, a.slices - 1)];
   auto f32 = [](uint32_t v) { return __builtin_bit_cast(float, v); };
   auto u32 = [](float v) { return __builtin_bit_cast(uint32_t, v); };
-  s.max = f32(wave_join(u32(mine.max), u32(-INFINITY), [&](uint32_t a, uint32_t b) {
-    return u32(fmaxf(f32(a), f32(b)));
+  s.max = f32(wave_join(u32(mine.max), u32(-INFINITY), [&](uint32_t v, uint32_t w) {
+    return u32(fmaxf(f32(v), f32(w)));
   }));
-  s.min = f32(wave_join(u32(mine.min), u32(INFINITY), [&](uint32_t a, uint32_t b) {
-    return u32(fminf(f32(a), f32(b)));
+  s.min = f32(wave_join(u32(mine.min), u32(INFINITY), [&](uint32_t v, uint32_t w) {
+    return u32(fminf(f32(v), f32(w)));
   }));
   s.top = (double)s.max;
   // Weights end at exp(-(shift + 1) ln 2), shift <= 51: d / T <= 36.1.
   s.range = fminf(37.f * s.t, s.max - s.min);
   s.step = s.range > 0.f ? kBins / s.range : 0.f;
+  if (threadIdx.x == 0) to = s;
 }
 
 // A row's memory in 16-byte chunks at 16-byte addresses; the elements of the first
@@ -308,10 +309,8 @@ __device__ inline V wave_sum(V v) {
 }
 // Where the running sum of the kBins entries at h first reaches `want` (1 or more): its
 // index and the sum before it; index kBins and the total where it does not.  By a
-// wavefront; a lane has 8 entries in turn (read from memory as they are, from LDS in
-// the order of slot(), in which 64 lanes read 64 neighbours).
+// wavefront; a lane has 8 entries in turn.
 constexpr int kLaneBins = kBins / 64;
-__device__ inline int slot(int entry) { return entry % kLaneBins * 64 + entry / kLaneBins; }
 struct Cross {
   int at;
   unsigned long long before;
@@ -320,12 +319,12 @@ template <typename V>
 struct Entries {
   V v[kLaneBins];
   unsigned long long sum, before, total;
-  __device__ explicit Entries(const V* h, bool slots = false) {
+  __device__ explicit Entries(const V* h) {
     const int lane = threadIdx.x & 63;
     sum = 0;
 #pragma unroll
     for (int i = 0; i < kLaneBins; ++i) {
-      v[i] = h[slots ? i * 64 + lane : lane * kLaneBins + i];
+      v[i] = h[lane * kLaneBins + i];
       sum += v[i];
     }
     before = wave_scan(sum);
@@ -383,6 +382,17 @@ template <typename V>
 __device__ inline V get(const V* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Whether this is the last of the row's workgroups to get here: to the first wavefront;
+// the others get false.
+__device__ inline bool last_of_row(unsigned int* arrived, int slices) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x >= 64) return false;
+  unsigned int before = 0;
+  if (threadIdx.x == 0)
+    before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return lane_of(before, 0) == (unsigned int)slices - 1;
+}
 
 // ceil(f w) for 0 < f < 1, at least 1; floor(f w), below w.  Exact: f has 24 bits.
 __device__ inline unsigned long long share_up(float f, unsigned long long w) {
@@ -420,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
       r.count[b] = 0;
     }
   }
-  if (slice == 0 && threadIdx.x == 0) r.listed = r.arrived = 0;
+  if (slice == 0 && threadIdx.x == 0) r.listed = r.arrived[0] = r.arrived[1] = 0;
   float mx = -INFINITY, mn = INFINITY;
   int at = INT_MAX;
   run.each([&](const auto& x, int chunk) {
@@ -455,8 +465,7 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
   const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
-  Settings s = settings_of(a, row);
-  if (!s.by_k && !s.by_p) return;
+  __shared__ Settings settings;
   __shared__ unsigned long long mass[kBins];
   __shared__ unsigned int count[kBins];
   __shared__ double pow16[16];
@@ -467,9 +476,10 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
     count[b] = 0;
   }
   if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  extremes(r, a.slices, s);
-  if (s.max == -INFINITY) return;
+  prepare(a, row, settings);
   __syncthreads();
+  const Settings s = settings;
+  if (!s.narrows()) return;
   run.each([&](const auto& x, int) {
 #pragma unroll
     for (int i = 0; i < Chunks<T>::E; ++i) {
@@ -486,86 +496,22 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_pick_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
-  Settings s = settings_of(a, row);
-  if (!s.by_k && !s.by_p) return;
-  __shared__ uint32_t list[kListMax];
-  __shared__ unsigned int n, at;
-  __shared__ int bins[3];
-  Row& r = a.rows[row];
-  Run<T> run(a, row, slice * kWaves + wave);
-  extremes(r, a.slices, s);
-  if (s.max == -INFINITY) return;
-  // the intervals of the thresholds: k's, and p's first and last possible
-  if (wave == 0) {
-    Cross k{kBins, 0};
-    if (s.by_k) k = Entries<unsigned int>(r.count).cross((unsigned long long)s.k);
-    Cross p{kBins, 0};
-    int lo = kBins, hi = -1;
-    unsigned long long least = 0;
-    if (s.by_p) {
-      // the weight that top-k leaves lies between that before its interval and that
-      // with all of it
-      const Entries<unsigned long long> m(r.mass);
-      least = k.at == kBins ? m.total : m.upto(k.at, false);
-      p = m.cross(share_up(s.p, least));
-      lo = min(p.at, k.at);
-      hi = k.at == kBins ? lo : min(m.cross(share_up(s.p, m.upto(k.at, true))).at, k.at);
-    }
-    if (threadIdx.x == 0) {
-      n = 0;
-      bins[0] = k.at;
-      bins[1] = lo;
-      bins[2] = hi;
-      if (slice == 0) {
-        r.kb = k.at;
-        r.above = k.before;
-        r.least = least;
-        r.pb = lo == hi && p.at == lo ? lo : kBins;
-        r.before = p.before;
-      }
-    }
-  }
-  __syncthreads();
-  const int kb = bins[0], lo = bins[1], hi = bins[2];
-  run.each([&](const auto& x, int) {
-#pragma unroll
-    for (int i = 0; i < Chunks<T>::E; ++i) {
-      const int b = bin_of(x[i], s);
-      if (b >= 0 && (b == kb || (b >= lo && b <= hi))) {
-        const unsigned int to = atomicAdd(&n, 1u);
-        if (to < kListMax) list[to] = key_of(x[i]);
-      }
-    }
-  });
-  __syncthreads();
-  if (n == 0) return;
-  if (threadIdx.x == 0) at = atomicAdd(&r.listed, n);
-  __syncthreads();
-  if (at >= kListMax) return;
-  const unsigned int room = min(n, kListMax - at);
-  for (unsigned int i = threadIdx.x; i < room; i += kThreads) r.list[at + i] = list[i];
-}
-
 // The largest value v among the candidates so that those >= v weigh `want` or more
-// (each 1, or its weight), and the sum of those above it.  Rounds of kDigits bits from
-// the highest in which the keys differ to the lowest (values of 16 bits need few).
-// `each(f)` calls f(key) for a thread's candidates.  A round's histogram is one of
-// three: while it is filled the next is cleared, which the round before last read, so
-// one barrier a round will do; every wavefront finds the digit for itself.
+// (each 1, or its weight); `want` becomes what those above it leave of it.  Rounds of
+// up to kDigits bits from the highest in which the keys differ to the lowest (values of
+// 16 bits need few).  `each(f)` calls f(key) for a thread's candidates.  A round's
+// histogram has a digit's sum in as many copies as fit, by lanes: few digits are many
+// candidates for each.  One of two: while it is filled the next is cleared.  The first
+// wavefront finds the digit.
 struct Select {
-  unsigned long long hist[3][kBins];
+  unsigned long long hist[2][kBins];
   unsigned long long red[kWaves];
+  unsigned long long want;
   uint32_t ones, zeros;  // bits that some key has set, and clear
-};
-struct Threshold {
-  uint32_t key;
-  unsigned long long above;
+  uint32_t found;
 };
 template <typename Each, typename Weight>
-__device__ inline Threshold select(Each each, Weight weight, unsigned long long want, Select& l) {
+__device__ inline uint32_t select(Each each, Weight weight, unsigned long long& want, Select& l) {
   uint32_t ones = 0, zeros = 0;
   each([&](uint32_t key) {
     ones |= key;
@@ -584,33 +530,165 @@ __device__ inline Threshold select(Each each, Weight weight, unsigned long long 
   }
   __syncthreads();
   ones = l.ones;
-  zeros = l.zeros;
-  const uint32_t differ = ones & zeros;
-  Threshold t{ones & ~differ, 0};
-  if (differ == 0) return t;
-  const int stop = __builtin_ctz(differ);
-  int left = 32 - __builtin_clz(differ);  // bits still open
-  // below `stop` the keys agree
+  const uint32_t differ = ones & l.zeros;
+  uint32_t found = ones & ~differ;
+  if (differ == 0) return found;
+  const int stop = __builtin_ctz(differ);  // below it the keys agree
+  int left = 32 - __builtin_clz(differ);   // bits still open
   for (int round = 0; left > stop; ++round) {
-    const int shift = max(left - kDigits, stop);
-    const uint32_t digits = (1u << (left - shift)) - 1;
-    unsigned long long* h = l.hist[round % 3];
-    if (threadIdx.x < kBins) l.hist[(round + 1) % 3][threadIdx.x] = 0;
+    const int shift = max(left - kDigits, stop), bits = left - shift;
+    const uint32_t digits = (1u << bits) - 1, copies = (uint32_t)kBins >> bits;
+    unsigned long long* h = l.hist[round % 2];
+    if (threadIdx.x < kBins) l.hist[(round + 1) % 2][threadIdx.x] = 0;
     each([&](uint32_t key) {
-      if (left == 32 || (key >> left) == (t.key >> left))
-        atomicAdd(&h[slot((int)(digits - ((key >> shift) & digits)))], weight(key));
+      if (left == 32 || (key >> left) == (found >> left))
+        atomicAdd(&h[(digits - ((key >> shift) & digits)) * copies +
+                     (threadIdx.x & (copies - 1))],
+                  weight(key));
     });
     __syncthreads();
-    const Cross c = Entries<unsigned long long>(h, true).cross(want);
-    const uint32_t digit = c.at < kBins ? digits - c.at : 0;  // (always found: want <= the sum)
-    t.key = (t.key & ~(digits << shift)) | (digit << shift);
-    if (c.at < kBins) {
-      t.above += c.before;
-      want -= c.before;
+    if (threadIdx.x < 64) {
+      const Entries<unsigned long long> e(h);
+      const Cross c = e.cross(want);
+      const uint32_t place = c.at < kBins ? c.at / copies : digits;  // (found: want <= the sum)
+      const unsigned long long above = copies > 1 ? e.upto((int)(place * copies), false) : c.before;
+      if (threadIdx.x == 0) {
+        l.found = found | (digits - place) << shift;
+        l.want = want - above;
+      }
     }
+    __syncthreads();
+    found = l.found;
+    want = l.want;
     left = shift;
   }
-  return t;
+  return found;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void
+sample_pick_kernel(const Args a) {
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
+  __shared__ Settings settings;
+  __shared__ double pow16[16];
+  __shared__ uint32_t list[kListMax];
+  __shared__ unsigned int n, at, last;
+  // Top-k's threshold is in interval kb (kBins: none, fewer values than k): `above`
+  // values and the weight `least` come before it.  Top-p's is in one of lo to hi; in
+  // pb, `before` it, where that is one for all that top-k may leave (else kBins).
+  __shared__ int kb, lo, hi, pb;
+  __shared__ unsigned long long above, least, before;
+  __shared__ Select l;
+  Row& r = a.rows[row];
+  Run<T> run(a, row, slice * kWaves + wave);
+  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
+  prepare(a, row, settings);
+  __syncthreads();
+  const Settings s = settings;
+  if (!s.narrows()) return;
+  if (wave == 0) {
+    Cross k{kBins, 0}, p{kBins, 0};
+    if (s.by_k) k = Entries<unsigned int>(r.count).cross((unsigned long long)s.k);
+    int p0 = kBins, p1 = -1;
+    unsigned long long w = 0;
+    if (s.by_p) {
+      // the weight that top-k leaves lies between that before its interval and that
+      // with all of it
+      const Entries<unsigned long long> m(r.mass);
+      w = k.at == kBins ? m.total : m.upto(k.at, false);
+      p = m.cross(share_up(s.p, w));
+      p0 = min(p.at, k.at);
+      p1 = k.at == kBins ? p0 : min(m.cross(share_up(s.p, m.upto(k.at, true))).at, k.at);
+    }
+    if (threadIdx.x == 0) {
+      n = 0;
+      kb = k.at;
+      above = k.before;
+      least = w;
+      lo = p0;
+      hi = p1;
+      pb = p0 == p1 && p.at == p0 ? p0 : kBins;
+      before = p.before;
+    }
+  }
+  __syncthreads();
+  {
+    const int b0 = kb, b1 = lo, b2 = hi;
+    run.each([&](const auto& x, int) {
+#pragma unroll
+      for (int i = 0; i < Chunks<T>::E; ++i) {
+        const int b = bin_of(x[i], s);
+        if (b >= 0 && (b == b0 || (b >= b1 && b <= b2))) {
+          const unsigned int to = atomicAdd(&n, 1u);
+          if (to < kListMax) list[to] = key_of(x[i]);
+        }
+      }
+    });
+  }
+  __syncthreads();
+  unsigned int listed = n;
+  if (a.slices > 1) {
+    if (threadIdx.x == 0 && n > 0) at = atomicAdd(&r.listed, n);
+    __syncthreads();
+    if (n > 0 && at < kListMax) {
+      const unsigned int room = min(n, kListMax - at);
+      for (unsigned int i = threadIdx.x; i < room; i += kThreads) put(&r.list[at + i], list[i]);
+    }
+    const bool is_last = last_of_row(&r.arrived[0], a.slices);
+    if (threadIdx.x == 0) last = is_last;
+    __syncthreads();
+    if (!last) return;
+    listed = get(&r.listed);
+    if (listed <= kListMax)
+      for (unsigned int i = threadIdx.x; i < listed; i += kThreads) list[i] = get(&r.list[i]);
+    __syncthreads();
+  }
+  // the values of interval b, from the list or, where that overflowed, the row
+  const bool in_list = listed <= kListMax;
+  const unsigned int candidates = in_list ? listed : (unsigned int)a.cols;
+  auto values = [&](int b) {
+    return [&, b](auto f) {
+      for (unsigned int i = threadIdx.x; i < candidates; i += kThreads) {
+        const float x = in_list ? value_of(list[i]) : Elem<T>::load(run.c.base + i);
+        if (bin_of(x, s) == b) f(key_of(x));
+      }
+    };
+  };
+  // top-k's threshold, then top-p's
+  uint32_t cut = 0;
+  unsigned long long ties = 0;
+  for (int by_p = kb < kBins ? 0 : 1; by_p <= (s.by_p ? 1 : 0); ++by_p) {
+    auto weight = [&](uint32_t key) {
+      return by_p ? weight_of(value_of(key), s, a.shift, pow16) : 1ull;
+    };
+    Cross c{kb, above};
+    unsigned long long want = (unsigned long long)s.k;
+    if (by_p) {
+      unsigned long long total = least;
+      if (kb < kBins) {
+        unsigned long long more = 0;
+        values(kb)([&](uint32_t key) {
+          if (key > cut) more += weight(key);
+        });
+        total += sum_of(more, l.red) + ties * weight(cut);
+      }
+      want = share_up(s.p, total);
+      c = Cross{pb, before};
+      if (c.at == kBins) c = Entries<unsigned long long>(r.mass).cross(want);
+    }
+    want -= c.before;
+    cut = select(values(c.at), weight, want, l);
+    // as many as reach it: want / weight, rounded up (below 2^23: the quotient in f64
+    // is off by one at most)
+    const unsigned long long w = max(weight(cut), 1ull);
+    ties = (unsigned long long)((double)want / (double)w);
+    while (ties * w < want) ++ties;
+    while (ties > 0 && (ties - 1) * w >= want) --ties;
+  }
+  if (threadIdx.x == 0) {
+    r.cut = cut;
+    r.ties = ties;
+  }
 }
 
 template <typename T>
@@ -618,21 +696,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) v
 sample_draw_kernel(const Args a) {
   const int row = blockIdx.y, slice = blockIdx.x, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Settings s = settings_of(a, row);
+  __shared__ Settings settings;
   Row& r = a.rows[row];
   __shared__ double pow16[16];
-  __shared__ Select l;
   Run<T> run(a, row, slice * kWaves + wave);
-  constexpr int kMine = kListMax / kThreads;
-  unsigned int listed = 0;
-  uint32_t mine[kMine];
-  if (s.by_k || s.by_p) {
-    listed = r.listed;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) mine[i] = r.list[i * kThreads + threadIdx.x];
-  }
   if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  extremes(r, a.slices, s);
+  prepare(a, row, settings);
+  __syncthreads();
+  const Settings s = settings;
   if (s.greedy || s.max == -INFINITY) {
     // the first largest; 0 where nothing is above -inf
     if (slice == 0 && threadIdx.x == 0) {
@@ -643,59 +714,8 @@ sample_draw_kernel(const Args a) {
     }
     return;
   }
-  __syncthreads();
-  // Kept: the values above `cut` and the first `ties` at it.
-  uint32_t cut = 0;
-  unsigned long long ties = 0;
-  if (s.by_k || s.by_p) {
-    // the values of interval b, from the list (a thread's few in registers) or, where
-    // that overflowed, the row
-    int bins[kMine];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      bins[i] = i * kThreads + threadIdx.x < listed ? bin_of(value_of(mine[i]), s) : -1;
-    auto values = [&](int b) {
-      return [&, b](auto f) {
-        if (listed <= kListMax) {
-#pragma unroll
-          for (int i = 0; i < kMine; ++i)
-            if (bins[i] == b) f(mine[i]);
-        } else {
-          const Chunks<T> c(a, row);
-          for (int ch = threadIdx.x; ch < c.count; ch += kThreads) {
-            float x[Chunks<T>::E];
-            c.load(ch, x);
-#pragma unroll
-            for (int i = 0; i < Chunks<T>::E; ++i)
-              if (bin_of(x[i], s) == b) f(key_of(x[i]));
-          }
-        }
-      };
-    };
-    auto weight = [&](uint32_t key) { return weight_of(value_of(key), s, a.shift, pow16); };
-    const int kb = r.kb;
-    unsigned long long total = r.least;
-    if (kb < kBins) {
-      const unsigned long long want = (unsigned long long)s.k - r.above;
-      const Threshold t = select(values(kb), [](uint32_t) { return 1ull; }, want, l);
-      cut = t.key;
-      ties = want - t.above;
-      if (s.by_p) {
-        unsigned long long above = 0;
-        values(kb)([&](uint32_t key) { above += key > cut ? weight(key) : 0; });
-        total += sum_of(above, l.red) + ties * weight(cut);
-      }
-    }
-    if (s.by_p) {
-      const unsigned long long want = share_up(s.p, total);
-      Cross c{r.pb, r.before};
-      if (c.at == kBins) c = Entries<unsigned long long>(r.mass).cross(want);
-      const Threshold t = select(values(c.at), weight, want - c.before, l);
-      cut = t.key;
-      const unsigned long long w = max(weight(cut), 1ull);
-      ties = (want - c.before - t.above + w - 1) / w;
-    }
-  }
+  const uint32_t cut = s.narrows() ? r.cut : 0;
+  const unsigned long long ties = s.narrows() ? r.ties : 0;
   // What is kept of the wavefront's run.
   unsigned long long mass = 0;
   unsigned int equal = 0;
@@ -714,13 +734,7 @@ sample_draw_kernel(const Args a) {
     put(&parts[slice * kWaves + wave].mass, mass);
     put(&parts[slice * kWaves + wave].ties, equal);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (wave != 0) return;
-  unsigned int arrived = 0;
-  if (lane == 0)
-    arrived = __hip_atomic_fetch_add(&r.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (lane_of(arrived, 0) != (unsigned int)a.slices - 1) return;
+  if (!last_of_row(&r.arrived[1], a.slices)) return;
   // The row's last workgroup has every part; its first wavefront draws.
   const unsigned long long even = cut ? kept_weight(value_of(cut), s, a.shift, pow16) : 0;
   // of n tokens at the threshold with `before` of them in front, the weight of those kept
@@ -812,7 +826,7 @@ sample_draw_kernel(const Args a) {
   }
 }
 
-// Slices of a row: workgroups of 1024 threads, two a CU, a chunk a thread or more.
+// Slices of a row: workgroups of 512 threads, four a CU, a chunk a thread or more.
 int most_slices(int rows) {
   return std::max(1, std::min(kMaxSlices, kWorkgroups / std::max(rows, 1)));
 }

@@ -21,7 +21,7 @@ constexpr int kStep = 4 * kBlock;  // tokens a step
 // become scores, its V where this one's has been multiplied: a step is always on its
 // way, in one set of registers.
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 16 ? 4 : D == 256 ? 1 : 2))) void
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void
 decode_int8_kernel(
     uint16_t* __restrict__ out, const uint16_t* __restrict__ q, int64_t q_row,
     const int8_t* __restrict__ kc, const int8_t* __restrict__ vc, const uint8_t* __restrict__ ks,
@@ -201,17 +201,38 @@ __global__ __launch_bounds__(64) void decode_int8_merge_kernel(
       out[row * D + lane + 64 * x] = f32_to_bf16_bits(den != 0.f ? num[x] / den : 0.f);
 }
 
-// How a launch over contexts of up to max_ctx tokens is cut.
+// How a launch over contexts of up to max_ctx tokens is cut, after sweeps of 1 to 96
+// parts and 4 or 8 wavefronts over 37 launches of 2 to 1600 (sequence, kv head) pairs
+// and 130 to 120000 tokens: within 3 % of the best of them in the mean, 14 % at worst.
+//   One part where contexts are short (the merge's launch takes 3 us) or fill the card
+//     by pairs: 32 x 320-768, 14 / 2 heads of 64, 6.6 us and 8.0 as four; 64 x 4096,
+//     32 / 8 of 128, 88 and 93 as two; but 16 x 8192-32768 145 as two, 128 as 48.
+//   Else as many as put one workgroup on each of 256 CUs (1 x 1537 of 32 / 8 x 128:
+//     15 us whole, 10 as 8 to 24 parts; 8 x 8000-16000 of 14 / 2 x 64: 50 whole, 12 as
+//     16), and for many or long sequences, whose lengths differ, no longer than 1344 tokens (11 x
+//     37-29000 of 24 / 4 x 96: 38 us as 6, 35 as 22 to 24, 40 as 64).  Not where head_dim
+//     256 leaves one workgroup to a CU: 5 x 968-20891 67 us as 6, 87 as 16.
+//   8 wavefronts a workgroup where workgroups are few, 4 where they are many (1024 pairs
+//     of 100-1000 tokens 36 us with 4, 44 with 8) or short.
 struct Int8Plan {
   int waves, part_len, parts;
 };
 Int8Plan plan_of(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_ctx) {
   const int groups = (num_heads / num_kv_heads + 15) / 16;
   const long long pairs = (long long)num_seqs * num_kv_heads * groups;
-  int len = 4096;
-  while (len > 256 && pairs * ((max_ctx + len - 1) / len) < 512) len /= 2;
-  if (len >= max_ctx) len = std::max(kStep, (max_ctx + kStep - 1) / kStep * kStep);
-  return {head_dim <= 192 ? 8 : 4, len, std::max(1, (int)(((long long)max_ctx + len - 1) / len))};
+  constexpr int kLongest = 21 * kStep;
+  long long parts = 1;
+  if (max_ctx > 768 && !(pairs >= 160 && max_ctx <= 7 * kLongest / 2)) {
+    parts = std::min({256 / pairs, (long long)max_ctx / 96, 32ll});
+    if (head_dim <= 192 && pairs > 8)
+      parts = std::max(parts, ((long long)max_ctx + kLongest - 1) / kLongest);
+    parts = std::max(parts, 1ll);
+  }
+  const long long len = ((max_ctx + parts - 1) / parts + kStep - 1) / kStep * kStep;
+  parts = std::max(1ll, (max_ctx + len - 1) / std::max(len, 1ll));
+  const bool eight = head_dim < 256 && pairs * parts <= 300 &&
+                     !(parts == 1 && head_dim > 64 && max_ctx <= 640);
+  return {eight ? 8 : 4, (int)std::max(len, (long long)kStep), (int)parts};
 }
 
 }  // namespace
@@ -285,14 +306,12 @@ int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_
       (uint16_t*)out, (const uint16_t*)q, q_row, k_cache, v_cache, k_scales, v_scales,         \
       block_tables, max_blocks_per_seq, context_lens, num_heads, num_kv_heads, G, head_groups, \
       num_blocks, scale * kInt8Log2e, np, plan.part_len, ws_o, ws_ml)
-#define PA_LAUNCH_DECODE_INT8(DD)                          \
-  do {                                                     \
-    if (DD == 256 || plan.waves == 4)                      \
-      PA_LAUNCH_DECODE_INT8_NW(DD, 4);                     \
-    else if (DD > 64 || plan.waves == 8)                   \
-      PA_LAUNCH_DECODE_INT8_NW(DD, (DD == 256 ? 4 : 8));   \
-    else                                                   \
-      PA_LAUNCH_DECODE_INT8_NW(DD, (DD > 64 ? 4 : 16));    \
+#define PA_LAUNCH_DECODE_INT8(DD)                         \
+  do {                                                    \
+    if (plan.waves == 4)                                  \
+      PA_LAUNCH_DECODE_INT8_NW(DD, 4);                    \
+    else                                                  \
+      PA_LAUNCH_DECODE_INT8_NW(DD, (DD == 256 ? 4 : 8));  \
   } while (0)
   switch (head_dim) {
     case 32: PA_LAUNCH_DECODE_INT8(32); break;

@@ -28,16 +28,19 @@ __device__ inline int scale_exponent(float a) {
   return e < -126 ? -126 : e;
 }
 
-// x 2^-e to the nearest integer, ties to even; NaN to 0, infinities to +-127.
-// (The product may overflow only for infinite x: |x| <= 127 2^e for the others.)
-__device__ inline int encode(float x, int e) {
-  const float y = rintf(ldexpf(x, -e));
-  return x != x ? 0 : (int)fminf(fmaxf(y, -127.f), 127.f);
+// x 2^-e to the nearest integer, ties to even, as the low byte: x 2^-e + 1.5 2^23 rounds
+// once, to an integer.  For |x| <= 127 2^e (`down` is 2^-e).
+__device__ inline uint32_t encode(float x, float down) {
+  return __builtin_bit_cast(uint32_t, __builtin_fmaf(x, down, 0x1.8p23f));
+}
+// The low bytes of four words.
+__device__ inline uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u),
+                               __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
 }
 
-template <typename T>
-struct Four {
-  T v[4];
+struct Eight {
+  float v[8];
 };
 
 // What the launch works on.
@@ -61,18 +64,21 @@ struct AppendArgs {
 // h < Hkv writes kv head h of K, Hkv + h of V, 2 Hkv + h rotates query head h.  A
 // block goes through it whole: its tokens' values in registers, the largest by lane
 // shuffles, so no launch reads the tokens twice and the blocks need no order.
-// A row of D values takes D / 4 lanes (4 values each), TPP rows at a time.
-// ALIGNED: rows by 8- or 16-byte loads.
+// A lane has 8 values of each of TPL neighbouring tokens: 16-byte loads of bf16 rows
+// where ALIGNED, and V's codes meet in LDS as words of neighbouring tokens.  ROPE
+// (K and q are rotated) is apart for its registers.
 // Bound by its chain of loads (offsets, table, old scale and codes) for a decode
 // step, by memory for prompts.
-template <typename T, int D, bool ALIGNED>
+template <typename T, int D, bool ALIGNED, bool ROPE>
 __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {
-  constexpr int LPR = D / 4;                       // lanes a row
-  constexpr int TPP = 64 / LPR;                    // rows at a time
-  constexpr int PASSES = (kBlock + TPP - 1) / TPP;
-  __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock * D];  // V: [dim][token]
+  constexpr int LPR = D / 8;  // lanes a row
+  constexpr int SUBS = 64 / LPR >= 16 ? 16 : 64 / LPR >= 8 ? 8 : 64 / LPR >= 4 ? 4 : 2;
+  constexpr int TPL = kBlock / SUBS;  // tokens a lane
+  // V's codes, [dim][token]; rows of 5 words, to spread the lanes over the banks
+  constexpr int PITCH = kBlock + 4;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[PITCH * D];
   const int lane = threadIdx.x, sub = lane / LPR, u = lane % LPR;
-  const bool on = sub < TPP;
+  const bool on = sub < SUBS;
   const int seq = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int col = blockIdx.y;
   const int part = col < a.Hkv ? 0 : col < 2 * a.Hkv ? 1 : 2;  // K, V, q
@@ -86,19 +92,18 @@ __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {
   const T* src = (const T*)(part == 0 ? a.key : part == 1 ? a.value : a.q) +
                  (int64_t)begin * row_stride + head * D;
   const int b0 = start / kBlock, nb = (int)(((int64_t)start + n - 1) / kBlock) - b0 + 1;
-  const bool rotate = a.inv_freq && part != 1;
-  auto load = [&](const T* p) -> Four<float> {
-    Four<float> r;
+  auto load = [&](const T* p) -> Eight {
+    Eight r;
     if constexpr (ALIGNED) {
-      struct __attribute__((aligned(4 * sizeof(T)))) V {
-        T v[4];
+      struct __attribute__((aligned(16))) V {
+        T v[8];
       };
       const V w = *reinterpret_cast<const V*>(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.v[i] = Elem<T>::load(w.v + i);
+      for (int i = 0; i < 8; ++i) r.v[i] = Elem<T>::load(w.v + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.v[i] = Elem<T>::load(p + i);
+      for (int i = 0; i < 8; ++i) r.v[i] = Elem<T>::load(p + i);
     }
     return r;
   };
@@ -113,23 +118,27 @@ __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {
     }
     // token `at` of the block is row at - first of this block's rows
     const T* rows = src + (int64_t)(b * kBlock - start) * row_stride;
-    Four<float> x[PASSES];
-    float amax = 0.f;
+    Eight x[TPL];
+    uint32_t most = 0;  // the largest magnitude's bits
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int at = p * TPP + sub;
+    for (int p = 0; p < TPL; ++p) {
+      const int at = sub * TPL + p;
       const bool mine = on && at >= first && at < last;
-      x[p] = Four<float>{{0.f, 0.f, 0.f, 0.f}};
-      if (mine) {
+      x[p] = Eight{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+      if (mine) x[p] = load(rows + (int64_t)at * row_stride + 8 * u);
+    }
+#pragma unroll
+    for (int p = 0; p < TPL; ++p) {
+      const int at = sub * TPL + p;
+      if (on && at >= first && at < last) {
         const T* row = rows + (int64_t)at * row_stride;
-        x[p] = load(row + 4 * u);
-        if (rotate) {
+        if (ROPE && part != 1) {
           // dims i < D / 2 and i + D / 2 form a pair
           const bool low = u < LPR / 2;
-          const int i0 = 4 * (low ? u : u - LPR / 2);
-          const Four<float> y = load(row + (low ? 4 * u + D / 2 : 4 * u - D / 2));
+          const int i0 = 8 * (low ? u : u - LPR / 2);
+          const Eight y = load(row + (low ? 8 * u + D / 2 : 8 * u - D / 2));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             float s, c;
             sincosf((float)(b * kBlock + at) * a.inv_freq[i0 + i], &s, &c);
             x[p].v[i] = low ? __builtin_fmaf(x[p].v[i], c, -(y.v[i] * s))
@@ -137,30 +146,54 @@ __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float m = fabsf(x[p].v[i]);
-          amax = m < INFINITY ? fmaxf(amax, m) : amax;  // (NaN fails the test too)
-        }
+        for (int i = 0; i < 8; ++i)
+          most = max(most, __builtin_bit_cast(uint32_t, x[p].v[i]) & 0x7FFFFFFFu);
       }
     }
     if (part == 2) {
       T* dst = const_cast<T*>(rows);
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int at = p * TPP + sub;
-        if (on && at >= first && at < last)
+      for (int p = 0; p < TPL; ++p) {
+        const int at = sub * TPL + p;
+        if (!on || at < first || at >= last) continue;
+        T* to = dst + (int64_t)at * row_stride + 8 * u;
+        if constexpr (ALIGNED) {
+          struct __attribute__((aligned(16))) V {
+            T v[8];
+          } w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            Elem<T>::store(dst + (int64_t)at * row_stride + 4 * u + i, x[p].v[i]);
+          for (int i = 0; i < 8; ++i) Elem<T>::store(w.v + i, x[p].v[i]);
+          *reinterpret_cast<V*>(to) = w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) Elem<T>::store(to + i, x[p].v[i]);
+        }
       }
       continue;
     }
+    auto wave_max = [](uint32_t v) -> uint32_t {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+      for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+      return v;
+    };
+    constexpr uint32_t kInf = 0x7F800000u;
+    most = wave_max(most);
+    const bool odd = most >= kInf;  // infinities or NaN: of the finite values, then
+    if (odd) {
+      most = 0;
+#pragma unroll
+      for (int p = 0; p < TPL; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t m = __builtin_bit_cast(uint32_t, x[p].v[i]) & 0x7FFFFFFFu;
+          most = max(most, m < kInf ? m : 0);
+        }
+      most = wave_max(most);
+    }
     const int64_t slice = (int64_t)id * a.Hkv + head;
     uint8_t* scale = (part == 0 ? a.k_scales : a.v_scales) + slice;
     int8_t* codes = (part == 0 ? a.k_cache : a.v_cache) + slice * (kBlock * D);
-    int e = scale_exponent(amax);
+    int e = scale_exponent(__builtin_bit_cast(float, most));
     int drop = 0;  // the kept codes move down by 2^drop
     if (first > 0) {
       const int old = (int)*scale - 127;
@@ -168,46 +201,80 @@ __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {
       drop = e - old;
     }
     if (lane == 0) *scale = (uint8_t)(e + 127);
-    auto kept = [&](int8_t c) -> int { return drop ? (int)rintf(ldexpf((float)c, -drop)) : c; };
-    if (part == 0) {
+    float down = ldexpf(1.f, -e);
+    if (odd) {  // in units of 2^e: NaN as 0, infinities as the largest codes
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int at = p * TPP + sub;
-        if (!on || at >= last || (at < first && drop == 0)) continue;
-        uint32_t* to = reinterpret_cast<uint32_t*>(codes + at * D + 4 * u);
-        uint32_t w = 0;
-        if (at < first) {
-          const uint32_t was = *to;
+      for (int p = 0; p < TPL; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w |= (uint32_t)(uint8_t)kept((int8_t)(was >> (8 * i))) << (8 * i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w |= (uint32_t)(uint8_t)encode(x[p].v[i], e) << (8 * i);
+        for (int i = 0; i < 8; ++i) {
+          const float v = x[p].v[i] * down;
+          x[p].v[i] = v != v ? 0.f : fminf(fmaxf(v, -127.f), 127.f);
         }
-        *to = w;
+      down = 1.f;
+    }
+    // four of the codes that were there
+    auto kept = [&](uint32_t w) -> uint32_t {
+      const float by = ldexpf(1.f, -drop);
+      return low_bytes(encode((float)(int8_t)w, by), encode((float)(int8_t)(w >> 8), by),
+                       encode((float)(int8_t)(w >> 16), by), encode((float)(int8_t)(w >> 24), by));
+    };
+    if (part == 0) {
+      if (drop) {
+        uint32_t* words = reinterpret_cast<uint32_t*>(codes);
+#pragma unroll 1
+        for (int i = lane; i < first * D / 4; i += 64) {
+          words[i] = kept(words[i]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < TPL; ++p) {
+        const int at = sub * TPL + p;
+        if (!on || at < first || at >= last) continue;
+        uint32_t c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = encode(x[p].v[i], down);
+        *reinterpret_cast<uint2*>(codes + at * D + 8 * u) =
+            uint2{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
       }
     } else {
       __syncthreads();  // the last block's rows have been read
+      if (on) {
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int at = p * TPP + sub;
-        if (on && at >= first && at < last)
+        for (int i = 0; i < 8; ++i) {
+          uint8_t* to = tile + (8 * u + i) * PITCH + sub * TPL;
+          uint32_t c[TPL < 4 ? 4 : TPL] = {};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tile[(4 * u + i) * kBlock + at] = (uint8_t)encode(x[p].v[i], e);
+          for (int p = 0; p < TPL; ++p) c[p] = encode(x[p].v[i], down);
+          const uint32_t w = low_bytes(c[0], c[1], c[2], c[3]);
+          if constexpr (TPL == 1) *to = (uint8_t)w;
+          if constexpr (TPL == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
+          if constexpr (TPL >= 4) *reinterpret_cast<uint32_t*>(to) = w;
+          if constexpr (TPL == 8)
+            reinterpret_cast<uint32_t*>(to)[1] = low_bytes(c[4], c[5], c[6], c[7]);
+        }
       }
       __syncthreads();
-      struct __attribute__((aligned(16))) Row {
-        int8_t c[kBlock];
+      // the bytes of word i that are tokens before t
+      auto before = [](int i, int t) -> uint32_t {
+        const int n = min(max(t - 4 * i, 0), 4);
+        return n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1;
       };
+#pragma unroll 1
       for (int d = lane; d < D; d += 64) {
+        struct __attribute__((aligned(16))) Row {
+          uint32_t w[kBlock / 4];
+        } r;
         Row* to = reinterpret_cast<Row*>(codes + d * kBlock);
-        Row r = *reinterpret_cast<const Row*>(tile + d * kBlock);
-        if (first > 0 || last < kBlock) {
-          const Row was = *to;
 #pragma unroll
-          for (int t = 0; t < kBlock; ++t) {
-            if (t < first) r.c[t] = (int8_t)kept(was.c[t]);
-            if (t >= last) r.c[t] = was.c[t];
+        for (int i = 0; i < kBlock / 4; ++i)
+          r.w[i] = *reinterpret_cast<const uint32_t*>(tile + d * PITCH + 4 * i);
+        if (first > 0 || last < kBlock) {
+          Row was = *to;
+#pragma unroll
+          for (int i = 0; i < kBlock / 4; ++i) {
+            const uint32_t old = before(i, first), fresh = before(i, last) & ~old;
+            if (drop) was.w[i] = (was.w[i] & ~old) | (kept(was.w[i]) & old);
+            r.w[i] = (r.w[i] & fresh) | (was.w[i] & ~fresh);
           }
         }
         *to = r;
@@ -288,17 +355,17 @@ extern "C" int32_t pa_append_int8(int8_t* k_cache, int8_t* v_cache, uint8_t* k_s
                      max_blocks_per_seq, num_tokens, max_tokens, chunks, num_heads, num_kv_heads,
                      head_dim, num_blocks};
   const int es = dtype == PA_DTYPE_BF16 ? 2 : 4;
-  const bool aligned =
-      ((uintptr_t)key | (uintptr_t)value | (uintptr_t)q) % (4 * es) == 0 &&
-      (key_stride | value_stride | (q ? q_stride : 0)) % 4 == 0;
+  const bool aligned = ((uintptr_t)key | (uintptr_t)value | (uintptr_t)q) % 16 == 0 &&
+                       (key_stride | value_stride | (q ? q_stride : 0)) * es % 16 == 0;
   const dim3 grid(num_seqs * chunks, columns);
   hipStream_t s = (hipStream_t)stream;
-#define PA_LAUNCH_APPEND(DD)                                                          \
-  (dtype == PA_DTYPE_BF16                                                             \
-       ? (aligned ? append_int8_kernel<uint16_t, DD, true><<<grid, 64, 0, s>>>(a)     \
-                  : append_int8_kernel<uint16_t, DD, false><<<grid, 64, 0, s>>>(a))   \
-       : (aligned ? append_int8_kernel<float, DD, true><<<grid, 64, 0, s>>>(a)        \
-                  : append_int8_kernel<float, DD, false><<<grid, 64, 0, s>>>(a)))
+#define PA_LAUNCH_APPEND_T(T, DD)                                                       \
+  (q ? (aligned ? append_int8_kernel<T, DD, true, true><<<grid, 64, 0, s>>>(a)          \
+                : append_int8_kernel<T, DD, false, true><<<grid, 64, 0, s>>>(a))        \
+     : (aligned ? append_int8_kernel<T, DD, true, false><<<grid, 64, 0, s>>>(a)         \
+                : append_int8_kernel<T, DD, false, false><<<grid, 64, 0, s>>>(a)))
+#define PA_LAUNCH_APPEND(DD) \
+  (dtype == PA_DTYPE_BF16 ? PA_LAUNCH_APPEND_T(uint16_t, DD) : PA_LAUNCH_APPEND_T(float, DD))
   switch (head_dim) {
     case 32: PA_LAUNCH_APPEND(32); break;
     case 64: PA_LAUNCH_APPEND(64); break;
@@ -308,6 +375,7 @@ extern "C" int32_t pa_append_int8(int8_t* k_cache, int8_t* v_cache, uint8_t* k_s
     default: PA_LAUNCH_APPEND(256); break;
   }
 #undef PA_LAUNCH_APPEND
+#undef PA_LAUNCH_APPEND_T
   return check_launch("pa_append_int8");
 }
 

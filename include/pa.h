@@ -347,7 +347,8 @@ int32_t pa_prefill_quantized(void* out, const void* q, const float* k_cache, con
 /* A cache of one byte an element that keeps 7 to 8 bits of precision: codes int8
  * in the block layouts above (K [NB, Hkv, 16, D], V [NB, Hkv, D, 16]) and a scale
  * byte for each (block, kv head) of each, k_scales / v_scales [NB, Hkv] uint8.  A
- * value is code * 2^(byte - 127); scale bytes are 1 to 254 (0 reads as scale 0).
+ * value is code * 2^(byte - 127); scale bytes are 1 to 254 (0 reads as scale 0), of
+ * pa_append_int8's 1 to 249.
  * No counterpart in the reference, whose quantised cache keeps int8 values in f32
  * with one scale for a block's K, V and heads (pa_kv_cache_create_quantized).
  * q and out are bf16, head_dim is 32, 64, 96, 128, 192 or 256
@@ -400,9 +401,11 @@ size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
 
 /* pa_decode over an int8 cache, arguments and conventions as there (any number of
  * query heads per kv head; calls that may overlap need workspaces of their own).
- * The scores are exact products of the codes with q rounded to 15 bits of its
- * row's largest value, probabilities times the V scale are rounded to bf16, sums
- * are f32.  A query row with a NaN or an infinity gives NaN. */
+ * The scores are exact products of the codes with q rounded to 2^-14 of its row's
+ * largest value, probabilities times the V scale are rounded to bf16, sums are f32.
+ * A query row with a NaN or an infinity gives NaN.  Where V's scale bytes are below
+ * 16 or above 240, probabilities times the scale may leave bf16's range: small
+ * values come out as 0, large ones as infinities or NaN. */
 int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
                        const uint8_t* k_scales, const uint8_t* v_scales,
                        const int32_t* block_tables, int32_t max_blocks_per_seq,
@@ -412,7 +415,7 @@ int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const in
                        pa_stream_t stream);
 
 /* pa_prefill over an int8 cache, arguments and conventions as there, arithmetic as
- * pa_decode_int8. */
+ * pa_decode_int8, but with q as it is. */
 int32_t pa_prefill_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
                         const uint8_t* k_scales, const uint8_t* v_scales,
                         const int32_t* block_tables, int32_t max_blocks_per_seq,

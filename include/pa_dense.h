@@ -266,7 +266,7 @@ int32_t pa_argmax(int64_t* out, const void* logits, int32_t rows, int32_t cols,
  *   logits  [rows, cols] of dtype with row_stride elements between rows (0 =
  *           cols), rows at any element; cols up to 2^22, rows up to 65535
  *   out     [rows] int64 (device)
- * Weights are formed in f64 and summed exactly in units of 2^-(62 - b), b =
+ * Weights are formed in f64 and summed exactly in units of 2^-min(51, 62 - b), b =
  * max(1, ceil(log2 cols)), of the largest: the draw is that of the formula but for
  * borders closer than a few of those times cols, and does not depend on the order
  * of anything.

@@ -1,8 +1,9 @@
 """pa_sample on the GPU: the very tokens of the definition in 64 bits.
 
-The kernel's weights are off by less than 2^-46 of themselves and half a unit of
-2^-(62 - b), b = ceil(log2 cols), so a running sum over n tokens is off by less than
-2^-46 of the total and n 2^-(63 - b); numpy's by n 2^-53 of it.  Where u or p is
+The kernel's weights are off by less than 2^-48 of themselves and half a unit of
+2^-min(51, 62 - b), b = ceil(log2 cols), so a running sum over n tokens is off by less
+than 2^-48 of the total and n 2^-(63 - b) or, for 1024 columns and fewer, n 2^-52;
+numpy's by n 2^-53 of it at most, and half of that over runs of equal steps.  Where u or p is
 nearer than that (over the total, which is 1 or more) to a border between two
 tokens, the tokens on both sides are right."""
 import numpy as np

@@ -2,8 +2,8 @@
 // and min-p, one uniform number a row.
 //
 // With M the row's largest logit a token weighs w = exp((x - M) / T).  Weights are
-// formed in f64 (an error of about 2^-48) and summed as integers of 2^-shift (44
-// bits for vocabularies up to 2^18): a sum does not depend on its order, so equal
+// formed in f64 (an error of about 2^-48) and summed as integers of 2^-shift (51
+// bits, 44 for vocabularies up to 2^18): a sum does not depend on its order, so equal
 // calls draw equal tokens, and a border between two tokens lies where the exact sums
 // have it but for a few 2^-44 of the row's total.  (Sums of 10^5 f32 weights would
 // move the borders by more than many tokens' weights.)

@@ -59,7 +59,7 @@ def prefill(lib, **kw):
     (prefill, dict(b=-1), -1), (prefill, dict(hq=5), -1), (prefill, dict(most=-1), -1),
     (prefill, dict(d=16), -3), (prefill, dict(out=None), -1), (prefill, dict(past=None), -1),
     (prefill, dict(k=C.c_void_p(264)), -1), (prefill, dict(out=C.c_void_p(260)), -1),
-    (prefill, dict(b=70000), -3), (prefill, dict(mbs=1 << 28), -3),
+    (prefill, dict(b=1 << 30), -3), (prefill, dict(mbs=1 << 28), -3),
     (prefill, dict(b=0), 0), (prefill, dict(t=0), 0), (prefill, dict(most=0), 0),
 ])
 def test_refusals(lib, call, kw, rc):

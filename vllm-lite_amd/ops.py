@@ -779,6 +779,13 @@ def linear_mx(x, weight, bias=None, act=ACT_NONE, residual=None, out=None, mx_ou
 # ---- the int8 cache (pa.h) --------------------------------------------------
 
 
+def _int8_like(t, shape, dtype, index):
+    """A contiguous tensor of `shape` on the device of this index: _mx_like for calls
+    that are as long as their checks (a device's index compares in half the time)."""
+    return (t.dtype is dtype and t.get_device() == index and t.is_contiguous() and
+            t.shape == shape)
+
+
 class Int8Cache:
     """One layer's int8 cache: codes k int8 [NB, H, 16, D] and v int8
     [NB, H, D, 16], scale bytes k_scales and v_scales uint8 [NB, H]; a value is
@@ -787,18 +794,23 @@ class Int8Cache:
     __slots__ = ("k", "v", "k_scales", "v_scales", "num_blocks", "num_kv_heads", "head_dim")
 
     def __init__(self, k, v, k_scales, v_scales):
-        if k.dim() != 4 or k.shape[2] != BLOCK_SIZE:
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != BLOCK_SIZE:
             raise ValueError("k must be [NB, H, 16, D]")
-        nb, h, _, d = k.shape
-        device = k.device
+        nb, h, _, d = shape
         if not k.is_cuda:
             raise ValueError("an int8 cache is on the device")
-        for name, t, shape, dtype in (("k", k, (nb, h, BLOCK_SIZE, d), torch.int8),
-                                      ("v", v, (nb, h, d, BLOCK_SIZE), torch.int8),
-                                      ("k_scales", k_scales, (nb, h), torch.uint8),
-                                      ("v_scales", v_scales, (nb, h), torch.uint8)):
-            if not _mx_like(t, shape, dtype, device):
-                _mx_refuse(name, t, shape, dtype, device)
+        i, codes, scales = k.get_device(), torch.int8, torch.uint8
+        if not (_int8_like(k, shape, codes, i) and
+                _int8_like(v, (nb, h, d, BLOCK_SIZE), codes, i) and
+                _int8_like(k_scales, (nb, h), scales, i) and
+                _int8_like(v_scales, (nb, h), scales, i)):
+            for name, x, s, dtype in (("k", k, shape, codes),
+                                      ("v", v, (nb, h, d, BLOCK_SIZE), codes),
+                                      ("k_scales", k_scales, (nb, h), scales),
+                                      ("v_scales", v_scales, (nb, h), scales)):
+                if not _int8_like(x, s, dtype, i):
+                    _mx_refuse(name, x, s, dtype, k.device)
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
         self.num_blocks, self.num_kv_heads, self.head_dim = nb, h, d
 
@@ -817,17 +829,19 @@ class Int8Cache:
                 self.v_scales.data_ptr())
 
 
-def _int8_index(name, t, shape, device):
-    if not _mx_like(t, shape, torch.int32, device):
-        _mx_refuse(name, t, shape, torch.int32, device)
+def _int8_index(name, t, n, index):
+    if not _int8_like(t, (n,), torch.int32, index):
+        _mx_refuse(name, t, (n,), torch.int32, f"cuda:{index}")
     return t.data_ptr()
 
 
-def _int8_tables(block_tables, device):
-    if block_tables.dim() != 2:
+def _int8_tables(tables, index):
+    shape = tables.shape
+    if len(shape) != 2:
         raise ValueError("block_tables must be [num_seqs, max_blocks_per_seq]")
-    _int8_index("block_tables", block_tables, block_tables.shape, device)
-    return block_tables.shape
+    if not _int8_like(tables, shape, torch.int32, index):
+        _mx_refuse("block_tables", tables, shape, torch.int32, f"cuda:{index}")
+    return shape
 
 
 def append_int8(cache, key, value, block_tables, cu_seq_tokens, context_lens, max_tokens, q=None,
@@ -839,28 +853,33 @@ def append_int8(cache, key, value, block_tables, cu_seq_tokens, context_lens, ma
     max_tokens: the most of any sequence.  With inv_freq (f32 [D / 2]), q
     [T, Hq, D] is rotated in place and the keys on their way."""
     device, h, d = cache.k.device, cache.num_kv_heads, cache.head_dim
-    b, mbs = _int8_tables(block_tables, device)
-    t = key.shape[0]
-    code = _dtype_code(key)
+    index = device.index
+    b, mbs = _int8_tables(block_tables, index)
+    shape, dtype = key.shape, key.dtype
+    t, code = shape[0] if shape else 0, _dtype_code(key)
     if (q is None) != (inv_freq is None):
         raise ValueError("q is rotated with inv_freq: both or neither")
     hq = 0 if q is None else q.shape[1] if q.dim() == 3 else 0
-    for name, x, heads in (("key", key, h), ("value", value, h), ("q", q, hq)):
-        if x is None:
-            continue
-        if x.shape != (t, heads, d) or heads == 0 or x.dtype != key.dtype or x.device != device:
-            raise ValueError(f"{name}: expected {key.dtype} [{t}, {heads or 'Hq'}, {d}] on "
+
+    def stride(name, x, heads):
+        if (x.shape != (t, heads, d) or heads == 0 or x.dtype is not dtype or
+                x.get_device() != index):
+            raise ValueError(f"{name}: expected {dtype} [{t}, {heads or 'Hq'}, {d}] on "
                              f"{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-        if not _rows_ok(x, heads, d):
+        row, head, one = x.stride()
+        if one != 1 or head != d or (t > 1 and row < heads * d):
             raise ValueError(f"{name}: rows must be contiguous [H, D], not overlapping")
+        return row if t > 1 else 0
+
+    ks, vs = stride("key", key, h), stride("value", value, h)
+    qs = 0 if q is None else stride("q", q, hq)
     if inv_freq is not None and not _mx_like(inv_freq, (d // 2,), torch.float32, device):
         _mx_refuse("inv_freq", inv_freq, (d // 2,), torch.float32, device)
-    _mx_call("pa_append_int8", device, *cache._ptrs(), key.data_ptr(),
-             key.stride(0) if t > 1 else 0, value.data_ptr(), value.stride(0) if t > 1 else 0,
-             None if q is None else q.data_ptr(), 0 if q is None or t <= 1 else q.stride(0),
+    _mx_call("pa_append_int8", device, *cache._ptrs(), key.data_ptr(), ks, value.data_ptr(), vs,
+             None if q is None else q.data_ptr(), qs,
              None if inv_freq is None else inv_freq.data_ptr(), block_tables.data_ptr(), mbs,
-             _int8_index("cu_seq_tokens", cu_seq_tokens, (b + 1,), device),
-             _int8_index("context_lens", context_lens, (b,), device), b, t, max_tokens, hq, h, d,
+             _int8_index("cu_seq_tokens", cu_seq_tokens, b + 1, index),
+             _int8_index("context_lens", context_lens, b, index), b, t, max_tokens, hq, h, d,
              cache.num_blocks, code)
 
 
@@ -870,7 +889,7 @@ def read_kv_int8(cache, block_ids, seq_len):
     device = cache.k.device
     if block_ids.dim() != 1:
         raise ValueError("block_ids must be one-dimensional")
-    ids = _int8_index("block_ids", block_ids, block_ids.shape, device)
+    ids = _int8_index("block_ids", block_ids, block_ids.shape[0], device.index)
     shape = (seq_len, cache.num_kv_heads, cache.head_dim)
     out_k, out_v = (torch.empty(shape, dtype=torch.float32, device=device) for _ in range(2))
     _mx_call("pa_read_kv_int8", device, *cache._ptrs(), ids, block_ids.shape[0], seq_len,
@@ -885,28 +904,28 @@ def decode_int8_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, max_
 
 
 def _int8_q(q, cache, out):
-    device = cache.k.device
-    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+    index, shape = cache.k.get_device(), q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError("q must be [rows, Hq, D]")
-    if not _mx_like(q, q.shape, torch.bfloat16, device):
-        _mx_refuse("q", q, q.shape, torch.bfloat16, device)
+    if not _int8_like(q, shape, torch.bfloat16, index):
+        _mx_refuse("q", q, shape, torch.bfloat16, f"cuda:{index}")
     if out is None:
-        return torch.empty_like(q)
-    if not _mx_like(out, q.shape, torch.bfloat16, device):
-        _mx_refuse("out", out, q.shape, torch.bfloat16, device)
-    return out
+        return torch.empty_like(q), shape
+    if not _int8_like(out, shape, torch.bfloat16, index):
+        _mx_refuse("out", out, shape, torch.bfloat16, f"cuda:{index}")
+    return out, shape
 
 
 def decode_int8(q, cache, block_tables, context_lens, max_context_len, scale=None, out=None,
                 workspace=None):
     """pa_decode_int8: q [B, Hq, D] bf16 -> out [B, Hq, D]."""
-    device, d = cache.k.device, cache.head_dim
-    out = _int8_q(q, cache, out)
-    n, hq, _ = q.shape
-    b, mbs = _int8_tables(block_tables, device)
+    device = cache.k.device
+    index = device.index
+    out, (n, hq, d) = _int8_q(q, cache, out)
+    b, mbs = _int8_tables(block_tables, index)
     if b != n:
         raise ValueError(f"block_tables of {b} sequences, q of {n}")
-    lens = _int8_index("context_lens", context_lens, (b,), device)
+    lens = _int8_index("context_lens", context_lens, b, index)
     if workspace is None:
         need = decode_int8_workspace_size(b, hq, cache.num_kv_heads, d, max_context_len)
         if need:
@@ -923,13 +942,13 @@ def decode_int8(q, cache, block_tables, context_lens, max_context_len, scale=Non
 
 def prefill_int8(q, cache, block_tables, cu_q_lens, past_lens, max_q_len, scale=None, out=None):
     """pa_prefill_int8: q [total_q, Hq, D] bf16 -> out [total_q, Hq, D]."""
-    device, d = cache.k.device, cache.head_dim
-    out = _int8_q(q, cache, out)
-    n, hq, _ = q.shape
-    b, mbs = _int8_tables(block_tables, device)
+    device = cache.k.device
+    index = device.index
+    out, (n, hq, d) = _int8_q(q, cache, out)
+    b, mbs = _int8_tables(block_tables, index)
     _mx_call("pa_prefill_int8", device, out.data_ptr(), q.data_ptr(), *cache._ptrs(),
-             block_tables.data_ptr(), mbs, _int8_index("cu_q_lens", cu_q_lens, (b + 1,), device),
-             _int8_index("past_lens", past_lens, (b,), device), b, n, max_q_len, hq,
+             block_tables.data_ptr(), mbs, _int8_index("cu_q_lens", cu_q_lens, b + 1, index),
+             _int8_index("past_lens", past_lens, b, index), b, n, max_q_len, hq,
              cache.num_kv_heads, d, cache.num_blocks,
              1.0 / math.sqrt(d) if scale is None else scale)
     return out

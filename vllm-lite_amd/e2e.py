@@ -30,6 +30,9 @@ device (pa_batch_advance; the block tables hold the whole generation).
 With weights quantised by Weights.pack_mx() every step runs the decoder block
 in MXFP8 (Engine._forward_mx): half the bytes of the projections' weights, the
 matrix cores at their FP8 rate.
+With Engine(kv_dtype=torch.int8) the cache holds int8 codes (pa_append_int8,
+pa_decode_int8, pa_prefill_int8 inside pa_batch_attention), and generate() with
+Sampling settings draws its tokens by pa_sample.
 The norm is chosen explicitly by ModelConfig.norm: "rms" (RMSNorm, what the
 benchmark configuration states) or "layer" (the zero-bias LayerNorm the
 reference's CausalLm constructs for these models,

@@ -19,6 +19,10 @@
 //                           the row's last workgroup, the token
 // 2 and 3 only where the call gives top_k or top_p; rows that do not use them pass
 // through.  Each kernel reads the logits once, in workgroups of a slice of a row.
+//
+// Bound by the launches and what each does once a row, one thing after the other, for
+// few rows: 1 x 151936 bf16 29 us, 32 rows 43; by f64 weights, formed twice, for many:
+// 253 x 50257 f32 80 us, of which the first kernel 11, at a copy's rate.
 #include <algorithm>
 #include <climits>
 

@@ -190,3 +190,85 @@ def test_frequencies(pa):
     assert np.all(np.diff(got) >= 0)  # in the order of the columns
     got = run(pa, x.repeat(n, 1), u, k=[2] * n)
     assert list(np.bincount(got, minlength=4)) == [2731, 0, 1365, 0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_launch_and_four_agree(pa, dtype):
+    """Many rows take their steps in one launch, few long ones in four: the same
+    tokens."""
+    rng = np.random.default_rng(7)
+    rows, cols = 600, 12007
+    x = (2.5 * rng.standard_normal((rows, cols))).astype(np.float32)
+    x[:60] = rng.integers(-3, 4, (60, cols))
+    x[60:80] = 1.5
+    x[80:120][rng.random((40, cols)) < 0.97] = -np.inf
+    x[120:140, 5] = 60.0
+    x[140:160][rng.random((20, cols)) < 0.5] = np.nan
+    logits = torch.from_numpy(x).to(DEV).to(dtype)
+    s = (rng.random(rows).astype(np.float32), rng.choice([0.0, 0.3, 1.0, 20.0], rows),
+         rng.choice([0, 1, 40, 9000], rows), rng.choice([1.0, 0.9, 0.4], rows),
+         rng.choice([0.0, 0.05], rows))
+    got = run(pa, logits, *s)
+    few = [run(pa, logits[i:i + 100], *(v[i:i + 100] for v in s)) for i in range(0, rows, 100)]
+    np.testing.assert_array_equal(got, np.concatenate(few))
+
+
+@pytest.mark.parametrize("cols", [8191, 8192, 8193])
+def test_short_rows_at_the_limit(pa, cols):
+    """Ties, masks, an outlier over values in one interval and odd strides, in rows
+    that take one launch and just not."""
+    rng = np.random.default_rng(cols)
+    rows = 24
+    x = (2.5 * rng.standard_normal((rows, cols))).astype(np.float32)
+    x[:6] = rng.integers(-3, 4, (6, cols))
+    x[6:10] = 1e-3 * x[6:10]
+    x[6:10, 3] = 60.0
+    x[10:14][rng.random((4, cols)) < 0.99] = -np.inf
+    x[14] = np.nan
+    x[15, 8:10] = np.inf
+    flat = torch.full((rows * (cols + 3) + 1,), 1e4, device=DEV)
+    logits = flat[1:].view(rows, cols + 3)[:, :cols]
+    logits.copy_(torch.from_numpy(x))
+    u = rng.random(rows).astype(np.float32)
+    t = np.where(np.arange(rows) // 2 == 3, 30.0, rng.choice([0.4, 1.0], rows))
+    check(pa, logits, u, t, rng.choice([0, 3, 50, 5000], rows), rng.choice([1.0, 0.8], rows),
+          rng.choice([0.0, 0.02], rows))
+    check(pa, logits, u, t)
+    # settings at their ends
+    h = x[20].astype(np.float64)
+    one = logits[20:21].expand(7, cols)
+    ts = [1e-30, 1e-3, 3e38, float("inf"), -1.0, float("nan"), 1e-45]
+    want = [sample_plain.draw(h, float(np.float32(0.37)), float(np.float32(v))) for v in ts]
+    assert list(run(pa, one, [0.37] * 7, ts)) == want
+    top, free = int(np.argmax(h)), sample_plain.draw(h, float(np.float32(0.73)))
+    ps = [0.0, -1.0, 1e-40, 1.0, 2.0, float("nan"), 1.5]
+    assert list(run(pa, one, [0.73] * 7, p=ps)) == [top] * 3 + [free] * 4
+
+
+def test_graphs_share_a_workspace(pa):
+    """Two captured draws, long rows and short ones, with one workspace, replayed in
+    turn over changing logits and numbers beside eager calls."""
+    rng = np.random.default_rng(8)
+    rows = 5
+    ws = torch.empty(pa.sample_workspace_size(rows), dtype=torch.uint8, device=DEV)
+    bufs, graphs = [], []
+    for cols in (30011, 700):
+        x, u = rows_of(rng, rows, cols, torch.bfloat16), dev(rng.random(rows), torch.float32)
+        opts = dict(temperature=dev([0.8] * rows, torch.float32),
+                    top_k=dev([0, 50, 3, 0, 999], torch.int32),
+                    top_p=dev([0.9, 0.9, 1.0, 1.0, 0.3], torch.float32))
+        pa.sample(x, u, workspace=ws, **opts)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = pa.sample(x, u, workspace=ws, **opts)
+        bufs.append((x, u, opts))
+        graphs.append((g, out))
+    for _ in range(4):
+        for (x, u, opts), (g, out) in zip(bufs, graphs):
+            x.copy_(rows_of(rng, *x.shape, x.dtype))
+            u.copy_(dev(rng.random(rows), torch.float32))
+            g.replay()
+            want = pa.sample(x, u, **opts)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)

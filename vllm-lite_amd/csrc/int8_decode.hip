@@ -5,8 +5,9 @@
 // merge through LDS.  Contexts of several parts leave a result for each in the
 // workspace, which a second launch merges.
 // Bound by memory: every code is read once, for all heads of its group: 64 x 4096 of
-// 32 / 8 heads of 128 87 us, 6.2 TB/s (two sets of registers a step, loaded together
-// ahead: 99).  Few sequences: by the loads' latency, 32 x 320-768 of 14 / 2 x 64 6.1 us.
+// 32 / 8 heads of 128 87 us, 6.2 TB/s (99 with a wavefront's steps side by side and
+// their ids behind the context length).  Few sequences: by the loads' latency, 32 x
+// 320-768 of 14 / 2 x 64 6.1 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -18,7 +18,9 @@
 //   4  sample_draw_kernel   the kept weight of every wavefront's run of tokens and, in
 //                           the row's last workgroup, the token
 // 2 and 3 only where the call gives top_k or top_p; rows that do not use them pass
-// through.  Each kernel reads the logits once, in workgroups of a slice of a row.
+// through.  Each kernel reads the logits once, in workgroups of a slice of a row.  Rows
+// of few tokens, and many rows, take all steps in one launch, a workgroup a row
+// (sample_row_kernel), with the same results.
 //
 // Bound by the launches and what each does once a row, one thing after the other, for
 // few rows: 1 x 151936 bf16 29 us, 32 rows 43; by f64 weights, formed twice, for many:
@@ -56,10 +58,12 @@ struct Row {
   Stats stats[kMaxSlices];
   unsigned long long mass[kBins];
   unsigned int count[kBins];
-  unsigned int list[kListMax];
   uint32_t cut;  // kept: the values above `cut` and the first `ties` at it
   unsigned long long ties;
   unsigned int listed, arrived[2];
+};
+struct RowSpace : Row {
+  uint32_t list[kListMax];
 };
 
 struct Args {
@@ -71,7 +75,7 @@ struct Args {
   const int32_t* top_k;
   const float* top_p;
   const float* min_p;
-  Row* rows;
+  RowSpace* rows;
   Part* parts;  // of (row, slice, wavefront)
   int cols, slices;
   int shift;  // weights in units of 2^-shift, at most 51
@@ -191,10 +195,10 @@ __device__ inline uint32_t wave_join(uint32_t v, uint32_t none, F f) {
 
 // The row's settings and, from its slices, extremes: formed by the first wavefront (a
 // CU's wavefronts share its issue slots), for all behind the next barrier.
-__device__ inline void prepare(const Args& a, int row, Settings& to) {
+__device__ inline void prepare(const Args& a, int row, const Row& r, Settings& to) {
   if (threadIdx.x >= 64) return;
   Settings s = settings_of(a, row);
-  const Stats& mine = a.rows[row].stats[min((int)threadIdx.x, a.slices - 1)];
+  const Stats& mine = r.stats[min((int)threadIdx.x, a.slices - 1)];
   auto f32 = [](uint32_t v) { return __builtin_bit_cast(float, v); };
   auto u32 = [](float v) { return __builtin_bit_cast(uint32_t, v); };
   s.max = f32(wave_join(u32(mine.max), u32(-INFINITY), [&](uint32_t v, uint32_t w) {
@@ -422,10 +426,10 @@ __device__ inline unsigned long long share_down(float f, unsigned long long w) {
   return (unsigned long long)(((unsigned __int128)m * w) >> down);
 }
 
+// Step 1 for a slice.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
-  Row& r = a.rows[row];
+__device__ inline void max_of_slice(const Args& a, int row, int slice, Row& r) {
+  const int wave = threadIdx.x >> 6;
   Run<T> run(a, row, slice * kWaves + wave);
   // what the next kernels add to
   if (a.top_k || a.top_p) {
@@ -465,7 +469,27 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
     r.stats[slice] = Stats{mx, mn, at, 0};
   }
 }
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(const Args a) {
+  max_of_slice<T>(a, blockIdx.y, blockIdx.x, a.rows[blockIdx.y]);
+}
 
+// Step 2 for a slice, into arrays in LDS (cleared; a barrier behind).
+template <typename T>
+__device__ inline void hist_of_slice(const Args& a, const Settings& s, Run<T>& run,
+                                     unsigned long long* mass, unsigned int* count,
+                                     const double* pow16) {
+  run.each([&](const auto& x, int) {
+#pragma unroll
+    for (int i = 0; i < Chunks<T>::E; ++i) {
+      const int b = bin_of(x[i], s);
+      if (b < 0) continue;
+      if (s.by_k) atomicAdd(&count[b], 1u);
+      if (s.by_p) atomicAdd(&mass[b], weight_of(x[i], s, a.shift, pow16));
+    }
+  });
+  __syncthreads();
+}
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
   const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
@@ -480,20 +504,11 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(const Args a) {
     count[b] = 0;
   }
   if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  prepare(a, row, settings);
+  prepare(a, row, r, settings);
   __syncthreads();
   const Settings s = settings;
   if (!s.narrows()) return;
-  run.each([&](const auto& x, int) {
-#pragma unroll
-    for (int i = 0; i < Chunks<T>::E; ++i) {
-      const int b = bin_of(x[i], s);
-      if (b < 0) continue;
-      if (s.by_k) atomicAdd(&count[b], 1u);
-      if (s.by_p) atomicAdd(&mass[b], weight_of(x[i], s, a.shift, pow16));
-    }
-  });
-  __syncthreads();
+  hist_of_slice<T>(a, s, run, mass, count, pow16);
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     if (count[b]) atomicAdd(&r.count[b], count[b]);
     if (mass[b]) atomicAdd(&r.mass[b], mass[b]);
@@ -569,27 +584,23 @@ __device__ inline uint32_t select(Each each, Weight weight, unsigned long long& 
   return found;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void
-sample_pick_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
-  __shared__ Settings settings;
-  __shared__ double pow16[16];
-  __shared__ uint32_t list[kListMax];
-  __shared__ unsigned int n, at, last;
+// Step 3 for a slice and, in the row's last workgroup, for the row.  WHOLE: the slice is
+// the row, its Row is in LDS.
+struct Pick {
+  uint32_t list[kListMax];
+  unsigned int n, at, last;
   // Top-k's threshold is in interval kb (kBins: none, fewer values than k): `above`
   // values and the weight `least` come before it.  Top-p's is in one of lo to hi; in
   // pb, `before` it, where that is one for all that top-k may leave (else kBins).
-  __shared__ int kb, lo, hi, pb;
-  __shared__ unsigned long long above, least, before;
-  __shared__ Select l;
-  Row& r = a.rows[row];
-  Run<T> run(a, row, slice * kWaves + wave);
-  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  prepare(a, row, settings);
-  __syncthreads();
-  const Settings s = settings;
-  if (!s.narrows()) return;
+  int kb, lo, hi, pb;
+  unsigned long long above, least, before;
+  Select l;
+};
+template <typename T, bool WHOLE>
+__device__ inline void pick_of_slice(const Args& a, const Settings& s, Run<T>& run, Row& r,
+                                     uint32_t* row_list, const double* pow16, Pick& sh) {
+  const int wave = threadIdx.x >> 6;
+  uint32_t* list = sh.list;
   if (wave == 0) {
     Cross k{kBins, 0}, p{kBins, 0};
     if (s.by_k) k = Entries<unsigned int>(r.count).cross((unsigned long long)s.k);
@@ -605,46 +616,49 @@ sample_pick_kernel(const Args a) {
       p1 = k.at == kBins ? p0 : min(m.cross(share_up(s.p, m.upto(k.at, true))).at, k.at);
     }
     if (threadIdx.x == 0) {
-      n = 0;
-      kb = k.at;
-      above = k.before;
-      least = w;
-      lo = p0;
-      hi = p1;
-      pb = p0 == p1 && p.at == p0 ? p0 : kBins;
-      before = p.before;
+      sh.n = 0;
+      sh.kb = k.at;
+      sh.above = k.before;
+      sh.least = w;
+      sh.lo = p0;
+      sh.hi = p1;
+      sh.pb = p0 == p1 && p.at == p0 ? p0 : kBins;
+      sh.before = p.before;
     }
   }
   __syncthreads();
+  const int kb = sh.kb;
   {
-    const int b0 = kb, b1 = lo, b2 = hi;
+    const int b0 = kb, b1 = sh.lo, b2 = sh.hi;
     run.each([&](const auto& x, int) {
 #pragma unroll
       for (int i = 0; i < Chunks<T>::E; ++i) {
         const int b = bin_of(x[i], s);
         if (b >= 0 && (b == b0 || (b >= b1 && b <= b2))) {
-          const unsigned int to = atomicAdd(&n, 1u);
+          const unsigned int to = atomicAdd(&sh.n, 1u);
           if (to < kListMax) list[to] = key_of(x[i]);
         }
       }
     });
   }
   __syncthreads();
-  unsigned int listed = n;
-  if (a.slices > 1) {
-    if (threadIdx.x == 0 && n > 0) at = atomicAdd(&r.listed, n);
+  unsigned int listed = sh.n;
+  if constexpr (!WHOLE) {
+    const unsigned int n = listed;
+    if (threadIdx.x == 0 && n > 0) sh.at = atomicAdd(&r.listed, n);
     __syncthreads();
+    const unsigned int at = sh.at;
     if (n > 0 && at < kListMax) {
       const unsigned int room = min(n, kListMax - at);
-      for (unsigned int i = threadIdx.x; i < room; i += kThreads) put(&r.list[at + i], list[i]);
+      for (unsigned int i = threadIdx.x; i < room; i += kThreads) put(&row_list[at + i], list[i]);
     }
     const bool is_last = last_of_row(&r.arrived[0], a.slices);
-    if (threadIdx.x == 0) last = is_last;
+    if (threadIdx.x == 0) sh.last = is_last;
     __syncthreads();
-    if (!last) return;
+    if (!sh.last) return;
     listed = get(&r.listed);
     if (listed <= kListMax)
-      for (unsigned int i = threadIdx.x; i < listed; i += kThreads) list[i] = get(&r.list[i]);
+      for (unsigned int i = threadIdx.x; i < listed; i += kThreads) list[i] = get(&row_list[i]);
     __syncthreads();
   }
   // the values of interval b, from the list or, where that overflowed, the row
@@ -665,23 +679,23 @@ sample_pick_kernel(const Args a) {
     auto weight = [&](uint32_t key) {
       return by_p ? weight_of(value_of(key), s, a.shift, pow16) : 1ull;
     };
-    Cross c{kb, above};
+    Cross c{kb, sh.above};
     unsigned long long want = (unsigned long long)s.k;
     if (by_p) {
-      unsigned long long total = least;
+      unsigned long long total = sh.least;
       if (kb < kBins) {
         unsigned long long more = 0;
         values(kb)([&](uint32_t key) {
           if (key > cut) more += weight(key);
         });
-        total += sum_of(more, l.red) + ties * weight(cut);
+        total += sum_of(more, sh.l.red) + ties * weight(cut);
       }
       want = share_up(s.p, total);
-      c = Cross{pb, before};
+      c = Cross{sh.pb, sh.before};
       if (c.at == kBins) c = Entries<unsigned long long>(r.mass).cross(want);
     }
     want -= c.before;
-    cut = select(values(c.at), weight, want, l);
+    cut = select(values(c.at), weight, want, sh.l);
     // as many as reach it: want / weight, rounded up (below 2^23: the quotient in f64
     // is off by one at most)
     const unsigned long long w = max(weight(cut), 1ull);
@@ -697,17 +711,26 @@ sample_pick_kernel(const Args a) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void
-sample_draw_kernel(const Args a) {
-  const int row = blockIdx.y, slice = blockIdx.x, lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+sample_pick_kernel(const Args a) {
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
   __shared__ Settings settings;
-  Row& r = a.rows[row];
   __shared__ double pow16[16];
+  __shared__ Pick sh;
+  RowSpace& r = a.rows[row];
   Run<T> run(a, row, slice * kWaves + wave);
   if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
-  prepare(a, row, settings);
+  prepare(a, row, r, settings);
   __syncthreads();
   const Settings s = settings;
+  if (s.narrows()) pick_of_slice<T, false>(a, s, run, r, r.list, pow16, sh);
+}
+
+// Step 4 for a slice and, in the row's last workgroup, for the row.
+template <typename T, bool WHOLE>
+__device__ inline void draw_of_slice(const Args& a, int row, int slice, const Settings& s,
+                                     Run<T>& run, Row& r, Part* parts, const double* pow16) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (s.greedy || s.max == -INFINITY) {
     // the first largest; 0 where nothing is above -inf
     if (slice == 0 && threadIdx.x == 0) {
@@ -733,12 +756,17 @@ sample_draw_kernel(const Args a) {
   });
   mass = wave_sum(mass);
   equal = wave_sum(equal);
-  Part* parts = a.parts + (int64_t)row * a.slices * kWaves;
-  if (lane == 0) {
-    put(&parts[slice * kWaves + wave].mass, mass);
-    put(&parts[slice * kWaves + wave].ties, equal);
+  if constexpr (WHOLE) {
+    if (lane == 0) parts[wave] = Part{mass, equal, 0};
+    __syncthreads();
+    if (wave != 0) return;
+  } else {
+    if (lane == 0) {
+      put(&parts[slice * kWaves + wave].mass, mass);
+      put(&parts[slice * kWaves + wave].ties, equal);
+    }
+    if (!last_of_row(&r.arrived[1], a.slices)) return;
   }
-  if (!last_of_row(&r.arrived[1], a.slices)) return;
   // The row's last workgroup has every part; its first wavefront draws.
   const unsigned long long even = cut ? kept_weight(value_of(cut), s, a.shift, pow16) : 0;
   // of n tokens at the threshold with `before` of them in front, the weight of those kept
@@ -752,8 +780,8 @@ sample_draw_kernel(const Args a) {
   for (int i = 0; i < kLaneParts; ++i) {
     const int at = lane * each + i;
     const bool there = i < each && at < count;
-    m[i] = there ? get(&parts[at].mass) : 0;
-    n_eq[i] = there ? get(&parts[at].ties) : 0;
+    m[i] = !there ? 0 : WHOLE ? parts[at].mass : get(&parts[at].mass);
+    n_eq[i] = !there ? 0 : WHOLE ? parts[at].ties : get(&parts[at].ties);
   }
 #pragma unroll
   for (int i = 0; i < kLaneParts; ++i) eq += n_eq[i];
@@ -830,11 +858,58 @@ sample_draw_kernel(const Args a) {
   }
 }
 
-// Slices of a row: workgroups of 512 threads, four a CU, a chunk a thread or more.
+template <typename T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void
+sample_draw_kernel(const Args a) {
+  const int row = blockIdx.y, slice = blockIdx.x, wave = threadIdx.x >> 6;
+  __shared__ Settings settings;
+  __shared__ double pow16[16];
+  Row& r = a.rows[row];
+  Run<T> run(a, row, slice * kWaves + wave);
+  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
+  prepare(a, row, r, settings);
+  __syncthreads();
+  draw_of_slice<T, false>(a, row, slice, settings, run, r,
+                          a.parts + (int64_t)row * a.slices * kWaves, pow16);
+}
+
+// All steps for a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void
+sample_row_kernel(const Args a) {
+  const int row = blockIdx.x, wave = threadIdx.x >> 6;
+  __shared__ Row r;
+  __shared__ Settings settings;
+  __shared__ double pow16[16];
+  __shared__ Pick sh;
+  __shared__ Part parts[kWaves];
+  if (threadIdx.x < 16) pow16[threadIdx.x] = kPow[threadIdx.x];
+  max_of_slice<T>(a, row, 0, r);
+  __syncthreads();
+  prepare(a, row, r, settings);
+  __syncthreads();
+  const Settings s = settings;
+  if (s.narrows()) {
+    Run<T> run(a, row, wave);
+    hist_of_slice<T>(a, s, run, r.mass, r.count, pow16);
+    Run<T> again(a, row, wave);
+    pick_of_slice<T, true>(a, s, again, r, nullptr, pow16, sh);
+    __syncthreads();
+  }
+  Run<T> run(a, row, wave);
+  draw_of_slice<T, true>(a, row, 0, s, run, r, parts, pow16);
+}
+
+// Slices of a row: workgroups of 512 threads, four a CU, a chunk a thread or more.  One,
+// and so one launch, where the row is short: us in four launches and in one, 32 rows of
+// 4096 28 / 18 bf16 and 27 / 21 f32, 1 x 8192 24.4 / 22.4 and 22.8 / 23.8, 32 x 8192 30 /
+// 25.6 and 28.7 / 28.2, 253 x 8192 36 / 27 and 37 / 30, but 32 x 16384 30 / 35; and where
+// two would be the most: 512 x 50257 128 / 122 and 134 / 125 (400 rows: 111 / 120).
 int most_slices(int rows) {
   return std::max(1, std::min(kMaxSlices, kWorkgroups / std::max(rows, 1)));
 }
-int slices_of(int rows, int chunks) {
+int slices_of(int rows, int cols, int chunks) {
+  if (cols <= 8192 || most_slices(rows) <= 2) return 1;
   return std::max(1, std::min(most_slices(rows), (chunks + kThreads - 1) / kThreads));
 }
 
@@ -844,7 +919,7 @@ int slices_of(int rows, int chunks) {
 using namespace pa;
 
 extern "C" size_t pa_sample_workspace_size(int32_t rows) {
-  return rows > 0 ? (size_t)rows * (sizeof(Row) + most_slices(rows) * kWaves * sizeof(Part)) : 0;
+  return rows > 0 ? (size_t)rows * (sizeof(RowSpace) + most_slices(rows) * kWaves * sizeof(Part)) : 0;
 }
 
 extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* uniform,
@@ -869,16 +944,23 @@ extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* unif
              PA_ERR_WORKSPACE, "pa_sample: workspace of %zu bytes (16-byte aligned) needed, %zu given",
              need, workspace ? workspace_bytes : 0);
   const int chunks = (int)(((int64_t)cols * es + 15) / 16) + 1;
-  const int slices = slices_of(rows, chunks);
+  const int slices = slices_of(rows, cols, chunks);
   int bits = 1;
   while ((1 << bits) < cols) ++bits;
-  const Args a{out, logits, row_stride, uniform, temperature, top_k, top_p, min_p, (Row*)workspace,
-               (Part*)((Row*)workspace + rows), cols, slices, std::min(62 - bits, 51)};
+  const Args a{out, logits, row_stride, uniform, temperature, top_k, top_p, min_p, (RowSpace*)workspace,
+               (Part*)((RowSpace*)workspace + rows), cols, slices, std::min(62 - bits, 51)};
   const dim3 grid(slices, rows);
   hipStream_t s = (hipStream_t)stream;
 #define PA_LAUNCH_SAMPLE(KERNEL)                                                   \
   (dtype == PA_DTYPE_BF16 ? KERNEL<uint16_t><<<grid, kThreads, 0, s>>>(a)          \
                           : KERNEL<float><<<grid, kThreads, 0, s>>>(a))
+  if (slices == 1) {
+    if (dtype == PA_DTYPE_BF16)
+      sample_row_kernel<uint16_t><<<rows, kThreads, 0, s>>>(a);
+    else
+      sample_row_kernel<float><<<rows, kThreads, 0, s>>>(a);
+    return check_launch("pa_sample");
+  }
   PA_LAUNCH_SAMPLE(sample_max_kernel);
   if (top_k || top_p) {
     PA_LAUNCH_SAMPLE(sample_hist_kernel);

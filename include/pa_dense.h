@@ -278,7 +278,7 @@ int32_t pa_sample(int64_t* out, const void* logits, const float* uniform,
                   const float* min_p, int32_t rows, int32_t cols, int64_t row_stride,
                   void* workspace, size_t workspace_bytes, int32_t dtype, pa_stream_t stream);
 
-/* Workspace bytes of pa_sample. */
+/* Workspace bytes of pa_sample (0, and workspace may be NULL, from 512 rows on). */
 size_t pa_sample_workspace_size(int32_t rows);
 
 #ifdef __cplusplus

@@ -38,6 +38,8 @@ def test_workspace_size(lib):
     size = lib.pa_sample_workspace_size
     assert size(0) == 0 and size(-3) == 0 and size(1) > 0 and size(7) == 7 * size(1)
     assert call(lib, rows=3, wsb=size(3) - 1) == -4
+    # many rows take a workgroup each
+    assert size(511) > 0 and size(512) == size(65535) == 0
 
 
 def test_wrapper_refuses_host_tensors(pa):

@@ -903,13 +903,14 @@ sample_row_kernel(const Args a) {
 // Slices of a row: workgroups of 512 threads, four a CU, a chunk a thread or more.  One,
 // and so one launch, where the row is short: us in four launches and in one, 32 rows of
 // 4096 28 / 18 bf16 and 27 / 21 f32, 1 x 8192 24.4 / 22.4 and 22.8 / 23.8, 32 x 8192 30 /
-// 25.6 and 28.7 / 28.2, 253 x 8192 36 / 27 and 37 / 30, but 32 x 16384 30 / 35; and where
-// two would be the most: 512 x 50257 128 / 122 and 134 / 125 (400 rows: 111 / 120).
+// 25.6 and 28.7 / 28.2, 253 x 8192 36 / 27 and 37 / 30, but 32 x 16384 30 / 35; and for
+// many rows: 512 x 50257 128 / 122 and 134 / 125, 400 x 50257 111 / 120.
+constexpr int kManyRows = 512;
 int most_slices(int rows) {
   return std::max(1, std::min(kMaxSlices, kWorkgroups / std::max(rows, 1)));
 }
 int slices_of(int rows, int cols, int chunks) {
-  if (cols <= 8192 || most_slices(rows) <= 2) return 1;
+  if (cols <= 8192 || rows >= kManyRows) return 1;
   return std::max(1, std::min(most_slices(rows), (chunks + kThreads - 1) / kThreads));
 }
 
@@ -919,7 +920,8 @@ int slices_of(int rows, int cols, int chunks) {
 using namespace pa;
 
 extern "C" size_t pa_sample_workspace_size(int32_t rows) {
-  return rows > 0 ? (size_t)rows * (sizeof(RowSpace) + most_slices(rows) * kWaves * sizeof(Part)) : 0;
+  if (rows <= 0 || rows >= kManyRows) return 0;  // (many: a workgroup a row)
+  return (size_t)rows * (sizeof(RowSpace) + most_slices(rows) * kWaves * sizeof(Part));
 }
 
 extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* uniform,
@@ -940,7 +942,7 @@ extern "C" int32_t pa_sample(int64_t* out, const void* logits, const float* unif
   const int es = dtype == PA_DTYPE_BF16 ? 2 : 4;
   PA_REQUIRE((uintptr_t)logits % es == 0, PA_ERR_INVALID_ARG, "pa_sample: logits not aligned");
   const size_t need = pa_sample_workspace_size(rows);
-  PA_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
+  PA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
              PA_ERR_WORKSPACE, "pa_sample: workspace of %zu bytes (16-byte aligned) needed, %zu given",
              need, workspace ? workspace_bytes : 0);
   const int chunks = (int)(((int64_t)cols * es + 15) / 16) + 1;

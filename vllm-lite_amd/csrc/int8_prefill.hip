@@ -83,8 +83,7 @@ prefill_int8_kernel(const PrefillArgs a) {
   constexpr int KT = key_tile<D>(), NB = KT / kBlock;
   constexpr int SPT = KT / 32 / KG;  // a wavefront's steps a tile
   static_assert(SPT >= 1, "a step for every group of wavefronts");
-  // EARLY: operands are read ahead (K two steps, V one), where the tiles are there and
-  // the registers too.
+  // EARLY: K's operands are read two steps ahead, where the tile is there.
   constexpr bool EARLY = SPT == 2;
   constexpr int NBUF = 3;  // operand buffers; tile kt + 2 is written during tile kt
   constexpr int ROWS = 16 * NT * (W / KG);
@@ -216,31 +215,37 @@ prefill_int8_kernel(const PrefillArgs a) {
     const int r0 = tile * ROWS + wt * 16 * NT;  // first row of this wavefront
     const bool active = r0 < rows;
 
-    // ---- the blocks' ids and scales: lane t holds those of block t of a group of GT
+    // ---- the blocks' places and scales: lane t holds those of block t of a group of GT
     // tiles.  Blocks behind the last and ids outside the pool read block 0.
+    const float scale = fabsf(a.scale_log2);
     auto load_ids = [&](int group) -> int32_t {
       return tab[min(group * 64 + lane, nblk - 1)];
     };
-    auto in_pool = [&](int32_t id) -> int32_t { return id >= 0 && id < a.num_blocks ? id : 0; };
-    int32_t ids = in_pool(load_ids(0)), ids_next = load_ids(1);  // of the tiles copied
-    uint32_t ksc, vsc, ksc_next, vsc_next;                       // of the tiles computed
-    {
-      const uint32_t s = (uint32_t)ids * (uint32_t)Hkv + kvh;
-      ksc = a.ks[s];
-      vsc = a.vs[s];
-      ksc_next = ksc;
-      vsc_next = vsc;
-    }
+    auto place_of = [&](int32_t id) -> uint32_t {
+      return (uint32_t)(id >= 0 && id < a.num_blocks ? id : 0) * (uint32_t)Hkv + kvh;
+    };
+    uint32_t places = place_of(load_ids(0));  // of the tiles copied
+    int32_t ids_next = load_ids(1);
+    // K's scale bytes, V's << 8, of the next group
+    uint32_t bytes_next = (uint32_t)a.ks[places] | (uint32_t)a.vs[places] << 8;
+    // of the tiles computed: the scores' factor, and 2^-e twice in bf16, e being the V
+    // scale's exponent (0 for a byte that no scale is, in blocks never written)
+    float factors;
+    uint32_t units;
+    auto next_scales = [&]() {
+      factors = scale * scale_of(bytes_next & 255);
+      const uint32_t v = bytes_next >> 8;
+      units = (v == 0 || v > 253 ? 127 : 254 - v) * 0x00800080u;
+    };
+    next_scales();
     // ---- staging: wavefront w copies and writes pieces 64 (w + n W) + lane.  Piece
     // i < KT D / 16 is chunk i % (D / 16) of key i / (D / 16); the others are dim i' % D
     // of block i' / D.
     auto copy_tile = [&](int kt) {
       if (kt % GT == 0 && kt > 0) {
-        ids = in_pool(ids_next);
+        places = place_of(ids_next);
         ids_next = load_ids(kt / GT + 1);
-        const uint32_t s = (uint32_t)ids * (uint32_t)Hkv + kvh;
-        ksc_next = a.ks[s];
-        vsc_next = a.vs[s];
+        bytes_next = (uint32_t)a.ks[places] | (uint32_t)a.vs[places] << 8;
       }
 #pragma unroll
       for (int n = 0; n < PPT; ++n) {
@@ -248,9 +253,9 @@ prefill_int8_kernel(const PrefillArgs a) {
         if (CHUNKS % W != 0 && ch >= CHUNKS) continue;
         const bool is_k = ch < CHUNKS / 2;
         const int i = (is_k ? ch : ch - CHUNKS / 2) * 64 + lane;
-        const uint32_t id = __shfl(ids, kt % GT * NB + i / D, 64);
-        const uint64_t off =
-            (uint64_t)(id * (uint32_t)Hkv + kvh) * (kBlock * D) + (uint32_t)(i % D) * 16;
+        const uint64_t off = (uint64_t)(uint32_t)__shfl((int)places, kt % GT * NB + i / D, 64) *
+                                 (kBlock * D) +
+                             (uint32_t)(i % D) * 16;
         const uint32_t to = (uint32_t)(uintptr_t)(
             __attribute__((address_space(3))) uint8_t*)&stage[kt & 1][ch * 1024];
         lds_copy16((const uint8_t*)(is_k ? a.kc : a.vc), off,
@@ -332,10 +337,11 @@ prefill_int8_kernel(const PrefillArgs a) {
     const bool bad_ids = __syncthreads_or(bad) != 0;
     f32x4 o[NT][DT];
     f32x4 lacc[NT];  // denominators
-    float nm[NT];    // minus the rows' maxima; INFINITY: none yet
+    float nm[NT];    // minus the rows' maxima; kNone: none yet
+    constexpr float kNone = 3.0e38f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      nm[nt] = INFINITY;
+      nm[nt] = kNone;
       lacc[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[nt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -378,12 +384,8 @@ prefill_int8_kernel(const PrefillArgs a) {
     auto next_buf = [](int buf, int n) -> int { return buf + n >= NBUF ? buf + n - NBUF : buf + n; };
     qk_load(0, kgrp);
     scores();
-    if constexpr (EARLY) {
-      qk_load(0, 1);
-      v_load(0, 0);
-    }
+    if constexpr (EARLY) qk_load(0, 1);
     const int last_pos = past + (min(rows, r0 + 16 * NT) - 1) / G;  // of this wavefront's rows
-    const float scale = fabsf(a.scale_log2);
 
     // During tile kt: this wavefront's share of the tile two on, and the copies of the
     // one four on.
@@ -401,28 +403,17 @@ prefill_int8_kernel(const PrefillArgs a) {
       const int kb = kt * KT + st * 32;
       const bool live = active && kb <= last_pos;
       if (FIRST && kt > 0) {
-        if (kt % GT == 0) {
-          ksc = ksc_next;
-          vsc = vsc_next;
-        }
+        if (kt % GT == 0) next_scales();
         barrier();
       }
       if (live) {
-        if constexpr (!EARLY) {
-          qk_load(next_buf(buf, 1), kgrp);
-          v_load(buf, st);
-        }
-        // the scales of the lane's block: a K scale of 2^(byte - 127); the V scale's
-        // exponent (0 for a byte that no scale is, in blocks never written)
-        const int at = kt % GT * NB + 2 * st;
-        const uint32_t k0 = __builtin_amdgcn_readlane(ksc, at),
-                       k1 = __builtin_amdgcn_readlane(ksc, at + 1),
-                       v0 = __builtin_amdgcn_readlane(vsc, at),
-                       v1 = __builtin_amdgcn_readlane(vsc, at + 1);
-        const uint32_t vb = j & 2 ? v1 : v0;
-        float f = scale * scale_of(j & 2 ? k1 : k0);
-        const int e = vb == 0 || vb > 253 ? 0 : (int)vb - 127;
-        const uint32_t one = (uint32_t)(127 - e) * 0x00800080u;
+        if constexpr (!EARLY) qk_load(next_buf(buf, 1), kgrp);
+        // the scales of the lane's block
+        const int at = 4 * (kt % GT * NB + 2 * st) + 4 * (j >> 1);
+        float f = __builtin_bit_cast(
+            float, __builtin_amdgcn_ds_bpermute(at, __builtin_bit_cast(int, factors)));
+        const uint32_t one = __builtin_amdgcn_ds_bpermute(at, (int)units);
+        const float e = (float)(127 - (int)(one >> 23));
         const bool tail = kt * KT + KT > key_end || bad_ids;
         if (tail || kb + 31 > past + r0 / G) {
           // keys behind the last, in blocks outside the pool or above a row's diagonal
@@ -449,8 +440,7 @@ prefill_int8_kernel(const PrefillArgs a) {
           const float m0 = max3(S[nt][0][0], S[nt][0][1], S[nt][0][2]);
           const float m1 = max3(S[nt][0][3], S[nt][1][0], S[nt][1][1]);
           lm[nt] = max3(m0, m1, max3(S[nt][1][2], S[nt][1][3], S[nt][1][3])) * f;
-          // (a row without keys so far has nm = inf: any score passes, and -inf + inf
-          // does not)
+          // (a row without keys so far: any score passes, and -inf + kNone does not)
           need |= lm[nt] + nm[nt] > 8.0f;
         }
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(need) != 0, 0)) {
@@ -459,7 +449,7 @@ prefill_int8_kernel(const PrefillArgs a) {
             float top = fmaxf(lm[nt], -nm[nt]);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float r = nm[nt] == INFINITY ? 1.f : __builtin_amdgcn_exp2f(-nm[nt] - top);
+            const float r = __builtin_amdgcn_exp2f(-nm[nt] - top);
             nm[nt] = -top;
             lacc[nt] *= r;
 #pragma unroll
@@ -468,7 +458,7 @@ prefill_int8_kernel(const PrefillArgs a) {
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float shift = (nm[nt] == INFINITY ? 0.f : nm[nt]) + (float)e;
+          const float shift = nm[nt] + e;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             pb[nt][i] = (__bf16)__builtin_amdgcn_exp2f(
@@ -478,8 +468,11 @@ prefill_int8_kernel(const PrefillArgs a) {
         // runs meanwhile: 347 us where 371 at the step's end, 397 behind the scores and
         // 293 without the writes (4 x 1024-2048 tokens on 0-4096, 32 / 8 heads of 128)
         if constexpr (FIRST) prepare(kt, buf);
-        __builtin_amdgcn_s_setprio(1);
         scores();
+        // (where K's operands are of no use any more: with both at once, head_dim 256
+        // keeps 68 registers in scratch and takes 149 us for 90, 128 keeps 12 and 368
+        // for 357)
+        v_load(buf, st);
         // (past the last tile what is read here is never used)
         if constexpr (EARLY) qk_load(next_buf(buf, 1), st);
 #pragma unroll
@@ -493,9 +486,7 @@ prefill_int8_kernel(const PrefillArgs a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           lacc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[nt], lacc[nt], 0, 0, 0);
-        if constexpr (EARLY) v_load(FIRST ? buf : next_buf(buf, 1), 1 - st);
       }
-      __builtin_amdgcn_s_setprio(0);
       if (FIRST && !live) prepare(kt, buf);
     };
 
@@ -506,7 +497,7 @@ prefill_int8_kernel(const PrefillArgs a) {
 
     if constexpr (KG == 2) {
       // The two groups' results, in the tiles' space.  A group that saw no key of a
-      // row (nm = inf) drops out.
+      // row (nm = kNone) drops out.
       static_assert(W / 2 * NT * (DT * 1024 + 512) <= (int)sizeof(Tiles), "space");
       float* mo = reinterpret_cast<float*>(&lds);
       float* mml = mo + W / 2 * NT * DT * 256;
@@ -528,8 +519,7 @@ prefill_int8_kernel(const PrefillArgs a) {
       for (int nt = 0; nt < NT; ++nt) {
         const float2 ml = *reinterpret_cast<const float2*>(mml + ((wt * NT + nt) * 64 + lane) * 2);
         const float m = -nm[nt], mx = fmaxf(m, ml.x);
-        const float fa = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-        const float fb = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+        const float fa = __builtin_amdgcn_exp2f(m - mx), fb = __builtin_amdgcn_exp2f(ml.x - mx);
         // (a row of NaN has no maximum, but sums of NaN)
         lacc[nt][0] = lacc[nt][0] * fa + ml.y * fb;
 #pragma unroll

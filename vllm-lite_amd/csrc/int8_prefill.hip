@@ -15,8 +15,8 @@
 //     same probabilities (as rounded) by 2^-exponent, exact.
 // The maximum is kept until a score passes it by 2^8.
 // Bound by vector instructions (softmax, conversions) beside the products: 4 x
-// 1055-2048 on 360-4096, 32 / 8 heads of 128, 370 us, 800 TFLOP/s; without the writes
-// of operands 320, and a bf16 cache's kernel, which has no conversions, 307.
+// 1055-2048 on 360-4096, 32 / 8 heads of 128, 360 us, 825 TFLOP/s; without the writes
+// of operands 305, and a bf16 cache's kernel, which has no conversions, 306.
 // KG = 2: half the wavefronts take the first 32 keys of each tile, half the second,
 // for launches of few rows; their results meet in LDS.
 #include <algorithm>
@@ -465,8 +465,8 @@ prefill_int8_kernel(const PrefillArgs a) {
                 __builtin_fmaf(S[nt][i >> 2][i & 3], f, shift));
         }
         // between the softmax and the products, which the other wavefront of this SIMD
-        // runs meanwhile: 347 us where 371 at the step's end, 397 behind the scores and
-        // 293 without the writes (4 x 1024-2048 tokens on 0-4096, 32 / 8 heads of 128)
+        // runs meanwhile (4 x 1100-2048 tokens on 100-4096, 32 / 8 heads of 128: 24 us
+        // less than at the step's end, 50 less than behind the scores)
         if constexpr (FIRST) prepare(kt, buf);
         scores();
         // (where K's operands are of no use any more: with both at once, head_dim 256

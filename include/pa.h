@@ -352,7 +352,8 @@ int32_t pa_prefill_quantized(void* out, const void* q, const float* k_cache, con
  * No counterpart in the reference, whose quantised cache keeps int8 values in f32
  * with one scale for a block's K, V and heads (pa_kv_cache_create_quantized).
  * q and out are bf16, head_dim is 32, 64, 96, 128, 192 or 256
- * (PA_ERR_UNSUPPORTED for others), code arrays are 16-byte aligned. */
+ * (PA_ERR_UNSUPPORTED for others), code arrays are 16-byte aligned, q 4-byte and out
+ * 8-byte (torch's tensors are, and their rows). */
 
 /* Appends tokens to their sequences' blocks.  Sequence s owns rows
  * cu_seq_tokens[s] .. cu_seq_tokens[s + 1] - 1 (n of them) and has

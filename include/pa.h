@@ -406,7 +406,8 @@ size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  * largest value, probabilities times the V scale are rounded to bf16, sums are f32.
  * A query row with a NaN or an infinity gives NaN.  Where V's scale bytes are below
  * 16 or above 240, probabilities times the scale may leave bf16's range: small
- * values come out as 0, large ones as infinities or NaN. */
+ * values come out as 0 (their keys count in the denominator all the same), large ones
+ * as infinities or NaN. */
 int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
                        const uint8_t* k_scales, const uint8_t* v_scales,
                        const int32_t* block_tables, int32_t max_blocks_per_seq,
@@ -416,7 +417,8 @@ int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const in
                        pa_stream_t stream);
 
 /* pa_prefill over an int8 cache, arguments and conventions as there, arithmetic as
- * pa_decode_int8, but with q as it is. */
+ * pa_decode_int8, but with q as it is, and without its loss of V's values under small
+ * scale bytes. */
 int32_t pa_prefill_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
                         const uint8_t* k_scales, const uint8_t* v_scales,
                         const int32_t* block_tables, int32_t max_blocks_per_seq,

@@ -11,8 +11,9 @@
 //     softmax's and the block's scale and the row's running maximum are one
 //     multiply-add of a score.
 //   Oᵀ += Vᵀ·Pᵀ, codes by probabilities that carry the V scale: its exponent goes
-//     into the exponential's argument.  The denominators are one more product, of the
-//     same probabilities (as rounded) by 2^-exponent, exact.
+//     into the exponential's argument (what is below 2^-32 of it into the operands,
+//     once they are written).  The denominators are one more product, of the same
+//     probabilities (as rounded) by 2^-exponent, exact.
 // The maximum is kept until a score passes it by 2^8.
 // Bound by vector instructions (softmax, conversions) beside the products: 4 x
 // 1055-2048 on 360-4096, 32 / 8 heads of 128, 360 us, 825 TFLOP/s; without the writes
@@ -65,6 +66,12 @@ struct PrefillArgs {
   float scale_log2;
 };
 
+// The least exponent of a V scale that the probabilities carry.  They are bf16 and the
+// denominators are theirs, so a weight below 2^(-126 - e) of the row's largest is lost:
+// with all of e (-126 in a block of zeros) every weight below 1.  What is below goes
+// into the values, which stay normal numbers (2^-126 is the least scale).
+constexpr int kLeast = -32;
+
 template <int D>
 constexpr int key_tile() {  // keys a tile: three buffers of K and V fit LDS
   return D <= 128 ? 64 : 32;
@@ -106,6 +113,7 @@ prefill_int8_kernel(const PrefillArgs a) {
   __shared__ int rank_seq[kMaxSeqs], rank_begin[kMaxSeqs], rank_len[kMaxSeqs],
       rank_past[kMaxSeqs], rank_tile0[kMaxSeqs], rank_of[kMaxSeqs], tile0_of[kMaxSeqs];
   __shared__ int tiles_in_all;
+  __shared__ float rest_of[64];  // see apply_rest
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -229,13 +237,16 @@ prefill_int8_kernel(const PrefillArgs a) {
     // K's scale bytes, V's << 8, of the next group
     uint32_t bytes_next = (uint32_t)a.ks[places] | (uint32_t)a.vs[places] << 8;
     // of the tiles computed: the scores' factor, and 2^-e twice in bf16, e being the V
-    // scale's exponent (0 for a byte that no scale is, in blocks never written)
+    // scale's exponent as far as the probabilities carry it: kLeast or more (0 for a byte
+    // that no scale is, in blocks never written)
     float factors;
     uint32_t units;
+    auto carried = [&](uint32_t v) -> uint32_t {  // e + 127
+      return v == 0 || v > 253 ? 127 : max(v, (uint32_t)(127 + kLeast));
+    };
     auto next_scales = [&]() {
       factors = scale * scale_of(bytes_next & 255);
-      const uint32_t v = bytes_next >> 8;
-      units = (v == 0 || v > 253 ? 127 : 254 - v) * 0x00800080u;
+      units = (254 - carried(bytes_next >> 8)) * 0x00800080u;
     };
     next_scales();
     // ---- staging: wavefront w copies and writes pieces 64 (w + n W) + lane.  Piece
@@ -293,6 +304,35 @@ prefill_int8_kernel(const PrefillArgs a) {
         codes_bf16x16(raw, first, second);
         reinterpret_cast<bf16x8*>(to)[0] = first;
         reinterpret_cast<bf16x8*>(to)[1] = second;
+      }
+    };
+    // What V's scales leave for the operands: this wavefront's pieces of a tile that it has
+    // written (they are its own until the next barrier) times the rest.  Apart from
+    // write_tile, word by word and from LDS, for the time and registers of tiles without.
+    int rest_at = 0;  // the next tile that may have a rest
+    auto apply_rest = [&](int kt, int buf) {
+      if (kt % GT == 0) {  // (its group's bytes are the last loaded)
+        const uint32_t v = bytes_next >> 8, r = 127 + v - carried(v);
+        const bool any = __builtin_amdgcn_ballot_w64(v != 0 && v <= 253 && r != 127) != 0;
+        rest_at = any ? kt : kt + GT;
+        // (every wavefront writes the same)
+        if (any) rest_of[lane] = v == 0 || v > 253 ? 1.f : scale_of(r);
+        if (!any) return;
+      }
+#pragma unroll 1
+      for (int ch = wave; ch < CHUNKS; ch += W) {
+        if (ch < CHUNKS / 2) continue;
+        const int i = (ch - CHUNKS / 2) * 64 + lane;
+        const float by = rest_of[kt % GT * NB + i / D];
+        uint32_t* at = reinterpret_cast<uint32_t*>(&lds.v[buf][(i % D) * VROW + (i / D) * 32]);
+#pragma unroll 1
+        for (int m = 0; m < 8; ++m) {
+          const uint32_t w = at[m];
+          const float lo = __builtin_bit_cast(float, w << 16) * by;
+          const float hi = __builtin_bit_cast(float, w & 0xFFFF0000u) * by;
+          at[m] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi),
+                                        __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+        }
       }
     };
     // LDS writes done, then a barrier; loads to registers stay in flight.
@@ -353,6 +393,8 @@ prefill_int8_kernel(const PrefillArgs a) {
       write_tile(1, 1, n_kt > 2);
       if (n_kt > 3) copy_tile(3);
     }
+    apply_rest(0, 0);
+    if (n_kt > 1 && rest_at <= 1) apply_rest(1, 1);
     barrier();
 
     f32x4 S[NT][2];
@@ -392,6 +434,7 @@ prefill_int8_kernel(const PrefillArgs a) {
     auto prepare = [&](int kt, int buf) __attribute__((always_inline)) {
       if (kt + 2 >= n_kt) return;
       write_tile(kt + 2, next_buf(buf, 2), kt + 3 < n_kt);
+      if (__builtin_expect(kt + 2 >= rest_at, 0)) apply_rest(kt + 2, next_buf(buf, 2));
       if (kt + 4 < n_kt) copy_tile(kt + 4);
     };
     // A step of 32 keys, step `st` of tile kt (in buffer buf): probabilities of S, the

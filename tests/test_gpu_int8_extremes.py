@@ -54,3 +54,59 @@ def test_values_of_zero_and_tiny_ones_beside_others(pa, hq, hkv, d, new, past):
     want, tol = int8_plain.attention(cache, q64[:len(ctx)], tables, ctx, list(enumerate(ctx)),
                                      scale)
     check(got, want, tol)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_scale_byte_0_reads_as_scale_0(pa, d):
+    """V blocks of any codes under byte 0, beside others: their values are zeros, their
+    keys are in the denominator."""
+    rng = np.random.default_rng(d)
+    hq, hkv, ctx = 4, 2, [200, 97, 40]
+    cache = int8_plain.random_cache(rng, 30, hkv, d)
+    zero = rng.random((30, hkv)) < 0.4
+    tables = make_tables(rng, [13, 7, 3], 30)
+    zero[tables[2, :3]] = True  # a sequence with no other
+    cache[3][zero] = 0
+    plain = (cache[0], np.where(zero[:, :, None, None], 0, cache[1]), cache[2], cache[3])
+    q, q64 = query(rng, 3, hq, d)
+    c, scale = on_device(pa, cache), 0.25 / math.sqrt(d)
+    want, tol = int8_plain.attention(plain, q64, tables, ctx, list(enumerate(ctx)), scale)
+    assert not want[2].any()
+    check(pa.decode_int8(q, c, i32(tables), i32(ctx), 200, scale=scale), want, tol)
+    check(pa.prefill_int8(q, c, i32(tables), i32([0, 1, 2, 3]), i32([x - 1 for x in ctx]), 1,
+                          scale=scale), want, tol)
+
+
+@pytest.mark.parametrize("byte", [1, 2, 94, 95, 96, 127, 249, 252, 253, 254])
+@pytest.mark.parametrize("d", [32, 128, 256])
+def test_every_value_scale_alone(pa, byte, d):
+    """One key, so out is its value, in both kernels: powers of two to the first and
+    the last scale."""
+    rng = np.random.default_rng(byte)
+    cache = int8_plain.random_cache(rng, 3, 2, d)
+    cache[1][:] = rng.integers(-1, 2, cache[1].shape)
+    cache[3][:] = byte
+    q, _ = query(rng, 2, 4, d)
+    c, tables = on_device(pa, cache), i32([[2], [1]])
+    want = torch.stack([pa.read_kv_int8(c, i32([b]), 1)[1][0] for b in (2, 1)])
+    want = want.repeat_interleave(2, 1)
+    assert torch.equal(want.abs().amax((1, 2)), torch.full((2,), 2.0 ** (byte - 127), device=DEV))
+    got = pa.prefill_int8(q, c, tables, i32([0, 1, 2]), i32([0, 0]), 1, scale=0.01)
+    assert torch.equal(got.float(), want)
+    assert torch.equal(pa.decode_int8(q, c, tables, i32([1, 1]), 1, scale=0.01).float(), want)
+
+
+def test_masked_blocks_of_the_largest_values(pa):
+    """An id outside the pool is replaced by block 0, here of the largest codes and
+    scale: nothing of it shows."""
+    rng = np.random.default_rng(3)
+    hq, hkv, d, ctx = 4, 2, 64, [100, 33]
+    cache = int8_plain.random_cache(rng, 12, hkv, d)
+    cache[1][0], cache[3][0] = 127, 254
+    tables = np.array([[1, -1, 2, 99, 3, 4, -5], [5, -1, 6, 0, 0, 0, 0]], np.int32)
+    q, q64 = query(rng, 2, hq, d)
+    c, scale = on_device(pa, cache), 0.02
+    want, tol = int8_plain.attention(cache, q64, tables, ctx, list(enumerate(ctx)), scale)
+    check(pa.decode_int8(q, c, i32(tables), i32(ctx), 100, scale=scale), want, tol)
+    check(pa.prefill_int8(q, c, i32(tables), i32([0, 1, 2]), i32([99, 32]), 1, scale=scale),
+          want, tol)

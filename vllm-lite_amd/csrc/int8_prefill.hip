@@ -237,12 +237,12 @@ prefill_int8_kernel(const PrefillArgs a) {
     // K's scale bytes, V's << 8, of the next group
     uint32_t bytes_next = (uint32_t)a.ks[places] | (uint32_t)a.vs[places] << 8;
     // of the tiles computed: the scores' factor, and 2^-e twice in bf16, e being the V
-    // scale's exponent as far as the probabilities carry it: kLeast or more (0 for a byte
-    // that no scale is, in blocks never written)
+    // scale's exponent as far as the probabilities carry it: kLeast to 126, whose 2^-e is
+    // a normal number
     float factors;
     uint32_t units;
     auto carried = [&](uint32_t v) -> uint32_t {  // e + 127
-      return v == 0 || v > 253 ? 127 : max(v, (uint32_t)(127 + kLeast));
+      return min(max(v, 127u + kLeast), 253u);
     };
     auto next_scales = [&]() {
       factors = scale * scale_of(bytes_next & 255);
@@ -307,17 +307,17 @@ prefill_int8_kernel(const PrefillArgs a) {
       }
     };
     // What V's scales leave for the operands: this wavefront's pieces of a tile that it has
-    // written (they are its own until the next barrier) times the rest.  Apart from
-    // write_tile, word by word and from LDS, for the time and registers of tiles without.
+    // written (they are its own until the next barrier) times the rest, 0 for scale byte 0.
+    // Apart from write_tile, word by word and from LDS, for the time and registers of
+    // tiles without.
     int rest_at = 0;  // the next tile that may have a rest
     auto apply_rest = [&](int kt, int buf) {
       if (kt % GT == 0) {  // (its group's bytes are the last loaded)
-        const uint32_t v = bytes_next >> 8, r = 127 + v - carried(v);
-        const bool any = __builtin_amdgcn_ballot_w64(v != 0 && v <= 253 && r != 127) != 0;
+        const uint32_t v = bytes_next >> 8, r = v ? 127 + v - carried(v) : 0;
+        const bool any = __builtin_amdgcn_ballot_w64(r != 127) != 0;
         rest_at = any ? kt : kt + GT;
-        // (every wavefront writes the same)
-        if (any) rest_of[lane] = v == 0 || v > 253 ? 1.f : scale_of(r);
         if (!any) return;
+        rest_of[lane] = scale_of(r);  // (every wavefront writes the same)
       }
 #pragma unroll 1
       for (int ch = wave; ch < CHUNKS; ch += W) {

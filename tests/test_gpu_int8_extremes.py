@@ -28,7 +28,8 @@ def test_values_of_zero_and_tiny_ones_beside_others(pa, hq, hkv, d, new, past):
     nb, total = sum(counts) + 2, sum(ctx)
     tables = make_tables(rng, counts, nb)
     cache = tuple(np.zeros_like(x) for x in int8_plain.random_cache(rng, nb, hkv, d))
-    size = rng.choice([0.0, 2.0 ** -90, 2.0 ** -40, 2.0 ** -24, 1.0, 4.0], (total // 16 + 2, hkv, 1))
+    size = rng.choice([0.0, 2.0 ** -90, 2.0 ** -40, 2.0 ** -24, 1.0, 4.0],
+                      (total // 16 + 2, hkv, 1))
     size[0], size[1] = 0.0, 2.0 ** -90
     key = rng.standard_normal((total, hkv, d)).astype(np.float32)
     value = (1 + 0.1 * rng.standard_normal((total, hkv, d))).astype(np.float32)
@@ -110,3 +111,38 @@ def test_masked_blocks_of_the_largest_values(pa):
     check(pa.decode_int8(q, c, i32(tables), i32(ctx), 100, scale=scale), want, tol)
     check(pa.prefill_int8(q, c, i32(tables), i32([0, 1, 2]), i32([99, 32]), 1, scale=scale),
           want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 32), (4, 2, 64), (6, 2, 96), (4, 1, 128),
+                                      (2, 1, 192), (2, 1, 256)])
+@pytest.mark.parametrize("scale", [0.02, -0.02])
+def test_infinite_queries_against_codes_of_one_sign(pa, hq, hkv, d, scale):
+    """Rows with an infinity, whose scores may all be -inf: NaN, as pa.h says, and the
+    rows beside them their values; zeros for one without keys."""
+    rng = np.random.default_rng(d)
+    new, past = [3, 40, 1, 70], [0, 0, 20, 33]
+    ctx = [a + b for a, b in zip(new, past)]
+    counts = [-(-c // 16) for c in ctx]
+    nb = sum(counts) + 1
+    cache = int8_plain.random_cache(rng, nb, hkv, d)
+    tables = make_tables(rng, counts, nb)
+    for s, sign in enumerate((1, -1, 1, -1)):  # dim 5 has codes of one sign
+        for b in tables[s, :counts[s]]:
+            cache[0][b, :, :, 5] = sign * (1 + np.abs(cache[0][b, :, :, 5] // 2))
+    tables[2] = -1  # no keys
+    q, q64 = query(rng, sum(new), hq, d)
+    hit = rng.random(sum(new)) < 0.5
+    hit[[0, 2, 3, 43]] = True
+    for r in np.flatnonzero(hit):
+        q[r, r % hq, 5] = q64[r, r % hq, 5] = math.inf if r % 3 else -math.inf
+        if r % hq:
+            q[r, 0, 5] = q64[r, 0, 5] = -q64[r, r % hq, 5]
+    c = on_device(pa, cache)
+    rows = [(s, past[s] + i + 1) for s in range(len(new)) for i in range(new[s])]
+    want, tol = int8_plain.attention(cache, q64, tables, ctx, rows, scale)
+    assert np.isnan(want).any() and not want[43].any()
+    check(pa.prefill_int8(q, c, i32(tables), i32(np.cumsum([0] + new)), i32(past), max(new),
+                          scale=scale), want, tol)
+    last = np.cumsum(new) - 1
+    check(pa.decode_int8(q[torch.from_numpy(last).to(DEV)], c, i32(tables), i32(ctx), max(ctx),
+                         scale=scale), want[last], tol[last])

@@ -579,7 +579,15 @@ prefill_int8_kernel(const PrefillArgs a) {
       if (row >= rows) continue;
       const int token = row / G, h = row - token * G;
       const float l = lacc[nt][0];
-      const float inv = l != 0.f ? 1.f / l : 0.f;
+      float inv = 1.f / l;
+      if (l == 0.f) {
+        // no keys, or all its scores are -inf (an infinity in q, against codes of one
+        // sign): 0 or, as other rows of infinities have it, NaN
+        bool keys = !bad_ids;
+        for (int b = 0; !keys && b <= min(pos[nt], key_end - 1) / kBlock; ++b)
+          keys = (uint32_t)tab[b] < (uint32_t)a.num_blocks;
+        inv = keys ? __builtin_nanf("") : 0.f;
+      }
       uint16_t* to = a.out + ((int64_t)(qr.begin + token) * a.Hq + kvh * G + h) * D + 4 * j;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {

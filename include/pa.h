@@ -417,8 +417,9 @@ int32_t pa_decode_int8(void* out, const void* q, const int8_t* k_cache, const in
                        pa_stream_t stream);
 
 /* pa_prefill over an int8 cache, arguments and conventions as there, arithmetic as
- * pa_decode_int8, but with q as it is, and without its loss of V's values under small
- * scale bytes. */
+ * pa_decode_int8, but with q as it is (its products with the codes, before their
+ * scale, are summed in f32: rows of 2^112 and more may leave its range and give NaN), and
+ * without its loss of V's values under small scale bytes. */
 int32_t pa_prefill_int8(void* out, const void* q, const int8_t* k_cache, const int8_t* v_cache,
                         const uint8_t* k_scales, const uint8_t* v_scales,
                         const int32_t* block_tables, int32_t max_blocks_per_seq,

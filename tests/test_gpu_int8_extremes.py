@@ -146,3 +146,20 @@ def test_infinite_queries_against_codes_of_one_sign(pa, hq, hkv, d, scale):
     last = np.cumsum(new) - 1
     check(pa.decode_int8(q[torch.from_numpy(last).to(DEV)], c, i32(tables), i32(ctx), max(ctx),
                          scale=scale), want[last], tol[last])
+
+
+def test_key_scale_byte_0_reads_as_scale_0(pa):
+    """Under byte 0 of K every score is 0, however large the query."""
+    rng = np.random.default_rng(4)
+    hq, hkv, d, ctx = 4, 2, 64, [100, 20]
+    cache = int8_plain.random_cache(rng, 12, hkv, d)
+    cache[2][:] = 0
+    plain = (np.zeros_like(cache[0]), *cache[1:])
+    tables = make_tables(rng, [7, 2], 12)
+    q, q64 = query(rng, 2, hq, d)
+    c, scale = on_device(pa, cache), 1.0
+    want, tol = int8_plain.attention(plain, q64, tables, ctx, list(enumerate(ctx)), scale)
+    check(pa.decode_int8(q * 2.0 ** 118, c, i32(tables), i32(ctx), 100, scale=scale), want, tol)
+    # (prefill's sums of q times codes are f32)
+    check(pa.prefill_int8(q * 2.0 ** 100, c, i32(tables), i32([0, 1, 2]), i32([99, 19]), 1,
+                          scale=scale), want, tol)

@@ -200,7 +200,8 @@ __device__ inline void int8_softmax(const i32x4 (&a)[4], uint32_t kscale, uint32
                                     bf16x8& p1) {
   // blocks that are not attended may hold any bytes
   const bool none = !whole && lim <= 0;
-  const float f = ldexpf(factor, none ? 0 : (int)kscale - 127);
+  // (a factor of 2^-1000 is 0, NaN stays)
+  const float f = ldexpf(factor, none ? 0 : kscale ? (int)kscale - 127 : -1000);
   const float fv = scale_of(none ? 127 : vscale);
   float x[16];
 #pragma unroll

@@ -163,3 +163,18 @@ def test_key_scale_byte_0_reads_as_scale_0(pa):
     # (prefill's sums of q times codes are f32)
     check(pa.prefill_int8(q * 2.0 ** 100, c, i32(tables), i32([0, 1, 2]), i32([99, 19]), 1,
                           scale=scale), want, tol)
+
+
+@pytest.mark.parametrize("power", [-126, -100, -60, 0, 60, 110])
+def test_queries_and_key_scales_of_opposite_sizes(pa, power):
+    """Queries of 2^power, keys of 70 * 2^-power: the scores are of normal size."""
+    rng = np.random.default_rng(power + 200)
+    hq, hkv, d, ctx = 4, 2, 64, [300, 97]
+    cache = int8_plain.random_cache(rng, 30, hkv, d, 1.0)
+    cache[2][:] = cache[2].astype(int) + 6 - power
+    tables = make_tables(rng, [19, 7], 30)
+    q = torch.from_numpy(rng.standard_normal((2, hq, d)) * 2.0 ** power).to(torch.bfloat16)
+    c, scale = on_device(pa, cache), 1.2e-3
+    want, tol = int8_plain.attention(cache, q.double().numpy(), tables, ctx,
+                                     list(enumerate(ctx)), scale)
+    check(pa.decode_int8(q.to(DEV), c, i32(tables), i32(ctx), 300, scale=scale), want, tol)

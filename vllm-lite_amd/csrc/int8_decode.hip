@@ -94,7 +94,7 @@ decode_int8_kernel(
       blocks.load_keys(next.kid, next.vid, c, j, k);
     }
     __builtin_amdgcn_sched_barrier(0);
-    int8_softmax<D>(a, kscale, v.scale, qv.factor, now.whole, now.lim, S, p0, p1);
+    int8_softmax<D>(a, kscale, v.scale, qv, now.whole, now.lim, S, p0, p1);
     __builtin_amdgcn_sched_barrier(0);
     int8_output<D>(v, p0, p1, S);
     if constexpr (decltype(more)::value) blocks.load_values(next.vid, c, v);

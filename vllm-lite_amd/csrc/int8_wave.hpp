@@ -49,7 +49,10 @@ template <int D>
 struct Int8Query {
   static constexpr int KS = (D + 63) / 64;  // reduction steps of 64 dims
   i32x4 hi[KS], lo[KS];
-  float factor;  // of a score: scale * log2(e) * 2^e; NaN for a row that is not finite
+  // Of a score: factor 2^e, scale * log2(e) by the row's unit; NaN for a row that is not
+  // finite.  (Apart, as the product may be below the floats and a score not.)
+  float factor;
+  int e;
 };
 
 // The 16-byte chunk of a K row that reduction step s reads in lane group j; a chunk
@@ -109,7 +112,8 @@ __device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, 
     q.hi[s] = i32x4{(int)hw[0], (int)hw[1], (int)hw[2], (int)hw[3]};
     q.lo[s] = i32x4{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
   }
-  q.factor = worse ? __builtin_nanf("") : ldexpf(scale_log2, e);
+  q.factor = worse ? __builtin_nanf("") : scale_log2;
+  q.e = e;
 }
 
 // A wavefront's online softmax: o unnormalised, m in the log2 domain, lsum this
@@ -196,12 +200,12 @@ __device__ inline void int8_scores(const Int8Keys<D>& st, const Int8Query<D>& q,
 // (wavefront-uniform).
 template <int D>
 __device__ inline void int8_softmax(const i32x4 (&a)[4], uint32_t kscale, uint32_t vscale,
-                                    float factor, bool whole, int lim, Int8State<D>& S, bf16x8& p0,
-                                    bf16x8& p1) {
+                                    const Int8Query<D>& q, bool whole, int lim, Int8State<D>& S,
+                                    bf16x8& p0, bf16x8& p1) {
   // blocks that are not attended may hold any bytes
   const bool none = !whole && lim <= 0;
   // (a factor of 2^-1000 is 0, NaN stays)
-  const float f = ldexpf(factor, none ? 0 : kscale ? (int)kscale - 127 : -1000);
+  const float f = ldexpf(q.factor, none ? 0 : kscale ? q.e + (int)kscale - 127 : -1000);
   const float fv = scale_of(none ? 127 : vscale);
   float x[16];
 #pragma unroll

@@ -178,3 +178,22 @@ def test_queries_and_key_scales_of_opposite_sizes(pa, power):
     want, tol = int8_plain.attention(cache, q.double().numpy(), tables, ctx,
                                      list(enumerate(ctx)), scale)
     check(pa.decode_int8(q.to(DEV), c, i32(tables), i32(ctx), 300, scale=scale), want, tol)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_decode_rounds_a_query_to_2_to_the_minus_14_of_its_largest(pa, sign):
+    """The largest with all its bits set and 63 values of 2^-13 of its power of two:
+    rounded by 2^-14 of the largest each at most (here not at all), their products with
+    two keys of 127 and -127 (and 0 for the largest) differ by 4: tanh(2) of the values
+    1 and -1, off by the rounding of probabilities and out, 2^-8 each."""
+    h = 2.0 ** -13
+    q = torch.full((1, 1, 64), h, dtype=torch.bfloat16, device=DEV)
+    q[0, 0, 0] = sign * (2 - 2.0 ** -7)
+    cache = tuple(np.zeros(s, t) for s, t in (((1, 1, 16, 64), np.int8), ((1, 1, 64, 16), np.int8),
+                                              ((1, 1), np.uint8), ((1, 1), np.uint8)))
+    cache[0][0, 0, 0, 1:], cache[0][0, 0, 1, 1:] = 127, -127
+    cache[1][0, 0, :, 0], cache[1][0, 0, :, 1] = 64, -64
+    cache[2][:], cache[3][:] = 127, 121
+    out = pa.decode_int8(q, on_device(pa, cache), i32([[0]]), i32([2]), 2,
+                         scale=2 / (63 * 127 * h)).float()
+    assert (out - math.tanh(2)).abs().max() <= 2.0 ** -7

@@ -91,11 +91,10 @@ __device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, 
   top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
   const bool worse = top >= 0x7F80u;
   const float amax = bf16_bits_to_f32((uint16_t)top);
-  // |x| 2^-e < 2^14 - 64: the largest is m 2^b, m < 2, so e = b - 13 gives less than
-  // 2^14 and hi at most 128 where m is near 2; e = b - 12 there
+  // |x| 2^-e < 2^14, the largest being m 2^b, m < 2, and e = b - 13.  (Subnormal rows are
+  // multiples of 2^-133: exact at e = -140.)
   const uint32_t u = __builtin_bit_cast(uint32_t, amax);
-  int e = (int)(u >> 23) - 127 - 13 + ((u & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
-  e = max(e, -140);
+  const int e = (int)(u >> 23) - 127 - 13;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     uint32_t hw[4], lw[4];
@@ -105,7 +104,8 @@ __device__ inline void int8_query(const uint16_t* row, int j, float scale_log2, 
     for (int i = 0; i < 16; ++i) {
       const float x = bf16_bits_to_f32((uint16_t)(raw[s][i / 2] >> (16 * (i & 1))));
       const int n = worse ? 0 : (int)rintf(ldexpf(x, -e));
-      const int hi = (n + 64) >> 7, lo = n - 128 * hi;
+      // |n| <= 2^14 - 64 (8 bits of the largest): hi from -128 to 127, lo from -63 to 64
+      const int hi = (n + 63) >> 7, lo = n - 128 * hi;
       hw[i / 4] |= (uint32_t)(uint8_t)hi << (8 * (i & 3));
       lw[i / 4] |= (uint32_t)(uint8_t)lo << (8 * (i & 3));
     }

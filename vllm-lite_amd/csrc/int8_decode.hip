@@ -42,8 +42,10 @@ decode_int8_kernel(
   const int begin = part * part_len;
   const int32_t* tab = tables + (int64_t)seq * mbs;
   // Lane t holds block t % 4 of the wavefront's step t / 4, for 16 steps.
+  // (Counted in blocks: tokens so far behind the largest context pass 31 bits.)
   auto load_ids = [&](int step) -> int32_t {
-    const int b = (begin + (wave + (step + lane / 4) * NW) * kStep) / kBlock + lane % 4;
+    const int b =
+        begin / kBlock + (wave + (step + lane / 4) * NW) * (kStep / kBlock) + lane % 4;
     return b < mbs ? tab[b] : -1;
   };
   int32_t ids = load_ids(0);

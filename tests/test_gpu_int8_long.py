@@ -24,3 +24,19 @@ def test_ids_are_read_inside_the_widest_table(pa):
     got = pa.decode_int8(q, on_device(pa, cache), tables, i32([ctx]), MBS * 16, scale=scale)
     want, tol = int8_plain.attention(cache, q64, ids, [ctx], [(0, ctx)], scale)
     check(got, want, tol)
+
+
+@pytest.mark.parametrize("ctx", [2 ** 31 - 70000000, 2 ** 31 - 5000])
+def test_parts_of_the_longest_contexts_are_merged(pa, ctx):
+    """All scores 0 and values 1 or -1, the same at every token: out is the value (the
+    sums are of multiples of 1 to 2^24 and, among 32 parts, off by 2^-20)."""
+    d = 32
+    cache = tuple(np.zeros(s, t) for s, t in (((2, 1, 16, d), np.int8), ((2, 1, d, 16), np.int8),
+                                              ((2, 1), np.uint8), ((2, 1), np.uint8)))
+    value = np.where(np.arange(d) % 3 == 0, -1, 1)
+    cache[1][:] = value[:, None]
+    cache[2][:] = cache[3][:] = 127
+    tables = torch.ones(1, MBS, dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 1, d, dtype=torch.bfloat16, device=DEV)
+    out = pa.decode_int8(q, on_device(pa, cache), tables, i32([ctx]), MBS * 16)
+    assert torch.equal(out[0, 0].float(), dev(value.astype(np.float32)))

@@ -160,7 +160,8 @@ __global__ __launch_bounds__(64) void decode_int8_merge_kernel(
   const float* o = ws_o + row * num_parts * D;
   float2 mine = ml[min(lane, num_parts - 1)];  // (parts without keys are not written)
   const int ctx = min(context_lens[row / Hq], mbs * kBlock);
-  const int np = min(num_parts, (max(ctx, 1) + part_len - 1) / part_len);
+  // (the part of the last token: ctx + part_len may pass 31 bits)
+  const int np = min(num_parts, (max(ctx, 1) - 1) / part_len + 1);
   float M = kInt8NoMax, num[DL], den = 0.f;
 #pragma unroll
   for (int x = 0; x < DL; ++x) num[x] = 0.f;

@@ -396,7 +396,8 @@ int32_t pa_read_kv_int8(const int8_t* k_cache, const int8_t* v_cache, const uint
                         int32_t seq_len, int32_t num_kv_heads, int32_t head_dim,
                         int32_t num_blocks, float* out_k, float* out_v, pa_stream_t stream);
 
-/* Bytes of workspace pa_decode_int8 needs for these sizes (0: none). */
+/* Bytes of workspace pa_decode_int8 needs for these sizes (0: none), or for fewer
+ * sequences and shorter contexts: it grows with both. */
 size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                      int32_t head_dim, int32_t max_context_len);
 

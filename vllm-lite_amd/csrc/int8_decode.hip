@@ -11,13 +11,14 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "int8_plan.hpp"
 #include "int8_wave.hpp"
 #include "pa_internal.hpp"
 
 namespace pa {
 namespace {
 
-constexpr int kStep = 4 * kBlock;  // tokens a step
+constexpr int kStep = kInt8Step;
 
 // Each wavefront takes every NW-th step of the part, so that its block ids are known
 // before the context length is.  The next step's K is loaded where this one's has
@@ -207,40 +208,6 @@ __global__ __launch_bounds__(64) void decode_int8_merge_kernel(
       out[row * D + lane + 64 * x] = f32_to_bf16_bits(den != 0.f ? num[x] / den : 0.f);
 }
 
-// How a launch over contexts of up to max_ctx tokens is cut, after sweeps of 1 to 96
-// parts and 4 or 8 wavefronts over 37 launches of 2 to 1600 (sequence, kv head) pairs
-// and 130 to 120000 tokens: within 3 % of the best of them in the mean, 14 % at worst.
-//   One part where contexts are short (the merge's launch takes 3 us) or fill the card
-//     by pairs: 32 x 320-768, 14 / 2 heads of 64, 6.6 us and 8.0 as four; 64 x 4096,
-//     32 / 8 of 128, 88 and 93 as two; but 16 x 8192-32768 145 as two, 128 as 48.
-//   Else as many as put one workgroup on each of 256 CUs (1 x 1537 of 32 / 8 x 128:
-//     15 us whole, 10 as 8 to 24 parts; 8 x 8000-16000 of 14 / 2 x 64: 50 whole, 12 as
-//     16), and for many or long sequences, whose lengths differ, no longer than 1344 tokens (11 x
-//     37-29000 of 24 / 4 x 96: 38 us as 6, 35 as 22 to 24, 40 as 64).  Not where head_dim
-//     256 leaves one workgroup to a CU: 5 x 968-20891 67 us as 6, 87 as 16.
-//   8 wavefronts a workgroup where workgroups are few, 4 where they are many (1024 pairs
-//     of 100-1000 tokens 36 us with 4, 44 with 8) or short.
-struct Int8Plan {
-  int waves, part_len, parts;
-};
-Int8Plan plan_of(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_ctx) {
-  const int groups = (num_heads / num_kv_heads + 15) / 16;
-  const long long pairs = (long long)num_seqs * num_kv_heads * groups;
-  constexpr int kLongest = 21 * kStep;
-  long long parts = 1;
-  if (max_ctx > 768 && !(pairs >= 160 && max_ctx <= 7 * kLongest / 2)) {
-    parts = std::min({256 / pairs, (long long)max_ctx / 96, 32ll});
-    if (head_dim <= 192 && pairs > 8)
-      parts = std::max(parts, ((long long)max_ctx + kLongest - 1) / kLongest);
-    parts = std::max(parts, 1ll);
-  }
-  const long long len = ((max_ctx + parts - 1) / parts + kStep - 1) / kStep * kStep;
-  parts = std::max(1ll, (max_ctx + len - 1) / std::max(len, 1ll));
-  const bool eight = head_dim < 256 && pairs * parts <= 300 &&
-                     !(parts == 1 && head_dim > 64 && max_ctx <= 640);
-  return {eight ? 8 : 4, (int)std::max(len, (long long)kStep), (int)parts};
-}
-
 }  // namespace
 }  // namespace pa
 
@@ -252,9 +219,8 @@ extern "C" size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_he
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
       head_dim <= 0 || max_context_len <= 0)
     return 0;
-  const Int8Plan p = plan_of(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len);
-  return p.parts == 1 ? 0
-                      : (size_t)num_seqs * num_heads * p.parts * (head_dim + 2) * sizeof(float);
+  return (size_t)int8_most_parts(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len) *
+         num_heads * (head_dim + 2) * sizeof(float);
 }
 
 namespace pa {
@@ -289,7 +255,7 @@ int32_t decode_int8_strided(void* out, const void* q, int64_t q_row, const int8_
                  q_row % 2 == 0 && (uintptr_t)out % 2 == 0,
              PA_ERR_INVALID_ARG, "pa_decode_int8: caches not 16-byte or q not 4-byte aligned");
   const int G = num_heads / num_kv_heads, head_groups = (G + 15) / 16;
-  const Int8Plan plan = plan_of(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len);
+  const Int8Plan plan = int8_plan(num_seqs, num_heads, num_kv_heads, head_dim, max_context_len);
   const int np = plan.parts;
   PA_REQUIRE(num_seqs <= 65535 && (long long)num_kv_heads * head_groups <= 65535 &&
                  (long long)num_blocks * num_kv_heads < (1ll << 32) && grid_fits(np, 512) &&

@@ -95,7 +95,9 @@ struct Settings {
   double rate, least;   // of y = 16 (max - x) / (T ln 2): the factor, and min-p's bound
   int k;
   bool greedy, by_k, by_p;
-  float range, step;    // intervals: of d = max - x up to range, step a unit
+  // intervals: of d = (max - x) / 2, which is a float where max - x is not, up to range,
+  // step a unit
+  float half, range, step;  // half: max / 2
   __device__ bool narrows() const { return (by_k || by_p) && max > -INFINITY; }
 };
 
@@ -154,7 +156,7 @@ __device__ inline unsigned long long kept_weight(float x, const Settings& s, int
 __device__ inline int bin_of(float x, const Settings& s) {
 #pragma clang fp contract(off)
   if (x == s.max) return 0;
-  const float d = s.max - x;
+  const float d = __builtin_fmaf(x, -0.5f, s.half);
   if (!(d <= s.range) || !(d < INFINITY)) return -1;
   return min((int)(d * s.step), kBins - 1);
 }
@@ -208,8 +210,9 @@ __device__ inline void prepare(const Args& a, int row, const Row& r, Settings& t
     return u32(fminf(f32(v), f32(w)));
   }));
   s.top = (double)s.max;
-  // Weights end at exp(-(shift + 1) ln 2), shift <= 51: d / T <= 36.1.
-  s.range = fminf(37.f * s.t, s.max - s.min);
+  // Weights end at exp(-(shift + 1) ln 2), shift <= 51: 2 d / T <= 36.1.
+  s.half = 0.5f * s.max;
+  s.range = fminf(18.5f * s.t, __builtin_fmaf(s.min, -0.5f, s.half));
   s.step = s.range > 0.f ? kBins / s.range : 0.f;
   if (threadIdx.x == 0) to = s;
 }

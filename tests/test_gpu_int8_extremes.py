@@ -197,3 +197,22 @@ def test_decode_rounds_a_query_to_2_to_the_minus_14_of_its_largest(pa, sign):
     out = pa.decode_int8(q, on_device(pa, cache), i32([[0]]), i32([2]), 2,
                          scale=2 / (63 * 127 * h)).float()
     assert (out - math.tanh(2)).abs().max() <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("scale,spread", [(0.125, 0.0), (3.0, 0.0), (-0.1, 3.0), (0.0, 2.0),
+                                          (1e-3, 40.0)])
+def test_prefill_of_scales_far_apart(pa, scale, spread):
+    """Peaked and flat softmaxes, a negative and a zero softmax scale, blocks whose
+    scales are far apart, in chunks."""
+    rng = np.random.default_rng(12)
+    hq, hkv, d, new, past = 4, 2, 64, [70, 33], [230, 0]
+    cache = int8_plain.random_cache(rng, 30, hkv, d, spread)
+    if spread > 8:
+        cache[2][:] = 121  # scores that are finite, values of any size
+    tables = make_tables(rng, [19, 3], 30)
+    q, q64 = query(rng, 103, hq, d)
+    got = pa.prefill_int8(q, on_device(pa, cache), i32(tables), i32([0, 70, 103]), i32(past), 70,
+                          scale=scale)
+    rows = [(s, past[s] + i + 1) for s in range(2) for i in range(new[s])]
+    want, tol = int8_plain.attention(cache, q64, tables, [300, 33], rows, scale)
+    check(got, want, tol)

@@ -224,7 +224,9 @@ int32_t pa_batch_qkv_rope_cache(pa_batch* batch, pa_kv_cache* cache, int32_t lay
  * the cache and q is final (pa_batch_qkv_rope_cache ran); attention only.
  * Allocates (once, grown on demand) the decode workspace; a call that would
  * grow it while `stream` is capturing returns PA_ERR_WORKSPACE instead (run
- * one eager step of the captured shape first). */
+ * one eager step of the captured shape first).  Growing frees the old one: a
+ * step captured before a larger one (more sequences, a larger capacity) ran
+ * has to be captured again; smaller ones leave it. */
 int32_t pa_batch_attention(pa_batch* batch, pa_kv_cache* cache, int32_t layer, int32_t num_heads,
                            void* q, int64_t q_stride, const void* key, int64_t key_stride,
                            const void* value, int64_t value_stride, const float* inv_freq,

@@ -68,7 +68,7 @@ struct AppendArgs {
 // where ALIGNED, and V's codes meet in LDS as words of neighbouring tokens.  ROPE
 // (K and q are rotated) is apart for its registers.
 // Bound by its chain of loads (offsets, table, old scale and codes) for a decode
-// step: 4.2 us for 32 tokens; by memory for prompts: 8192 tokens of 8 x 128 bf16 15.6
+// step: 4.2 us for 32 tokens; by memory for prompts: 9434 tokens of 8 x 128 bf16 15.6
 // us, 3.7 TB/s (22 with 4 values a lane and codes by compares and conversions).
 template <typename T, int D, bool ALIGNED, bool ROPE>
 __global__ __launch_bounds__(64) void append_int8_kernel(const AppendArgs a) {

@@ -224,7 +224,7 @@ prefill_int8_kernel(const PrefillArgs a) {
     const bool active = r0 < rows;
 
     // ---- the blocks' places and scales: lane t holds those of block t of a group of GT
-    // tiles.  Blocks behind the last and ids outside the pool read block 0.
+    // tiles.  Blocks behind the last read the last, ids outside the pool block 0.
     const float scale = fabsf(a.scale_log2);
     auto load_ids = [&](int group) -> int32_t {
       return tab[min(group * 64 + lane, nblk - 1)];

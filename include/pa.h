@@ -405,7 +405,8 @@ size_t pa_decode_int8_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  * query heads per kv head; calls that may overlap need workspaces of their own).
  * The scores are exact products of the codes with q rounded to 2^-14 of its row's
  * largest value, probabilities times the V scale are rounded to bf16, sums are f32.
- * A query row with a NaN or an infinity gives NaN.  Where V's scale bytes are below
+ * A query row with a NaN or an infinity gives NaN; so does one of which all scores, or
+ * the largest, are beyond f32's range.  Where V's scale bytes are below
  * 16 or above 240, probabilities times the scale may leave bf16's range: small
  * values come out as 0 (their keys count in the denominator all the same), large ones
  * as infinities or NaN. */

@@ -216,3 +216,32 @@ def test_prefill_of_scales_far_apart(pa, scale, spread):
     rows = [(s, past[s] + i + 1) for s in range(2) for i in range(new[s])]
     want, tol = int8_plain.attention(cache, q64, tables, [300, 33], rows, scale)
     check(got, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d,ctx", [(4, 2, 64, [40, 300, 7]), (32, 8, 128, [1500, 3]),
+                                          (2, 1, 256, [100, 17])])
+def test_scores_below_the_floats(pa, hq, hkv, d, ctx):
+    """A finite query against keys so large that all of a row's scores are below f32's
+    range: NaN, not the 0 of a row without keys; where some key's score is a float, its
+    value."""
+    rng = np.random.default_rng(d)
+    counts = [-(-c // 16) for c in ctx]
+    nb = sum(counts) + 1
+    cache = int8_plain.random_cache(rng, nb, hkv, d)
+    cache[0][:] = -1 - np.abs(cache[0] // 2)
+    cache[2][:] = 200
+    tables = make_tables(rng, counts, nb)
+    # the second sequence's first block: scores that are floats, the largest token 1's, 0
+    cache[0][tables[1, 0], :, 1], cache[2][tables[1, 0]] = 0, 100
+    tables[0, 0] = -1
+    c = on_device(pa, cache)
+    q = torch.full((len(ctx), hq, d), 2.0 ** 70, dtype=torch.bfloat16, device=DEV)
+    want = np.full(q.shape, np.nan)
+    v = int8_plain.values(cache[1], cache[3])[tables[1, 0], :, :, 1]
+    want[1] = np.repeat(v, hq // hkv, 0)
+    tol = 2.0 ** -7 * np.abs(want)
+    check(pa.decode_int8(q, c, i32(tables), i32(ctx), max(ctx), scale=1.0), want, tol)
+    check(pa.prefill_int8(q, c, i32(tables), i32(range(len(ctx) + 1)), i32([n - 1 for n in ctx]),
+                          1, scale=1.0), want, tol)
+    none = torch.full_like(i32(tables), -1)
+    assert not pa.decode_int8(q, c, none, i32(ctx), max(ctx), scale=1.0).any()

@@ -85,6 +85,7 @@ decode_int8_kernel(
                 j, scale_log2, qv);
   Int8State<D> S;
   S.init();
+  int keys = 0;  // whether block j had any
   auto step = [&](int s, auto more) {
     i32x4 a[4];
     bf16x8 p0, p1;
@@ -98,6 +99,7 @@ decode_int8_kernel(
     }
     __builtin_amdgcn_sched_barrier(0);
     int8_softmax<D>(a, kscale, v.scale, qv, now.whole, now.lim, S, p0, p1);
+    keys |= now.lim;
     __builtin_amdgcn_sched_barrier(0);
     int8_output<D>(v, p0, p1, S);
     if constexpr (decltype(more)::value) blocks.load_values(next.vid, c, v);
@@ -105,6 +107,7 @@ decode_int8_kernel(
   };
   for (int s = 0; s + 1 < steps; ++s) step(s, std::true_type{});
   if (steps > 0) step(steps - 1, std::false_type{});
+  if (S.m == kInt8NoMax && __builtin_amdgcn_ballot_w64(keys != 0) != 0) S.m = kInt8AllBelow;
   float lsum = S.lsum;
   lsum += __shfl_xor(lsum, 16, 64);
   lsum += __shfl_xor(lsum, 32, 64);
@@ -135,8 +138,7 @@ decode_int8_kernel(
       den += a * sml[w][h][1];
     }
     if (num_parts == 1) {
-      // den is 0 for a row without keys; NaN goes through
-      out[row0 * D + i] = f32_to_bf16_bits(den != 0.f ? num / den : 0.f);
+      out[row0 * D + i] = f32_to_bf16_bits(int8_quotient(num, den, m));
     } else {
       const int64_t at = (row0 + h) * num_parts + part;
       ws_o[at * D + d] = num;
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(64) void decode_int8_merge_kernel(
 #pragma unroll
   for (int x = 0; x < DL; ++x)
     if (lane + 64 * x < D)
-      out[row * D + lane + 64 * x] = f32_to_bf16_bits(den != 0.f ? num[x] / den : 0.f);
+      out[row * D + lane + 64 * x] = f32_to_bf16_bits(int8_quotient(num[x], den, M));
 }
 
 }  // namespace

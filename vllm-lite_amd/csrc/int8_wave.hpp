@@ -23,8 +23,15 @@ namespace pa {
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInt8Log2e = 1.4426950408889634f;
-// "No maximum yet": below any score, and m - m is 0.
+// "No maximum yet": below any score, and m - m is 0.  And where there were keys, all of
+// whose scores are -inf: no maximum either, but a row of only such is no row without keys.
 constexpr float kInt8NoMax = -3.0e38f;
+constexpr float kInt8AllBelow = -2.9e38f;
+// A row's output from its numerator, denominator and maximum: 0 for one without keys; NaN
+// goes through.
+__device__ inline float int8_quotient(float num, float den, float m) {
+  return den != 0.f ? num / den : m == kInt8AllBelow ? __builtin_nanf("") : 0.f;
+}
 
 // Four int8 codes of w as floats, and pairs of those as bf16 (exact: the low half
 // of such a float is 0).
